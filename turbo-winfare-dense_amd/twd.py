@@ -153,6 +153,17 @@ _SIGS = {
     "twd_validate_sampling": (C.c_int, [_f32, _f32, _i32, _f32]),
     "twd_generate_head": (C.c_int, [_vp, _u32, _u32, _u32, _u64, _vp]),
     "twd_head_bytes": (_u64, [_u32, _u32, _u32]),
+    "twd_mx_quantize": (C.c_int, [_vp, C.c_int, _u64, _u32, _u64, _vp, _vp, _vp]),
+    "twd_mx_dequantize": (C.c_int, [_vp, _vp, _u64, _u32, _vp, C.c_int, _u64, _vp]),
+    "twd_mxhead_create": (C.c_int, [_vp, _vp, _u32, _u32, _f32, _vp, C.POINTER(_vp)]),
+    "twd_mxhead_destroy": (None, [_vp]),
+    "twd_mxhead_info": (C.c_int, [_vp, C.POINTER(_u32), C.POINTER(_u32), C.POINTER(_f32), C.POINTER(_u64)]),
+    "twd_mxhead_logits": (C.c_int, [_vp, _vp, _u32, _u64, _vp, C.c_int, _u64, _vp]),
+    "twd_mxhead_logits_mx": (C.c_int, [_vp, _vp, _vp, _u32, _vp, C.c_int, _u64, _vp]),
+    "twd_sampler_create": (C.c_int, [_u32, _u32, C.POINTER(_vp)]),
+    "twd_sampler_destroy": (None, [_vp]),
+    "twd_sampler_sample": (C.c_int, [_vp, _vp, C.c_int, _u32, _u32, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                     _vp, _vp]),
     "twd_probe_read_bandwidth": (C.c_int, [_vp, _u64, _u32, _u32, _vp, C.POINTER(_f32),
                                            C.POINTER(_u64)]),
 }
@@ -712,6 +723,198 @@ class LMHead:
                                            _ptr(history), _ptr(logits), _ptr(tokens),
                                            _stream(stream)))
         return tokens, logits
+
+
+# ---- microscaled 4-bit floating point, and sampling from given random numbers -----------------------
+
+F32, BF16, F16 = 0, 1, 2
+
+
+def _type_of(t, what: str) -> int:
+    import torch
+    code = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}.get(t.dtype)
+    if code is None:
+        raise ValueError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
+    return code
+
+
+def _on_device(*tensors):
+    """A guard that makes the tensors' one device the current one for the call."""
+    import torch
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on {dev} and {t.device} in one call")
+    if dev.type != "cuda":
+        raise ValueError(f"device tensors are needed, not tensors on {dev}")
+    return torch.cuda.device(dev)
+
+
+def _matrix(t, what: str):
+    """(rows, cols, row stride) of a 2-D tensor whose columns are adjacent."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{what} must be two-dimensional with adjacent columns")
+    return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _buffer(t, shape, dtype, what: str):
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+    return t
+
+
+def mx_quantize(x, codes=None, scales=None, stream=None):
+    """Rows of a float32, bfloat16 or float16 device tensor [rows, cols] in microscaled 4-bit floating
+    point (twd_mx_quantize): (codes uint8 [rows, cols / 2], scales uint8 [rows, cols / 32])."""
+    import torch
+    kind = _type_of(x, "x")
+    rows, cols, stride = _matrix(x, "x")
+    with _on_device(x, codes, scales):
+        if codes is None:
+            codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
+        if scales is None:
+            scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
+        _buffer(codes, (rows, cols // 2), torch.uint8, "codes")
+        _buffer(scales, (rows, cols // 32), torch.uint8, "scales")
+        _check(lib.twd_mx_quantize(_ptr(x), kind, rows, cols, stride, _ptr(codes), _ptr(scales), _stream(stream)))
+    return codes, scales
+
+
+def mx_dequantize(codes, scales, dtype=None, out=None, stream=None):
+    """The values that codes and scales stand for (twd_mx_dequantize), in `dtype` (bfloat16) or out's."""
+    import torch
+    rows, half, _ = _matrix(codes, "codes")
+    _buffer(codes, (rows, half), torch.uint8, "codes")
+    _buffer(scales, (rows, half // 16), torch.uint8, "scales")
+    with _on_device(codes, scales, out):
+        if out is None:
+            out = torch.empty(rows, 2 * half, dtype=dtype or torch.bfloat16, device=codes.device)
+        elif tuple(out.shape) != (rows, 2 * half) or (dtype is not None and out.dtype != dtype):
+            raise ValueError(f"out must be of shape {(rows, 2 * half)} and of dtype, where that is given")
+        kind = _type_of(out, "out")
+        _, _, stride = _matrix(out, "out")
+        _check(lib.twd_mx_dequantize(_ptr(codes), _ptr(scales), rows, 2 * half, _ptr(out), kind, stride,
+                                     _stream(stream)))
+    return out
+
+
+class MxHead:
+    """An LM head in microscaled 4-bit floating point, resident in HBM (twd_mxhead)."""
+
+    def __init__(self, codes, scales, softcap: float = 0.0, stream=None):
+        """codes uint8 [vocab, d_model / 2] and scales uint8 [vocab, d_model / 32] on the device; they may
+        be freed afterwards."""
+        import torch
+        self.handle = None
+        vocab, half, _ = _matrix(codes, "codes")
+        _buffer(codes, (vocab, half), torch.uint8, "codes")
+        _buffer(scales, (vocab, half // 16), torch.uint8, "scales")
+        h = C.c_void_p()
+        with _on_device(codes, scales):
+            _check(lib.twd_mxhead_create(_ptr(codes), _ptr(scales), vocab, 2 * half, softcap, _stream(stream),
+                                         C.byref(h)))
+        self.handle = h
+        self.device = codes.device
+        self.vocab, self.d_model, self.softcap = vocab, 2 * half, softcap
+        n = _u64()
+        _check(lib.twd_mxhead_info(h, None, None, None, C.byref(n)))
+        self.nbytes = n.value
+
+    @classmethod
+    def from_weights(cls, w, softcap: float = 0.0, stream=None) -> "MxHead":
+        """Quantises float32, bfloat16 or float16 weights [vocab, d_model] (mx_quantize)."""
+        codes, scales = mx_quantize(w, stream=stream)
+        return cls(codes, scales, softcap, stream)
+
+    def close(self):
+        if self.handle:
+            lib.twd_mxhead_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _out(self, rows: int, out):
+        import torch
+        if out is None:
+            out = torch.empty(rows, self.vocab, dtype=torch.float32, device=self.device)
+        if tuple(out.shape) != (rows, self.vocab):
+            raise ValueError(f"out must be of shape {(rows, self.vocab)}")
+        return out, _type_of(out, "out"), _matrix(out, "out")[2]
+
+    def logits(self, hidden, out=None, stream=None):
+        """Logits of bfloat16 hidden rows [rows, d_model] (or their bits in int16), in out's float32 or
+        bfloat16 (float32 where none is given)."""
+        import torch
+        rows, d, stride = _matrix(hidden, "hidden")
+        if d != self.d_model or hidden.dtype not in (torch.bfloat16, torch.int16):
+            raise ValueError(f"hidden must be bfloat16 [rows, {self.d_model}]")
+        with _on_device(hidden, out):
+            out, kind, out_stride = self._out(rows, out)
+            _check(lib.twd_mxhead_logits(self.handle, _ptr(hidden), rows, stride, _ptr(out), kind, out_stride,
+                                         _stream(stream)))
+        return out
+
+    def logits_mx(self, codes, scales, out=None, stream=None):
+        """Logits of hidden rows that mx_quantize brought into the format too."""
+        import torch
+        rows = codes.shape[0]
+        _buffer(codes, (rows, self.d_model // 2), torch.uint8, "codes")
+        _buffer(scales, (rows, self.d_model // 32), torch.uint8, "scales")
+        with _on_device(codes, scales, out):
+            out, kind, out_stride = self._out(rows, out)
+            _check(lib.twd_mxhead_logits_mx(self.handle, _ptr(codes), _ptr(scales), rows, _ptr(out), kind,
+                                            out_stride, _stream(stream)))
+        return out
+
+
+class Sampler:
+    """Scratch for sampling with temperature, top-k, top-p and min-p from given draws (twd_sampler)."""
+
+    def __init__(self, max_vocab: int, max_rows: int = MAX_ROWS):
+        self.handle = None
+        h = C.c_void_p()
+        _check(lib.twd_sampler_create(max_vocab, max_rows, C.byref(h)))
+        self.handle = h
+        self.max_vocab, self.max_rows = max_vocab, max_rows
+
+    def close(self):
+        if self.handle:
+            lib.twd_sampler_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def sample(self, logits, uniform, temperature=None, top_k=None, top_p=None, min_p=None, tokens=None,
+               logprobs=None, kept=None, stream=None):
+        """One id per row of float32, bfloat16 or float16 logits [rows, vocab] (twd_sampler_sample). uniform
+        and, where given, temperature, top_p and min_p are float32 device tensors [rows], top_k int32; tokens
+        (int32, made where not given, and returned; -1: a degenerate row), logprobs (float32) and kept (int32)
+        receive the results."""
+        import torch
+        kind = _type_of(logits, "logits")
+        rows, vocab, stride = _matrix(logits, "logits")
+        with _on_device(logits, uniform, temperature, top_k, top_p, min_p, tokens, logprobs, kept):
+            for t, what in ((uniform, "uniform"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"),
+                            (logprobs, "logprobs")):
+                if t is not None:
+                    _buffer(t, (rows,), torch.float32, what)
+            for t, what in ((top_k, "top_k"), (tokens, "tokens"), (kept, "kept")):
+                if t is not None:
+                    _buffer(t, (rows,), torch.int32, what)
+            if tokens is None:
+                tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+            _check(lib.twd_sampler_sample(self.handle, _ptr(logits), kind, vocab, rows, stride, _ptr(temperature),
+                                          _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(tokens),
+                                          _ptr(logprobs), _ptr(kept), _stream(stream)))
+        return tokens
 
 
 def probe_read_bandwidth(buf, waves: int = 32768, launches: int = 50, stream=None):
