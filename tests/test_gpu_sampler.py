@@ -177,6 +177,18 @@ def test_extreme_parameters():
     check(dev(a[:10]), [0.7] * 10, [40] * 10, None, [-1.0] * 10, us, tag="draws")
 
 
+@pytest.mark.parametrize("vocab", [9, 6000])
+def test_min_p_above_one_and_zero_thresholds(vocab):
+    """min_p above 1 keeps the first of the largest; a threshold at 0, and limits met exactly."""
+    a = np.full((6, vocab), 2.0, np.float32)
+    a[2:, 4:] = 0.0
+    a[4, 4::2] = -0.0
+    a[5, 1:] = 2.0 - np.float32(math.log(2.0))
+    mps = [1.5, math.inf, math.exp(-2.0), math.exp(-2.0) * 0.999999, math.exp(-2.0) * 0.999999, 0.4999999]
+    check(dev(a), [1.0] * 6, None, None, mps, [0.7] * 6, tag="min_p")
+    check(dev(a), [1.0] * 6, [0, 2, 3, 4, 5, 6], [0.3] * 6, mps, [0.9] * 6, tag="min_p and more")
+
+
 def test_draws_cover_the_kept_ids():
     """One row under a thousand evenly spread draws: every id comes as often as its weight says."""
     import torch
