@@ -21,6 +21,7 @@ namespace {
 
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
 typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
@@ -205,40 +206,44 @@ __global__ __launch_bounds__(kQuantThreads) void mx_dequantize_kernel(DequantArg
 
 // ---- the head's layout in HBM ---------------------------------------------------------------------
 //
-// A tile is 16 vocabulary rows; a chunk is 128 columns, four blocks. Both matrix instructions used
-// here (16x16x128 on 4-bit operands, and four 16x16x32 on bf16 ones, whose columns may be taken in
-// any order as long as both operands agree) let lane l = 16 kg + r hold row r's block kg of a chunk:
-//   codes  [tile][chunk][lane] 16 bytes, the block's 32 elements
-//   scales [tile][quad of chunks][lane] 4 bytes, byte j the scale of that lane's block in chunk 4q + j
+// A group is 64 vocabulary rows, four tiles of 16; a chunk is 128 columns, four blocks; a quad is four
+// chunks. Both matrix instructions used here (16x16x128 on 4-bit operands, and four 16x16x32 on bf16 ones,
+// whose columns may be taken in any order as long as both operands agree) let lane l = 16 kg + r hold row
+// r's block kg of a chunk:
+//   codes  [group][chunk][tile][lane] 16 bytes, the block's 32 elements
+//   scales [group][quad][tile][lane] 4 bytes, byte c the scale of that lane's block in the quad's chunk c
 // so a load instruction of a wave moves 1 KB (codes) or 256 B (scales) of contiguous memory, and every
-// lane's elements share the lane's own scale. Rows past the vocabulary and columns past d_model are
-// zero codes; their scales are 0 (2^-127).
+// lane's elements share the lane's own scale. Row r of tile j is the group's vocabulary row
+// 16 (r / 4) + 4 j + r % 4: a product's lane then holds, over the four tiles, 16 logits in a row of one
+// hidden row. Rows past the vocabulary and columns past d_model are zero codes with scale byte 0 (2^-127).
 constexpr uint32_t kMxChunkK = 128;
-constexpr uint32_t kMxTileRows = 16;
+constexpr uint32_t kMxGroupRows = 64;
+
+__device__ __forceinline__ uint32_t group_row(uint32_t tile, uint32_t r) { return 16 * (r / 4) + 4 * tile + r % 4; }
 
 __global__ __launch_bounds__(256) void mx_repack_kernel(const uint8_t* __restrict__ codes,
                                                        const uint8_t* __restrict__ scales, uint32_t vocab,
                                                        uint32_t d, uint32_t chunks, u32x4_t* __restrict__ out_codes,
                                                        uint32_t* __restrict__ out_scales, uint32_t* bad) {
-    const uint32_t lane = threadIdx.x % 64, kg = lane / 16, r = lane % 16;
+    const uint32_t lane = threadIdx.x % 64, tile = threadIdx.x / 64, kg = lane / 16, r = lane % 16;
     const uint32_t blocks = d / kMxBlock, quads = (chunks + 3) / 4;
-    const uint64_t tile = blockIdx.x;
-    const uint64_t row = tile * kMxTileRows + r;
-    for (uint32_t q = threadIdx.x / 64; q < quads; q += 4) {
+    const uint64_t group = blockIdx.x;
+    const uint64_t row = group * kMxGroupRows + group_row(tile, r);
+    for (uint32_t q = 0; q < quads; ++q) {
         uint32_t sc = 0;
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t chunk = 4 * q + j, b = 4 * chunk + kg;
+        for (uint32_t c = 0; c < 4; ++c) {
+            const uint32_t chunk = 4 * q + c, b = 4 * chunk + kg;
             if (chunk >= chunks) break;
-            u32x4_t c = {0, 0, 0, 0};
+            u32x4_t w = {0, 0, 0, 0};
             if (row < vocab && b < blocks) {
-                c = *reinterpret_cast<const u32x4_t*>(codes + row * (d / 2) + 16ull * b);
+                w = *reinterpret_cast<const u32x4_t*>(codes + row * (d / 2) + 16ull * b);
                 const uint32_t s = scales[row * blocks + b];
                 if (s > 227u) *bad = 1;  // above 2^100, NaN among them
-                sc |= s << (8 * j);
+                sc |= s << (8 * c);
             }
-            out_codes[(tile * chunks + chunk) * 64 + lane] = c;
+            out_codes[((group * chunks + chunk) * 4 + tile) * 64 + lane] = w;
         }
-        out_scales[(tile * quads + q) * 64 + lane] = sc;
+        out_scales[((group * quads + q) * 4 + tile) * 64 + lane] = sc;
     }
 }
 
@@ -247,9 +252,10 @@ __global__ __launch_bounds__(256) void mx_repack_kernel(const uint8_t* __restric
 }  // namespace twd
 
 struct twd_mxhead {
-    uint32_t vocab, d, chunks, quads, tiles;
+    uint32_t vocab, d, chunks, quads, groups;
     float softcap;
     int device;
+    int cus;
     twd::u32x4_t* codes;
     uint32_t* scales;
     uint64_t bytes;
@@ -267,62 +273,401 @@ struct MxArgs {
     uint64_t x_stride;
     void* out;
     uint64_t out_stride;
-    uint32_t vocab, d, chunks, quads, rows;
+    uint32_t vocab, d, chunks, quads, groups, rows;
     float softcap;
 };
 
 __device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = static_cast<uint16_t>(bf16_bits(v)); }
 
-// One wave per tile of 16 vocabulary rows and 16 hidden rows.
+__device__ __forceinline__ float cap_logit(float v, float cap) { return cap > 0.0f ? cap * tanhf(v / cap) : v; }
+
+__device__ __forceinline__ i32x8_t mx_operand(u32x4_t v) {  // 4-bit operands fill half the registers
+    const i32x4_t x = __builtin_bit_cast(i32x4_t, v);
+    return __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1);
+}
+
+// One chunk's product of a 16-row weight tile and 16 quantised hidden rows; C: which byte of the weights'
+// scale word. The hidden rows' scale is the low byte of xs.
+template <int C>
+__device__ __forceinline__ f32x4_t mfma_mx(u32x4_t w, uint32_t ws, u32x4_t x, uint32_t xs, f32x4_t acc) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(w), mx_operand(x), acc, 4, 4, C,
+                                                            static_cast<int>(ws), 0, static_cast<int>(xs));
+}
+
+// Eight elements of a code word times their scale, exact in bf16.
+__device__ __forceinline__ bf16x8_t widen(uint32_t w, float s) {
+    u32x4_t e;
+    e[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+    e[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+    e[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+    e[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+    return __builtin_bit_cast(bf16x8_t, e);
+}
+__device__ __forceinline__ float scale_float(uint32_t word, int c) { return __uint_as_float(((word >> (8 * c)) & 255u) << 23); }
+
+// A barrier that waits for the wave's LDS accesses only: loads on their way into registers stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
+constexpr int kStreamed = 2;  // non-temporal: read once
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(bytes), 0x00027000);
+}
+
+// ---- up to 16 hidden rows: the weights stream past rows held in registers ---------------------------
+//
+// Bound by the read of the head. The waves of a team split d_model by quads: a wave keeps its quad of the
+// hidden rows in registers for the whole launch and streams its quad of one group after another, kRing
+// chunks (4 KB each) ahead of the arithmetic. The teams' sums over the quads meet in LDS, two buffers in
+// turn, so that one barrier a group is enough and no load waits at it.
+constexpr uint32_t kSmallRows = 16;
+constexpr uint32_t kSmallWaves = 12;  // 168 registers each
+constexpr uint32_t kRing = 4;
+
 template <bool MX, typename Out>
-__global__ __launch_bounds__(256) void mx_logits_kernel(MxArgs a) {
+__global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a, uint32_t teams, uint32_t cols) {
+    extern __shared__ float part[];  // [2][team][quad][cols][64]
     const uint32_t lane = threadIdx.x % 64, kg = lane / 16, r = lane % 16;
-    const uint32_t tile = blockIdx.x * 4 + threadIdx.x / 64;
-    if (tile * kMxTileRows >= a.vocab) return;
-    const uint32_t m = blockIdx.y * 16 + r;
-    const bool have = m < a.rows;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t team = wave / a.quads, quad = wave % a.quads;
     const uint32_t blocks = a.d / kMxBlock;
-    f32x4_t acc = {0, 0, 0, 0};
-    uint32_t sc = 0;
-    for (uint32_t c = 0; c < a.chunks; ++c) {
-        const u32x4_t w = a.codes[(static_cast<uint64_t>(tile) * a.chunks + c) * 64 + lane];
-        if (c % 4 == 0) sc = a.scales[(static_cast<uint64_t>(tile) * a.quads + c / 4) * 64 + lane];
-        const uint32_t s = (sc >> (8 * (c % 4))) & 255u, b = 4 * c + kg;
-        if constexpr (MX) {
-            u32x4_t x = {0, 0, 0, 0};
-            uint32_t xs = 0;
-            if (have && b < blocks) {
-                x = *reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(a.x) + m * (a.d / 2ull) + 16ull * b);
-                xs = a.xs[static_cast<uint64_t>(m) * blocks + b];
-            }
-            const i32x8_t wa = {static_cast<int>(w[0]), static_cast<int>(w[1]), static_cast<int>(w[2]), static_cast<int>(w[3])};
-            const i32x8_t xb = {static_cast<int>(x[0]), static_cast<int>(x[1]), static_cast<int>(x[2]), static_cast<int>(x[3])};
-            acc = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, xb, acc, 4, 4, 0, static_cast<int>(s), 0,
-                                                                   static_cast<int>(xs));
-        } else {
-            const float sv = __uint_as_float(s << 23);
-            const uint16_t* row = static_cast<const uint16_t*>(a.x) + m * a.x_stride + 32ull * b;
+    const uint32_t here = min(4u, a.chunks - 4 * quad);  // chunks of this wave
+
+    u32x4_t x[MX ? 4 : 16] = {};
+    uint32_t xs[MX ? 4 : 1] = {};
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                u32x4_t x = {0, 0, 0, 0};
-                if (have && b < blocks) x = *reinterpret_cast<const u32x4_t*>(row + 8 * t);
-                u32x4_t e;
-                e[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[t], sv, 0));
-                e[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[t], sv, 1));
-                e[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[t], sv, 2));
-                e[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[t], sv, 3));
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, e),
-                                                              __builtin_bit_cast(bf16x8_t, x), acc, 0, 0, 0);
+    for (int c = 0; c < 4; ++c) {
+        const uint32_t b = 16 * quad + 4 * c + kg;
+        if (r < a.rows && b < blocks) {
+            if constexpr (MX) {
+                x[c] = *reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(a.x) + r * (a.d / 2ull) + 16ull * b);
+                xs[c] = a.xs[static_cast<uint64_t>(r) * blocks + b];
+            } else {
+                const uint16_t* row = static_cast<const uint16_t*>(a.x) + r * a.x_stride + 32ull * b;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) x[4 * c + t] = *reinterpret_cast<const u32x4_t*>(row + 8 * t);
             }
         }
     }
-    if (!have) return;
-    Out* out = static_cast<Out*>(a.out) + m * a.out_stride;
+
+    const uint32_t step = gridDim.x * teams;
+    // Buffer loads: the base in scalar registers, one lane offset for all. Past the quad's end (the last quad)
+    // the last chunk comes again, whose hidden columns are zero.
+    auto codes_of = [&](uint32_t g) {
+        return make_rsrc(a.codes + (static_cast<uint64_t>(g) * a.chunks + 4 * quad) * 256, here * 4096);
+    };
+    auto scales_of = [&](uint32_t g) {
+        return make_rsrc(a.scales + (static_cast<uint64_t>(g) * a.quads + quad) * 256, 1024);
+    };
+    auto load_codes = [&](const __amdgpu_buffer_rsrc_t& at, uint32_t c, u32x4_t (&to)[4]) {
+        const int chunk = static_cast<int>(min(c, here - 1) * 4096);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t v = tile * kMxTileRows + 4 * kg + i;
-        if (v < a.vocab) store_logit(out + v, a.softcap > 0.0f ? a.softcap * tanhf(acc[i] / a.softcap) : acc[i]);
+        for (int j = 0; j < 4; ++j)
+            to[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(at, lane * 16 + 1024 * j, chunk, kStreamed));
+    };
+    auto load_scales = [&](const __amdgpu_buffer_rsrc_t& at, uint32_t (&to)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[j] = __builtin_amdgcn_raw_buffer_load_b32(at, lane * 4 + 256 * j, 0, kStreamed);
+    };
+    u32x4_t w[kRing][4];
+    uint32_t ws[4];
+    const uint32_t last = a.groups - 1, g0 = min(blockIdx.x * teams + team, last);
+    {
+        const auto codes = codes_of(g0), scales = scales_of(g0);
+#pragma unroll
+        for (uint32_t c = 0; c < kRing; ++c) {
+            load_codes(codes, c, w[c]);
+            if (c == 0) load_scales(scales, ws);
+            __builtin_amdgcn_sched_barrier(0);  // the loads in the order of their use, here and in every turn
+        }
+    }
+    uint32_t buf = 0;
+    // every wave of the block takes the same number of turns
+    for (uint32_t base = blockIdx.x * teams; base < a.groups; base += step) {
+        const uint32_t g = base + team, next = min(g + step, last);
+        const auto codes = codes_of(next), scales = scales_of(next);
+        f32x4_t acc[4] = {};
+        uint32_t s[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = ws[j];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (MX) {
+                    if (c == 0) acc[j] = mfma_mx<0>(w[c][j], s[j], x[c], xs[c], acc[j]);
+                    if (c == 1) acc[j] = mfma_mx<1>(w[c][j], s[j], x[c], xs[c], acc[j]);
+                    if (c == 2) acc[j] = mfma_mx<2>(w[c][j], s[j], x[c], xs[c], acc[j]);
+                    if (c == 3) acc[j] = mfma_mx<3>(w[c][j], s[j], x[c], xs[c], acc[j]);
+                } else {
+                    const float f = scale_float(s[j], c);
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            widen(w[c][j][t], f), __builtin_bit_cast(bf16x8_t, x[4 * c + t]), acc[j], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);  // one tile's widened codes at a time
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            load_codes(codes, c, w[c]);
+            if (c == 0) load_scales(scales, ws);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        float* mine = part + (static_cast<uint64_t>(buf * teams + team) * a.quads + quad) * cols * 64;
+        if (r < cols) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4_t*>(mine + r * 64 + 16 * kg + 4 * j) = acc[j];
+        }
+        lds_barrier();
+        // the team's waves share the sums: element e is hidden row e / 64, vocabulary row e % 64
+        for (uint32_t e = quad * 64 + lane; e < a.rows * 64; e += a.quads * 64) {
+            const float* p = part + static_cast<uint64_t>(buf * teams + team) * a.quads * cols * 64 + e;
+            float y = p[0];
+            for (uint32_t q = 1; q < a.quads; ++q) y += p[q * cols * 64];
+            const uint64_t v = static_cast<uint64_t>(g) * kMxGroupRows + e % 64;
+            if (v < a.vocab) store_logit(static_cast<Out*>(a.out) + (e / 64) * a.out_stride + v, cap_logit(y, a.softcap));
+        }
+        buf ^= 1;
+    }
+}
+
+// ---- more hidden rows: tiles of 256 vocabulary rows by 16 NT hidden rows -----------------------------
+//
+// Four waves, a group of weights each, read straight from memory a chunk ahead; the hidden rows' tile goes
+// through LDS, loaded there without registers one stage ahead into the other of two buffers. A stage is a
+// chunk of bf16 rows (256 bytes a row) or a quad of quantised ones (4 x 64 bytes a row and 16 scales).
+constexpr uint32_t kTileWaves = 4;
+constexpr int kVmcnt0 = 0x0F70;  // s_waitcnt vmcnt(0), no other counter
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <typename Out>
+__device__ __forceinline__ void store_logits(Out* p, const float* y, uint32_t n) {  // n of 16
+    if (n >= 16) {
+        if constexpr (sizeof(Out) == 4) {
+            __builtin_memcpy(p, y, 64);
+        } else {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = bf16_bits(y[2 * i]) | (bf16_bits(y[2 * i + 1]) << 16);
+            __builtin_memcpy(p, w, 32);
+        }
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i)
+            if (i < n) store_logit(p + i, y[i]);
+    }
+}
+
+template <bool MX, int NT, typename Out>
+__global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void mx_tile_kernel(MxArgs a) {
+    constexpr uint32_t kRows = 16 * NT;
+    constexpr uint32_t kStage = NT * 256;  // 16-byte pieces of a stage
+    __shared__ u32x4_t buf0[kStage], buf1[kStage];
+    __shared__ uint32_t sc0[MX ? kRows * 4 : 1], sc1[MX ? kRows * 4 : 1];
+    const uint32_t lane = threadIdx.x % 64, kg = lane / 16, r = lane % 16;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    // Blocks go to the XCDs in turn. An XCD's blocks take the hidden rows' tiles of one stretch of vocabulary
+    // after another, so the weights come to its L2 once; the last stretch, which may be short, goes first.
+    const uint32_t row_tiles = (a.rows + kRows - 1) / kRows, stretches = (a.groups + kTileWaves - 1) / kTileWaves;
+    const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
+    const uint32_t stretch_up = turn / row_tiles * 8 + xcd;
+    if (stretch_up >= stretches) return;
+    const uint32_t stretch = stretches - 1 - stretch_up;
+    const uint32_t m0 = turn % row_tiles * kRows;
+    const uint32_t group = stretch * kTileWaves + wave;
+    const bool have_group = group < a.groups;
+    const uint64_t g = min(group, a.groups - 1);
+    const uint32_t blocks = a.d / kMxBlock;
+
+    // The stage's hidden rows, NT pieces of 1 KB a wave: `row` and `byte` say which 16 bytes of a row's stage
+    // a lane brings. bf16: [row][16 pieces], the pieces of a row exchanged by the row's number so that a
+    // fragment's reads of one piece in 16 rows meet 16 different banks. Quantised: [chunk][tile][lane].
+    const uint32_t row_bytes = static_cast<uint32_t>(MX ? a.d / 2 : 2 * a.x_stride);
+    const uint32_t width = MX ? a.d / 2 : 2 * a.d, stages = width / 256;  // whole stages; the rest follows
+    auto row_of = [&](uint32_t i) {
+        const uint32_t p = i * kTileWaves + wave;
+        return min(m0 + (MX ? 16 * (p % NT) + r : 4 * p + lane / 16), a.rows - 1) - m0;
+    };
+    auto byte_of = [&](uint32_t i) {
+        const uint32_t p = i * kTileWaves + wave;
+        return MX ? 64 * (p / NT) + 16 * kg : 16 * ((lane ^ (4 * p + lane / 16)) % 16);
+    };
+    const char* x0 = static_cast<const char*>(a.x) + static_cast<uint64_t>(m0) * row_bytes;
+    const uint32_t rows_here = min(a.rows - m0, kRows);
+    const auto rsrc = make_rsrc(x0, (rows_here - 1) * row_bytes + width);
+    uint32_t off[NT];
+#pragma unroll
+    for (uint32_t i = 0; i < NT; ++i) off[i] = row_of(i) * row_bytes + byte_of(i);
+    auto fetch = [&](uint32_t stage, u32x4_t* to) {
+        const int at = __builtin_amdgcn_readfirstlane(static_cast<int>(stage * 256));
+#pragma unroll
+        for (uint32_t i = 0; i < NT; ++i)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + (i * kTileWaves + wave) * 64), 16,
+                                                     static_cast<int>(off[i]), at, 0, 0);
+    };
+    // the quantised stage's scales, [row][chunk] with four blocks' bytes each: through registers, so that they
+    // too travel beside the arithmetic
+    constexpr uint32_t kScales = MX ? (kRows * 4 + kTileWaves * 64 - 1) / (kTileWaves * 64) : 0;
+    uint32_t sc_next[MX ? kScales : 1];
+    auto fetch_scales = [&](uint32_t stage) {
+#pragma unroll
+        for (uint32_t i = 0; i < kScales; ++i) {
+            const uint32_t e = i * kTileWaves * 64 + threadIdx.x;
+            const uint32_t m = min(m0 + e / 4, a.rows - 1), b = 16 * stage + 4 * (e % 4);
+            __builtin_memcpy(&sc_next[i], a.xs + static_cast<uint64_t>(m) * blocks + b, 4);
+        }
+    };
+    auto write_scales = [&](uint32_t* to) {
+#pragma unroll
+        for (uint32_t i = 0; i < kScales; ++i) {
+            const uint32_t e = i * kTileWaves * 64 + threadIdx.x;
+            if (e < kRows * 4) to[e] = sc_next[i];
+        }
+    };
+    f32x4_t acc[4][NT] = {};
+    const u32x4_t* codes = a.codes + g * a.chunks * 256;
+    const uint32_t* scales = a.scales + g * a.quads * 256;
+    // w, ws: the chunk's codes and the quad's scales; wn, wsn: the next ones, on their way
+    u32x4_t w[4], wn[4];
+    uint32_t ws[4], wsn[4];
+    auto load_codes = [&](uint32_t c) {
+        const uint32_t cn = min(c, a.chunks - 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wn[j] = codes[(cn * 4 + j) * 64 + lane];
+    };
+    auto load_scales = [&](uint32_t q) {
+        const uint32_t qn = min(q, a.quads - 1);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) wsn[j] = scales[(qn * 4 + j) * 64 + lane];
+    };
+    // x(n, t): the hidden fragment of tile n and step t
+    auto chunk_bf16 = [&](uint32_t c, auto x) {
+        float f[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(((ws[j] >> (8 * (c % 4))) & 255u) << 23);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            __builtin_amdgcn_sched_barrier(0);  // one step's operands at a time: more would not fit beside the sums
+            bf16x8_t e[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) e[j] = widen(w[j][t], f[j]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const bf16x8_t y = __builtin_bit_cast(bf16x8_t, x(n, t));
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e[j], y, acc[j][n], 0, 0, 0);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = wn[j], ws[j] = c % 4 == 3 ? wsn[j] : ws[j];
+    };
+    // x(n, c), xs(n, c): the hidden fragment of tile n and chunk c of the quad, and its scale in the low byte
+    auto quad_mx = [&](uint32_t q, uint32_t chunks, auto x, auto xs) {
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) {
+            if (c < chunks) {
+                if (c > 0) load_codes(4 * q + c + 1);
+                __builtin_amdgcn_sched_barrier(0);  // the loads first, then their chunk of arithmetic
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const u32x4_t y = x(n, c);
+                    const uint32_t ys = xs(n, c);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        if (c == 0) acc[j][n] = mfma_mx<0>(w[j], ws[j], y, ys, acc[j][n]);
+                        if (c == 1) acc[j][n] = mfma_mx<1>(w[j], ws[j], y, ys, acc[j][n]);
+                        if (c == 2) acc[j][n] = mfma_mx<2>(w[j], ws[j], y, ys, acc[j][n]);
+                        if (c == 3) acc[j][n] = mfma_mx<3>(w[j], ws[j], y, ys, acc[j][n]);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) w[j] = wn[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ws[j] = wsn[j];
+    };
+    // Loads are waited for in the order of their issue, so the weights' come before the hidden rows'.
+    auto ahead = [&](uint32_t s) {
+        load_codes(MX ? 4 * s + 1 : s + 1);
+        if (MX || s % 4 == 0) load_scales(MX ? s + 1 : s / 4 + 1);
+    };
+    auto stage = [&](uint32_t s, const u32x4_t* x, const uint32_t* xs, u32x4_t* to, uint32_t* to_xs) {
+        __syncthreads();  // stage s has arrived, and nobody reads the other buffer
+        ahead(s);
+        if (s + 1 < stages) {
+            if constexpr (MX) fetch_scales(s + 1);
+            fetch(s + 1, to);
+        }
+        if constexpr (MX)
+            quad_mx(s, 4, [&](int n, uint32_t c) { return x[(c * NT + n) * 64 + lane]; },
+                    [&](int n, uint32_t c) { return xs[(16 * n + r) * 4 + c] >> (8 * kg); });
+        else
+            chunk_bf16(s, [&](int n, int t) { return x[(16 * n + r) * 16 + ((4 * kg + t) ^ r)]; });
+        if constexpr (MX) {
+            if (s + 1 < stages) write_scales(to_xs);
+        }
+        // the next stage's loads into LDS are done before the barrier that hands it over; quantised, the next
+        // chunk's codes, the last four loads issued, may still be on their way
+        __builtin_amdgcn_s_waitcnt(MX ? kVmcnt0 + 4 : kVmcnt0);
+    };
+    load_codes(0);
+    load_scales(0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = wn[j], ws[j] = wsn[j];
+    if (stages > 0) {
+        fetch(0, buf0);
+        if constexpr (MX) fetch_scales(0), write_scales(sc0);
+        __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    }
+    for (uint32_t s = 0; s < stages; s += 2) {
+        stage(s, buf0, sc0, buf1, sc1);
+        if (s + 1 >= stages) break;
+        stage(s + 1, buf1, sc1, buf0, sc0);
+    }
+    if (stages * 256 < width) {  // the columns past the last whole stage, straight from memory
+        ahead(stages);
+        if constexpr (MX) {
+            quad_mx(stages, a.chunks - 4 * stages,
+                    [&](int n, uint32_t c) {
+                        const uint32_t m = min(m0 + 16 * n + r, a.rows - 1), b = 16 * stages + 4 * c + kg;
+                        u32x4_t y = {0, 0, 0, 0};
+                        if (b < blocks)
+                            y = *reinterpret_cast<const u32x4_t*>(static_cast<const uint8_t*>(a.x) + m * (a.d / 2ull) + 16ull * b);
+                        return y;
+                    },
+                    [&](int n, uint32_t c) {
+                        const uint32_t m = min(m0 + 16 * n + r, a.rows - 1), b = 16 * stages + 4 * c + kg;
+                        return b < blocks ? static_cast<uint32_t>(a.xs[static_cast<uint64_t>(m) * blocks + b]) : 0u;
+                    });
+        } else {
+            chunk_bf16(stages, [&](int n, int t) {
+                const uint32_t m = min(m0 + 16 * n + r, a.rows - 1), b = 4 * stages + kg;
+                u32x4_t y = {0, 0, 0, 0};
+                if (b < blocks)
+                    y = *reinterpret_cast<const u32x4_t*>(static_cast<const uint16_t*>(a.x) + m * a.x_stride + 32ull * b + 8 * t);
+                return y;
+            });
+        }
+    }
+    const uint64_t v = g * kMxGroupRows + 16 * kg;
+    if (!have_group || v >= a.vocab) return;
+    const uint32_t n_v = static_cast<uint32_t>(min(a.vocab - v, static_cast<uint64_t>(16)));
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        const uint32_t m = m0 + 16 * n + r;
+        if (m >= a.rows) continue;
+        float y[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[4 * j + i] = cap_logit(acc[j][n][i], a.softcap);
+        store_logits(static_cast<Out*>(a.out) + m * a.out_stride + v, y, n_v);
     }
 }
 
@@ -357,16 +702,45 @@ int check_device(const twd_mxhead* h) {
     return TWD_OK;
 }
 
-template <bool MX>
-int launch_logits(const MxArgs& a, int out_type, hipStream_t s) {
-    const uint32_t tiles = (a.vocab + kMxTileRows - 1) / kMxTileRows;
-    const dim3 grid((tiles + 3) / 4, (a.rows + 15) / 16);
-    if (out_type == TWD_F32)
-        mx_logits_kernel<MX, float><<<grid, 256, 0, s>>>(a);
-    else
-        mx_logits_kernel<MX, uint16_t><<<grid, 256, 0, s>>>(a);
+// The small kernels' sums take more LDS than a launch may ask for by default.
+int enable_small() {
+    constexpr int kMost = 2 * kSmallWaves * kSmallRows * 64 * sizeof(float);
+    for (const void* k : {reinterpret_cast<const void*>(mx_small_kernel<false, float>),
+                          reinterpret_cast<const void*>(mx_small_kernel<false, uint16_t>),
+                          reinterpret_cast<const void*>(mx_small_kernel<true, float>),
+                          reinterpret_cast<const void*>(mx_small_kernel<true, uint16_t>)})
+        TWD_HIP(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    return TWD_OK;
+}
+
+template <bool MX, int NT, typename Out>
+int launch_tile(const MxArgs& a, hipStream_t s) {
+    const uint32_t row_tiles = (a.rows + 16 * NT - 1) / (16 * NT), stretches = (a.groups + kTileWaves - 1) / kTileWaves;
+    const uint64_t blocks = static_cast<uint64_t>((stretches + 7) / 8) * 8 * row_tiles;
+    if (blocks > 0x7FFFFFFFull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
+    mx_tile_kernel<MX, NT, Out><<<static_cast<uint32_t>(blocks), kTileWaves * 64, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
     return TWD_OK;
+}
+
+template <bool MX, typename Out>
+int launch_typed(const twd_mxhead* h, const MxArgs& a, hipStream_t s) {
+    if (a.rows <= kSmallRows && a.quads <= kSmallWaves) {
+        const uint32_t teams = kSmallWaves / a.quads;
+        const uint32_t blocks = min((a.groups + teams - 1) / teams, static_cast<uint32_t>(h->cus));
+        const uint32_t lds = 2 * teams * a.quads * a.rows * 64 * sizeof(float);
+        mx_small_kernel<MX, Out><<<blocks, teams * a.quads * 64, lds, s>>>(a, teams, a.rows);
+        TWD_HIP(hipGetLastError());
+        return TWD_OK;
+    }
+    if (a.rows <= 32) return launch_tile<MX, 2, Out>(a, s);
+    if (a.rows <= 64) return launch_tile<MX, 4, Out>(a, s);
+    return launch_tile<MX, 8, Out>(a, s);
+}
+
+template <bool MX>
+int launch_logits(const twd_mxhead* h, const MxArgs& a, int out_type, hipStream_t s) {
+    return out_type == TWD_F32 ? launch_typed<MX, float>(h, a, s) : launch_typed<MX, uint16_t>(h, a, s);
 }
 
 constexpr uint32_t kMxMaxRows = 65536;
@@ -445,11 +819,13 @@ TWD_API int twd_mxhead_create(const uint8_t* codes, const uint8_t* scales, uint3
     if (!(softcap >= 0.0f) || softcap > 3.0e38f) return fail(TWD_E_INVALID, "softcap must be finite and >= 0 (0: none)");
     if (!aligned(codes, 16)) return fail(TWD_E_INVALID, "codes must start at a multiple of 16 bytes");
     const uint32_t chunks = (d_model + kMxChunkK - 1) / kMxChunkK, quads = (chunks + 3) / 4;
-    const uint32_t tiles = (vocab + kMxTileRows - 1) / kMxTileRows;
-    const uint64_t code_bytes = static_cast<uint64_t>(tiles) * chunks * 1024, scale_bytes = static_cast<uint64_t>(tiles) * quads * 256;
+    const uint32_t groups = (vocab + kMxGroupRows - 1) / kMxGroupRows;
+    const uint64_t code_bytes = static_cast<uint64_t>(groups) * chunks * 4096, scale_bytes = static_cast<uint64_t>(groups) * quads * 1024;
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    int dev = 0;
+    int dev = 0, cus = 0;
     TWD_HIP(hipGetDevice(&dev));
+    if (const int rc = enable_small()) return rc;
+    TWD_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
     void* mem = nullptr;
     TWD_HIP(hipMalloc(&mem, code_bytes + scale_bytes + 16));
     uint8_t* base = static_cast<uint8_t*>(mem);
@@ -457,9 +833,9 @@ TWD_API int twd_mxhead_create(const uint8_t* codes, const uint8_t* scales, uint3
     u32x4_t* oc = static_cast<u32x4_t*>(mem);
     uint32_t* os = reinterpret_cast<uint32_t*>(base + code_bytes);
     uint32_t bad = 0;
-    hipError_t e = hipMemcpyAsync(bad_dev, &bad, sizeof(bad), hipMemcpyHostToDevice, s);
+    hipError_t e = hipMemsetAsync(bad_dev, 0, sizeof(bad), s);
     if (e == hipSuccess) {
-        mx_repack_kernel<<<tiles, 256, 0, s>>>(codes, scales, vocab, d_model, chunks, oc, os, bad_dev);
+        mx_repack_kernel<<<groups, 256, 0, s>>>(codes, scales, vocab, d_model, chunks, oc, os, bad_dev);
         e = hipGetLastError();
     }
     if (e == hipSuccess) e = hipMemcpyAsync(&bad, bad_dev, sizeof(bad), hipMemcpyDeviceToHost, s);
@@ -469,8 +845,8 @@ TWD_API int twd_mxhead_create(const uint8_t* codes, const uint8_t* scales, uint3
         if (e != hipSuccess) return hip_fail(e, "repacking the head");
         return fail(TWD_E_UNSUPPORTED, "a block scale exceeds 2^100 or is NaN");
     }
-    twd_mxhead* h = new (std::nothrow) twd_mxhead{vocab, d_model, chunks, quads, tiles, softcap, dev, oc, os,
-                                                  code_bytes + scale_bytes};
+    twd_mxhead* h = new (std::nothrow) twd_mxhead{vocab, d_model, chunks, quads, groups, softcap, dev, cus, oc,
+                                                  os, code_bytes + scale_bytes};
     if (!h) {
         (void)hipFree(mem);
         return fail(TWD_E_INVALID, "out of host memory");
@@ -506,8 +882,8 @@ TWD_API int twd_mxhead_logits(const twd_mxhead* head, const uint16_t* hidden_bf1
         return fail(TWD_E_INVALID, "the hidden rows' stride must be a multiple of 8 and at least d_model");
     if ((rc = check_device(head))) return rc;
     const MxArgs a{head->codes, head->scales, hidden_bf16, nullptr, hidden_stride, logits, logits_stride,
-                   head->vocab, head->d, head->chunks, head->quads, rows, head->softcap};
-    return launch_logits<false>(a, logits_type, static_cast<hipStream_t>(stream));
+                   head->vocab, head->d, head->chunks, head->quads, head->groups, rows, head->softcap};
+    return launch_logits<false>(head, a, logits_type, static_cast<hipStream_t>(stream));
 }
 
 TWD_API int twd_mxhead_logits_mx(const twd_mxhead* head, const uint8_t* codes, const uint8_t* scales, uint32_t rows,
@@ -518,8 +894,8 @@ TWD_API int twd_mxhead_logits_mx(const twd_mxhead* head, const uint8_t* codes, c
     if (!scales) return fail(TWD_E_INVALID, "null argument");
     if ((rc = check_device(head))) return rc;
     const MxArgs a{head->codes, head->scales, codes, scales, head->d, logits, logits_stride,
-                   head->vocab, head->d, head->chunks, head->quads, rows, head->softcap};
-    return launch_logits<true>(a, logits_type, static_cast<hipStream_t>(stream));
+                   head->vocab, head->d, head->chunks, head->quads, head->groups, rows, head->softcap};
+    return launch_logits<true>(head, a, logits_type, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"
