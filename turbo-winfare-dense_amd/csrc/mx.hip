@@ -657,7 +657,7 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
     }
     const uint64_t v = g * kMxGroupRows + 16 * kg;
     if (!have_group || v >= a.vocab) return;
-    const uint32_t n_v = static_cast<uint32_t>(min(a.vocab - v, static_cast<uint64_t>(16)));
+    const uint32_t n_v = v + 16 <= a.vocab ? 16u : a.vocab - static_cast<uint32_t>(v);
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         const uint32_t m = m0 + 16 * n + r;

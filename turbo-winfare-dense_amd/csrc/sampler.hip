@@ -56,52 +56,42 @@ __device__ __forceinline__ Scale scale_of(float t) {
     return s;
 }
 
-// 2^((j + 0.5) / 8 + 37), j = 0..7
-__device__ __forceinline__ double eighth(uint32_t j) {
-    constexpr double k[8] = {0x1.0b5586cf9890fp+37, 0x1.2387a6e756238p+37, 0x1.3dea64c123422p+37, 0x1.5ab07dd485429p+37,
-                             0x1.7a11473eb0187p+37, 0x1.9c49182a3f090p+37, 0x1.c199bdd85529cp+37, 0x1.ea4afa2a490dap+37};
-    return k[j];
-}
-
 // The weight's octave floor(z) and its eighth of it, both rising with l, and the weight's 38 bits.
 struct Weight {
     double oct;
     uint32_t sub;
     uint64_t q;
 };
+// FAR: |z| may reach 2^45, where neighbouring floats lie more octaves apart than any sum holds and z has no
+// fraction left: the weight is its octave's middle then. A caller that knows better leaves the test out.
+template <bool FAR = true>
 __device__ __forceinline__ Weight weight_of(float l, const Scale& c) {
 #pragma clang fp contract(off)
-    // (contracted, zh - oct would be formed from the unrounded product, whose excess `rest` adds again)
     const double ld = l;
     const double zh = ld * c.hi;
-    const double oct = __builtin_floor(zh);
-    const double fr = zh - oct;
-    uint32_t sub = static_cast<uint32_t>(fr * 8.0);
-    sub = sub < 7u ? sub : 7u;
-    // past 2^45 neighbouring floats lie more octaves apart than any sum holds, and z has no fraction left
-    const bool far = !(__builtin_fabs(zh) < 0x1p45);
-    const double rest = far ? 0.0 : fma(ld, c.hi, -zh) + ld * c.lo;
-    // 2^((sub + 0.5) / 8) e^t with |t| <= ln2 / 16, by its degree-6 Taylor polynomial (6e-14 relative)
-    const double t = (fr - (static_cast<double>(sub) * 0.125 + 0.0625) + rest) * 0.6931471805599453;
-    double p = fma(t, 1.0 / 720.0, 1.0 / 120.0);
-    p = fma(t, p, 1.0 / 24.0);
-    p = fma(t, p, 1.0 / 6.0);
-    p = fma(t, p, 0.5);
-    p = fma(t, p, 1.0);
-    p = fma(t, p, 1.0);
     Weight w;
-    w.oct = oct;
-    w.sub = sub;
+    w.oct = __builtin_floor(zh);
+    const double mid = w.oct + 0.5;
+    double t = fma(ld, c.hi, -mid);  // z less the octave's middle, rounded once, so rising with l
+    if (FAR) t = __builtin_fabs(zh) < 0x1p45 ? t : 0.0;
+    const uint32_t sub = static_cast<uint32_t>(fma(t, 8.0, 4.0));
+    w.sub = sub < 7u ? sub : 7u;
+    if (FAR) t = __builtin_fabs(zh) < 0x1p45 ? fma(ld, c.lo, t) : t;
+    else t = fma(ld, c.lo, t);
+    // 2^(37.5 + t), |t| <= 0.5: the degree-9 polynomial through the Chebyshev nodes (2e-14 relative)
+    constexpr double k = 0x1.6a09e667f3bcdp+37;
+    double p = fma(t, 0x1.b6571de2f2351p-24 * k, 0x1.63ef969a64d3cp-20 * k);
+    p = fma(t, p, 0x1.ffcb76789860fp-17 * k);
+    p = fma(t, p, 0x1.43088e257f341p-13 * k);
+    p = fma(t, p, 0x1.5d87fe908f88ap-10 * k);
+    p = fma(t, p, 0x1.3b2ab72b175eep-7 * k);
+    p = fma(t, p, 0x1.c6b08d7044119p-5 * k);
+    p = fma(t, p, 0x1.ebfbdff8149f2p-3 * k);
+    p = fma(t, p, 0x1.62e42fefa39f7p-1 * k);
+    p = fma(t, p, 0x1.000000000003dp+0 * k);
     // + 2^52 leaves the nearest integer in the low mantissa bits
-    w.q = __builtin_bit_cast(uint64_t, eighth(sub) * p + 0x1p52) & 0xFFFFFFFFFFFFFull;
+    w.q = __builtin_bit_cast(uint64_t, p + 0x1p52) & 0xFFFFFFFFFFFFFull;
     return w;
-}
-
-// The weight in units of the row's sums, `top` being the octave of the largest.
-__device__ __forceinline__ u128 in_sum(const Weight& w, double top) {
-    const double down = top - w.oct;
-    if (!(down < 80.0)) return 0;
-    return (static_cast<u128>(w.q) << kSumShift) >> static_cast<int>(down);
 }
 
 // floor(f s) and ceil(f s) of a float f in [0, 1) and a sum: f is m 2^-k with a 24-bit m.
@@ -186,6 +176,7 @@ struct RowState {
     uint32_t count_k;   // and under bin_k
     uint32_t listed;    // entries in the deciding bins
     uint32_t appended;  // of these, on the list so far
+    uint32_t key[4];    // keys of the bins' entries: key[0] .. key[1] - 1 of lo .. hi, key[2] .. key[3] - 1 of bin_k
 };
 
 struct SamplerScratch {
@@ -249,25 +240,35 @@ __device__ __forceinline__ u128 shfl_up_u128(u128 v, int d) {
 constexpr uint32_t kRowThreads = 1024;
 constexpr uint32_t kRowWaves = kRowThreads / 64;
 
-// Running sums over the block's threads (each includes its own), and the total. All threads call.
+__device__ __forceinline__ u128 shfl_xor_u128(u128 v, int d) {
+    const uint64_t lo = shfl_xor_u64(static_cast<uint64_t>(v), d), hi = shfl_xor_u64(static_cast<uint64_t>(v >> 64), d);
+    return static_cast<u128>(hi) << 64 | lo;
+}
+
+// Running sums over the threads of the block's first WAVES waves (each includes its own), and the total, which
+// every thread gets. All threads call.
 struct ScanMem {
     u128 w[kRowWaves];
     uint32_t n[kRowWaves];
 };
+template <uint32_t WAVES>
 __device__ __forceinline__ void block_scan(uint32_t& n, u128& w, uint32_t* n_all, u128* w_all, ScanMem& mem) {
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    n = wave_incl_scan_u32(n);
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const u128 o = shfl_up_u128(w, d);
-        if (lane >= static_cast<uint32_t>(d)) w += o;
-    }
     __syncthreads();
-    if (lane == 63) mem.n[wave] = n, mem.w[wave] = w;
+    if (wave < WAVES) {
+        n = wave_incl_scan_u32(n);
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const u128 o = shfl_up_u128(w, d);
+            if (lane >= static_cast<uint32_t>(d)) w += o;
+        }
+        if (lane == 63) mem.n[wave] = n, mem.w[wave] = w;
+    }
     __syncthreads();
     uint32_t nb = 0, na = 0;
     u128 wb = 0, wa = 0;
-    for (uint32_t i = 0; i < kRowWaves; ++i) {
+#pragma unroll
+    for (uint32_t i = 0; i < WAVES; ++i) {
         if (i == wave) nb = na, wb = wa;
         na += mem.n[i], wa += mem.w[i];
     }
@@ -276,61 +277,81 @@ __device__ __forceinline__ void block_scan(uint32_t& n, u128& w, uint32_t* n_all
 }
 
 constexpr uint32_t kSliceThreads = 256;
+constexpr uint32_t kCopies = 4;  // of a slice's bins, by lane, so that a wave's equal bins meet less often
 
 template <typename T>
 __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs a) {
-    __shared__ uint64_t bins[kBins];
-    __shared__ uint64_t s_best[kSliceThreads / 64];
-    __shared__ uint32_t s_live[kSliceThreads / 64], s_bad[kSliceThreads / 64];
+    __shared__ uint64_t bins[kBins][kCopies];
+    __shared__ uint32_t s_key[kSliceThreads / 64], s_live[kSliceThreads / 64], s_bad[kSliceThreads / 64], s_idx;
     const uint32_t t = threadIdx.x, slice = blockIdx.x, lane = t % 64, wave = t / 64;
     const uint64_t r = blockIdx.y;
     const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
-    constexpr uint32_t kLoads = kSlice / kSliceThreads / kVec<T>;
-    float v[kLoads * kVec<T>];
+    constexpr uint32_t kLoads = kSlice / kSliceThreads / kVec<T>, kEach = kLoads * kVec<T>;
+    float v[kEach];
     const uint32_t i0 = slice * kSlice + t * kVec<T>;
 #pragma unroll
     for (uint32_t j = 0; j < kLoads; ++j)
         load_vec<T>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab, v + j * kVec<T>);
-    bins[t] = 0;
-    uint64_t best = 0;
-    uint32_t live = 0, bad = 0;
+    const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
 #pragma unroll
-    for (uint32_t j = 0; j < kLoads * kVec<T>; ++j) {
+    for (uint32_t i = 0; i < kCopies; ++i) bins[t][i] = 0;
+    if (t == 0) s_idx = ~0u;
+    const Scale c = scale_of(temp);
+    const float far = static_cast<float>(0x1p44 / c.hi);
+    float best = -INFINITY;
+    uint32_t live = 0, bad = 0, is_far = 0;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
         bad |= v[j] < INFINITY ? 0u : 1u;
-        if (v[j] > -INFINITY) {
-            ++live;
-            const uint64_t k = rank_key(v[j], i0 + (j / kVec<T>) * kSliceThreads * kVec<T> + j % kVec<T>);
-            best = k > best ? k : best;
-        }
+        live += v[j] > -INFINITY ? 1u : 0u;
+        is_far |= __builtin_fabsf(v[j]) < far || !(v[j] > -INFINITY) ? 0u : 1u;
+        best = v[j] > best ? v[j] : best;
     }
-    best = wave_max_u64(best);
+    uint32_t key = float_key(best);
+    key = wave_reduce(key, 0u, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
     live = wave_reduce(live, 0u, [](uint32_t x, uint32_t y) { return x + y; });
-    bad = wave_reduce(bad, 0u, [](uint32_t x, uint32_t y) { return x | y; });
-    if (lane == 0) s_best[wave] = best, s_live[wave] = live, s_bad[wave] = bad;
+    bad = wave_reduce(bad | is_far << 1, 0u, [](uint32_t x, uint32_t y) { return x | y; });
+    if (lane == 0) s_key[wave] = key, s_live[wave] = live, s_bad[wave] = bad;
     __syncthreads();
     live = 0;
 #pragma unroll
     for (uint32_t i = 0; i < kSliceThreads / 64; ++i) {
-        best = s_best[i] > best ? s_best[i] : best;
+        key = s_key[i] > key ? s_key[i] : key;
         live += s_live[i], bad |= s_bad[i];
     }
-    const uint64_t at = r * a.s.slices + slice;
-    if (t == 0) a.s.head[at] = SliceHead{best, live, bad};
-    const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
-    if (live == 0 || !(temp > 0.0f)) return;
-    const Scale c = scale_of(temp);
-    const double top = weight_of(rank_value(best), c).oct;
+    best = key_float(key);
+    uint32_t idx = ~0u;
 #pragma unroll
-    for (uint32_t j = 0; j < kLoads * kVec<T>; ++j) {
-        if (v[j] > -INFINITY && v[j] < INFINITY) {
-            const Weight w = weight_of(v[j], c);
+    for (uint32_t j = kEach; j-- > 0;)
+        if (v[j] == best) idx = i0 + (j / kVec<T>) * kSliceThreads * kVec<T> + j % kVec<T>;
+    if (idx != ~0u) atomicMin(&s_idx, idx);
+    if (live != 0 && temp > 0.0f) {
+        const double top = weight_of(best, c).oct;
+        auto add = [&](const Weight& w) {
             const uint32_t b = bin_of(w, top);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b]),
+            atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b][lane % kCopies]),
                       static_cast<unsigned long long>(1ull << kCountBit | mass_of(w, b, top)));
+        };
+        if (bad == 0) {
+#pragma unroll
+            for (uint32_t j = 0; j < kEach; ++j)
+                if (v[j] > -INFINITY) add(weight_of<false>(v[j], c));
+        } else {
+#pragma unroll
+            for (uint32_t j = 0; j < kEach; ++j)
+                if (v[j] > -INFINITY && v[j] < INFINITY) add(weight_of(v[j], c));
         }
     }
     __syncthreads();
-    a.s.bins[at * kBins + t] = bins[t];
+    const uint64_t at = r * a.s.slices + slice;
+    if (t == 0)
+        a.s.head[at] = SliceHead{live ? static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - s_idx) : 0, live, bad & 1u};
+    if (live != 0 && temp > 0.0f) {
+        uint64_t x = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kCopies; ++i) x += bins[t][i];
+        a.s.bins[at * kBins + t] = x;
+    }
 }
 static_assert(kBins == kSliceThreads, "a bin per thread");
 
@@ -342,8 +363,10 @@ __device__ __forceinline__ uint32_t row_bin(uint32_t b, uint32_t shift, uint32_t
     *down = (b >> 3) + shift - kTailOct;
     return kTail;
 }
-__device__ __forceinline__ uint32_t slice_shift(double top, double slice_top) {
-    const double d = top - slice_top;
+constexpr uint32_t kNoSlice = 255;  // the shift of a slice without live entries, whose bins are not written
+__device__ __forceinline__ uint32_t slice_shift(const SliceHead& h, double top, const Scale& c) {
+    if (h.live == 0) return kNoSlice;
+    const double d = top - __builtin_floor(static_cast<double>(rank_value(h.best)) * c.hi);
     return d < 128.0 ? static_cast<uint32_t>(d) : 128u;
 }
 
@@ -372,40 +395,81 @@ __device__ uint64_t least_kept(uint64_t best, float min_p, const Scale& c) {
     return static_cast<uint64_t>(float_key(l)) << 32;
 }
 
+// The least key whose entry lies in a bin of at most b, by a wave: bins fall with rising keys, so each round
+// cuts the range by 64. `above`: a key past every entry's, taken where no key below it qualifies.
+__device__ uint32_t least_key(int b, uint32_t above, double top, const Scale& c) {
+    uint64_t lo = 0x00800000u, hi = above;  // from -FLT_MAX's key; hi qualifies
+    const uint32_t lane = threadIdx.x % 64;
+    while (lo < hi) {
+        const uint64_t step = (hi - lo + 63) / 64;
+        const uint64_t k = lo + step * lane;
+        const bool yes = k >= hi || static_cast<int>(bin_of(weight_of(key_float(static_cast<uint32_t>(k)), c), top)) <= b;
+        const uint32_t first = static_cast<uint32_t>(__builtin_ctzll(__ballot(yes) | 1ull << 63));
+        if (!(__ballot(yes) >> 63) && first == 63) {  // none of the 64: it lies past the last
+            lo = lo + step * 63 + 1;
+            continue;
+        }
+        const uint64_t at = lo + step * first;
+        hi = at < hi ? at : hi;
+        if (first != 0) lo = lo + step * (first - 1) + 1;
+        else lo = hi;
+    }
+    return static_cast<uint32_t>(hi);
+}
+
+// What every wave of a block learns of its row from the slices' heads.
+struct RowHead {
+    uint64_t best;
+    uint32_t live, bad;
+    SliceHead own[kMaxSlices / 64];  // of slices lane and lane + 64
+};
+__device__ __forceinline__ RowHead read_heads(const SampleArgs& a, uint64_t r) {
+    const uint32_t lane = threadIdx.x % 64;
+    RowHead h{0, 0, 0, {}};
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSlices / 64; ++i) {
+        h.own[i] = SliceHead{0, 0, 0};
+        if (lane + 64 * i < a.slices) h.own[i] = a.s.head[r * a.s.slices + lane + 64 * i];
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSlices / 64; ++i) {
+        h.best = h.own[i].best > h.best ? h.own[i].best : h.best;
+        h.live += h.own[i].live, h.bad |= h.own[i].bad;
+    }
+    h.best = wave_max_u64(h.best);
+    h.live = wave_reduce(h.live, 0u, [](uint32_t x, uint32_t y) { return x + y; });
+    h.bad = wave_reduce(h.bad, 0u, [](uint32_t x, uint32_t y) { return x | y; });
+    return h;
+}
+
+// A slice's bins lie 256 apart: thread t reads bin t % 256 of slices t / 256, 4 + t / 256, ... The first 64
+// slices' come in one go, ahead of everything that decides what they mean.
+constexpr uint32_t kBatch = 64 * kBins / kRowThreads;
+
 __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a) {
     __shared__ unsigned long long mass[kBins];
-    __shared__ uint32_t count[kBins];
+    __shared__ uint32_t count[kBins], counts[kBins], found[3], s_bin_m;
     __shared__ u128 sums[kBins];
-    __shared__ uint32_t counts[kBins];
-    __shared__ unsigned long long s_best;
-    __shared__ uint32_t s_live, s_bad, found[3];
-    __shared__ uint8_t shift[kMaxSlices];
+    __shared__ uint64_t s_rank_m;
+    __shared__ RowState s_st;
     __shared__ ScanMem scan;
-    const uint32_t t = threadIdx.x;
+    const uint32_t t = threadIdx.x, lane = t % 64;
     const uint64_t r = blockIdx.x;
-    if (t == 0) s_best = 0, s_live = 0, s_bad = 0;
-    if (t < kBins) mass[t] = 0, count[t] = 0;
-    if (t < 3) found[t] = kBins;
-    __syncthreads();
-    const SliceHead* head = a.s.head + r * a.s.slices;
-    SliceHead mine{0, 0, 0};
-    if (t < a.slices) {
-        mine = head[t];
-        atomicMax(&s_best, static_cast<unsigned long long>(mine.best));
-        atomicAdd(&s_live, mine.live);
-        atomicOr(&s_bad, mine.bad);
-    }
-    __syncthreads();
+    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
+    uint64_t x[kBatch];
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i) x[i] = t + i * kRowThreads < a.slices * kBins ? bins[t + i * kRowThreads] : 0;
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f, u = a.p.uniform[r];
     const float top_p = a.p.top_p ? a.p.top_p[r] : 1.0f, min_p = a.p.min_p ? a.p.min_p[r] : 0.0f;
     const int32_t top_k = a.p.top_k ? a.p.top_k[r] : 0;
-    const uint64_t best = s_best;
-    const uint32_t live = s_live;
-    const bool none = s_bad != 0 || live == 0 || temp != temp || u != u || top_p != top_p || min_p != min_p;
+    const RowHead head = read_heads(a, r);
+    const uint64_t best = head.best;
+    const uint32_t live = head.live;
+    const bool none = head.bad != 0 || live == 0 || temp != temp || u != u || top_p != top_p || min_p != min_p;
     if (none || temp <= 0.0f) {
         if (t == 0) {
             a.s.state[r].done = 1;
-            a.s.state[r].lo = 1, a.s.state[r].hi = 0, a.s.state[r].bin_k = kBins, a.s.state[r].listed = 0;
+            a.s.state[r].listed = 0;
             a.o.tokens[r] = none ? TWD_TOKEN_DEGENERATE : rank_index(best);
             if (a.o.logprobs) a.o.logprobs[r] = none ? __uint_as_float(0x7FC00000u) : 0.0f;
             if (a.o.kept) a.o.kept[r] = none ? 0 : 1;
@@ -413,195 +477,192 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         return;
     }
     const Scale c = scale_of(temp);
-    const float m = rank_value(best);
-    const double top = weight_of(m, c).oct;
-    if (t < a.slices)
-        shift[t] = static_cast<uint8_t>(mine.live ? slice_shift(top, weight_of(rank_value(mine.best), c).oct) : 255u);
-    __syncthreads();
-    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
-    for (uint32_t i = t; i < a.slices * kBins; i += kRowThreads) {
-        const uint32_t sh = shift[i / kBins];
-        if (sh == 255u) continue;  // an empty slice writes no bins
-        const uint64_t x = bins[i];
-        if (x == 0) continue;
-        uint32_t down;
-        const uint32_t b = row_bin(i % kBins, sh, &down);
-        atomicAdd(&mass[b], static_cast<unsigned long long>(down < 64 ? (x & kMassMask) >> down : 0));
-        atomicAdd(&count[b], static_cast<uint32_t>(x >> kCountBit));
+    const double top = weight_of(rank_value(best), c).oct;
+    if (t < kBins) mass[t] = 0, count[t] = 0;
+    if (t < 3) found[t] = kBins;
+    if (t == kRowThreads - 64) {  // the last wave, while the others add
+        s_rank_m = 0, s_bin_m = kBins;
+        if (min_p > 0.0f) {
+            const uint64_t rank = least_kept(best, min_p, c);
+            const float l = rank_value(rank);
+            s_rank_m = rank;
+            s_bin_m = l > -INFINITY ? bin_of(weight_of(l, c), top) : kBins;
+        }
     }
+    uint32_t shift[kMaxSlices / 64];
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSlices / 64; ++i) shift[i] = slice_shift(head.own[i], top, c);
+    __syncthreads();
+    auto add = [&](uint64_t v, uint32_t slice) {
+        const uint32_t sh = __builtin_amdgcn_readlane(slice < 64 ? shift[0] : shift[1], slice % 64);
+        if (sh == kNoSlice || v == 0) return;
+        uint32_t down;
+        const uint32_t b = row_bin(t % kBins, sh, &down);
+        atomicAdd(&mass[b], static_cast<unsigned long long>(down < 64 ? (v & kMassMask) >> down : 0));
+        atomicAdd(&count[b], static_cast<uint32_t>(v >> kCountBit));
+    };
+    const uint32_t slice0 = __builtin_amdgcn_readfirstlane(t / kBins);
+#pragma unroll
+    for (uint32_t i = 0; i < kBatch; ++i)
+        if (slice0 + i * (kRowThreads / kBins) < a.slices) add(x[i], slice0 + i * (kRowThreads / kBins));
+    for (uint32_t s0 = 64 + slice0; s0 < a.slices; s0 += kRowThreads / kBins) add(bins[s0 * kBins + t % kBins], s0);
     __syncthreads();
     uint32_t n = t < kBins ? count[t] : 0, n_all;
     u128 w = t < kBins ? unit(mass[t], t) : 0, w_all;
-    block_scan(n, w, &n_all, &w_all, scan);
-    if (t < kBins) counts[t] = n, sums[t] = w;
-    if (t < kBins) a.s.counts[r * kBins + t] = n, a.s.sums[r * kBins + t] = w;
+    block_scan<kBins / 64>(n, w, &n_all, &w_all, scan);
+    if (t < kBins) {
+        counts[t] = n, sums[t] = w;
+        a.s.counts[r * kBins + t] = n, a.s.sums[r * kBins + t] = w;
+    }
     __syncthreads();
     // the bin each limit cuts in: the first whose running number or sum reaches it
     const uint32_t k = top_k > 0 && static_cast<uint32_t>(top_k) < live ? static_cast<uint32_t>(top_k) : 0;
-    if (t < kBins && k != 0 && counts[t] >= k && (t == 0 || counts[t - 1] < k)) found[0] = t;
+    if (t < kBins && k != 0 && n >= k && (t == 0 || counts[t - 1] < k)) found[0] = t;
     __syncthreads();
     const uint32_t bin_k = found[0];
     const bool use_p = top_p < 1.0f;
     if (use_p && t < kBins) {
         // the top-k's sum lies between those of the bins under and with its cut
         const u128 low = part_of(top_p, k ? (bin_k ? sums[bin_k - 1] : 0) : w_all, true);
-        const u128 high = part_of(top_p, k ? sums[bin_k] : w_all, true);
-        auto reaches = [&](uint32_t b, u128 x) { return counts[b] >= 1 && sums[b] >= x; };
+        const u128 high = k ? part_of(top_p, sums[bin_k], true) : low;
+        auto reaches = [&](uint32_t b, u128 v) { return counts[b] >= 1 && sums[b] >= v; };
         if (reaches(t, low) && (t == 0 || !reaches(t - 1, low))) found[1] = t;
         if (reaches(t, high) && (t == 0 || !reaches(t - 1, high))) found[2] = t;
     }
     __syncthreads();
-    if (t != 0) return;
-    RowState st{};
     uint32_t lo = kBins, hi = kBins;
     if (use_p)
         lo = found[1], hi = found[2];
     else if (k)
         lo = hi = bin_k;
     bool need_k = use_p && k;
-    if (min_p > 0.0f) {
-        st.rank_m = least_kept(best, min_p, c);
-        const float l = rank_value(st.rank_m);
-        const uint32_t b = l > -INFINITY ? bin_of(weight_of(l, c), top) : kBins;
-        if (b < lo) lo = hi = b, need_k = false;  // the other limits cut deeper
-        if (b < hi) hi = b;
+    const uint32_t bin_m = s_bin_m;
+    if (bin_m < lo) lo = hi = bin_m, need_k = false;  // the other limits cut deeper
+    if (bin_m < hi) hi = bin_m;
+    const bool any = lo < kBins;
+    if (t == 0) {
+        RowState& st = s_st;
+        st.top = top, st.best = best, st.rank_m = s_rank_m, st.all = w_all, st.live = live, st.k = k, st.use_p = use_p;
+        st.bin_k = need_k ? bin_k : kBins, st.done = 0, st.appended = 0;
+        st.lo = any ? lo : 1, st.hi = any ? hi : 0;
+        st.below_l = any && lo ? sums[lo - 1] : 0, st.count_l = any && lo ? counts[lo - 1] : 0;
+        st.listed = any ? counts[hi] - st.count_l : 0;
+        st.below_k = need_k && bin_k ? sums[bin_k - 1] : 0, st.count_k = need_k && bin_k ? counts[bin_k - 1] : 0;
+        if (need_k && bin_k > hi) st.listed += counts[bin_k] - st.count_k;
     }
-    st.top = top, st.best = best, st.all = w_all, st.live = live, st.k = k, st.use_p = use_p;
-    st.bin_k = need_k ? bin_k : kBins;
-    if (lo < kBins) {
-        st.lo = lo, st.hi = hi;
-        st.below_l = lo ? sums[lo - 1] : 0, st.count_l = lo ? counts[lo - 1] : 0;
-        st.listed = counts[hi] - st.count_l;
-    } else {
-        st.lo = 1, st.hi = 0;
+    // the keys that bound those bins, a wave each
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(t / 64), above = static_cast<uint32_t>(best >> 32) + 1;
+    if (wave < 4) {
+        uint32_t key = 0;
+        if (wave < 2 ? any : need_k) {
+            const uint32_t b0 = wave < 2 ? lo : bin_k, b1 = wave < 2 ? hi : bin_k;
+            key = wave % 2 == 0 ? least_key(static_cast<int>(b1), above, top, c)
+                                : (b0 == 0 ? above : least_key(static_cast<int>(b0) - 1, above, top, c));
+        }
+        if (lane == 0) s_st.key[wave] = key;
     }
-    if (need_k) {
-        st.below_k = bin_k ? sums[bin_k - 1] : 0, st.count_k = bin_k ? counts[bin_k - 1] : 0;
-        if (bin_k > hi) st.listed += counts[bin_k] - st.count_k;
-    }
-    a.s.state[r] = st;
+    __syncthreads();
+    if (t < sizeof(RowState) / 4) reinterpret_cast<uint32_t*>(a.s.state + r)[t] = reinterpret_cast<const uint32_t*>(&s_st)[t];
 }
+static_assert(sizeof(RowState) % 4 == 0 && sizeof(RowState) / 4 <= kRowThreads, "copied by words");
 
 template <typename T>
 __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArgs a) {
-    __shared__ uint32_t s_n, s_base, s_any;
+    __shared__ uint32_t s_n, s_base;
     __shared__ uint64_t s_rank[kSlice];
     const uint32_t t = threadIdx.x, slice = blockIdx.x;
     const uint64_t r = blockIdx.y;
     RowState* st = a.s.state + r;
-    const uint32_t lo = st->lo, hi = st->hi, bin_k = st->bin_k;
-    if (st->listed == 0 || st->listed > kListCap) return;
+    const uint32_t listed = st->listed, k0 = st->key[0], k1 = st->key[1], k2 = st->key[2], k3 = st->key[3];
     const SliceHead h = a.s.head[r * a.s.slices + slice];
-    if (h.live == 0) return;
-    const Scale c = scale_of(a.p.temperature ? a.p.temperature[r] : 1.0f);
-    const double top = st->top;
-    const uint32_t sh = slice_shift(top, weight_of(rank_value(h.best), c).oct);
-    if (t == 0) s_n = 0, s_any = 0;
+    if (listed == 0 || listed > kListCap || h.live == 0) return;
+    const uint32_t most = static_cast<uint32_t>(h.best >> 32);
+    if (most < k0 && (k2 == k3 || most < k2)) return;  // all of the slice lies below
+    if (t == 0) s_n = 0;
     __syncthreads();
-    uint32_t down;
-    const uint32_t b = row_bin(t, sh, &down);
-    if (((b >= lo && b <= hi) || b == bin_k) && a.s.bins[(r * a.s.slices + slice) * kBins + t] != 0) s_any = 1;
-    __syncthreads();
-    if (!s_any) return;
     const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
     constexpr uint32_t kLoads = kSlice / kSliceThreads / kVec<T>;
     const uint32_t i0 = slice * kSlice + t * kVec<T>;
+    float v[kLoads * kVec<T>];
 #pragma unroll
-    for (uint32_t j = 0; j < kLoads; ++j) {
-        float v[kVec<T>];
-        const uint32_t i = i0 + j * kSliceThreads * kVec<T>;
-        load_vec<T>(row, i, a.vocab, v);
+    for (uint32_t j = 0; j < kLoads; ++j) load_vec<T>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab, v + j * kVec<T>);
 #pragma unroll
-        for (uint32_t e = 0; e < kVec<T>; ++e) {
-            if (v[e] > -INFINITY) {
-                const uint32_t x = bin_of(weight_of(v[e], c), top);
-                if ((x >= lo && x <= hi) || x == bin_k) s_rank[atomicAdd(&s_n, 1u)] = rank_key(v[e], i + e);
-            }
-        }
+    for (uint32_t j = 0; j < kLoads * kVec<T>; ++j) {
+        const uint32_t k = float_key(v[j]);
+        // (-inf's key lies under every bin's)
+        if (k - k0 < k1 - k0 || k - k2 < k3 - k2)
+            s_rank[atomicAdd(&s_n, 1u)] =
+                static_cast<uint64_t>(k) << 32 | (0xFFFFFFFFu - (i0 + (j / kVec<T>) * kSliceThreads * kVec<T> + j % kVec<T>));
     }
     __syncthreads();
-    if (t == 0) s_base = atomicAdd(&st->appended, s_n);
+    if (t == 0 && s_n != 0) s_base = atomicAdd(&st->appended, s_n);
     __syncthreads();
     // the bins' own numbers say how many come: the list holds them all
     for (uint32_t i = t; i < s_n; i += kSliceThreads)
         if (s_base + i < kListCap) a.s.list[r * kListCap + s_base + i] = s_rank[i];
 }
 
-// Ranks in falling order, n <= kListCap, through LDS. A few are placed by counting the larger ones.
-__device__ void sort_ranks(uint64_t* x, uint32_t n) {
-    const uint32_t t = threadIdx.x;
-    if (n <= 256) {
-        uint64_t mine = 0;
-        uint32_t pos = 0;
-        const uint32_t e = t / 4, part = t % 4;
-        if (e < n) {
-            mine = x[e];
-            for (uint32_t i = part; i < n; i += 4) pos += x[i] > mine ? 1u : 0u;
-        }
-        pos += __shfl_xor(pos, 1);
-        pos += __shfl_xor(pos, 2);
-        __syncthreads();
-        if (e < n && part == 0) x[pos] = mine;
-        __syncthreads();
-        return;
-    }
-    uint32_t size = 512;
-    while (size < n) size *= 2;
-    for (uint32_t i = n + t; i < size; i += kRowThreads) x[i] = 0;
-    for (uint32_t len = 2; len <= size; len *= 2) {
-        for (uint32_t step = len / 2; step > 0; step /= 2) {
-            __syncthreads();
-            for (uint32_t i = t; i < size / 2; i += kRowThreads) {
-                const uint32_t p = 2 * i - (i & (step - 1)), q = p + step;
-                const uint64_t u = x[p], v = x[q];
-                if (((p & len) == 0) == (u < v)) x[p] = v, x[q] = u;
-            }
-        }
-    }
-    __syncthreads();
-}
+constexpr uint32_t kSmall = 256;    // entries that are ranked against each other directly
+constexpr uint32_t kFinThreads = 512, kFinWaves = kFinThreads / 64;  // 256 registers each: 128 did not hold the sums
+constexpr uint32_t kParts = kFinThreads;  // parts that a range of ranks is cut into
+constexpr int kHalf = 39;           // sums of parts are held in two halves, split here (a weight has up to 78 bits)
 
 struct FinishMem {
     uint64_t rank[kListCap];
+    uint32_t part_n[kParts];
+    unsigned long long part_lo[kParts], part_hi[kParts];
+    uint64_t small[kSmall];
+    u128 small_w[kSmall];
     ScanMem scan;
     u128 slice[kMaxSlices];
     unsigned long long in_slice[kMaxSlices];
-    uint32_t digit_n[kBins];
-    unsigned long long digit_w[kBins];
-    uint64_t cut, cut2;
-    u128 sum, want;
-    uint32_t n, pick, id, last;
+    unsigned long long least, most;
+    uint64_t cut;
+    u128 sum, base_w, want;
+    uint32_t n, base_n, pick, id, last;
 };
 
 template <typename T>
-__global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a) {
     __shared__ FinishMem sm;
-    const uint32_t t = threadIdx.x;
+    const uint32_t t = threadIdx.x, lane = t % 64;
     const uint64_t r = blockIdx.x;
     const RowState& st = a.s.state[r];
-    if (st.done) return;
+    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
+    // read ahead: the bins that the draw adds up, and the list
+    constexpr uint32_t kTurn = kFinThreads / 16;  // slices that the block adds up at a time
+    uint64_t ahead[2][16];
+    const uint32_t done = st.done, listed = st.listed;
+#pragma unroll
+    for (uint32_t j = 0; j < 2; ++j)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i)
+            ahead[j][i] = j * kTurn + t / 16 < a.slices ? bins[(j * kTurn + t / 16) * kBins + t % 16 + 16 * i] : 0;
+    const RowHead head = read_heads(a, r);
     const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f, u = a.p.uniform[r];
     const float top_p = a.p.top_p ? a.p.top_p[r] : 1.0f;
+    if (done) return;
     const Scale c = scale_of(temp);
     const double top = st.top;
-    const uint32_t lo = st.lo, hi = st.hi, listed = st.listed;
+    const uint32_t lo = st.lo, hi = st.hi;
     const bool on_list = listed <= kListCap;
     auto weight = [&](float l, uint32_t* bin) {
         const Weight w = weight_of(l, c);
         *bin = bin_of(w, top);
         return mass_of(w, *bin, top);
     };
-    // f(rank, bin, mass) of every entry in the row's bins b0 .. b1
+    // f(rank, bin, mass) of every entry in the row's bins b0 .. b1: from the list, or, where equal or nearly
+    // equal logits are too many for it, from the row
     auto members = [&](uint32_t b0, uint32_t b1, auto f) {
         if (on_list) {
-            for (uint32_t i = t; i < listed; i += kRowThreads) {
+            for (uint32_t i = t; i < listed; i += kFinThreads) {
                 uint32_t b;
                 const uint64_t m = weight(rank_value(sm.rank[i]), &b);
                 if (b >= b0 && b <= b1) f(sm.rank[i], b, m);
             }
         } else {
-            for (uint32_t i = t; i < a.vocab; i += kRowThreads) {
+            for (uint32_t i = t; i < a.vocab; i += kFinThreads) {
                 const float l = load_logit<T>(row, i);
                 if (!(l > -INFINITY)) continue;
                 uint32_t b;
@@ -610,130 +671,106 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
             }
         }
     };
-    // In one bin, by digits of the rank from the top: the largest rank such that the entries of at least
-    // it number `n` or weigh `w` (whichever `by_sum` says; all of them where they do not reach that).
-    // Returns it, and the weight of those entries.
-    auto select = [&](uint32_t bin, uint32_t n, u128 w, bool by_sum, u128* sum) {
-        uint64_t prefix = 0;
-        uint32_t n_done = 0;
-        u128 w_done = 0;
-        for (int sft = 56; sft >= 0; sft -= 8) {
+    // Among the entries of bins b0 .. b1, with base_n entries of sum base_w before them: the rank of the one
+    // that brings the number to n, or the sum to w (by_sum); 0 where none does. *sum: the sum with it. While
+    // they are many, the range of their ranks is cut into parts and the part that holds it kept.
+    auto select = [&](uint32_t b0, uint32_t b1, uint32_t base_n, u128 base_w, bool by_sum, uint32_t n, u128 w, u128* sum) {
+        uint64_t r0 = 0, r1 = ~0ull;
+        for (;;) {
             __syncthreads();
-            if (t < kBins) sm.digit_n[t] = 0, sm.digit_w[t] = 0;
-            if (t == 0) sm.pick = 0;
+            if (t == 0) sm.n = 0, sm.least = ~0ull, sm.most = 0, sm.cut = 0, sm.sum = 0;
             __syncthreads();
-            members(bin, bin, [&](uint64_t k, uint32_t, uint64_t m) {
-                if (sft < 56 && (k >> (sft + 8)) != (prefix >> (sft + 8))) return;
-                const uint32_t d = 255u - (static_cast<uint32_t>(k >> sft) & 255u);
-                atomicAdd(&sm.digit_n[d], 1u);
-                atomicAdd(&sm.digit_w[d], static_cast<unsigned long long>(m));
+            uint64_t least = ~0ull, most = 0;
+            members(b0, b1, [&](uint64_t k, uint32_t b, uint64_t m) {
+                if (k < r0 || k > r1) return;
+                const uint32_t at = atomicAdd(&sm.n, 1u);
+                if (at < kSmall) sm.small[at] = k, sm.small_w[at] = unit(m, b);
+                least = k < least ? k : least, most = k > most ? k : most;
             });
-            __syncthreads();
-            uint32_t x = t < kBins ? sm.digit_n[t] : 0, x_all;
-            const uint32_t own = x;
-            u128 y = t < kBins ? unit(sm.digit_w[t], bin) : 0, y_all;
-            const u128 own_w = y;
-            block_scan(x, y, &x_all, &y_all, sm.scan);
-            // the digit at which the running number or sum reaches the target, or the last one there is
-            const bool here = own != 0 && (by_sum ? w_done + y >= w && w_done + y - own_w < w
-                                                  : n_done + x >= n && n_done + x - own < n);
-            const bool end = own != 0 && x == x_all && (by_sum ? w_done + y < w : n_done + x < n);
-            const bool first = by_sum && w <= w_done && own != 0 && x == own;
-            if (here || end || first) sm.pick = t, sm.n = n_done + x - own, sm.sum = w_done + y - own_w;
-            __syncthreads();
-            prefix |= static_cast<uint64_t>(255u - sm.pick) << sft;
-            n_done = sm.n, w_done = sm.sum;
-            if (sft == 0) w_done += unit(sm.digit_w[sm.pick], bin);
-        }
-        __syncthreads();
-        *sum = w_done;
-        return prefix;
-    };
-
-    uint64_t cut = 0;  // ranks of at least this are kept
-    if (on_list && listed != 0) {
-        for (uint32_t i = t; i < listed; i += kRowThreads) sm.rank[i] = a.s.list[r * kListCap + i];
-        __syncthreads();
-        sort_ranks(sm.rank, listed);
-        // running sums along the list, four entries to a thread; lo .. hi come first, bin_k after them or
-        // among them
-        constexpr uint32_t kEach = kListCap / kRowThreads;
-        uint32_t bin[kEach], n = 0, n_all;
-        u128 w[kEach], run = 0, w_all;
-#pragma unroll
-        for (uint32_t j = 0; j < kEach; ++j) {
-            const uint32_t i = kEach * t + j;
-            bin[j] = kBins + 1, w[j] = 0;
-            if (i < listed) {
-                const uint64_t m = weight(rank_value(sm.rank[i]), &bin[j]);
-                w[j] = unit(m, bin[j]);
+            if (!on_list || listed > kSmall) {
+                most = wave_max_u64(most);
+                least = ~wave_max_u64(~least);
+                if (lane == 0) atomicMax(&sm.most, static_cast<unsigned long long>(most)), atomicMin(&sm.least, static_cast<unsigned long long>(least));
             }
-            run += w[j];
-            n += i < listed && bin[j] < st.bin_k ? 1u : 0u;
-        }
-        const u128 own = run;
-        uint32_t n_before = n;
-        block_scan(n_before, run, &n_all, &w_all, sm.scan);
-        if (t == 0) sm.cut = 0, sm.cut2 = 0, sm.sum = st.all, sm.want = 0;
-        __syncthreads();
-        u128 before = run - own;
-        if (st.use_p) {
-            if (st.bin_k < kBins) {
-                // the top-k's last entry is number k - count_k of its bin; the sum under that bin is known,
-                // and the list's own sum where the bin begins
-                const uint32_t at = n_all + (st.k - st.count_k) - 1;
-                u128 x = before;
-#pragma unroll
-                for (uint32_t j = 0; j < kEach; ++j) {
-                    const uint32_t i = kEach * t + j;
-                    if (i == n_all) sm.want = x;
-                    x += w[j];
-                    if (i == at) sm.cut = sm.rank[i], sm.sum = x;
+            __syncthreads();
+            const uint32_t have = sm.n;
+            if (have <= kSmall) {
+                // two threads to an entry add up those of larger rank
+                const uint32_t e = t / 2;
+                if (e < have) {
+                    const uint64_t mine = sm.small[e];
+                    uint32_t more = 0;
+                    u128 over = 0;
+                    for (uint32_t i = t % 2; i < have; i += 2) {
+                        const bool larger = sm.small[i] > mine;
+                        more += larger ? 1u : 0u;
+                        over += larger ? sm.small_w[i] : 0;
+                    }
+                    more += __shfl_xor(more, 1);
+                    over += shfl_xor_u128(over, 1);
+                    const u128 before = base_w + over, with = before + sm.small_w[e];
+                    if (t % 2 == 0 && (by_sum ? before < w && with >= w : base_n + more + 1 == n)) sm.cut = mine, sm.sum = with;
                 }
                 __syncthreads();
-                if (t == 0) sm.sum = st.below_k + (sm.sum - sm.want);
-                __syncthreads();
+                *sum = sm.sum;
+                return sm.cut;
             }
-            const u128 want = part_of(top_p, sm.sum, true);
-            u128 x = st.below_l + before;
-#pragma unroll
-            for (uint32_t j = 0; j < kEach; ++j) {
-                const uint32_t i = kEach * t + j;
-                const bool in = i < listed && bin[j] >= lo && bin[j] <= hi;
-                const u128 y = x + w[j];
-                // the entry that reaches the target; the first one where none is needed
-                if (in && ((y >= want && x < want) || (i == 0 && want <= x))) sm.cut2 = sm.rank[i];
-                x = y;
-            }
+            r0 = sm.least, r1 = sm.most;
+            const uint64_t range = r1 - r0;
+            const int sft = range < kParts ? 0 : 55 - __builtin_clzll(range);  // range >> sft < 512
+            for (uint32_t i = t; i < kParts; i += kFinThreads) sm.part_n[i] = 0, sm.part_lo[i] = 0, sm.part_hi[i] = 0;
+            if (t == 0) sm.pick = kParts;
             __syncthreads();
-            cut = sm.cut > sm.cut2 ? sm.cut : sm.cut2;
-        } else if (st.k != 0 && st.count_l < st.k && st.k - st.count_l <= listed) {
-            cut = sm.rank[st.k - st.count_l - 1];
-        }
-    } else if (listed != 0) {
-        // more entries than the list holds: equal or nearly equal logits. The row itself is read for each digit.
-        u128 sum = st.all;
-        const u128* sums = a.s.sums + r * kBins;
-        const uint32_t* counts = a.s.counts + r * kBins;
-        uint64_t cut_k = 0;
-        if (st.use_p && st.bin_k < kBins) {
-            cut_k = select(st.bin_k, st.k - st.count_k, 0, false, &sum);
-            sum += st.below_k;
-        } else if (!st.use_p && st.k != 0 && st.count_l < st.k && counts[hi] >= st.k) {
-            cut_k = select(lo, st.k - st.count_l, 0, false, &sum);
-        }
-        cut = cut_k;
-        if (st.use_p) {
-            const u128 want = part_of(top_p, sum, true);
-            uint32_t b = lo;
-            while (b < hi && !(counts[b] >= 1 && sums[b] >= want)) ++b;
-            const u128 under = b ? sums[b - 1] : 0;
-            // (not reached: min-p cuts before)
-            if (counts[b] >= 1 && (sums[b] >= want || b == kTail)) {
-                const uint64_t x = select(b, 0, want > under ? want - under : 0, true, &sum);
-                cut = x > cut ? x : cut;
+            members(b0, b1, [&](uint64_t k, uint32_t b, uint64_t m) {
+                if (k < r0 || k > r1) return;
+                const uint32_t d = kParts - 1 - static_cast<uint32_t>((k - r0) >> sft);  // falling
+                const u128 x = unit(m, b);
+                atomicAdd(&sm.part_n[d], 1u);
+                atomicAdd(&sm.part_lo[d], static_cast<unsigned long long>(static_cast<uint64_t>(x) & ((1ull << kHalf) - 1)));
+                atomicAdd(&sm.part_hi[d], static_cast<unsigned long long>(x >> kHalf));
+            });
+            __syncthreads();
+            const uint32_t own_n = sm.part_n[t];
+            const u128 own = (static_cast<u128>(sm.part_hi[t]) << kHalf) + sm.part_lo[t];
+            uint32_t x = own_n, x_all;
+            u128 y = own, y_all;
+            block_scan<kFinWaves>(x, y, &x_all, &y_all, sm.scan);
+            if (own_n != 0 && (by_sum ? base_w + y >= w && base_w + y - own < w : base_n + x >= n && base_n + x - own_n < n))
+                sm.pick = t, sm.base_n = base_n + x - own_n, sm.base_w = base_w + y - own;
+            __syncthreads();
+            if (sm.pick == kParts) {
+                *sum = base_w + y_all;
+                return static_cast<uint64_t>(0);
             }
+            base_n = sm.base_n, base_w = sm.base_w;
+            const uint64_t from = r0 + (static_cast<uint64_t>(kParts - 1 - sm.pick) << sft);
+            const uint64_t to = from + ((uint64_t{1} << sft) - 1);
+            r1 = to < r1 ? to : r1, r0 = from;
         }
+    };
+
+    if (on_list) {
+        for (uint32_t i = t; i < listed; i += kFinThreads) sm.rank[i] = a.s.list[r * kListCap + i];
+        __syncthreads();
+    }
+    // top-k's cut by number, then top-p's by its share of the top-k's sum
+    uint64_t cut = 0;  // ranks of at least this are kept
+    u128 sum = st.all;
+#pragma unroll 1
+    for (int by_sum = 0; by_sum < 2; ++by_sum) {
+        const bool in_k = by_sum == 0 && st.bin_k < kBins;
+        const u128 want = by_sum ? part_of(top_p, sum, true) : 0;
+        if (by_sum ? !st.use_p : (st.use_p ? !in_k : st.k == 0)) continue;
+        uint64_t x = st.best;
+        if (in_k || (lo <= hi && (by_sum == 0 || want > 0))) {
+            u128 with;
+            x = select(in_k ? st.bin_k : lo, in_k ? st.bin_k : hi, in_k ? st.count_k : st.count_l,
+                       in_k ? st.below_k : st.below_l, by_sum != 0, st.k, want, &with);
+            if (by_sum == 0) sum = with;
+        } else if (lo > hi) {
+            x = 0;
+        }
+        cut = x > cut ? x : cut;
     }
     cut = st.rank_m > cut ? st.rank_m : cut;
 
@@ -744,7 +781,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     if (!all) weight(rank_value(cut), &full);
     __syncthreads();
     if (t < kMaxSlices) sm.in_slice[t] = 0, sm.slice[t] = 0;
-    if (t == 0) sm.n = 0;
+    if (t == 0) sm.n = 0, sm.last = 0, sm.id = ~0u;
+    uint32_t shift[kMaxSlices / 64];
+#pragma unroll
+    for (uint32_t i = 0; i < kMaxSlices / 64; ++i) shift[i] = slice_shift(head.own[i], top, c);
     __syncthreads();
     if (!all) {
         members(full, full, [&](uint64_t k, uint32_t, uint64_t m) {
@@ -753,77 +793,77 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
             atomicAdd(&sm.n, 1u);
         });
     }
-    __syncthreads();
-    const SliceHead* head = a.s.head + r * a.s.slices;
-    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
-    for (uint32_t s0 = t / 64; s0 < a.slices; s0 += kRowWaves) {  // a wave per slice, four bins a lane
-        const SliceHead h = head[s0];
-        u128 w = 0;
-        if (h.live != 0) {
-            const uint32_t sh = slice_shift(top, weight_of(rank_value(h.best), c).oct);
+    // sixteen threads to a slice, sixteen of its bins each
+    auto add = [&](uint32_t slice, uint32_t sh, auto bin_at) {
+        u128 x = 0;
 #pragma unroll
-            for (uint32_t j = 0; j < kBins / 64; ++j) {
-                uint32_t down;
-                const uint32_t b = row_bin(64 * j + t % 64, sh, &down);
-                if (b < full) {
-                    const uint64_t x = bins[s0 * kBins + 64 * j + t % 64];
-                    w += unit(down < 64 ? (x & kMassMask) >> down : 0, b);
-                }
-            }
+        for (uint32_t i = 0; i < 16; ++i) {
+            uint32_t down;
+            const uint32_t b = row_bin(t % 16 + 16 * i, sh, &down);
+            const uint64_t v = bin_at(i);
+            if (b < full) x += unit(down < 64 ? (v & kMassMask) >> down : 0, b);
         }
 #pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const u128 o = shfl_up_u128(w, d);
-            if (t % 64 >= static_cast<uint32_t>(d)) w += o;
-        }
-        if (t % 64 == 63) sm.slice[s0] = w + (all ? 0 : unit(sm.in_slice[s0], full));
+        for (int d = 1; d < 16; d *= 2) x += shfl_xor_u128(x, d);
+        if (t % 16 == 0 && sh != kNoSlice) sm.slice[slice] = x;
+    };
+#pragma unroll
+    for (uint32_t j = 0; j < kMaxSlices / kTurn; ++j) {
+        const uint32_t s0 = j * kTurn + t / 16, sh = __shfl(shift[j * kTurn / 64], s0 % 64);
+        if (s0 >= a.slices) continue;
+        if (j < 2)
+            add(s0, sh, [&](uint32_t i) { return ahead[j < 2 ? j : 0][i]; });
+        else
+            add(s0, sh, [&](uint32_t i) { return bins[s0 * kBins + t % 16 + 16 * i]; });
     }
     __syncthreads();
     uint32_t n = 0, n_all;
-    u128 w = t < a.slices ? sm.slice[t] : 0, kept;
-    const u128 own = w;
-    block_scan(n, w, &n_all, &kept, sm.scan);
+    u128 own = 0, kept;
+    if (t < a.slices)
+        own = sm.slice[t] + (all ? 0 : unit(sm.in_slice[t], full));
+    u128 w = own;
+    block_scan<kMaxSlices / 64>(n, w, &n_all, &kept, sm.scan);
     const u128 want = u < 1.0f ? part_of(u, kept, false) : kept - 1;  // the first running sum past this is drawn
-    if (w > want && w - own <= want) sm.pick = t, sm.want = want - (w - own);
-    if (t == 0) sm.last = 0, sm.id = ~0u;
+    if (t < a.slices && w > want && w - own <= want) sm.pick = t, sm.want = want - (w - own);
     __syncthreads();
     const uint32_t slice = sm.pick;
     const u128 rest = sm.want;
-    constexpr uint32_t kEach = kSlice / kRowThreads;
-    u128 e[kEach], run = 0, sum;
+    constexpr uint32_t kEach = kSlice / kFinThreads;
+    u128 e[kEach], run = 0, ignored;
     const uint32_t i0 = slice * kSlice + kEach * t;
     uint32_t last = 0;
+    float v[kEach];
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) v[j] = i0 + j < a.vocab ? load_logit<T>(row, i0 + j) : -INFINITY;
 #pragma unroll
     for (uint32_t j = 0; j < kEach; ++j) {
         e[j] = 0;
-        if (i0 + j < a.vocab) {
-            const float l = load_logit<T>(row, i0 + j);
-            if (l > -INFINITY && rank_key(l, i0 + j) >= cut) {
-                uint32_t b;
-                const uint64_t m = weight(l, &b);
-                e[j] = unit(m, b);
-                if (e[j] != 0) last = i0 + j + 1;
-            }
+        if (v[j] > -INFINITY && rank_key(v[j], i0 + j) >= cut) {
+            uint32_t b;
+            const uint64_t m = weight(v[j], &b);
+            e[j] = unit(m, b);
+            if (e[j] != 0) last = i0 + j + 1;
         }
         run += e[j];
     }
     const u128 mine = run;
     if (last) atomicMax(&sm.last, last);
-    block_scan(n, run, &n_all, &sum, sm.scan);
+    block_scan<kFinWaves>(n, run, &n_all, &ignored, sm.scan);
     u128 x = run - mine;
 #pragma unroll
     for (uint32_t j = 0; j < kEach; ++j) {
-        if (x <= rest && x + e[j] > rest) sm.id = i0 + j;
+        if (x <= rest && x + e[j] > rest) sm.id = i0 + j, sm.sum = e[j];
         x += e[j];
     }
     __syncthreads();
-    if (t == 0) {
-        // (the deepest bin's sum may exceed its entries' own by their last bits: the last of them then)
-        const uint32_t id = sm.id != ~0u ? sm.id : sm.last - 1;
+    // (the deepest bin's sum may exceed its entries' own by their last bits: the last of them then)
+    const uint32_t id = sm.id != ~0u ? sm.id : sm.last - 1;
+    if (id - i0 < kEach) {
+        u128 drawn = e[0];
+#pragma unroll
+        for (uint32_t j = 1; j < kEach; ++j) drawn = id == i0 + j ? e[j] : drawn;
         a.o.tokens[r] = id;
-        uint32_t b;
-        const uint64_t m = weight(load_logit<T>(row, id), &b);
-        if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(unit(m, b)) / to_double(kept)));
+        if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(drawn) / to_double(kept)));
         if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(all ? st.live : (full ? a.s.counts[r * kBins + full - 1] : 0) + sm.n);
     }
 }
@@ -834,7 +874,7 @@ void launch(const SampleArgs& a, uint32_t rows, hipStream_t s) {
     sample_slices_kernel<T><<<grid, kSliceThreads, 0, s>>>(a);
     sample_limits_kernel<<<rows, kRowThreads, 0, s>>>(a);
     sample_collect_kernel<T><<<grid, kSliceThreads, 0, s>>>(a);
-    sample_finish_kernel<T><<<rows, kRowThreads, 0, s>>>(a);
+    sample_finish_kernel<T><<<rows, kFinThreads, 0, s>>>(a);
 }
 
 }  // namespace
