@@ -64,8 +64,19 @@ struct Weight {
 };
 // FAR: |z| may reach 2^45, where neighbouring floats lie more octaves apart than any sum holds and z has no
 // fraction left: the weight is its octave's middle then. A caller that knows better leaves the test out.
+// 2^(37.5 + t), |t| <= 0.5: the degree-9 polynomial through the Chebyshev nodes (2e-14 relative). A kernel that
+// evaluates it for every logit takes the coefficients as an argument, in scalar registers: as literals each
+// would be moved into a register pair before its use.
+constexpr double kRoot = 0x1.6a09e667f3bcdp+37;
+struct Exp2Poly {
+    double c[10];
+};
+constexpr Exp2Poly kExp2Poly{{0x1.000000000003dp+0 * kRoot, 0x1.62e42fefa39f7p-1 * kRoot, 0x1.ebfbdff8149f2p-3 * kRoot,
+                              0x1.c6b08d7044119p-5 * kRoot, 0x1.3b2ab72b175eep-7 * kRoot, 0x1.5d87fe908f88ap-10 * kRoot,
+                              0x1.43088e257f341p-13 * kRoot, 0x1.ffcb76789860fp-17 * kRoot, 0x1.63ef969a64d3cp-20 * kRoot,
+                              0x1.b6571de2f2351p-24 * kRoot}};
 template <bool FAR = true>
-__device__ __forceinline__ Weight weight_of(float l, const Scale& c) {
+__device__ __forceinline__ Weight weight_of(float l, const Scale& c, const Exp2Poly& k = kExp2Poly) {
 #pragma clang fp contract(off)
     const double ld = l;
     const double zh = ld * c.hi;
@@ -78,17 +89,9 @@ __device__ __forceinline__ Weight weight_of(float l, const Scale& c) {
     w.sub = sub < 7u ? sub : 7u;
     if (FAR) t = __builtin_fabs(zh) < 0x1p45 ? fma(ld, c.lo, t) : t;
     else t = fma(ld, c.lo, t);
-    // 2^(37.5 + t), |t| <= 0.5: the degree-9 polynomial through the Chebyshev nodes (2e-14 relative)
-    constexpr double k = 0x1.6a09e667f3bcdp+37;
-    double p = fma(t, 0x1.b6571de2f2351p-24 * k, 0x1.63ef969a64d3cp-20 * k);
-    p = fma(t, p, 0x1.ffcb76789860fp-17 * k);
-    p = fma(t, p, 0x1.43088e257f341p-13 * k);
-    p = fma(t, p, 0x1.5d87fe908f88ap-10 * k);
-    p = fma(t, p, 0x1.3b2ab72b175eep-7 * k);
-    p = fma(t, p, 0x1.c6b08d7044119p-5 * k);
-    p = fma(t, p, 0x1.ebfbdff8149f2p-3 * k);
-    p = fma(t, p, 0x1.62e42fefa39f7p-1 * k);
-    p = fma(t, p, 0x1.000000000003dp+0 * k);
+    double p = fma(t, k.c[9], k.c[8]);
+#pragma unroll
+    for (int i = 7; i >= 0; --i) p = fma(t, p, k.c[i]);
     // + 2^52 leaves the nearest integer in the low mantissa bits
     w.q = __builtin_bit_cast(uint64_t, p + 0x1p52) & 0xFFFFFFFFFFFFFull;
     return w;
@@ -174,6 +177,7 @@ struct RowState {
     uint32_t use_p;
     uint32_t count_l;   // entries in bins under lo
     uint32_t count_k;   // and under bin_k
+    uint32_t in_l, in_k;  // entries in bins lo .. hi, and in bin_k
     uint32_t listed;    // entries in the deciding bins
     uint32_t appended;  // of these, on the list so far
     uint32_t key[4];    // keys of the bins' entries: key[0] .. key[1] - 1 of lo .. hi, key[2] .. key[3] - 1 of bin_k
@@ -184,8 +188,7 @@ struct SamplerScratch {
     SliceHead* head;  // [rows][slices]
     RowState* state;  // [rows]
     uint64_t* list;   // [rows][kListCap] ranks
-    u128* sums;       // [rows][kBins] sum of the weights up to a bin
-    uint32_t* counts; // [rows][kBins]
+    u128* under;      // [rows][slices] a slice's sum of the weights in bins under lo
     uint32_t slices;  // of max_vocab
 };
 
@@ -196,6 +199,7 @@ struct SampleArgs {
     SampleParams p;
     SampleOut o;
     SamplerScratch s;
+    Exp2Poly poly;
 };
 
 // 16 bytes of logits from any address (the hardware splits an unaligned load itself).
@@ -230,14 +234,35 @@ __device__ __forceinline__ u128 unit(uint64_t mass, uint32_t bin) {
     return (static_cast<u128>(mass) << kSumShift) >> (bin >> 3);
 }
 
-__device__ __forceinline__ u128 shfl_up_u128(u128 v, int d) {
-    uint64_t lo = static_cast<uint64_t>(v), hi = static_cast<uint64_t>(v >> 64);
-    lo = static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(lo), d));
-    hi = static_cast<uint64_t>(__shfl_up(static_cast<unsigned long long>(hi), d));
-    return static_cast<u128>(hi) << 64 | lo;
+// Sums travel between lanes in two halves of 39 bits and more, each of which adds up by itself: a step is a
+// register move per half, where carrying 128 bits would take four LDS round trips.
+constexpr int kHalf = 39;
+struct Halves {
+    uint64_t lo, hi;
+};
+__device__ __forceinline__ Halves halve(u128 x) {
+    return Halves{static_cast<uint64_t>(x) & ((uint64_t{1} << kHalf) - 1), static_cast<uint64_t>(x >> kHalf)};
+}
+__device__ __forceinline__ u128 join(const Halves& h) { return (static_cast<u128>(h.hi) << kHalf) + h.lo; }
+__device__ __forceinline__ uint64_t wave_incl_scan_u64(uint64_t x) {
+    x += dpp_move<0x111>(uint64_t{0}, x);
+    x += dpp_move<0x112>(uint64_t{0}, x);
+    x += dpp_move<0x114>(uint64_t{0}, x);
+    x += dpp_move<0x118>(uint64_t{0}, x);
+    x += dpp_move<0x142, 0xA>(uint64_t{0}, x);
+    x += dpp_move<0x143, 0xC>(uint64_t{0}, x);
+    return x;
+}
+// The sum over a row of 16 lanes, in each of them.
+__device__ __forceinline__ uint64_t sum_of_16(uint64_t x) {
+    x += dpp_move<0xB1>(uint64_t{0}, x);
+    x += dpp_move<0x4E>(uint64_t{0}, x);
+    x += dpp_move<0x141>(uint64_t{0}, x);
+    x += dpp_move<0x140>(uint64_t{0}, x);
+    return x;
 }
 
-constexpr uint32_t kRowThreads = 1024;
+constexpr uint32_t kRowThreads = 512;
 constexpr uint32_t kRowWaves = kRowThreads / 64;
 
 __device__ __forceinline__ u128 shfl_xor_u128(u128 v, int d) {
@@ -257,11 +282,8 @@ __device__ __forceinline__ void block_scan(uint32_t& n, u128& w, uint32_t* n_all
     __syncthreads();
     if (wave < WAVES) {
         n = wave_incl_scan_u32(n);
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-            const u128 o = shfl_up_u128(w, d);
-            if (lane >= static_cast<uint32_t>(d)) w += o;
-        }
+        const Halves h = halve(w);
+        w = join(Halves{wave_incl_scan_u64(h.lo), wave_incl_scan_u64(h.hi)});
         if (lane == 63) mem.n[wave] = n, mem.w[wave] = w;
     }
     __syncthreads();
@@ -327,19 +349,22 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
     if (idx != ~0u) atomicMin(&s_idx, idx);
     if (live != 0 && temp > 0.0f) {
         const double top = weight_of(best, c).oct;
-        auto add = [&](const Weight& w) {
-            const uint32_t b = bin_of(w, top);
-            atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b][lane % kCopies]),
-                      static_cast<unsigned long long>(1ull << kCountBit | mass_of(w, b, top)));
+        auto add = [&](float l, const Weight& w) {
+            uint32_t b = (static_cast<uint32_t>(top - w.oct) << 3) + 7u - w.sub;
+            uint64_t m = w.q;
+            if (!(top - w.oct < static_cast<double>(kTailOct) + 0.5)) b = bin_of(w, top), m = mass_of(w, b, top);
+            if (l > -INFINITY)
+                atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b][lane % kCopies]),
+                          static_cast<unsigned long long>(1ull << kCountBit | m));
         };
         if (bad == 0) {
+            // masked entries take the largest one's place in the arithmetic, so that nothing branches there
 #pragma unroll
-            for (uint32_t j = 0; j < kEach; ++j)
-                if (v[j] > -INFINITY) add(weight_of<false>(v[j], c));
+            for (uint32_t j = 0; j < kEach; ++j) add(v[j], weight_of<false>(v[j] > -INFINITY ? v[j] : best, c, a.poly));
         } else {
 #pragma unroll
             for (uint32_t j = 0; j < kEach; ++j)
-                if (v[j] > -INFINITY && v[j] < INFINITY) add(weight_of(v[j], c));
+                if (v[j] < INFINITY) add(v[j], weight_of(v[j] > -INFINITY ? v[j] : best, c));
         }
     }
     __syncthreads();
@@ -370,29 +395,29 @@ __device__ __forceinline__ uint32_t slice_shift(const SliceHead& h, double top, 
     return d < 128.0 ? static_cast<uint32_t>(d) : 128u;
 }
 
-// The next float below and above (the key under 0's is -0's, which float_key takes for 0).
-__device__ __forceinline__ float float_below(float l) {
-    const uint32_t k = float_key(l);
-    return key_float(k == 0x80000000u ? k - 2 : k - 1);
-}
-__device__ __forceinline__ float float_above(float l) {
-    const uint32_t k = float_key(l) + 1;
-    return key_float(k == 0x7FFFFFFFu ? k + 1 : k);
-}
-
-// The least rank that min-p keeps: (l - M) log2(e) / T >= log2(min_p); the best one where none does.
+// The least rank that min-p keeps, by a wave: (l - M) log2(e) / T >= log2(min_p); the best one where none does.
 __device__ uint64_t least_kept(uint64_t best, float min_p, const Scale& c) {
     const float m = rank_value(best);
+    const uint32_t key_m = static_cast<uint32_t>(best >> 32), lane = threadIdx.x % 64;
+    constexpr uint32_t kLeast = 0x007FFFFFu;  // -inf's key
     const double lim = log2(static_cast<double>(min_p));
     auto keeps = [&](float l) { return (static_cast<double>(l) - static_cast<double>(m)) * c.hi >= lim; };
     if (!keeps(m)) return best;
-    if (c.hi == 0.0) return static_cast<uint64_t>(float_key(-INFINITY)) << 32;
-    float l = static_cast<float>(static_cast<double>(m) + lim / c.hi);
-    l = l < m ? l : m;
-    // the quotient and the sum are rounded, the float once more: a few steps at most
-    for (int i = 0; i < 8 && l > -INFINITY && keeps(float_below(l)); ++i) l = float_below(l);
-    for (int i = 0; i < 8 && l < m && !keeps(l); ++i) l = float_above(l);
-    return static_cast<uint64_t>(float_key(l)) << 32;
+    if (c.hi == 0.0) return static_cast<uint64_t>(kLeast) << 32;
+    // the quotient and the sum are rounded, the float once more: it lies a few floats around their result
+    uint32_t k = float_key(static_cast<float>(static_cast<double>(m) + lim / c.hi));
+    k = k < key_m ? k : key_m;
+    for (;;) {
+        const uint32_t from = k > kLeast + 32 ? k - 32 : kLeast;
+        const uint64_t yes = __ballot(from + lane >= key_m || keeps(key_float(from + lane)));
+        if (yes == 0) {
+            k = from + 64 + 32;
+        } else if ((yes & 1) != 0 && from > kLeast) {
+            k = from - 31;
+        } else {
+            return static_cast<uint64_t>(from + static_cast<uint32_t>(__builtin_ctzll(yes))) << 32;
+        }
+    }
 }
 
 // The least key whose entry lies in a bin of at most b, by a wave: bins fall with rising keys, so each round
@@ -442,9 +467,10 @@ __device__ __forceinline__ RowHead read_heads(const SampleArgs& a, uint64_t r) {
     return h;
 }
 
-// A slice's bins lie 256 apart: thread t reads bin t % 256 of slices t / 256, 4 + t / 256, ... The first 64
-// slices' come in one go, ahead of everything that decides what they mean.
-constexpr uint32_t kBatch = 64 * kBins / kRowThreads;
+// Sixteen threads to a slice, sixteen of its bins each; the first 64 slices' come in one go, ahead of everything
+// that decides what they mean.
+constexpr uint32_t kTurn = kRowThreads / 16;  // slices at a time
+constexpr uint32_t kAhead = 64 / kTurn;
 
 __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a) {
     __shared__ unsigned long long mass[kBins];
@@ -453,16 +479,24 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
     __shared__ uint64_t s_rank_m;
     __shared__ RowState s_st;
     __shared__ ScanMem scan;
-    const uint32_t t = threadIdx.x, lane = t % 64;
+    const uint32_t t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
     const uint64_t r = blockIdx.x;
-    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
-    uint64_t x[kBatch];
-#pragma unroll
-    for (uint32_t i = 0; i < kBatch; ++i) x[i] = t + i * kRowThreads < a.slices * kBins ? bins[t + i * kRowThreads] : 0;
+    const RowHead head = read_heads(a, r);
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f, u = a.p.uniform[r];
     const float top_p = a.p.top_p ? a.p.top_p[r] : 1.0f, min_p = a.p.min_p ? a.p.min_p[r] : 0.0f;
     const int32_t top_k = a.p.top_k ? a.p.top_k[r] : 0;
-    const RowHead head = read_heads(a, r);
+    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
+    auto load = [&](uint32_t slice, uint64_t (&x)[16]) {
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) x[i] = slice < a.slices ? bins[slice * kBins + t % 16 + 16 * i] : 0;
+    };
+    uint64_t ahead[kAhead][16];
+#pragma unroll
+    for (uint32_t j = 0; j < kAhead; ++j) load(j * kTurn + t / 16, ahead[j]);
+    if (t < kBins) mass[t] = 0, count[t] = 0;
+    if (t < 3) found[t] = kBins;
+    if (t == 0) s_rank_m = 0, s_bin_m = kBins;
+    __syncthreads();
     const uint64_t best = head.best;
     const uint32_t live = head.live;
     const bool none = head.bad != 0 || live == 0 || temp != temp || u != u || top_p != top_p || min_p != min_p;
@@ -478,58 +512,66 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
     }
     const Scale c = scale_of(temp);
     const double top = weight_of(rank_value(best), c).oct;
-    if (t < kBins) mass[t] = 0, count[t] = 0;
-    if (t < 3) found[t] = kBins;
-    if (t == kRowThreads - 64) {  // the last wave, while the others add
-        s_rank_m = 0, s_bin_m = kBins;
-        if (min_p > 0.0f) {
-            const uint64_t rank = least_kept(best, min_p, c);
-            const float l = rank_value(rank);
-            s_rank_m = rank;
-            s_bin_m = l > -INFINITY ? bin_of(weight_of(l, c), top) : kBins;
-        }
-    }
     uint32_t shift[kMaxSlices / 64];
 #pragma unroll
     for (uint32_t i = 0; i < kMaxSlices / 64; ++i) shift[i] = slice_shift(head.own[i], top, c);
-    __syncthreads();
-    auto add = [&](uint64_t v, uint32_t slice) {
-        const uint32_t sh = __builtin_amdgcn_readlane(slice < 64 ? shift[0] : shift[1], slice % 64);
-        if (sh == kNoSlice || v == 0) return;
-        uint32_t down;
-        const uint32_t b = row_bin(t % kBins, sh, &down);
-        atomicAdd(&mass[b], static_cast<unsigned long long>(down < 64 ? (v & kMassMask) >> down : 0));
-        atomicAdd(&count[b], static_cast<uint32_t>(v >> kCountBit));
-    };
-    const uint32_t slice0 = __builtin_amdgcn_readfirstlane(t / kBins);
+    // f(slice, its shift, its sixteen bins of this thread), all slices in turn
+    auto slices = [&](auto f) {
 #pragma unroll
-    for (uint32_t i = 0; i < kBatch; ++i)
-        if (slice0 + i * (kRowThreads / kBins) < a.slices) add(x[i], slice0 + i * (kRowThreads / kBins));
-    for (uint32_t s0 = 64 + slice0; s0 < a.slices; s0 += kRowThreads / kBins) add(bins[s0 * kBins + t % kBins], s0);
+        for (uint32_t j = 0; j < kMaxSlices / kTurn; ++j) {
+            if (j * kTurn >= a.slices) break;
+            const uint32_t slice = j * kTurn + t / 16, sh = __shfl(shift[j * kTurn / 64], slice % 64);
+            if (j < kAhead) {
+                f(slice, sh, ahead[j < kAhead ? j : 0]);
+            } else {
+                uint64_t x[16];
+                load(slice, x);
+                f(slice, sh, x);
+            }
+        }
+    };
+    slices([&](uint32_t, uint32_t sh, const uint64_t (&x)[16]) {
+        if (sh == kNoSlice) return;  // (its bins are not written)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            if (x[i] == 0) continue;
+            uint32_t down;
+            const uint32_t b = row_bin(t % 16 + 16 * i, sh, &down);
+            atomicAdd(&mass[b], static_cast<unsigned long long>(down < 64 ? (x[i] & kMassMask) >> down : 0));
+            atomicAdd(&count[b], static_cast<uint32_t>(x[i] >> kCountBit));
+        }
+    });
+    if (wave == kRowThreads / 64 - 1 && min_p > 0.0f) {
+        const uint64_t rank = least_kept(best, min_p, c);
+        const float l = rank_value(rank);
+        const uint32_t b = l > -INFINITY ? bin_of(weight_of(l, c), top) : kBins;
+        if (lane == 0) s_rank_m = rank, s_bin_m = b;
+    }
     __syncthreads();
     uint32_t n = t < kBins ? count[t] : 0, n_all;
     u128 w = t < kBins ? unit(mass[t], t) : 0, w_all;
     block_scan<kBins / 64>(n, w, &n_all, &w_all, scan);
-    if (t < kBins) {
-        counts[t] = n, sums[t] = w;
-        a.s.counts[r * kBins + t] = n, a.s.sums[r * kBins + t] = w;
-    }
+    if (t < kBins) counts[t] = n, sums[t] = w;
     __syncthreads();
     // the bin each limit cuts in: the first whose running number or sum reaches it
     const uint32_t k = top_k > 0 && static_cast<uint32_t>(top_k) < live ? static_cast<uint32_t>(top_k) : 0;
-    if (t < kBins && k != 0 && n >= k && (t == 0 || counts[t - 1] < k)) found[0] = t;
-    __syncthreads();
-    const uint32_t bin_k = found[0];
     const bool use_p = top_p < 1.0f;
-    if (use_p && t < kBins) {
-        // the top-k's sum lies between those of the bins under and with its cut
-        const u128 low = part_of(top_p, k ? (bin_k ? sums[bin_k - 1] : 0) : w_all, true);
-        const u128 high = k ? part_of(top_p, sums[bin_k], true) : low;
-        auto reaches = [&](uint32_t b, u128 v) { return counts[b] >= 1 && sums[b] >= v; };
-        if (reaches(t, low) && (t == 0 || !reaches(t - 1, low))) found[1] = t;
-        if (reaches(t, high) && (t == 0 || !reaches(t - 1, high))) found[2] = t;
+    if (k != 0) {
+        if (t < kBins && n >= k && (t == 0 || counts[t - 1] < k)) found[0] = t;
+        __syncthreads();
     }
-    __syncthreads();
+    const uint32_t bin_k = found[0];
+    if (use_p) {
+        if (t < kBins) {
+            // the top-k's sum lies between those of the bins under and with its cut
+            const u128 low = part_of(top_p, k ? (bin_k ? sums[bin_k - 1] : 0) : w_all, true);
+            const u128 high = k ? part_of(top_p, sums[bin_k], true) : low;
+            auto reaches = [&](uint32_t b, u128 v) { return counts[b] >= 1 && sums[b] >= v; };
+            if (reaches(t, low) && (t == 0 || !reaches(t - 1, low))) found[1] = t;
+            if (reaches(t, high) && (t == 0 || !reaches(t - 1, high))) found[2] = t;
+        }
+        __syncthreads();
+    }
     uint32_t lo = kBins, hi = kBins;
     if (use_p)
         lo = found[1], hi = found[2];
@@ -540,18 +582,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
     if (bin_m < lo) lo = hi = bin_m, need_k = false;  // the other limits cut deeper
     if (bin_m < hi) hi = bin_m;
     const bool any = lo < kBins;
-    if (t == 0) {
-        RowState& st = s_st;
-        st.top = top, st.best = best, st.rank_m = s_rank_m, st.all = w_all, st.live = live, st.k = k, st.use_p = use_p;
-        st.bin_k = need_k ? bin_k : kBins, st.done = 0, st.appended = 0;
-        st.lo = any ? lo : 1, st.hi = any ? hi : 0;
-        st.below_l = any && lo ? sums[lo - 1] : 0, st.count_l = any && lo ? counts[lo - 1] : 0;
-        st.listed = any ? counts[hi] - st.count_l : 0;
-        st.below_k = need_k && bin_k ? sums[bin_k - 1] : 0, st.count_k = need_k && bin_k ? counts[bin_k - 1] : 0;
-        if (need_k && bin_k > hi) st.listed += counts[bin_k] - st.count_k;
-    }
     // the keys that bound those bins, a wave each
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(t / 64), above = static_cast<uint32_t>(best >> 32) + 1;
+    const uint32_t above = static_cast<uint32_t>(best >> 32) + 1;
     if (wave < 4) {
         uint32_t key = 0;
         if (wave < 2 ? any : need_k) {
@@ -561,15 +593,39 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         }
         if (lane == 0) s_st.key[wave] = key;
     }
+    // every slice's sum under them: what the draw starts from
+    slices([&](uint32_t slice, uint32_t sh, const uint64_t (&x)[16]) {
+        u128 sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            uint32_t down;
+            const uint32_t b = row_bin(t % 16 + 16 * i, sh, &down);
+            if (b < lo && sh != kNoSlice) sum += unit(down < 64 ? (x[i] & kMassMask) >> down : 0, b);
+        }
+        const Halves h = halve(sum);
+        sum = join(Halves{sum_of_16(h.lo), sum_of_16(h.hi)});
+        if (t % 16 == 0 && slice < a.slices) a.s.under[r * a.s.slices + slice] = sum;
+    });
+    if (t == kRowThreads - 1) {
+        RowState& st = s_st;
+        st.top = top, st.best = best, st.rank_m = s_rank_m, st.all = w_all, st.live = live, st.k = k, st.use_p = use_p;
+        st.bin_k = need_k ? bin_k : kBins, st.done = 0, st.appended = 0;
+        st.lo = any ? lo : 1, st.hi = any ? hi : 0;
+        st.below_l = any && lo ? sums[lo - 1] : 0, st.count_l = any && lo ? counts[lo - 1] : 0;
+        st.in_l = st.listed = any ? counts[hi] - st.count_l : 0;
+        st.below_k = need_k && bin_k ? sums[bin_k - 1] : 0, st.count_k = need_k && bin_k ? counts[bin_k - 1] : 0;
+        st.in_k = need_k ? counts[bin_k] - st.count_k : 0;
+        if (need_k && bin_k > hi) st.listed += st.in_k;
+    }
     __syncthreads();
     if (t < sizeof(RowState) / 4) reinterpret_cast<uint32_t*>(a.s.state + r)[t] = reinterpret_cast<const uint32_t*>(&s_st)[t];
 }
 static_assert(sizeof(RowState) % 4 == 0 && sizeof(RowState) / 4 <= kRowThreads, "copied by words");
+static_assert(kRowThreads % 64 == 0 && kBins <= kRowThreads, "a thread to a bin");
 
 template <typename T>
 __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArgs a) {
     __shared__ uint32_t s_n, s_base;
-    __shared__ uint64_t s_rank[kSlice];
     const uint32_t t = threadIdx.x, slice = blockIdx.x;
     const uint64_t r = blockIdx.y;
     RowState* st = a.s.state + r;
@@ -581,41 +637,47 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArg
     if (t == 0) s_n = 0;
     __syncthreads();
     const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
-    constexpr uint32_t kLoads = kSlice / kSliceThreads / kVec<T>;
+    constexpr uint32_t kLoads = kSlice / kSliceThreads / kVec<T>, kEach = kLoads * kVec<T>;
     const uint32_t i0 = slice * kSlice + t * kVec<T>;
-    float v[kLoads * kVec<T>];
+    float v[kEach];
 #pragma unroll
     for (uint32_t j = 0; j < kLoads; ++j) load_vec<T>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab, v + j * kVec<T>);
+    auto decides = [&](uint32_t k) { return k - k0 < k1 - k0 || k - k2 < k3 - k2; };  // (-inf's key lies under all)
+    uint32_t hits = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kLoads * kVec<T>; ++j) {
+    for (uint32_t j = 0; j < kEach; ++j) hits += decides(float_key(v[j])) ? 1u : 0u;
+    uint32_t at = hits ? atomicAdd(&s_n, hits) : 0;
+    __syncthreads();
+    if (s_n == 0) return;
+    if (t == 0) s_base = atomicAdd(&st->appended, s_n);
+    __syncthreads();
+    if (hits == 0) return;
+    at += s_base;
+#pragma unroll
+    for (uint32_t j = 0; j < kEach; ++j) {
         const uint32_t k = float_key(v[j]);
-        // (-inf's key lies under every bin's)
-        if (k - k0 < k1 - k0 || k - k2 < k3 - k2)
-            s_rank[atomicAdd(&s_n, 1u)] =
+        if (!decides(k)) continue;
+        // the bins' own numbers say how many come: the list holds them all
+        if (at < kListCap)
+            a.s.list[r * kListCap + at] =
                 static_cast<uint64_t>(k) << 32 | (0xFFFFFFFFu - (i0 + (j / kVec<T>) * kSliceThreads * kVec<T> + j % kVec<T>));
+        ++at;
     }
-    __syncthreads();
-    if (t == 0 && s_n != 0) s_base = atomicAdd(&st->appended, s_n);
-    __syncthreads();
-    // the bins' own numbers say how many come: the list holds them all
-    for (uint32_t i = t; i < s_n; i += kSliceThreads)
-        if (s_base + i < kListCap) a.s.list[r * kListCap + s_base + i] = s_rank[i];
 }
 
-constexpr uint32_t kSmall = 256;    // entries that are ranked against each other directly
-constexpr uint32_t kFinThreads = 512, kFinWaves = kFinThreads / 64;  // 256 registers each: 128 did not hold the sums
+constexpr uint32_t kFinThreads = 512, kFinWaves = kFinThreads / 64;
+constexpr uint32_t kSmall = 256;          // entries that are ranked against each other directly
 constexpr uint32_t kParts = kFinThreads;  // parts that a range of ranks is cut into
-constexpr int kHalf = 39;           // sums of parts are held in two halves, split here (a weight has up to 78 bits)
 
 struct FinishMem {
     uint64_t rank[kListCap];
+    uint64_t weight[kListCap];  // its bin above bit 48, the weight below
     uint32_t part_n[kParts];
     unsigned long long part_lo[kParts], part_hi[kParts];
     uint64_t small[kSmall];
     u128 small_w[kSmall];
     ScanMem scan;
-    u128 slice[kMaxSlices];
-    unsigned long long in_slice[kMaxSlices];
+    unsigned long long slice_lo[kMaxSlices], slice_hi[kMaxSlices];
     unsigned long long least, most;
     uint64_t cut;
     u128 sum, base_w, want;
@@ -624,24 +686,16 @@ struct FinishMem {
 
 template <typename T>
 __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a) {
-    __shared__ FinishMem sm;
+    extern __shared__ char finish_mem[];
+    FinishMem& sm = *reinterpret_cast<FinishMem*>(finish_mem);
     const uint32_t t = threadIdx.x, lane = t % 64;
     const uint64_t r = blockIdx.x;
     const RowState& st = a.s.state[r];
-    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
-    // read ahead: the bins that the draw adds up, and the list
-    constexpr uint32_t kTurn = kFinThreads / 16;  // slices that the block adds up at a time
-    uint64_t ahead[2][16];
     const uint32_t done = st.done, listed = st.listed;
-#pragma unroll
-    for (uint32_t j = 0; j < 2; ++j)
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i)
-            ahead[j][i] = j * kTurn + t / 16 < a.slices ? bins[(j * kTurn + t / 16) * kBins + t % 16 + 16 * i] : 0;
-    const RowHead head = read_heads(a, r);
-    const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f, u = a.p.uniform[r];
     const float top_p = a.p.top_p ? a.p.top_p[r] : 1.0f;
+    const u128 under = t < a.slices ? a.s.under[r * a.s.slices + t] : 0;
+    const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
     if (done) return;
     const Scale c = scale_of(temp);
     const double top = st.top;
@@ -652,14 +706,24 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
         *bin = bin_of(w, top);
         return mass_of(w, *bin, top);
     };
-    // f(rank, bin, mass) of every entry in the row's bins b0 .. b1: from the list, or, where equal or nearly
-    // equal logits are too many for it, from the row
+    if (t < kMaxSlices) sm.slice_lo[t] = 0, sm.slice_hi[t] = 0;
+    if (t == 0) sm.last = 0, sm.id = ~0u;
+    if (on_list) {
+        for (uint32_t i = t; i < listed; i += kFinThreads) {
+            const uint64_t k = a.s.list[r * kListCap + i];
+            uint32_t b;
+            const uint64_t m = weight(rank_value(k), &b);
+            sm.rank[i] = k, sm.weight[i] = static_cast<uint64_t>(b) << 48 | m;
+        }
+    }
+    // f(rank, bin, weight) of every entry in the row's bins b0 .. b1: from the list, or, where equal or nearly
+    // equal logits are too many for it, from the row. (A thread meets the same entries of the list each time.)
     auto members = [&](uint32_t b0, uint32_t b1, auto f) {
         if (on_list) {
             for (uint32_t i = t; i < listed; i += kFinThreads) {
-                uint32_t b;
-                const uint64_t m = weight(rank_value(sm.rank[i]), &b);
-                if (b >= b0 && b <= b1) f(sm.rank[i], b, m);
+                const uint64_t x = sm.weight[i];
+                const uint32_t b = static_cast<uint32_t>(x >> 48);
+                if (b >= b0 && b <= b1) f(sm.rank[i], b, x & 0xFFFFFFFFFFFFull);
             }
         } else {
             for (uint32_t i = t; i < a.vocab; i += kFinThreads) {
@@ -671,30 +735,24 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
             }
         }
     };
-    // Among the entries of bins b0 .. b1, with base_n entries of sum base_w before them: the rank of the one
-    // that brings the number to n, or the sum to w (by_sum); 0 where none does. *sum: the sum with it. While
-    // they are many, the range of their ranks is cut into parts and the part that holds it kept.
-    auto select = [&](uint32_t b0, uint32_t b1, uint32_t base_n, u128 base_w, bool by_sum, uint32_t n, u128 w, u128* sum) {
-        uint64_t r0 = 0, r1 = ~0ull;
-        for (;;) {
+    // Among the entries of bins b0 .. b1, `have` of them, ranks r0 .. r1, with base_n entries of sum base_w before
+    // them: the rank of the one that brings the number to n, or the sum to w (by_sum); 0 where none does. *sum:
+    // the sum with it. While they are many, the range of their ranks is cut into parts and the part that holds it
+    // kept.
+    auto select = [&](uint32_t b0, uint32_t b1, uint32_t have, uint64_t r0, uint64_t r1, uint32_t base_n, u128 base_w,
+                      bool by_sum, uint32_t n, u128 w, u128* sum) {
+        for (bool first = true;; first = false) {
             __syncthreads();
-            if (t == 0) sm.n = 0, sm.least = ~0ull, sm.most = 0, sm.cut = 0, sm.sum = 0;
+            if (t == 0) sm.n = 0, sm.least = ~0ull, sm.most = 0, sm.cut = 0, sm.sum = 0, sm.pick = kParts;
+            sm.part_n[t] = 0, sm.part_lo[t] = 0, sm.part_hi[t] = 0;
             __syncthreads();
-            uint64_t least = ~0ull, most = 0;
-            members(b0, b1, [&](uint64_t k, uint32_t b, uint64_t m) {
-                if (k < r0 || k > r1) return;
-                const uint32_t at = atomicAdd(&sm.n, 1u);
-                if (at < kSmall) sm.small[at] = k, sm.small_w[at] = unit(m, b);
-                least = k < least ? k : least, most = k > most ? k : most;
-            });
-            if (!on_list || listed > kSmall) {
-                most = wave_max_u64(most);
-                least = ~wave_max_u64(~least);
-                if (lane == 0) atomicMax(&sm.most, static_cast<unsigned long long>(most)), atomicMin(&sm.least, static_cast<unsigned long long>(least));
-            }
-            __syncthreads();
-            const uint32_t have = sm.n;
             if (have <= kSmall) {
+                members(b0, b1, [&](uint64_t k, uint32_t b, uint64_t m) {
+                    if (k < r0 || k > r1) return;
+                    const uint32_t at = atomicAdd(&sm.n, 1u);
+                    if (at < kSmall) sm.small[at] = k, sm.small_w[at] = unit(m, b);
+                });
+                __syncthreads();
                 // two threads to an entry add up those of larger rank
                 const uint32_t e = t / 2;
                 if (e < have) {
@@ -715,44 +773,48 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
                 *sum = sm.sum;
                 return sm.cut;
             }
-            r0 = sm.least, r1 = sm.most;
+            if (!first) {  // equal logits: their ranks fill little of the range
+                uint64_t least = ~0ull, most = 0;
+                members(b0, b1, [&](uint64_t k, uint32_t, uint64_t) {
+                    if (k < r0 || k > r1) return;
+                    least = k < least ? k : least, most = k > most ? k : most;
+                });
+                most = wave_max_u64(most);
+                least = ~wave_max_u64(~least);
+                if (lane == 0)
+                    atomicMax(&sm.most, static_cast<unsigned long long>(most)), atomicMin(&sm.least, static_cast<unsigned long long>(least));
+                __syncthreads();
+                r0 = sm.least, r1 = sm.most;
+            }
             const uint64_t range = r1 - r0;
             const int sft = range < kParts ? 0 : 55 - __builtin_clzll(range);  // range >> sft < 512
-            for (uint32_t i = t; i < kParts; i += kFinThreads) sm.part_n[i] = 0, sm.part_lo[i] = 0, sm.part_hi[i] = 0;
-            if (t == 0) sm.pick = kParts;
-            __syncthreads();
             members(b0, b1, [&](uint64_t k, uint32_t b, uint64_t m) {
                 if (k < r0 || k > r1) return;
                 const uint32_t d = kParts - 1 - static_cast<uint32_t>((k - r0) >> sft);  // falling
-                const u128 x = unit(m, b);
+                const Halves x = halve(unit(m, b));
                 atomicAdd(&sm.part_n[d], 1u);
-                atomicAdd(&sm.part_lo[d], static_cast<unsigned long long>(static_cast<uint64_t>(x) & ((1ull << kHalf) - 1)));
-                atomicAdd(&sm.part_hi[d], static_cast<unsigned long long>(x >> kHalf));
+                atomicAdd(&sm.part_lo[d], static_cast<unsigned long long>(x.lo));
+                atomicAdd(&sm.part_hi[d], static_cast<unsigned long long>(x.hi));
             });
             __syncthreads();
             const uint32_t own_n = sm.part_n[t];
-            const u128 own = (static_cast<u128>(sm.part_hi[t]) << kHalf) + sm.part_lo[t];
+            const u128 own = join(Halves{sm.part_lo[t], sm.part_hi[t]});
             uint32_t x = own_n, x_all;
             u128 y = own, y_all;
             block_scan<kFinWaves>(x, y, &x_all, &y_all, sm.scan);
             if (own_n != 0 && (by_sum ? base_w + y >= w && base_w + y - own < w : base_n + x >= n && base_n + x - own_n < n))
-                sm.pick = t, sm.base_n = base_n + x - own_n, sm.base_w = base_w + y - own;
+                sm.pick = t, sm.n = own_n, sm.base_n = base_n + x - own_n, sm.base_w = base_w + y - own;
             __syncthreads();
             if (sm.pick == kParts) {
                 *sum = base_w + y_all;
-                return static_cast<uint64_t>(0);
+                return uint64_t{0};
             }
-            base_n = sm.base_n, base_w = sm.base_w;
-            const uint64_t from = r0 + (static_cast<uint64_t>(kParts - 1 - sm.pick) << sft);
-            const uint64_t to = from + ((uint64_t{1} << sft) - 1);
+            base_n = sm.base_n, base_w = sm.base_w, have = sm.n;
+            const uint64_t from = r0 + (static_cast<uint64_t>(kParts - 1 - sm.pick) << sft), to = from + ((uint64_t{1} << sft) - 1);
             r1 = to < r1 ? to : r1, r0 = from;
         }
     };
 
-    if (on_list) {
-        for (uint32_t i = t; i < listed; i += kFinThreads) sm.rank[i] = a.s.list[r * kListCap + i];
-        __syncthreads();
-    }
     // top-k's cut by number, then top-p's by its share of the top-k's sum
     uint64_t cut = 0;  // ranks of at least this are kept
     u128 sum = st.all;
@@ -763,8 +825,10 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
         if (by_sum ? !st.use_p : (st.use_p ? !in_k : st.k == 0)) continue;
         uint64_t x = st.best;
         if (in_k || (lo <= hi && (by_sum == 0 || want > 0))) {
+            const uint32_t key0 = st.key[in_k ? 2 : 0], key1 = st.key[in_k ? 3 : 1];
             u128 with;
-            x = select(in_k ? st.bin_k : lo, in_k ? st.bin_k : hi, in_k ? st.count_k : st.count_l,
+            x = select(in_k ? st.bin_k : lo, in_k ? st.bin_k : hi, in_k ? st.in_k : st.in_l, static_cast<uint64_t>(key0) << 32,
+                       (static_cast<uint64_t>(key1) << 32) - 1, in_k ? st.count_k : st.count_l,
                        in_k ? st.below_k : st.below_l, by_sum != 0, st.k, want, &with);
             if (by_sum == 0) sum = with;
         } else if (lo > hi) {
@@ -775,52 +839,23 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
     cut = st.rank_m > cut ? st.rank_m : cut;
 
     // ---- the draw: kept weights by slice, then through the slice
-    const bool all = lo > hi;
-    // every entry in bins under `full` is kept, and of bin `full` those that reach the cut
-    uint32_t full = kBins;
-    if (!all) weight(rank_value(cut), &full);
     __syncthreads();
-    if (t < kMaxSlices) sm.in_slice[t] = 0, sm.slice[t] = 0;
-    if (t == 0) sm.n = 0, sm.last = 0, sm.id = ~0u;
-    uint32_t shift[kMaxSlices / 64];
-#pragma unroll
-    for (uint32_t i = 0; i < kMaxSlices / 64; ++i) shift[i] = slice_shift(head.own[i], top, c);
+    if (t == 0) sm.n = 0;
     __syncthreads();
-    if (!all) {
-        members(full, full, [&](uint64_t k, uint32_t, uint64_t m) {
+    if (lo <= hi) {
+        members(lo, hi, [&](uint64_t k, uint32_t b, uint64_t m) {
             if (k < cut) return;
-            atomicAdd(&sm.in_slice[rank_index(k) / kSlice], static_cast<unsigned long long>(m));
+            const Halves x = halve(unit(m, b));
+            const uint32_t slice = rank_index(k) / kSlice;
+            atomicAdd(&sm.slice_lo[slice], static_cast<unsigned long long>(x.lo));
+            atomicAdd(&sm.slice_hi[slice], static_cast<unsigned long long>(x.hi));
             atomicAdd(&sm.n, 1u);
         });
-    }
-    // sixteen threads to a slice, sixteen of its bins each
-    auto add = [&](uint32_t slice, uint32_t sh, auto bin_at) {
-        u128 x = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-            uint32_t down;
-            const uint32_t b = row_bin(t % 16 + 16 * i, sh, &down);
-            const uint64_t v = bin_at(i);
-            if (b < full) x += unit(down < 64 ? (v & kMassMask) >> down : 0, b);
-        }
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) x += shfl_xor_u128(x, d);
-        if (t % 16 == 0 && sh != kNoSlice) sm.slice[slice] = x;
-    };
-#pragma unroll
-    for (uint32_t j = 0; j < kMaxSlices / kTurn; ++j) {
-        const uint32_t s0 = j * kTurn + t / 16, sh = __shfl(shift[j * kTurn / 64], s0 % 64);
-        if (s0 >= a.slices) continue;
-        if (j < 2)
-            add(s0, sh, [&](uint32_t i) { return ahead[j < 2 ? j : 0][i]; });
-        else
-            add(s0, sh, [&](uint32_t i) { return bins[s0 * kBins + t % 16 + 16 * i]; });
     }
     __syncthreads();
     uint32_t n = 0, n_all;
     u128 own = 0, kept;
-    if (t < a.slices)
-        own = sm.slice[t] + (all ? 0 : unit(sm.in_slice[t], full));
+    if (t < a.slices) own = under + join(Halves{sm.slice_lo[t], sm.slice_hi[t]});
     u128 w = own;
     block_scan<kMaxSlices / 64>(n, w, &n_all, &kept, sm.scan);
     const u128 want = u < 1.0f ? part_of(u, kept, false) : kept - 1;  // the first running sum past this is drawn
@@ -833,8 +868,9 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
     const uint32_t i0 = slice * kSlice + kEach * t;
     uint32_t last = 0;
     float v[kEach];
+    static_assert(kEach % kVec<T> == 0, "whole loads");
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) v[j] = i0 + j < a.vocab ? load_logit<T>(row, i0 + j) : -INFINITY;
+    for (uint32_t j = 0; j < kEach; j += kVec<T>) load_vec<T>(row, i0 + j, a.vocab, v + j);
 #pragma unroll
     for (uint32_t j = 0; j < kEach; ++j) {
         e[j] = 0;
@@ -850,10 +886,12 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
     if (last) atomicMax(&sm.last, last);
     block_scan<kFinWaves>(n, run, &n_all, &ignored, sm.scan);
     u128 x = run - mine;
+    if (x <= rest && run > rest) {
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        if (x <= rest && x + e[j] > rest) sm.id = i0 + j, sm.sum = e[j];
-        x += e[j];
+        for (uint32_t j = 0; j < kEach; ++j) {
+            if (x <= rest && x + e[j] > rest) sm.id = i0 + j;
+            x += e[j];
+        }
     }
     __syncthreads();
     // (the deepest bin's sum may exceed its entries' own by their last bits: the last of them then)
@@ -864,7 +902,7 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
         for (uint32_t j = 1; j < kEach; ++j) drawn = id == i0 + j ? e[j] : drawn;
         a.o.tokens[r] = id;
         if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(drawn) / to_double(kept)));
-        if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(all ? st.live : (full ? a.s.counts[r * kBins + full - 1] : 0) + sm.n);
+        if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(lo > hi ? st.live : st.count_l + sm.n);
     }
 }
 
@@ -874,7 +912,7 @@ void launch(const SampleArgs& a, uint32_t rows, hipStream_t s) {
     sample_slices_kernel<T><<<grid, kSliceThreads, 0, s>>>(a);
     sample_limits_kernel<<<rows, kRowThreads, 0, s>>>(a);
     sample_collect_kernel<T><<<grid, kSliceThreads, 0, s>>>(a);
-    sample_finish_kernel<T><<<rows, kFinThreads, 0, s>>>(a);
+    sample_finish_kernel<T><<<rows, kFinThreads, sizeof(FinishMem), s>>>(a);
 }
 
 }  // namespace
@@ -906,9 +944,15 @@ TWD_API int twd_sampler_create(uint32_t max_vocab, uint32_t max_rows, twd_sample
     s->max_vocab = max_vocab, s->max_rows = max_rows, s->device = dev;
     const uint64_t slices = (max_vocab + kSlice - 1) / kSlice, rows = max_rows;
     const uint64_t bins = rows * slices * kBins * sizeof(uint64_t), list = rows * kListCap * sizeof(uint64_t);
-    const uint64_t sums = rows * kBins * sizeof(u128), states = (rows * sizeof(RowState) + 255) / 256 * 256;
-    const uint64_t heads = rows * slices * sizeof(SliceHead), counts = rows * kBins * sizeof(uint32_t);
-    const hipError_t e = hipMalloc(&s->block, bins + list + sums + states + heads + counts);
+    const uint64_t under = rows * slices * sizeof(u128), states = (rows * sizeof(RowState) + 255) / 256 * 256;
+    const uint64_t heads = rows * slices * sizeof(SliceHead);
+    hipError_t e = hipSuccess;
+    for (const void* f : {reinterpret_cast<const void*>(sample_finish_kernel<float>),
+                          reinterpret_cast<const void*>(sample_finish_kernel<Bf16>),
+                          reinterpret_cast<const void*>(sample_finish_kernel<Fp16>)})
+        if (e == hipSuccess)
+            e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(FinishMem)));
+    if (e == hipSuccess) e = hipMalloc(&s->block, bins + list + under + states + heads);
     if (e != hipSuccess) {
         delete s;
         return hip_fail(e, "allocating the sampler's scratch");
@@ -916,10 +960,9 @@ TWD_API int twd_sampler_create(uint32_t max_vocab, uint32_t max_rows, twd_sample
     char* at = static_cast<char*>(s->block);
     s->scratch.bins = reinterpret_cast<uint64_t*>(at), at += bins;
     s->scratch.list = reinterpret_cast<uint64_t*>(at), at += list;
-    s->scratch.sums = reinterpret_cast<u128*>(at), at += sums;
+    s->scratch.under = reinterpret_cast<u128*>(at), at += under;
     s->scratch.state = reinterpret_cast<RowState*>(at), at += states;
-    s->scratch.head = reinterpret_cast<SliceHead*>(at), at += heads;
-    s->scratch.counts = reinterpret_cast<uint32_t*>(at);
+    s->scratch.head = reinterpret_cast<SliceHead*>(at);
     s->scratch.slices = static_cast<uint32_t>(slices);
     *out = s;
     return TWD_OK;
@@ -954,7 +997,7 @@ TWD_API int twd_sampler_sample(twd_sampler* sampler, const void* logits, int typ
     if (rc) return rc;
     const SampleArgs args{logits, row_stride, vocab, (vocab + kSlice - 1) / kSlice,
                           SampleParams{temperature, top_k, top_p, min_p, uniform}, SampleOut{tokens, logprobs, kept},
-                          sampler->scratch};
+                          sampler->scratch, kExp2Poly};
     if (type == TWD_F32)
         launch<float>(args, rows, s);
     else if (type == TWD_BF16)
