@@ -56,7 +56,8 @@ __device__ __forceinline__ Scale scale_of(float t) {
     return s;
 }
 
-// The weight's octave floor(z) and its eighth of it, both rising with l, and the weight's 38 bits.
+// The weight's octave floor(z), the eighth of it that z lies in, counted from the top, and the weight's 38 bits.
+// The octave rises with l, and the eighth falls within it.
 struct Weight {
     double oct;
     uint32_t sub;
@@ -85,7 +86,7 @@ __device__ __forceinline__ Weight weight_of(float l, const Scale& c, const Exp2P
     const double mid = w.oct + 0.5;
     double t = fma(ld, c.hi, -mid);  // z less the octave's middle, rounded once, so rising with l
     if (FAR) t = __builtin_fabs(zh) < 0x1p45 ? t : 0.0;
-    const uint32_t sub = static_cast<uint32_t>(fma(t, 8.0, 4.0));
+    const uint32_t sub = static_cast<uint32_t>(fma(t, -8.0, 4.0));
     w.sub = sub < 7u ? sub : 7u;
     if (FAR) t = __builtin_fabs(zh) < 0x1p45 ? fma(ld, c.lo, t) : t;
     else t = fma(ld, c.lo, t);
@@ -157,9 +158,9 @@ constexpr int kCountBit = 51;
 constexpr uint64_t kMassMask = (1ull << kCountBit) - 1;
 
 struct SliceHead {
-    uint64_t best;  // largest rank of the live entries (0: none)
-    uint32_t live;
-    uint32_t bad;   // a NaN or +inf was seen
+    uint64_t best;     // largest rank of the live entries (0: none)
+    uint32_t weighed;  // its bins are written
+    uint32_t bad;      // a NaN or +inf was seen
 };
 
 struct RowState {
@@ -222,7 +223,7 @@ __device__ __forceinline__ void load_vec(const void* row, uint32_t i, uint32_t v
 __device__ __forceinline__ uint32_t bin_of(const Weight& w, double top) {
     const double down = top - w.oct;
     if (!(down < static_cast<double>(kTailOct + 1))) return kTail;
-    return (static_cast<uint32_t>(down) << 3) + 7u - w.sub;
+    return (static_cast<uint32_t>(down) << 3) + w.sub;
 }
 __device__ __forceinline__ uint64_t mass_of(const Weight& w, uint32_t bin, double top) {
     if (bin != kTail) return w.q;
@@ -304,7 +305,7 @@ constexpr uint32_t kCopies = 4;  // of a slice's bins, by lane, so that a wave's
 template <typename T>
 __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs a) {
     __shared__ uint64_t bins[kBins][kCopies];
-    __shared__ uint32_t s_key[kSliceThreads / 64], s_live[kSliceThreads / 64], s_bad[kSliceThreads / 64], s_idx;
+    __shared__ uint32_t s_key[kSliceThreads / 64], s_bad[kSliceThreads / 64], s_idx;
     const uint32_t t = threadIdx.x, slice = blockIdx.x, lane = t % 64, wave = t / 64;
     const uint64_t r = blockIdx.y;
     const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
@@ -319,59 +320,63 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
     for (uint32_t i = 0; i < kCopies; ++i) bins[t][i] = 0;
     if (t == 0) s_idx = ~0u;
     const Scale c = scale_of(temp);
-    const float far = static_cast<float>(0x1p44 / c.hi);
     float best = -INFINITY;
-    uint32_t live = 0, bad = 0, is_far = 0;
+    uint64_t nan = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        bad |= v[j] < INFINITY ? 0u : 1u;
-        live += v[j] > -INFINITY ? 1u : 0u;
-        is_far |= __builtin_fabsf(v[j]) < far || !(v[j] > -INFINITY) ? 0u : 1u;
-        best = v[j] > best ? v[j] : best;
+    for (uint32_t j = 0; j < kEach; j += 2) {
+        nan |= __ballot(__builtin_isunordered(v[j], v[j + 1]));
+        best = fmaxf(best, fmaxf(v[j], v[j + 1]));
     }
-    uint32_t key = float_key(best);
-    key = wave_reduce(key, 0u, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
-    live = wave_reduce(live, 0u, [](uint32_t x, uint32_t y) { return x + y; });
-    bad = wave_reduce(bad | is_far << 1, 0u, [](uint32_t x, uint32_t y) { return x | y; });
-    if (lane == 0) s_key[wave] = key, s_live[wave] = live, s_bad[wave] = bad;
+    const uint32_t own = float_key(best);
+    uint32_t key = wave_reduce(own, 0u, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
+    if (lane == 0) s_key[wave] = key, s_bad[wave] = nan != 0 ? 1u : 0u;
     __syncthreads();
-    live = 0;
+    uint32_t bad = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < kSliceThreads / 64; ++i) {
-        key = s_key[i] > key ? s_key[i] : key;
-        live += s_live[i], bad |= s_bad[i];
-    }
+    for (uint32_t i = 0; i < kSliceThreads / 64; ++i) key = s_key[i] > key ? s_key[i] : key, bad |= s_bad[i];
     best = key_float(key);
-    uint32_t idx = ~0u;
+    bad |= best < INFINITY ? 0u : 1u;
+    const bool live = best > -INFINITY;
+    if (own == key) {
+        uint32_t idx = ~0u;
 #pragma unroll
-    for (uint32_t j = kEach; j-- > 0;)
-        if (v[j] == best) idx = i0 + (j / kVec<T>) * kSliceThreads * kVec<T> + j % kVec<T>;
-    if (idx != ~0u) atomicMin(&s_idx, idx);
-    if (live != 0 && temp > 0.0f) {
+        for (uint32_t j = kEach; j-- > 0;)
+            if (v[j] == best) idx = i0 + (j / kVec<T>) * kSliceThreads * kVec<T> + j % kVec<T>;
+        atomicMin(&s_idx, idx);
+    }
+    const bool weigh = live && bad == 0 && temp > 0.0f;  // a row with a NaN or +inf, and a greedy one, needs no weights
+    if (weigh) {
         const double top = weight_of(best, c).oct;
-        auto add = [&](float l, const Weight& w) {
-            uint32_t b = (static_cast<uint32_t>(top - w.oct) << 3) + 7u - w.sub;
-            uint64_t m = w.q;
-            if (!(top - w.oct < static_cast<double>(kTailOct) + 0.5)) b = bin_of(w, top), m = mass_of(w, b, top);
-            if (l > -INFINITY)
-                atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b][lane % kCopies]),
-                          static_cast<unsigned long long>(1ull << kCountBit | m));
-        };
-        if (bad == 0) {
-            // masked entries take the largest one's place in the arithmetic, so that nothing branches there
+        if (__builtin_fabs(top) < 0x1p44) {
+            // Nothing branches on an entry's value, and only the counting leaves masked ones out. (An entry so far
+            // down that its z holds no fraction shifts to nothing.)
 #pragma unroll
-            for (uint32_t j = 0; j < kEach; ++j) add(v[j], weight_of<false>(v[j] > -INFINITY ? v[j] : best, c, a.poly));
+            for (uint32_t j = 0; j < kEach; ++j) {
+                const Weight w = weight_of<false>(v[j], c, a.poly);
+                uint32_t d = static_cast<uint32_t>(top - w.oct);
+                d = d < kTailOct + 63 ? d : kTailOct + 63;
+                const uint32_t b = d << 3 | w.sub;
+                const uint64_t m = w.q >> ((d > kTailOct ? d : kTailOct) - kTailOct);
+                if (v[j] > -INFINITY)
+                    atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b < kTail ? b : kTail][lane % kCopies]),
+                              static_cast<unsigned long long>(1ull << kCountBit | m));
+            }
         } else {
-#pragma unroll
-            for (uint32_t j = 0; j < kEach; ++j)
-                if (v[j] < INFINITY) add(v[j], weight_of(v[j] > -INFINITY ? v[j] : best, c));
+#pragma unroll 1
+            for (uint32_t i = slice * kSlice + t; i < min(a.vocab, (slice + 1) * kSlice); i += kSliceThreads) {
+                const float l = load_logit<T>(row, i);
+                if (!(l > -INFINITY)) continue;
+                const Weight w = weight_of(l, c);
+                const uint32_t b = bin_of(w, top);
+                atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b][lane % kCopies]),
+                          static_cast<unsigned long long>(1ull << kCountBit | mass_of(w, b, top)));
+            }
         }
     }
     __syncthreads();
     const uint64_t at = r * a.s.slices + slice;
-    if (t == 0)
-        a.s.head[at] = SliceHead{live ? static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - s_idx) : 0, live, bad & 1u};
-    if (live != 0 && temp > 0.0f) {
+    if (t == 0) a.s.head[at] = SliceHead{live ? static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - s_idx) : 0, weigh ? 1u : 0u, bad};
+    if (weigh) {
         uint64_t x = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kCopies; ++i) x += bins[t][i];
@@ -388,9 +393,9 @@ __device__ __forceinline__ uint32_t row_bin(uint32_t b, uint32_t shift, uint32_t
     *down = (b >> 3) + shift - kTailOct;
     return kTail;
 }
-constexpr uint32_t kNoSlice = 255;  // the shift of a slice without live entries, whose bins are not written
+constexpr uint32_t kNoSlice = 255;  // the shift of a slice whose bins are not written
 __device__ __forceinline__ uint32_t slice_shift(const SliceHead& h, double top, const Scale& c) {
-    if (h.live == 0) return kNoSlice;
+    if (h.weighed == 0) return kNoSlice;
     const double d = top - __builtin_floor(static_cast<double>(rank_value(h.best)) * c.hi);
     return d < 128.0 ? static_cast<uint32_t>(d) : 128u;
 }
@@ -445,12 +450,12 @@ __device__ uint32_t least_key(int b, uint32_t above, double top, const Scale& c)
 // What every wave of a block learns of its row from the slices' heads.
 struct RowHead {
     uint64_t best;
-    uint32_t live, bad;
+    uint32_t bad;
     SliceHead own[kMaxSlices / 64];  // of slices lane and lane + 64
 };
 __device__ __forceinline__ RowHead read_heads(const SampleArgs& a, uint64_t r) {
     const uint32_t lane = threadIdx.x % 64;
-    RowHead h{0, 0, 0, {}};
+    RowHead h{0, 0, {}};
 #pragma unroll
     for (uint32_t i = 0; i < kMaxSlices / 64; ++i) {
         h.own[i] = SliceHead{0, 0, 0};
@@ -459,10 +464,9 @@ __device__ __forceinline__ RowHead read_heads(const SampleArgs& a, uint64_t r) {
 #pragma unroll
     for (uint32_t i = 0; i < kMaxSlices / 64; ++i) {
         h.best = h.own[i].best > h.best ? h.own[i].best : h.best;
-        h.live += h.own[i].live, h.bad |= h.own[i].bad;
+        h.bad |= h.own[i].bad;
     }
     h.best = wave_max_u64(h.best);
-    h.live = wave_reduce(h.live, 0u, [](uint32_t x, uint32_t y) { return x + y; });
     h.bad = wave_reduce(h.bad, 0u, [](uint32_t x, uint32_t y) { return x | y; });
     return h;
 }
@@ -498,8 +502,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
     if (t == 0) s_rank_m = 0, s_bin_m = kBins;
     __syncthreads();
     const uint64_t best = head.best;
-    const uint32_t live = head.live;
-    const bool none = head.bad != 0 || live == 0 || temp != temp || u != u || top_p != top_p || min_p != min_p;
+    const bool none = head.bad != 0 || best == 0 || temp != temp || u != u || top_p != top_p || min_p != min_p;
     if (none || temp <= 0.0f) {
         if (t == 0) {
             a.s.state[r].done = 1;
@@ -551,6 +554,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
     uint32_t n = t < kBins ? count[t] : 0, n_all;
     u128 w = t < kBins ? unit(mass[t], t) : 0, w_all;
     block_scan<kBins / 64>(n, w, &n_all, &w_all, scan);
+    const uint32_t live = n_all;
     if (t < kBins) counts[t] = n, sums[t] = w;
     __syncthreads();
     // the bin each limit cuts in: the first whose running number or sum reaches it
@@ -631,7 +635,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArg
     RowState* st = a.s.state + r;
     const uint32_t listed = st->listed, k0 = st->key[0], k1 = st->key[1], k2 = st->key[2], k3 = st->key[3];
     const SliceHead h = a.s.head[r * a.s.slices + slice];
-    if (listed == 0 || listed > kListCap || h.live == 0) return;
+    if (listed == 0 || listed > kListCap || h.weighed == 0) return;
     const uint32_t most = static_cast<uint32_t>(h.best >> 32);
     if (most < k0 && (k2 == k3 || most < k2)) return;  // all of the slice lies below
     if (t == 0) s_n = 0;
