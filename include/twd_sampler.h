@@ -28,7 +28,7 @@ extern "C" {
  * holds a NaN or +inf logit or no entry above -inf, and one whose T, top_p, min_p or uniform is NaN,
  * gives TWD_TOKEN_DEGENERATE, a NaN logprob and 0 kept.
  *
- * Sums are integers (weights of 38 bits), so results do not depend on the launch, the batch or the
+ * Sums are integers (weights of 37 bits), so results do not depend on the launch, the batch or the
  * run. logits are rows of `type` with row_stride elements between them, at any alignment of that type, and
  * stay as they are. A sampler holds the scratch of up to max_rows (4,096) rows of up to max_vocab
  * (524,288) entries; its calls are ordered across streams as a selector's are, and replays of captured

@@ -9,8 +9,8 @@
 //
 // Arithmetic. Sums decide, so they may not depend on the order in which threads add: weights are
 // fixed-point numbers and sums are integers. With z = l log2(e) / T (formed in two doubles), a weight is
-// 2^floor(z) times the fraction's power of two, rounded to 38 bits (2^-38 relative); sums are held in 128
-// bits whose unit is 2^-78 of the largest weight's octave, so nothing above that is dropped. Every decision
+// 2^floor(z) times the fraction's power of two, rounded to 37 bits (2^-37 relative); sums are held in 128
+// bits whose unit is 2^-77 of the largest weight's octave, so nothing above that is dropped. Every decision
 // is then an exact comparison of integers, and equal logits have equal weights.
 #include <hip/hip_runtime.h>
 
@@ -26,7 +26,6 @@ namespace {
 
 typedef unsigned __int128 u128;
 
-constexpr int kWeightBits = 38;  // a weight is 2^37 .. 2^38 times its octave
 constexpr int kSumShift = 40;    // sums: the largest octave's weights shifted left by this
 
 struct SampleParams {
@@ -56,7 +55,7 @@ __device__ __forceinline__ Scale scale_of(float t) {
     return s;
 }
 
-// The weight's octave floor(z), the eighth of it that z lies in, counted from the top, and the weight's 38 bits.
+// The weight's octave floor(z), the eighth of it that z lies in, counted from the top, and the weight's 37 bits.
 // The octave rises with l, and the eighth falls within it.
 struct Weight {
     double oct;
@@ -65,10 +64,11 @@ struct Weight {
 };
 // FAR: |z| may reach 2^45, where neighbouring floats lie more octaves apart than any sum holds and z has no
 // fraction left: the weight is its octave's middle then. A caller that knows better leaves the test out.
-// 2^(37.5 + t), |t| <= 0.5: the degree-9 polynomial through the Chebyshev nodes (2e-14 relative). A kernel that
+// 2^(36.5 + t) less 2^-30 of it, so that 8,192 of them stay under 2^50; |t| <= 0.5: the degree-9 polynomial
+// through the Chebyshev nodes (2e-14 relative). A kernel that
 // evaluates it for every logit takes the coefficients as an argument, in scalar registers: as literals each
 // would be moved into a register pair before its use.
-constexpr double kRoot = 0x1.6a09e667f3bcdp+37;
+constexpr double kRoot = 0x1.6a09e667f3bcdp+36 * (1.0 - 0x1p-30);
 struct Exp2Poly {
     double c[10];
 };
@@ -138,23 +138,23 @@ constexpr uint32_t kLogitBytes<float> = 4;
 
 // ---- the four launches -------------------------------------------------------------------------------
 //
-//   slices   every slice of 4,096 entries: its largest rank, and its entries' numbers and weights by bin
+//   slices   every slice of 8,192 entries: its largest rank, and its entries' numbers and weights by bin
 //   limits   per row: the slices' bins added up, and the bins in which the limits cut
 //   collect  every slice: its entries in those bins, onto the row's list
 //   finish   per row: the list in order, the cuts, and the draw
 //
 // A bin is an eighth of an octave of weight. A slice counts from its own largest octave down (its row's is
 // not known yet), 256 bins to a slice, the last one for all that lies deeper; octaves are absolute, so the
-// slices' bins line up. A bin's entries share an octave, so its sum of 38-bit weights is one integer; the
+// slices' bins line up. A bin's entries share an octave, so its sum of 37-bit weights is one integer; the
 // last bin's are brought to its octave (2^-31 of the largest) first.
-constexpr uint32_t kSlice = 4096;
+constexpr uint32_t kSlice = 8192;
 constexpr uint32_t kBins = 256;
 constexpr uint32_t kTail = kBins - 1;
 constexpr uint32_t kTailOct = kTail >> 3;
 constexpr uint32_t kListCap = 4096;
 constexpr uint32_t kMaxSlices = 524288 / kSlice;
-// A bin of a slice: entries above bit 51, the sum of their weights (at most 4096 * 2^38 and a little) below.
-constexpr int kCountBit = 51;
+// A bin of a slice: its entries' number from bit 50 on, the sum of their weights below.
+constexpr int kCountBit = 50;
 constexpr uint64_t kMassMask = (1ull << kCountBit) - 1;
 
 struct SliceHead {
@@ -299,7 +299,7 @@ __device__ __forceinline__ void block_scan(uint32_t& n, u128& w, uint32_t* n_all
     *n_all = na, *w_all = wa;
 }
 
-constexpr uint32_t kSliceThreads = 256;
+constexpr uint32_t kSliceThreads = 512;
 constexpr uint32_t kCopies = 4;  // of a slice's bins, by lane, so that a wave's equal bins meet less often
 
 template <typename T>
@@ -316,8 +316,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
     for (uint32_t j = 0; j < kLoads; ++j)
         load_vec<T>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab, v + j * kVec<T>);
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < kCopies; ++i) bins[t][i] = 0;
+    for (uint32_t i = t; i < kBins * kCopies; i += kSliceThreads) bins[i / kCopies][i % kCopies] = 0;
     if (t == 0) s_idx = ~0u;
     const Scale c = scale_of(temp);
     float best = -INFINITY;
@@ -376,14 +375,14 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
     __syncthreads();
     const uint64_t at = r * a.s.slices + slice;
     if (t == 0) a.s.head[at] = SliceHead{live ? static_cast<uint64_t>(key) << 32 | (0xFFFFFFFFu - s_idx) : 0, weigh ? 1u : 0u, bad};
-    if (weigh) {
+    if (weigh && t < kBins) {
         uint64_t x = 0;
 #pragma unroll
         for (uint32_t i = 0; i < kCopies; ++i) x += bins[t][i];
         a.s.bins[at * kBins + t] = x;
     }
 }
-static_assert(kBins == kSliceThreads, "a bin per thread");
+static_assert(kMaxSlices <= 64, "a lane to a slice");
 
 // The row's bin of a slice's bin, `shift` octaves under the row's largest, and what to shift its sum by.
 __device__ __forceinline__ uint32_t row_bin(uint32_t b, uint32_t shift, uint32_t* down) {
@@ -400,85 +399,71 @@ __device__ __forceinline__ uint32_t slice_shift(const SliceHead& h, double top, 
     return d < 128.0 ? static_cast<uint32_t>(d) : 128u;
 }
 
-// The least rank that min-p keeps, by a wave: (l - M) log2(e) / T >= log2(min_p); the best one where none does.
+// The least key at which `yes` holds, by a wave: it holds from there up to `above`, where it is taken to hold.
+// First the 64 keys around the guess, then, had that been further off, cuts by 64.
+constexpr uint32_t kLeast = 0x007FFFFFu;  // -inf's key: below every entry's
+template <typename F>
+__device__ __forceinline__ uint32_t least_key(uint32_t guess, uint32_t above, F yes) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint64_t lo = kLeast + 1, hi = above;  // it lies between, hi included
+    uint64_t from = guess > lo + 32 ? (guess < hi ? guess : hi) - 32 : lo;
+    uint64_t step = 1;
+    for (;;) {
+        const uint64_t x = from + lane * step;
+        const uint64_t set = __ballot(x >= hi || yes(key_float(static_cast<uint32_t>(x))));
+        if (set == 0) {
+            lo = from + 63 * step + 1;
+        } else {
+            const uint32_t first = static_cast<uint32_t>(__builtin_ctzll(set));
+            const uint64_t at = from + first * step;
+            hi = at < hi ? at : hi;
+            if (first != 0) lo = from + (first - 1) * step + 1;
+        }
+        if (lo >= hi) return static_cast<uint32_t>(hi);
+        from = lo, step = (hi - lo + 63) / 64;
+    }
+}
+
+// The least rank that min-p keeps: (l - M) log2(e) / T >= log2(min_p); the best one where none does.
 __device__ uint64_t least_kept(uint64_t best, float min_p, const Scale& c) {
     const float m = rank_value(best);
-    const uint32_t key_m = static_cast<uint32_t>(best >> 32), lane = threadIdx.x % 64;
-    constexpr uint32_t kLeast = 0x007FFFFFu;  // -inf's key
     const double lim = log2(static_cast<double>(min_p));
     auto keeps = [&](float l) { return (static_cast<double>(l) - static_cast<double>(m)) * c.hi >= lim; };
     if (!keeps(m)) return best;
     if (c.hi == 0.0) return static_cast<uint64_t>(kLeast) << 32;
     // the quotient and the sum are rounded, the float once more: it lies a few floats around their result
-    uint32_t k = float_key(static_cast<float>(static_cast<double>(m) + lim / c.hi));
-    k = k < key_m ? k : key_m;
-    for (;;) {
-        const uint32_t from = k > kLeast + 32 ? k - 32 : kLeast;
-        const uint64_t yes = __ballot(from + lane >= key_m || keeps(key_float(from + lane)));
-        if (yes == 0) {
-            k = from + 64 + 32;
-        } else if ((yes & 1) != 0 && from > kLeast) {
-            k = from - 31;
-        } else {
-            return static_cast<uint64_t>(from + static_cast<uint32_t>(__builtin_ctzll(yes))) << 32;
-        }
-    }
+    const uint32_t guess = float_key(static_cast<float>(static_cast<double>(m) + lim / c.hi));
+    return static_cast<uint64_t>(least_key(guess, static_cast<uint32_t>(best >> 32), keeps)) << 32;
 }
 
-// The least key whose entry lies in a bin of at most b, by a wave: bins fall with rising keys, so each round
-// cuts the range by 64. `above`: a key past every entry's, taken where no key below it qualifies.
-__device__ uint32_t least_key(int b, uint32_t above, double top, const Scale& c) {
-    uint64_t lo = 0x00800000u, hi = above;  // from -FLT_MAX's key; hi qualifies
-    const uint32_t lane = threadIdx.x % 64;
-    while (lo < hi) {
-        const uint64_t step = (hi - lo + 63) / 64;
-        const uint64_t k = lo + step * lane;
-        const bool yes = k >= hi || static_cast<int>(bin_of(weight_of(key_float(static_cast<uint32_t>(k)), c), top)) <= b;
-        const uint32_t first = static_cast<uint32_t>(__builtin_ctzll(__ballot(yes) | 1ull << 63));
-        if (!(__ballot(yes) >> 63) && first == 63) {  // none of the 64: it lies past the last
-            lo = lo + step * 63 + 1;
-            continue;
-        }
-        const uint64_t at = lo + step * first;
-        hi = at < hi ? at : hi;
-        if (first != 0) lo = lo + step * (first - 1) + 1;
-        else lo = hi;
-    }
-    return static_cast<uint32_t>(hi);
+// The least key whose entry lies in a bin of at most b (bins fall with rising logits): where z reaches the bin's
+// lower end.
+__device__ uint32_t bin_key(uint32_t b, uint32_t above, double top, const Scale& c) {
+    if (b >= kTail) return kLeast + 1;
+    const double z = top + 1.0 - 0.125 * static_cast<double>(b + 1);
+    const uint32_t guess = c.hi > 0.0 ? float_key(static_cast<float>(z / c.hi)) : above;
+    return least_key(guess, above, [&](float l) { return bin_of(weight_of(l, c), top) <= b; });
 }
 
 // What every wave of a block learns of its row from the slices' heads.
 struct RowHead {
     uint64_t best;
     uint32_t bad;
-    SliceHead own[kMaxSlices / 64];  // of slices lane and lane + 64
+    SliceHead own;  // of slice `lane`
 };
 __device__ __forceinline__ RowHead read_heads(const SampleArgs& a, uint64_t r) {
     const uint32_t lane = threadIdx.x % 64;
-    RowHead h{0, 0, {}};
-#pragma unroll
-    for (uint32_t i = 0; i < kMaxSlices / 64; ++i) {
-        h.own[i] = SliceHead{0, 0, 0};
-        if (lane + 64 * i < a.slices) h.own[i] = a.s.head[r * a.s.slices + lane + 64 * i];
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < kMaxSlices / 64; ++i) {
-        h.best = h.own[i].best > h.best ? h.own[i].best : h.best;
-        h.bad |= h.own[i].bad;
-    }
-    h.best = wave_max_u64(h.best);
-    h.bad = wave_reduce(h.bad, 0u, [](uint32_t x, uint32_t y) { return x | y; });
+    RowHead h{0, 0, {0, 0, 0}};
+    if (lane < a.slices) h.own = a.s.head[r * a.s.slices + lane];
+    h.best = wave_max_u64(h.own.best);
+    h.bad = wave_reduce(h.own.bad, 0u, [](uint32_t x, uint32_t y) { return x | y; });
     return h;
 }
 
-// Sixteen threads to a slice, sixteen of its bins each; the first 64 slices' come in one go, ahead of everything
-// that decides what they mean.
-constexpr uint32_t kTurn = kRowThreads / 16;  // slices at a time
-constexpr uint32_t kAhead = 64 / kTurn;
-
 __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a) {
-    __shared__ unsigned long long mass[kBins];
-    __shared__ uint32_t count[kBins], counts[kBins], found[3], s_bin_m;
+    __shared__ uint64_t mass[kRowThreads];
+    __shared__ uint32_t count[kRowThreads], counts[kBins], found[3], s_bin_m, s_tail_n;
+    __shared__ unsigned long long s_tail;
     __shared__ u128 sums[kBins];
     __shared__ uint64_t s_rank_m;
     __shared__ RowState s_st;
@@ -489,18 +474,6 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f, u = a.p.uniform[r];
     const float top_p = a.p.top_p ? a.p.top_p[r] : 1.0f, min_p = a.p.min_p ? a.p.min_p[r] : 0.0f;
     const int32_t top_k = a.p.top_k ? a.p.top_k[r] : 0;
-    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
-    auto load = [&](uint32_t slice, uint64_t (&x)[16]) {
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) x[i] = slice < a.slices ? bins[slice * kBins + t % 16 + 16 * i] : 0;
-    };
-    uint64_t ahead[kAhead][16];
-#pragma unroll
-    for (uint32_t j = 0; j < kAhead; ++j) load(j * kTurn + t / 16, ahead[j]);
-    if (t < kBins) mass[t] = 0, count[t] = 0;
-    if (t < 3) found[t] = kBins;
-    if (t == 0) s_rank_m = 0, s_bin_m = kBins;
-    __syncthreads();
     const uint64_t best = head.best;
     const bool none = head.bad != 0 || best == 0 || temp != temp || u != u || top_p != top_p || min_p != min_p;
     if (none || temp <= 0.0f) {
@@ -514,36 +487,45 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         return;
     }
     const Scale c = scale_of(temp);
+    const uint32_t shift = slice_shift(head.own, weight_of(rank_value(best), c).oct, c);
     const double top = weight_of(rank_value(best), c).oct;
-    uint32_t shift[kMaxSlices / 64];
-#pragma unroll
-    for (uint32_t i = 0; i < kMaxSlices / 64; ++i) shift[i] = slice_shift(head.own[i], top, c);
-    // f(slice, its shift, its sixteen bins of this thread), all slices in turn
-    auto slices = [&](auto f) {
-#pragma unroll
-        for (uint32_t j = 0; j < kMaxSlices / kTurn; ++j) {
-            if (j * kTurn >= a.slices) break;
-            const uint32_t slice = j * kTurn + t / 16, sh = __shfl(shift[j * kTurn / 64], slice % 64);
-            if (j < kAhead) {
-                f(slice, sh, ahead[j < kAhead ? j : 0]);
-            } else {
-                uint64_t x[16];
-                load(slice, x);
-                f(slice, sh, x);
-            }
-        }
-    };
-    slices([&](uint32_t, uint32_t sh, const uint64_t (&x)[16]) {
-        if (sh == kNoSlice) return;  // (its bins are not written)
+    // Two threads to a bin of the row, every other slice each: a slice's bin 8 `shift` above it. What lies deeper
+    // than the row's last but one bin adds up in that last one.
+    const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
+    const uint32_t bin = t % kBins;
+    constexpr uint32_t kEvery = kRowThreads / kBins, kTurns = kMaxSlices / kEvery;
+    const uint32_t s0 = __builtin_amdgcn_readfirstlane(t / kBins);
+    uint64_t m = 0, tail = 0;
+    uint32_t n_bin = 0, n_tail = 0;
+#pragma unroll 1
+    for (uint32_t j = 0; j < kTurns && j * kEvery < a.slices; j += 16) {
+        uint64_t x[16], y[16];
 #pragma unroll
         for (uint32_t i = 0; i < 16; ++i) {
-            if (x[i] == 0) continue;
-            uint32_t down;
-            const uint32_t b = row_bin(t % 16 + 16 * i, sh, &down);
-            atomicAdd(&mass[b], static_cast<unsigned long long>(down < 64 ? (x[i] & kMassMask) >> down : 0));
-            atomicAdd(&count[b], static_cast<uint32_t>(x[i] >> kCountBit));
+            const uint32_t slice = s0 + (j + i) * kEvery;
+            const uint32_t sh = slice < a.slices ? __builtin_amdgcn_readlane(shift, slice) : kNoSlice;
+            const uint64_t* from = bins + slice * kBins;
+            x[i] = sh != kNoSlice && bin < kTail && bin >= 8 * sh ? from[bin - 8 * sh] : 0;
+            y[i] = sh != kNoSlice && bin + 8 * sh >= kTail ? from[bin] : 0;
         }
-    });
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            const uint32_t slice = s0 + (j + i) * kEvery;
+            const uint32_t sh = slice < a.slices ? __builtin_amdgcn_readlane(shift, slice) : 0;
+            m += x[i] & kMassMask, n_bin += static_cast<uint32_t>(x[i] >> kCountBit);
+            const uint32_t down = (bin >> 3) + sh - kTailOct;
+            tail += down < 64 ? (y[i] & kMassMask) >> down : 0, n_tail += static_cast<uint32_t>(y[i] >> kCountBit);
+        }
+    }
+    if (t < 3) found[t] = kBins;
+    if (t == 0) s_rank_m = 0, s_bin_m = kBins, s_tail = 0, s_tail_n = 0;
+    mass[t] = m, count[t] = n_bin;
+    __syncthreads();
+    if (__ballot(n_tail != 0) != 0) {
+        tail = wave_reduce(tail, uint64_t{0}, [](uint64_t p, uint64_t q) { return p + q; });
+        n_tail = wave_reduce(n_tail, 0u, [](uint32_t p, uint32_t q) { return p + q; });
+        if (lane == 0) atomicAdd(&s_tail, static_cast<unsigned long long>(tail)), atomicAdd(&s_tail_n, n_tail);
+    }
     if (wave == kRowThreads / 64 - 1 && min_p > 0.0f) {
         const uint64_t rank = least_kept(best, min_p, c);
         const float l = rank_value(rank);
@@ -551,8 +533,14 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         if (lane == 0) s_rank_m = rank, s_bin_m = b;
     }
     __syncthreads();
-    uint32_t n = t < kBins ? count[t] : 0, n_all;
-    u128 w = t < kBins ? unit(mass[t], t) : 0, w_all;
+    uint32_t n = 0, n_all;
+    u128 w = 0, w_all;
+    if (t < kBins) {
+        m = t == kTail ? s_tail : 0, n = t == kTail ? s_tail_n : 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kEvery; ++i) m += mass[i * kBins + t], n += count[i * kBins + t];
+        w = unit(m, t);
+    }
     block_scan<kBins / 64>(n, w, &n_all, &w_all, scan);
     const uint32_t live = n_all;
     if (t < kBins) counts[t] = n, sums[t] = w;
@@ -592,24 +580,10 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         uint32_t key = 0;
         if (wave < 2 ? any : need_k) {
             const uint32_t b0 = wave < 2 ? lo : bin_k, b1 = wave < 2 ? hi : bin_k;
-            key = wave % 2 == 0 ? least_key(static_cast<int>(b1), above, top, c)
-                                : (b0 == 0 ? above : least_key(static_cast<int>(b0) - 1, above, top, c));
+            key = wave % 2 == 0 ? bin_key(b1, above, top, c) : (b0 == 0 ? above : bin_key(b0 - 1, above, top, c));
         }
         if (lane == 0) s_st.key[wave] = key;
     }
-    // every slice's sum under them: what the draw starts from
-    slices([&](uint32_t slice, uint32_t sh, const uint64_t (&x)[16]) {
-        u128 sum = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-            uint32_t down;
-            const uint32_t b = row_bin(t % 16 + 16 * i, sh, &down);
-            if (b < lo && sh != kNoSlice) sum += unit(down < 64 ? (x[i] & kMassMask) >> down : 0, b);
-        }
-        const Halves h = halve(sum);
-        sum = join(Halves{sum_of_16(h.lo), sum_of_16(h.hi)});
-        if (t % 16 == 0 && slice < a.slices) a.s.under[r * a.s.slices + slice] = sum;
-    });
     if (t == kRowThreads - 1) {
         RowState& st = s_st;
         st.top = top, st.best = best, st.rank_m = s_rank_m, st.all = w_all, st.live = live, st.k = k, st.use_p = use_p;
@@ -635,6 +609,26 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArg
     RowState* st = a.s.state + r;
     const uint32_t listed = st->listed, k0 = st->key[0], k1 = st->key[1], k2 = st->key[2], k3 = st->key[3];
     const SliceHead h = a.s.head[r * a.s.slices + slice];
+    if (st->done) return;
+    // the slice's sum under the deciding bins: what the draw starts from
+    if (t < 64) {
+        const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
+        const uint32_t lo = st->lo <= st->hi ? st->lo : kBins, sh = slice_shift(h, st->top, scale_of(temp));
+        u128 sum = 0;
+        if (sh != kNoSlice) {
+            const uint64_t* bins = a.s.bins + (r * a.s.slices + slice) * kBins;
+#pragma unroll
+            for (uint32_t i = 0; i < kBins / 64; ++i) {
+                uint32_t down;
+                const uint32_t b = row_bin(64 * i + t, sh, &down);
+                if (b < lo) sum += unit(down < 64 ? (bins[64 * i + t] & kMassMask) >> down : 0, b);
+            }
+        }
+        const Halves x = halve(sum);
+        auto add = [](uint64_t p, uint64_t q) { return p + q; };
+        sum = join(Halves{wave_reduce(x.lo, uint64_t{0}, add), wave_reduce(x.hi, uint64_t{0}, add)});
+        if (t == 0) a.s.under[r * a.s.slices + slice] = sum;
+    }
     if (listed == 0 || listed > kListCap || h.weighed == 0) return;
     const uint32_t most = static_cast<uint32_t>(h.best >> 32);
     if (most < k0 && (k2 == k3 || most < k2)) return;  // all of the slice lies below
@@ -796,6 +790,28 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
                 if (k < r0 || k > r1) return;
                 const uint32_t d = kParts - 1 - static_cast<uint32_t>((k - r0) >> sft);  // falling
                 const Halves x = halve(unit(m, b));
+                // Equal logits meet in one part: where a wave's first entry has company, the lanes that hold its part
+                // and its weight add up as one.
+                bool todo = true;
+                for (uint32_t turn = 0; turn < 16; ++turn) {
+                    const uint32_t d0 = __builtin_amdgcn_readfirstlane(d);
+                    const uint64_t m0 = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(m >> 32))) << 32 |
+                                        __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(m));
+                    const bool same = d == d0 && m == m0;
+                    const uint64_t mates = __ballot(same);
+                    const uint32_t number = static_cast<uint32_t>(__builtin_popcountll(mates));
+                    if (number < 4) break;
+                    if (same) {
+                        if (static_cast<uint32_t>(__builtin_ctzll(mates)) == lane) {
+                            atomicAdd(&sm.part_n[d], number);
+                            atomicAdd(&sm.part_lo[d], static_cast<unsigned long long>(x.lo * number));
+                            atomicAdd(&sm.part_hi[d], static_cast<unsigned long long>(x.hi * number));
+                        }
+                        todo = false;
+                        break;
+                    }
+                }
+                if (!todo) return;
                 atomicAdd(&sm.part_n[d], 1u);
                 atomicAdd(&sm.part_lo[d], static_cast<unsigned long long>(x.lo));
                 atomicAdd(&sm.part_hi[d], static_cast<unsigned long long>(x.hi));
@@ -868,46 +884,47 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
     const uint32_t slice = sm.pick;
     const u128 rest = sm.want;
     constexpr uint32_t kEach = kSlice / kFinThreads;
-    u128 e[kEach], run = 0, ignored;
+    u128 run = 0, ignored;
     const uint32_t i0 = slice * kSlice + kEach * t;
+    constexpr uint32_t kWeighs = 1u << 20;  // above every index
     uint32_t last = 0;
     float v[kEach];
     static_assert(kEach % kVec<T> == 0, "whole loads");
 #pragma unroll
     for (uint32_t j = 0; j < kEach; j += kVec<T>) load_vec<T>(row, i0 + j, a.vocab, v + j);
+    auto drawn = [&](uint32_t j) -> u128 {
+        if (!(v[j] > -INFINITY && rank_key(v[j], i0 + j) >= cut)) return 0;
+        uint32_t b;
+        const uint64_t m = weight(v[j], &b);
+        return unit(m, b);
+    };
 #pragma unroll
     for (uint32_t j = 0; j < kEach; ++j) {
-        e[j] = 0;
-        if (v[j] > -INFINITY && rank_key(v[j], i0 + j) >= cut) {
-            uint32_t b;
-            const uint64_t m = weight(v[j], &b);
-            e[j] = unit(m, b);
-            if (e[j] != 0) last = i0 + j + 1;
-        }
-        run += e[j];
+        const u128 e = drawn(j);
+        if (v[j] > -INFINITY && rank_key(v[j], i0 + j) >= cut) last = e != 0 ? (i0 + j + 1) | kWeighs : (last > kWeighs ? last : i0 + j + 1);
+        run += e;
     }
     const u128 mine = run;
     if (last) atomicMax(&sm.last, last);
     block_scan<kFinWaves>(n, run, &n_all, &ignored, sm.scan);
-    u128 x = run - mine;
-    if (x <= rest && run > rest) {
-#pragma unroll
-        for (uint32_t j = 0; j < kEach; ++j) {
-            if (x <= rest && x + e[j] > rest) sm.id = i0 + j;
-            x += e[j];
-        }
-    }
+    const u128 start = run - mine;
+    if (start <= rest && run > rest) sm.id = t;
     __syncthreads();
     // (the deepest bin's sum may exceed its entries' own by their last bits: the last of them then)
-    const uint32_t id = sm.id != ~0u ? sm.id : sm.last - 1;
-    if (id - i0 < kEach) {
-        u128 drawn = e[0];
+    const bool found = sm.id != ~0u;
+    const uint32_t end = (sm.last & (kWeighs - 1)) - 1;
+    if (t != (found ? sm.id : (end - slice * kSlice) / kEach)) return;
+    u128 x = start, e = 0;
+    uint32_t id = 0;
 #pragma unroll
-        for (uint32_t j = 1; j < kEach; ++j) drawn = id == i0 + j ? e[j] : drawn;
-        a.o.tokens[r] = id;
-        if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(drawn) / to_double(kept)));
-        if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(lo > hi ? st.live : st.count_l + sm.n);
+    for (uint32_t j = 0; j < kEach; ++j) {
+        const u128 y = drawn(j);
+        if (found ? y != 0 && x <= rest : i0 + j == end) e = y, id = i0 + j;
+        x += y;
     }
+    a.o.tokens[r] = id;
+    if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(e) / to_double(kept)));
+    if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(lo > hi ? st.live : st.count_l + sm.n);
 }
 
 template <typename T>
