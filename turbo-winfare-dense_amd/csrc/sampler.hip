@@ -16,6 +16,7 @@
 
 #include <cmath>
 #include <new>
+#include <type_traits>
 
 #include "twd_internal.h"
 #include "twd_sampler.h"
@@ -121,8 +122,12 @@ template <>
 __device__ __forceinline__ float load_logit<float>(const void* row, uint32_t i) {
     return static_cast<const float*>(row)[i];
 }
-struct Bf16 {};
-struct Fp16 {};
+struct Bf16 {
+    static constexpr uint32_t kMasked = 0xFF80u;  // -inf
+};
+struct Fp16 {
+    static constexpr uint32_t kMasked = 0xFC00u;
+};
 template <>
 __device__ __forceinline__ float load_logit<Bf16>(const void* row, uint32_t i) {
     return __uint_as_float(static_cast<uint32_t>(static_cast<const uint16_t*>(row)[i]) << 16);
@@ -139,10 +144,12 @@ constexpr uint32_t kLogitBytes<float> = 4;
 // ---- the four launches -------------------------------------------------------------------------------
 //
 //   slices   every slice of 8,192 entries: its largest rank, and its entries' numbers and weights by bin
-//   limits   per row: the slices' bins added up, and the bins in which the limits cut
+//   limits   per row: the slices' bins added up, the bins in which the limits cut, and every slice's sum under them
 //   collect  every slice: its entries in those bins, onto the row's list
-//   finish   per row: the list in order, the cuts, and the draw
+//   finish   per row: the cuts among the listed entries, and the draw
 //
+// (limits, collect and finish as one block per row measured 78 us instead of 43 us for 64 rows of 262,144: one
+// compute unit reads a row at 30 GB/s or so where all of them read it in 8 us.)
 // A bin is an eighth of an octave of weight. A slice counts from its own largest octave down (its row's is
 // not known yet), 256 bins to a slice, the last one for all that lies deeper; octaves are absolute, so the
 // slices' bins line up. A bin's entries share an octave, so its sum of 37-bit weights is one integer; the
@@ -203,20 +210,40 @@ struct SampleArgs {
     Exp2Poly poly;
 };
 
-// 16 bytes of logits from any address (the hardware splits an unaligned load itself).
+// 16 bytes of logits from any address (the hardware splits an unaligned load itself): entries i .. of a row, moved
+// down to end with the row where they would pass its end. `first`: the first one's index; those under i are the
+// neighbour's. No lane branches and nothing is converted yet, so that the loads of several calls travel together.
+// TINY: rows shorter than a load, which are read one by one.
 template <typename T>
 constexpr uint32_t kVec = 16 / kLogitBytes<T>;
-template <typename T>
-__device__ __forceinline__ void load_vec(const void* row, uint32_t i, uint32_t vocab, float* v) {
-    if (i + kVec<T> <= vocab) {
-        uint32_t w[4];
-        __builtin_memcpy(w, static_cast<const char*>(row) + static_cast<uint64_t>(i) * kLogitBytes<T>, 16);
+struct Vec {
+    uint32_t w[4];
+    uint32_t first;
+};
+template <typename T, bool TINY>
+__device__ __forceinline__ Vec load_vec(const void* row, uint32_t i, uint32_t vocab) {
+    Vec v;
+    if constexpr (TINY) {
+        v.first = i;
 #pragma unroll
-        for (uint32_t j = 0; j < kVec<T>; ++j) v[j] = load_logit<T>(w, j);
+        for (uint32_t j = 0; j < 4; ++j) {
+            uint32_t bits[2];
+#pragma unroll
+            for (uint32_t h = 0; h < kVec<T> / 4; ++h) {
+                const uint32_t e = i + j * (kVec<T> / 4) + h;
+                if constexpr (kLogitBytes<T> == 4) {
+                    bits[h] = e < vocab ? static_cast<const uint32_t*>(row)[e] : 0xFF800000u;
+                } else {
+                    bits[h] = e < vocab ? static_cast<const uint16_t*>(row)[e] : T::kMasked;
+                }
+            }
+            v.w[j] = kLogitBytes<T> == 4 ? bits[0] : bits[0] | bits[kVec<T> / 4 - 1] << 16;
+        }
     } else {
-#pragma unroll
-        for (uint32_t j = 0; j < kVec<T>; ++j) v[j] = i + j < vocab ? load_logit<T>(row, i + j) : -INFINITY;
+        v.first = i < vocab - kVec<T> ? i : vocab - kVec<T>;
+        __builtin_memcpy(v.w, static_cast<const char*>(row) + static_cast<uint64_t>(v.first) * kLogitBytes<T>, 16);
     }
+    return v;
 }
 
 // The bin of a weight counted from octave `top`, and its integer in that bin.
@@ -302,7 +329,7 @@ __device__ __forceinline__ void block_scan(uint32_t& n, u128& w, uint32_t* n_all
 constexpr uint32_t kSliceThreads = 512;
 constexpr uint32_t kCopies = 4;  // of a slice's bins, by lane, so that a wave's equal bins meet less often
 
-template <typename T>
+template <typename T, bool TINY>
 __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs a) {
     __shared__ uint64_t bins[kBins][kCopies];
     __shared__ uint32_t s_key[kSliceThreads / 64], s_bad[kSliceThreads / 64], s_idx;
@@ -312,9 +339,9 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
     constexpr uint32_t kLoads = kSlice / kSliceThreads / kVec<T>, kEach = kLoads * kVec<T>;
     float v[kEach];
     const uint32_t i0 = slice * kSlice + t * kVec<T>;
+    Vec raw[kLoads];
 #pragma unroll
-    for (uint32_t j = 0; j < kLoads; ++j)
-        load_vec<T>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab, v + j * kVec<T>);
+    for (uint32_t j = 0; j < kLoads; ++j) raw[j] = load_vec<T, TINY>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab);
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
     for (uint32_t i = t; i < kBins * kCopies; i += kSliceThreads) bins[i / kCopies][i % kCopies] = 0;
     if (t == 0) s_idx = ~0u;
@@ -322,9 +349,19 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
     float best = -INFINITY;
     uint64_t nan = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; j += 2) {
-        nan |= __ballot(__builtin_isunordered(v[j], v[j + 1]));
-        best = fmaxf(best, fmaxf(v[j], v[j + 1]));
+    for (uint32_t j = 0; j < kLoads; ++j) {
+#pragma unroll
+        for (uint32_t e = 0; e < kVec<T>; ++e) v[j * kVec<T> + e] = load_logit<T>(raw[j].w, e);
+        const uint32_t over = i0 + j * kSliceThreads * kVec<T> - raw[j].first;
+        if (__ballot(over != 0) != 0) {  // the row's end: the neighbour's entries, or none at all
+#pragma unroll
+            for (uint32_t e = 0; e < kVec<T>; ++e) v[j * kVec<T> + e] = e < over ? -INFINITY : v[j * kVec<T> + e];
+        }
+#pragma unroll
+        for (uint32_t e = j * kVec<T>; e < (j + 1) * kVec<T>; e += 2) {
+            nan |= __ballot(__builtin_isunordered(v[e], v[e + 1]));
+            best = fmaxf(best, fmaxf(v[e], v[e + 1]));
+        }
     }
     const uint32_t own = float_key(best);
     uint32_t key = wave_reduce(own, 0u, [](uint32_t x, uint32_t y) { return x > y ? x : y; });
@@ -340,7 +377,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
         uint32_t idx = ~0u;
 #pragma unroll
         for (uint32_t j = kEach; j-- > 0;)
-            if (v[j] == best) idx = i0 + (j / kVec<T>) * kSliceThreads * kVec<T> + j % kVec<T>;
+            if (v[j] == best) idx = raw[j / kVec<T>].first + j % kVec<T>;
         atomicMin(&s_idx, idx);
     }
     const bool weigh = live && bad == 0 && temp > 0.0f;  // a row with a NaN or +inf, and a greedy one, needs no weights
@@ -461,12 +498,10 @@ __device__ __forceinline__ RowHead read_heads(const SampleArgs& a, uint64_t r) {
 }
 
 __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a) {
-    __shared__ uint64_t mass[kRowThreads];
-    __shared__ uint32_t count[kRowThreads], counts[kBins], found[3], s_bin_m, s_tail_n;
+    __shared__ uint64_t mass[kRowThreads], s_rank_m;
+    __shared__ uint32_t count[kRowThreads], counts[kBins], found[3], s_key[4], s_bin_m, s_tail_n;
     __shared__ unsigned long long s_tail;
     __shared__ u128 sums[kBins];
-    __shared__ uint64_t s_rank_m;
-    __shared__ RowState s_st;
     __shared__ ScanMem scan;
     const uint32_t t = threadIdx.x, lane = t % 64, wave = __builtin_amdgcn_readfirstlane(t / 64);
     const uint64_t r = blockIdx.x;
@@ -487,65 +522,78 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         return;
     }
     const Scale c = scale_of(temp);
-    const uint32_t shift = slice_shift(head.own, weight_of(rank_value(best), c).oct, c);
     const double top = weight_of(rank_value(best), c).oct;
-    // Two threads to a bin of the row, every other slice each: a slice's bin 8 `shift` above it. What lies deeper
-    // than the row's last but one bin adds up in that last one.
+    const uint32_t shift = slice_shift(head.own, top, c);
+
+    // ---- the row's bins. Two threads to a bin, every other slice each: a slice's bin 8 `shift` above it. What lies
+    // deeper than the row's last but one bin adds up in that last one.
     const uint64_t* bins = a.s.bins + r * a.s.slices * kBins;
-    const uint32_t bin = t % kBins;
-    constexpr uint32_t kEvery = kRowThreads / kBins, kTurns = kMaxSlices / kEvery;
-    const uint32_t s0 = __builtin_amdgcn_readfirstlane(t / kBins);
-    uint64_t m = 0, tail = 0;
-    uint32_t n_bin = 0, n_tail = 0;
+    {
+        const uint32_t bin = t % kBins;
+        constexpr uint32_t kEvery = kRowThreads / kBins, kTurns = kMaxSlices / kEvery;
+        const uint32_t s0 = __builtin_amdgcn_readfirstlane(t / kBins);
+        uint64_t m = 0, tail = 0;
+        uint32_t n_bin = 0, n_tail = 0;
 #pragma unroll 1
-    for (uint32_t j = 0; j < kTurns && j * kEvery < a.slices; j += 16) {
-        uint64_t x[16], y[16];
+        for (uint32_t j = 0; j < kTurns && j * kEvery < a.slices; j += 16) {
+            uint64_t x[16], y[16];
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-            const uint32_t slice = s0 + (j + i) * kEvery;
-            const uint32_t sh = slice < a.slices ? __builtin_amdgcn_readlane(shift, slice) : kNoSlice;
-            const uint64_t* from = bins + slice * kBins;
-            x[i] = sh != kNoSlice && bin < kTail && bin >= 8 * sh ? from[bin - 8 * sh] : 0;
-            y[i] = sh != kNoSlice && bin + 8 * sh >= kTail ? from[bin] : 0;
-        }
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t slice = s0 + (j + i) * kEvery;
+                const uint32_t sh = __builtin_amdgcn_readlane(shift, slice);  // (kNoSlice past the last)
+                // (every lane loads, so that the loads travel together; what does not count is dropped after)
+                const uint64_t* from = bins + min(slice, a.slices - 1) * kBins;
+                x[i] = from[max(bin, 8 * sh) - 8 * sh];
+                y[i] = 0;
+                if ((bin | 63) + 8 * sh >= kTail) y[i] = from[bin];  // a wave's lanes alike
+            }
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i) {
-            const uint32_t slice = s0 + (j + i) * kEvery;
-            const uint32_t sh = slice < a.slices ? __builtin_amdgcn_readlane(shift, slice) : 0;
-            m += x[i] & kMassMask, n_bin += static_cast<uint32_t>(x[i] >> kCountBit);
-            const uint32_t down = (bin >> 3) + sh - kTailOct;
-            tail += down < 64 ? (y[i] & kMassMask) >> down : 0, n_tail += static_cast<uint32_t>(y[i] >> kCountBit);
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t slice = s0 + (j + i) * kEvery;
+                const uint32_t sh = __builtin_amdgcn_readlane(shift, slice);
+                if (sh == kNoSlice || bin >= kTail || bin < 8 * sh) x[i] = 0;
+                if (sh == kNoSlice || bin + 8 * sh < kTail) y[i] = 0;
+            }
+#pragma unroll
+            for (uint32_t i = 0; i < 16; ++i) {
+                const uint32_t slice = s0 + (j + i) * kEvery;
+                const uint32_t sh = __builtin_amdgcn_readlane(shift, slice);
+                m += x[i] & kMassMask, n_bin += static_cast<uint32_t>(x[i] >> kCountBit);
+                const uint32_t down = (bin >> 3) + sh - kTailOct;
+                tail += down < 64 ? (y[i] & kMassMask) >> down : 0, n_tail += static_cast<uint32_t>(y[i] >> kCountBit);
+            }
         }
+        if (t < 3) found[t] = kBins;
+        if (t == 0) s_rank_m = 0, s_bin_m = kBins, s_tail = 0, s_tail_n = 0;
+        mass[t] = m, count[t] = n_bin;
+        __syncthreads();
+        if (__ballot(n_tail != 0) != 0) {
+            tail = wave_reduce(tail, uint64_t{0}, [](uint64_t p, uint64_t q) { return p + q; });
+            n_tail = wave_reduce(n_tail, 0u, [](uint32_t p, uint32_t q) { return p + q; });
+            if (lane == 0) atomicAdd(&s_tail, static_cast<unsigned long long>(tail)), atomicAdd(&s_tail_n, n_tail);
+        }
+        if (wave == kRowThreads / 64 - 1 && min_p > 0.0f) {
+            const uint64_t rank = least_kept(best, min_p, c);
+            const float l = rank_value(rank);
+            const uint32_t b = l > -INFINITY ? bin_of(weight_of(l, c), top) : kBins;
+            if (lane == 0) s_rank_m = rank, s_bin_m = b;
+        }
+        __syncthreads();
     }
-    if (t < 3) found[t] = kBins;
-    if (t == 0) s_rank_m = 0, s_bin_m = kBins, s_tail = 0, s_tail_n = 0;
-    mass[t] = m, count[t] = n_bin;
-    __syncthreads();
-    if (__ballot(n_tail != 0) != 0) {
-        tail = wave_reduce(tail, uint64_t{0}, [](uint64_t p, uint64_t q) { return p + q; });
-        n_tail = wave_reduce(n_tail, 0u, [](uint32_t p, uint32_t q) { return p + q; });
-        if (lane == 0) atomicAdd(&s_tail, static_cast<unsigned long long>(tail)), atomicAdd(&s_tail_n, n_tail);
-    }
-    if (wave == kRowThreads / 64 - 1 && min_p > 0.0f) {
-        const uint64_t rank = least_kept(best, min_p, c);
-        const float l = rank_value(rank);
-        const uint32_t b = l > -INFINITY ? bin_of(weight_of(l, c), top) : kBins;
-        if (lane == 0) s_rank_m = rank, s_bin_m = b;
-    }
-    __syncthreads();
-    uint32_t n = 0, n_all;
+    uint32_t n = 0, live;
     u128 w = 0, w_all;
     if (t < kBins) {
-        m = t == kTail ? s_tail : 0, n = t == kTail ? s_tail_n : 0;
+        uint64_t m = t == kTail ? s_tail : 0;
+        n = t == kTail ? s_tail_n : 0;
 #pragma unroll
-        for (uint32_t i = 0; i < kEvery; ++i) m += mass[i * kBins + t], n += count[i * kBins + t];
+        for (uint32_t i = 0; i < kRowThreads / kBins; ++i) m += mass[i * kBins + t], n += count[i * kBins + t];
         w = unit(m, t);
     }
-    block_scan<kBins / 64>(n, w, &n_all, &w_all, scan);
-    const uint32_t live = n_all;
+    block_scan<kBins / 64>(n, w, &live, &w_all, scan);
     if (t < kBins) counts[t] = n, sums[t] = w;
     __syncthreads();
-    // the bin each limit cuts in: the first whose running number or sum reaches it
+
+    // ---- the bin each limit cuts in: the first whose running number or sum reaches it
     const uint32_t k = top_k > 0 && static_cast<uint32_t>(top_k) < live ? static_cast<uint32_t>(top_k) : 0;
     const bool use_p = top_p < 1.0f;
     if (k != 0) {
@@ -564,6 +612,8 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         }
         __syncthreads();
     }
+    // lo .. hi: the bins whose entries decide (lo = kBins: none, every live entry is kept); need_k: those of bin_k
+    // do too, for the top-k's sum
     uint32_t lo = kBins, hi = kBins;
     if (use_p)
         lo = found[1], hi = found[2];
@@ -574,116 +624,138 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
     if (bin_m < lo) lo = hi = bin_m, need_k = false;  // the other limits cut deeper
     if (bin_m < hi) hi = bin_m;
     const bool any = lo < kBins;
-    // the keys that bound those bins, a wave each
-    const uint32_t above = static_cast<uint32_t>(best >> 32) + 1;
+    const u128 below_l = any && lo ? sums[lo - 1] : 0, below_k = need_k && bin_k ? sums[bin_k - 1] : 0;
+    const uint32_t count_l = any && lo ? counts[lo - 1] : 0, count_k = need_k && bin_k ? counts[bin_k - 1] : 0;
+    const uint32_t in_l = any ? counts[hi] - count_l : 0, in_k = need_k ? counts[bin_k] - count_k : 0;
+    const uint32_t listed = in_l + (need_k && bin_k > hi ? in_k : 0);
+    
+    // ---- the keys that bound those bins, a wave each, and every slice's sum under them: what the draw starts from.
+    // key[0] .. key[1] - 1: entries of lo .. hi; key[2] .. key[3] - 1: of bin_k
     if (wave < 4) {
+        const uint32_t above = static_cast<uint32_t>(best >> 32) + 1;
         uint32_t key = 0;
         if (wave < 2 ? any : need_k) {
-            const uint32_t b0 = wave < 2 ? lo : bin_k, b1 = wave < 2 ? hi : bin_k;
-            key = wave % 2 == 0 ? bin_key(b1, above, top, c) : (b0 == 0 ? above : bin_key(b0 - 1, above, top, c));
+            const uint32_t b0 = wave < 2 ? lo : bin_k, b1 = wave < 2 ? hi : bin_k, b = wave % 2 == 0 ? b1 : b0 - 1;
+            key = wave % 2 != 0 && b0 == 0 ? above : bin_key(b, above, top, c);
         }
-        if (lane == 0) s_st.key[wave] = key;
+        if (lane == 0) s_key[wave] = key;
     }
-    if (t == kRowThreads - 1) {
-        RowState& st = s_st;
-        st.top = top, st.best = best, st.rank_m = s_rank_m, st.all = w_all, st.live = live, st.k = k, st.use_p = use_p;
-        st.bin_k = need_k ? bin_k : kBins, st.done = 0, st.appended = 0;
-        st.lo = any ? lo : 1, st.hi = any ? hi : 0;
-        st.below_l = any && lo ? sums[lo - 1] : 0, st.count_l = any && lo ? counts[lo - 1] : 0;
-        st.in_l = st.listed = any ? counts[hi] - st.count_l : 0;
-        st.below_k = need_k && bin_k ? sums[bin_k - 1] : 0, st.count_k = need_k && bin_k ? counts[bin_k - 1] : 0;
-        st.in_k = need_k ? counts[bin_k] - st.count_k : 0;
-        if (need_k && bin_k > hi) st.listed += st.in_k;
+#pragma unroll 1
+    for (uint32_t s0 = 0; s0 < a.slices; s0 += kRowThreads / 16) {  // sixteen threads to a slice, sixteen of its bins each
+        const uint32_t slice = s0 + t / 16, sh = __shfl(shift, slice % 64);
+        uint64_t x[16];
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) x[i] = bins[min(slice, a.slices - 1) * kBins + t % 16 + 16 * i];
+        u128 sum = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) {
+            uint32_t down;
+            const uint32_t b = row_bin(t % 16 + 16 * i, sh, &down);
+            if (b < lo && sh != kNoSlice) sum += unit(down < 64 ? (x[i] & kMassMask) >> down : 0, b);
+        }
+        const Halves h = halve(sum);
+        sum = join(Halves{sum_of_16(h.lo), sum_of_16(h.hi)});
+        if (t % 16 == 0 && slice < a.slices) a.s.under[r * a.s.slices + slice] = sum;
     }
     __syncthreads();
-    if (t < sizeof(RowState) / 4) reinterpret_cast<uint32_t*>(a.s.state + r)[t] = reinterpret_cast<const uint32_t*>(&s_st)[t];
+    if (t == 0) {
+        RowState& st = a.s.state[r];
+        st.top = top, st.best = best, st.rank_m = s_rank_m, st.all = w_all, st.live = live, st.k = k, st.use_p = use_p;
+        st.bin_k = need_k ? bin_k : kBins, st.done = 0, st.appended = 0, st.lo = any ? lo : 1, st.hi = any ? hi : 0;
+        st.below_l = below_l, st.count_l = count_l, st.in_l = in_l;
+        st.below_k = below_k, st.count_k = count_k, st.in_k = in_k, st.listed = listed;
+        for (uint32_t i = 0; i < 4; ++i) st.key[i] = s_key[i];
+    }
 }
-static_assert(sizeof(RowState) % 4 == 0 && sizeof(RowState) / 4 <= kRowThreads, "copied by words");
-static_assert(kRowThreads % 64 == 0 && kBins <= kRowThreads, "a thread to a bin");
 
-template <typename T>
+template <typename T, bool TINY>
 __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArgs a) {
     __shared__ uint32_t s_n, s_base;
-    const uint32_t t = threadIdx.x, slice = blockIdx.x;
+    const uint32_t t = threadIdx.x, slice = blockIdx.x, lane = t % 64;
     const uint64_t r = blockIdx.y;
     RowState* st = a.s.state + r;
     const uint32_t listed = st->listed, k0 = st->key[0], k1 = st->key[1], k2 = st->key[2], k3 = st->key[3];
-    const SliceHead h = a.s.head[r * a.s.slices + slice];
-    if (st->done) return;
-    // the slice's sum under the deciding bins: what the draw starts from
-    if (t < 64) {
-        const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
-        const uint32_t lo = st->lo <= st->hi ? st->lo : kBins, sh = slice_shift(h, st->top, scale_of(temp));
-        u128 sum = 0;
-        if (sh != kNoSlice) {
-            const uint64_t* bins = a.s.bins + (r * a.s.slices + slice) * kBins;
-#pragma unroll
-            for (uint32_t i = 0; i < kBins / 64; ++i) {
-                uint32_t down;
-                const uint32_t b = row_bin(64 * i + t, sh, &down);
-                if (b < lo) sum += unit(down < 64 ? (bins[64 * i + t] & kMassMask) >> down : 0, b);
-            }
-        }
-        const Halves x = halve(sum);
-        auto add = [](uint64_t p, uint64_t q) { return p + q; };
-        sum = join(Halves{wave_reduce(x.lo, uint64_t{0}, add), wave_reduce(x.hi, uint64_t{0}, add)});
-        if (t == 0) a.s.under[r * a.s.slices + slice] = sum;
-    }
-    if (listed == 0 || listed > kListCap || h.weighed == 0) return;
-    const uint32_t most = static_cast<uint32_t>(h.best >> 32);
-    if (most < k0 && (k2 == k3 || most < k2)) return;  // all of the slice lies below
+    const uint32_t most = static_cast<uint32_t>(a.s.head[r * a.s.slices + slice].best >> 32);
+    if (listed == 0 || listed > kListCap) return;
+    const bool two = k2 < k3 && k2 < k0;  // a bin_k past lo .. hi
+    if (most < (two ? k2 : k0)) return;   // all of the slice lies below
     if (t == 0) s_n = 0;
-    __syncthreads();
     const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
-    constexpr uint32_t kLoads = kSlice / kSliceThreads / kVec<T>, kEach = kLoads * kVec<T>;
+    constexpr uint32_t kLoads = kSlice / kSliceThreads / kVec<T>;
     const uint32_t i0 = slice * kSlice + t * kVec<T>;
-    float v[kEach];
+    Vec v[kLoads];
 #pragma unroll
-    for (uint32_t j = 0; j < kLoads; ++j) load_vec<T>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab, v + j * kVec<T>);
-    auto decides = [&](uint32_t k) { return k - k0 < k1 - k0 || k - k2 < k3 - k2; };  // (-inf's key lies under all)
-    uint32_t hits = 0;
+    for (uint32_t j = 0; j < kLoads; ++j) v[j] = load_vec<T, TINY>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab);
+    __syncthreads();
+    // the lanes whose entry e of load j decides (keys order as their floats do; -inf lies under all)
+    const float f0 = key_float(k0), f1 = key_float(k1), f2 = key_float(k2), f3 = key_float(k3);
+    uint64_t in[kLoads][kVec<T>];
+    uint32_t number = 0;
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) hits += decides(float_key(v[j])) ? 1u : 0u;
-    uint32_t at = hits ? atomicAdd(&s_n, hits) : 0;
+    for (uint32_t j = 0; j < kLoads; ++j) {
+#pragma unroll
+        for (uint32_t e = 0; e < kVec<T>; ++e) {
+            const float l = load_logit<T>(v[j].w, e);
+            in[j][e] = __ballot(l >= f0) & __ballot(l < f1);
+            if (two) in[j][e] |= __ballot(l >= f2) & __ballot(l < f3);
+        }
+        const uint32_t over = i0 + j * kSliceThreads * kVec<T> - v[j].first;
+        if (__ballot(over != 0) != 0) {  // the row's end: a lane holds its neighbour's entries first
+#pragma unroll
+            for (uint32_t e = 0; e < kVec<T>; ++e) in[j][e] &= __ballot(e >= over);
+        }
+#pragma unroll
+        for (uint32_t e = 0; e < kVec<T>; ++e) number += static_cast<uint32_t>(__builtin_popcountll(in[j][e]));
+    }
+    uint32_t at = 0;
+    if (lane == 0 && number != 0) at = atomicAdd(&s_n, number);
     __syncthreads();
     if (s_n == 0) return;
     if (t == 0) s_base = atomicAdd(&st->appended, s_n);
     __syncthreads();
-    if (hits == 0) return;
-    at += s_base;
+    if (number == 0) return;
+    at = __builtin_amdgcn_readfirstlane(at) + s_base;
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        const uint32_t k = float_key(v[j]);
-        if (!decides(k)) continue;
-        // the bins' own numbers say how many come: the list holds them all
-        if (at < kListCap)
-            a.s.list[r * kListCap + at] =
-                static_cast<uint64_t>(k) << 32 | (0xFFFFFFFFu - (i0 + (j / kVec<T>) * kSliceThreads * kVec<T> + j % kVec<T>));
-        ++at;
+    for (uint32_t j = 0; j < kLoads; ++j) {
+#pragma unroll
+        for (uint32_t e = 0; e < kVec<T>; ++e) {
+            if (in[j][e] == 0) continue;
+            const uint32_t to = at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in[j][e] >> 32),
+                                                              __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in[j][e]), 0));
+            // the bins' own numbers say how many come: the list holds them all
+            if ((in[j][e] >> lane & 1) != 0 && to < kListCap)
+                a.s.list[r * kListCap + to] = rank_key(load_logit<T>(v[j].w, e), v[j].first + e);
+            at += static_cast<uint32_t>(__builtin_popcountll(in[j][e]));
+        }
     }
 }
 
-constexpr uint32_t kFinThreads = 512, kFinWaves = kFinThreads / 64;
-constexpr uint32_t kSmall = 256;          // entries that are ranked against each other directly
-constexpr uint32_t kParts = kFinThreads;  // parts that a range of ranks is cut into
+constexpr uint32_t kSmall = 64;           // entries that are ranked against each other directly
+constexpr uint32_t kParts = kRowThreads;  // parts that a range of ranks is cut into
+constexpr uint32_t kStageEach = kSlice / kRowThreads, kStageStride = kStageEach + 1;  // a thread's entries, an odd way apart
 
 struct FinishMem {
-    uint64_t rank[kListCap];
-    uint64_t weight[kListCap];  // its bin above bit 48, the weight below
+    union {
+        struct {
+            uint64_t rank[kListCap];
+            uint64_t weight[kListCap];  // its bin above bit 48, the weight below
+        };
+        float stage[kRowThreads * kStageStride];
+    };
     uint32_t part_n[kParts];
     unsigned long long part_lo[kParts], part_hi[kParts];
     uint64_t small[kSmall];
     u128 small_w[kSmall];
-    ScanMem scan;
     unsigned long long slice_lo[kMaxSlices], slice_hi[kMaxSlices];
+    ScanMem scan;
     unsigned long long least, most;
     uint64_t cut;
     u128 sum, base_w, want;
     uint32_t n, base_n, pick, id, last;
 };
 
-template <typename T>
-__global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a) {
+template <typename T, bool TINY>
+__global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a) {
     extern __shared__ char finish_mem[];
     FinishMem& sm = *reinterpret_cast<FinishMem*>(finish_mem);
     const uint32_t t = threadIdx.x, lane = t % 64;
@@ -692,13 +764,13 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
     const uint32_t done = st.done, listed = st.listed;
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f, u = a.p.uniform[r];
     const float top_p = a.p.top_p ? a.p.top_p[r] : 1.0f;
-    const u128 under = t < a.slices ? a.s.under[r * a.s.slices + t] : 0;
-    const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
+    const u128 under = a.s.under[r * a.s.slices + min(t, a.slices - 1)];
     if (done) return;
+    const void* row = static_cast<const char*>(a.logits) + r * a.stride * kLogitBytes<T>;
     const Scale c = scale_of(temp);
     const double top = st.top;
-    const uint32_t lo = st.lo, hi = st.hi;
-    const bool on_list = listed <= kListCap;
+    const uint32_t lo = st.lo, hi = st.hi, k = st.k, bin_k = st.bin_k;
+    const bool on_list = listed <= kListCap, any = lo <= hi, use_p = st.use_p != 0, need_k = bin_k < kBins;
     auto weight = [&](float l, uint32_t* bin) {
         const Weight w = weight_of(l, c);
         *bin = bin_of(w, top);
@@ -707,30 +779,31 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
     if (t < kMaxSlices) sm.slice_lo[t] = 0, sm.slice_hi[t] = 0;
     if (t == 0) sm.last = 0, sm.id = ~0u;
     if (on_list) {
-        for (uint32_t i = t; i < listed; i += kFinThreads) {
-            const uint64_t k = a.s.list[r * kListCap + i];
+#pragma unroll 1
+        for (uint32_t i = t; i < listed; i += kRowThreads) {
+            const uint64_t rank = a.s.list[r * kListCap + i];
             uint32_t b;
-            const uint64_t m = weight(rank_value(k), &b);
-            sm.rank[i] = k, sm.weight[i] = static_cast<uint64_t>(b) << 48 | m;
+            const uint64_t m = weight(rank_value(rank), &b);
+            sm.rank[i] = rank, sm.weight[i] = static_cast<uint64_t>(b) << 48 | m;
         }
     }
     // f(rank, bin, weight) of every entry in the row's bins b0 .. b1: from the list, or, where equal or nearly
     // equal logits are too many for it, from the row. (A thread meets the same entries of the list each time.)
     auto members = [&](uint32_t b0, uint32_t b1, auto f) {
-        if (on_list) {
-            for (uint32_t i = t; i < listed; i += kFinThreads) {
+        const uint32_t end = on_list ? listed : a.vocab;
+#pragma unroll 1
+        for (uint32_t i = t; i < end; i += kRowThreads) {
+            uint64_t rank, m;
+            uint32_t b;
+            if (on_list) {
                 const uint64_t x = sm.weight[i];
-                const uint32_t b = static_cast<uint32_t>(x >> 48);
-                if (b >= b0 && b <= b1) f(sm.rank[i], b, x & 0xFFFFFFFFFFFFull);
-            }
-        } else {
-            for (uint32_t i = t; i < a.vocab; i += kFinThreads) {
+                rank = sm.rank[i], b = static_cast<uint32_t>(x >> 48), m = x & 0xFFFFFFFFFFFFull;
+            } else {
                 const float l = load_logit<T>(row, i);
                 if (!(l > -INFINITY)) continue;
-                uint32_t b;
-                const uint64_t m = weight(l, &b);
-                if (b >= b0 && b <= b1) f(rank_key(l, i), b, m);
+                rank = rank_key(l, i), m = weight(l, &b);
             }
+            if (b >= b0 && b <= b1) f(rank, b, m);
         }
     };
     // Among the entries of bins b0 .. b1, `have` of them, ranks r0 .. r1, with base_n entries of sum base_w before
@@ -742,35 +815,36 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
         for (bool first = true;; first = false) {
             __syncthreads();
             if (t == 0) sm.n = 0, sm.least = ~0ull, sm.most = 0, sm.cut = 0, sm.sum = 0, sm.pick = kParts;
-            sm.part_n[t] = 0, sm.part_lo[t] = 0, sm.part_hi[t] = 0;
-            __syncthreads();
             if (have <= kSmall) {
+                __syncthreads();
                 members(b0, b1, [&](uint64_t k, uint32_t b, uint64_t m) {
                     if (k < r0 || k > r1) return;
                     const uint32_t at = atomicAdd(&sm.n, 1u);
                     if (at < kSmall) sm.small[at] = k, sm.small_w[at] = unit(m, b);
                 });
                 __syncthreads();
-                // two threads to an entry add up those of larger rank
-                const uint32_t e = t / 2;
+                // eight threads to an entry add up those of larger rank
+                const uint32_t e = t / 8;
                 if (e < have) {
                     const uint64_t mine = sm.small[e];
                     uint32_t more = 0;
                     u128 over = 0;
-                    for (uint32_t i = t % 2; i < have; i += 2) {
+                    for (uint32_t i = t % 8; i < have; i += 8) {
                         const bool larger = sm.small[i] > mine;
                         more += larger ? 1u : 0u;
                         over += larger ? sm.small_w[i] : 0;
                     }
-                    more += __shfl_xor(more, 1);
-                    over += shfl_xor_u128(over, 1);
+#pragma unroll
+                    for (int d = 1; d < 8; d *= 2) more += __shfl_xor(more, d), over += shfl_xor_u128(over, d);
                     const u128 before = base_w + over, with = before + sm.small_w[e];
-                    if (t % 2 == 0 && (by_sum ? before < w && with >= w : base_n + more + 1 == n)) sm.cut = mine, sm.sum = with;
+                    if (t % 8 == 0 && (by_sum ? before < w && with >= w : base_n + more + 1 == n)) sm.cut = mine, sm.sum = with;
                 }
                 __syncthreads();
                 *sum = sm.sum;
                 return sm.cut;
             }
+            sm.part_n[t] = 0, sm.part_lo[t] = 0, sm.part_hi[t] = 0;
+            __syncthreads();
             if (!first) {  // equal logits: their ranks fill little of the range
                 uint64_t least = ~0ull, most = 0;
                 members(b0, b1, [&](uint64_t k, uint32_t, uint64_t) {
@@ -790,9 +864,10 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
                 if (k < r0 || k > r1) return;
                 const uint32_t d = kParts - 1 - static_cast<uint32_t>((k - r0) >> sft);  // falling
                 const Halves x = halve(unit(m, b));
-                // Equal logits meet in one part: where a wave's first entry has company, the lanes that hold its part
+                // Equal logits meet in one part: while a wave's first entry has company, the lanes that hold its part
                 // and its weight add up as one.
                 bool todo = true;
+#pragma unroll 1
                 for (uint32_t turn = 0; turn < 16; ++turn) {
                     const uint32_t d0 = __builtin_amdgcn_readfirstlane(d);
                     const uint64_t m0 = static_cast<uint64_t>(__builtin_amdgcn_readfirstlane(static_cast<uint32_t>(m >> 32))) << 32 |
@@ -821,7 +896,7 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
             const u128 own = join(Halves{sm.part_lo[t], sm.part_hi[t]});
             uint32_t x = own_n, x_all;
             u128 y = own, y_all;
-            block_scan<kFinWaves>(x, y, &x_all, &y_all, sm.scan);
+            block_scan<kRowWaves>(x, y, &x_all, &y_all, sm.scan);
             if (own_n != 0 && (by_sum ? base_w + y >= w && base_w + y - own < w : base_n + x >= n && base_n + x - own_n < n))
                 sm.pick = t, sm.n = own_n, sm.base_n = base_n + x - own_n, sm.base_w = base_w + y - own;
             __syncthreads();
@@ -835,24 +910,22 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
         }
     };
 
-    // top-k's cut by number, then top-p's by its share of the top-k's sum
+    // ---- top-k's cut by number, then top-p's by its share of the top-k's sum
     uint64_t cut = 0;  // ranks of at least this are kept
     u128 sum = st.all;
 #pragma unroll 1
     for (int by_sum = 0; by_sum < 2; ++by_sum) {
-        const bool in_k = by_sum == 0 && st.bin_k < kBins;
+        const bool for_k = by_sum == 0 && need_k;
         const u128 want = by_sum ? part_of(top_p, sum, true) : 0;
-        if (by_sum ? !st.use_p : (st.use_p ? !in_k : st.k == 0)) continue;
+        if (by_sum ? !use_p : (use_p ? !for_k : k == 0)) continue;
         uint64_t x = st.best;
-        if (in_k || (lo <= hi && (by_sum == 0 || want > 0))) {
-            const uint32_t key0 = st.key[in_k ? 2 : 0], key1 = st.key[in_k ? 3 : 1];
+        if (for_k || by_sum == 0 || want > 0) {
+            const uint32_t key0 = st.key[for_k ? 2 : 0], key1 = st.key[for_k ? 3 : 1];
             u128 with;
-            x = select(in_k ? st.bin_k : lo, in_k ? st.bin_k : hi, in_k ? st.in_k : st.in_l, static_cast<uint64_t>(key0) << 32,
-                       (static_cast<uint64_t>(key1) << 32) - 1, in_k ? st.count_k : st.count_l,
-                       in_k ? st.below_k : st.below_l, by_sum != 0, st.k, want, &with);
+            x = select(for_k ? bin_k : lo, for_k ? bin_k : hi, for_k ? st.in_k : st.in_l, static_cast<uint64_t>(key0) << 32,
+                       (static_cast<uint64_t>(key1) << 32) - 1, for_k ? st.count_k : st.count_l, for_k ? st.below_k : st.below_l,
+                       by_sum != 0, k, want, &with);
             if (by_sum == 0) sum = with;
-        } else if (lo > hi) {
-            x = 0;
         }
         cut = x > cut ? x : cut;
     }
@@ -862,7 +935,7 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
     __syncthreads();
     if (t == 0) sm.n = 0;
     __syncthreads();
-    if (lo <= hi) {
+    if (any) {
         members(lo, hi, [&](uint64_t k, uint32_t b, uint64_t m) {
             if (k < cut) return;
             const Halves x = halve(unit(m, b));
@@ -881,59 +954,81 @@ __global__ __launch_bounds__(kFinThreads) void sample_finish_kernel(SampleArgs a
     const u128 want = u < 1.0f ? part_of(u, kept, false) : kept - 1;  // the first running sum past this is drawn
     if (t < a.slices && w > want && w - own <= want) sm.pick = t, sm.want = want - (w - own);
     __syncthreads();
-    const uint32_t slice = sm.pick;
+    const uint32_t first = sm.pick * kSlice;
     const u128 rest = sm.want;
-    constexpr uint32_t kEach = kSlice / kFinThreads;
-    u128 run = 0, ignored;
-    const uint32_t i0 = slice * kSlice + kEach * t;
-    constexpr uint32_t kWeighs = 1u << 20;  // above every index
-    uint32_t last = 0;
-    float v[kEach];
-    static_assert(kEach % kVec<T> == 0, "whole loads");
+    // the slice through LDS: read in rows, summed by thread
+    Vec part[kStageEach / kVec<T>];
 #pragma unroll
-    for (uint32_t j = 0; j < kEach; j += kVec<T>) load_vec<T>(row, i0 + j, a.vocab, v + j);
-    auto drawn = [&](uint32_t j) -> u128 {
-        if (!(v[j] > -INFINITY && rank_key(v[j], i0 + j) >= cut)) return 0;
+    for (uint32_t j = 0; j < kStageEach / kVec<T>; ++j) part[j] = load_vec<T, TINY>(row, first + (j * kRowThreads + t) * kVec<T>, a.vocab);
+#pragma unroll
+    for (uint32_t j = 0; j < kStageEach / kVec<T>; ++j) {
+        const uint32_t i = (j * kRowThreads + t) * kVec<T>, over = first + i - part[j].first;
+#pragma unroll
+        for (uint32_t e = 0; e < kVec<T>; ++e) {
+            // a lane at the row's end holds entries from `over` under its own on: it drops them and masks the rest
+            const uint32_t to = e >= over ? i + e - over : i + kVec<T> - 1 - e;
+            sm.stage[to / kStageEach * kStageStride + to % kStageEach] = e >= over ? load_logit<T>(part[j].w, e) : -INFINITY;
+        }
+    }
+    __syncthreads();
+    constexpr uint32_t kWeighs = 1u << 20;  // above every index
+    const uint32_t i0 = first + kStageEach * t;
+    auto drawn = [&](uint32_t j, bool* keeps) -> u128 {
+        const float l = sm.stage[t * kStageStride + j];
+        *keeps = l > -INFINITY && rank_key(l, i0 + j) >= cut;
+        if (!*keeps) return 0;
         uint32_t b;
-        const uint64_t m = weight(v[j], &b);
+        const uint64_t m = weight(l, &b);
         return unit(m, b);
     };
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        const u128 e = drawn(j);
-        if (v[j] > -INFINITY && rank_key(v[j], i0 + j) >= cut) last = e != 0 ? (i0 + j + 1) | kWeighs : (last > kWeighs ? last : i0 + j + 1);
+    u128 run = 0;
+    uint32_t last = 0;
+#pragma unroll 2
+    for (uint32_t j = 0; j < kStageEach; ++j) {
+        bool keeps;
+        const u128 e = drawn(j, &keeps);
+        if (keeps) last = e != 0 ? (i0 + j + 1) | kWeighs : (last > kWeighs ? last : i0 + j + 1);
         run += e;
     }
     const u128 mine = run;
-    if (last) atomicMax(&sm.last, last);
-    block_scan<kFinWaves>(n, run, &n_all, &ignored, sm.scan);
+    last = wave_reduce(last, 0u, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
+    if (lane == 0 && last != 0) atomicMax(&sm.last, last);
+    u128 ignored;
+    block_scan<kRowWaves>(n, run, &n_all, &ignored, sm.scan);
     const u128 start = run - mine;
     if (start <= rest && run > rest) sm.id = t;
     __syncthreads();
     // (the deepest bin's sum may exceed its entries' own by their last bits: the last of them then)
     const bool found = sm.id != ~0u;
     const uint32_t end = (sm.last & (kWeighs - 1)) - 1;
-    if (t != (found ? sm.id : (end - slice * kSlice) / kEach)) return;
+    if (t != (found ? sm.id : (end - first) / kStageEach)) return;
     u128 x = start, e = 0;
     uint32_t id = 0;
-#pragma unroll
-    for (uint32_t j = 0; j < kEach; ++j) {
-        const u128 y = drawn(j);
+#pragma unroll 1
+    for (uint32_t j = 0; j < kStageEach; ++j) {
+        bool keeps;
+        const u128 y = drawn(j, &keeps);
         if (found ? y != 0 && x <= rest : i0 + j == end) e = y, id = i0 + j;
         x += y;
     }
     a.o.tokens[r] = id;
     if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(e) / to_double(kept)));
-    if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(lo > hi ? st.live : st.count_l + sm.n);
+    if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(any ? st.count_l + sm.n : st.live);
 }
+static_assert(kBins <= kRowThreads && kMaxSlices <= 64, "a thread to a bin, a lane to a slice");
 
 template <typename T>
 void launch(const SampleArgs& a, uint32_t rows, hipStream_t s) {
-    const dim3 grid(a.slices, rows);
-    sample_slices_kernel<T><<<grid, kSliceThreads, 0, s>>>(a);
-    sample_limits_kernel<<<rows, kRowThreads, 0, s>>>(a);
-    sample_collect_kernel<T><<<grid, kSliceThreads, 0, s>>>(a);
-    sample_finish_kernel<T><<<rows, kFinThreads, sizeof(FinishMem), s>>>(a);
+    const auto all = [&](auto tiny) {
+        sample_slices_kernel<T, decltype(tiny)::value><<<dim3(a.slices, rows), kSliceThreads, 0, s>>>(a);
+        sample_limits_kernel<<<rows, kRowThreads, 0, s>>>(a);
+        sample_collect_kernel<T, decltype(tiny)::value><<<dim3(a.slices, rows), kSliceThreads, 0, s>>>(a);
+        sample_finish_kernel<T, decltype(tiny)::value><<<rows, kRowThreads, sizeof(FinishMem), s>>>(a);
+    };
+    if (a.vocab < kVec<T>)
+        all(std::true_type{});
+    else
+        all(std::false_type{});
 }
 
 }  // namespace
@@ -965,12 +1060,15 @@ TWD_API int twd_sampler_create(uint32_t max_vocab, uint32_t max_rows, twd_sample
     s->max_vocab = max_vocab, s->max_rows = max_rows, s->device = dev;
     const uint64_t slices = (max_vocab + kSlice - 1) / kSlice, rows = max_rows;
     const uint64_t bins = rows * slices * kBins * sizeof(uint64_t), list = rows * kListCap * sizeof(uint64_t);
-    const uint64_t under = rows * slices * sizeof(u128), states = (rows * sizeof(RowState) + 255) / 256 * 256;
+    const uint64_t under = rows * slices * sizeof(u128), states = rows * sizeof(RowState);
     const uint64_t heads = rows * slices * sizeof(SliceHead);
     hipError_t e = hipSuccess;
-    for (const void* f : {reinterpret_cast<const void*>(sample_finish_kernel<float>),
-                          reinterpret_cast<const void*>(sample_finish_kernel<Bf16>),
-                          reinterpret_cast<const void*>(sample_finish_kernel<Fp16>)})
+    for (const void* f : {reinterpret_cast<const void*>(sample_finish_kernel<float, false>),
+                          reinterpret_cast<const void*>(sample_finish_kernel<Bf16, false>),
+                          reinterpret_cast<const void*>(sample_finish_kernel<Fp16, false>),
+                          reinterpret_cast<const void*>(sample_finish_kernel<float, true>),
+                          reinterpret_cast<const void*>(sample_finish_kernel<Bf16, true>),
+                          reinterpret_cast<const void*>(sample_finish_kernel<Fp16, true>)})
         if (e == hipSuccess)
             e = hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(sizeof(FinishMem)));
     if (e == hipSuccess) e = hipMalloc(&s->block, bins + list + under + states + heads);
