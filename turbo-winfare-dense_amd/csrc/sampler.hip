@@ -281,6 +281,14 @@ __device__ __forceinline__ uint64_t wave_incl_scan_u64(uint64_t x) {
     x += dpp_move<0x143, 0xC>(uint64_t{0}, x);
     return x;
 }
+// The same inside each row of 16 lanes.
+__device__ __forceinline__ uint64_t row_incl_scan_u64(uint64_t x) {
+    x += dpp_move<0x111>(uint64_t{0}, x);
+    x += dpp_move<0x112>(uint64_t{0}, x);
+    x += dpp_move<0x114>(uint64_t{0}, x);
+    x += dpp_move<0x118>(uint64_t{0}, x);
+    return x;
+}
 // The sum over a row of 16 lanes, in each of them.
 __device__ __forceinline__ uint64_t sum_of_16(uint64_t x) {
     x += dpp_move<0xB1>(uint64_t{0}, x);
@@ -972,22 +980,23 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     }
     __syncthreads();
     constexpr uint32_t kWeighs = 1u << 20;  // above every index
-    const uint32_t i0 = first + kStageEach * t;
-    auto drawn = [&](uint32_t j, bool* keeps) -> u128 {
-        const float l = sm.stage[t * kStageStride + j];
-        *keeps = l > -INFINITY && rank_key(l, i0 + j) >= cut;
-        if (!*keeps) return 0;
+    // the weight of entry j of thread `by`, where it is kept
+    auto drawn = [&](uint32_t by, uint32_t j, float l) -> u128 {
+        if (!(l > -INFINITY) || rank_key(l, first + kStageEach * by + j) < cut) return 0;
         uint32_t b;
         const uint64_t m = weight(l, &b);
         return unit(m, b);
     };
+    const float floor_l = key_float(static_cast<uint32_t>(cut >> 32));  // (NaN for no cut: nothing lies below it)
     u128 run = 0;
     uint32_t last = 0;
-#pragma unroll 2
+#pragma unroll 1
     for (uint32_t j = 0; j < kStageEach; ++j) {
-        bool keeps;
-        const u128 e = drawn(j, &keeps);
-        if (keeps) last = e != 0 ? (i0 + j + 1) | kWeighs : (last > kWeighs ? last : i0 + j + 1);
+        const float l = sm.stage[t * kStageStride + j];
+        if (__ballot(l > -INFINITY && !(l < floor_l)) == 0) continue;
+        const u128 e = drawn(t, j, l);
+        const uint32_t i = first + kStageEach * t + j;
+        if (l > -INFINITY && rank_key(l, i) >= cut) last = e != 0 ? (i + 1) | kWeighs : (last > kWeighs ? last : i + 1);
         run += e;
     }
     const u128 mine = run;
@@ -996,24 +1005,24 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     u128 ignored;
     block_scan<kRowWaves>(n, run, &n_all, &ignored, sm.scan);
     const u128 start = run - mine;
-    if (start <= rest && run > rest) sm.id = t;
+    if (start <= rest && run > rest) sm.id = t, sm.want = rest - start;
     __syncthreads();
-    // (the deepest bin's sum may exceed its entries' own by their last bits: the last of them then)
+    // One thread's sixteen entries hold it: a lane to each. (The deepest bin's sum may exceed its entries' own by
+    // their last bits: the last of them then.)
+    static_assert(kStageEach == 16, "a row of lanes");
+    if (t >= kStageEach) return;
     const bool found = sm.id != ~0u;
-    const uint32_t end = (sm.last & (kWeighs - 1)) - 1;
-    if (t != (found ? sm.id : (end - first) / kStageEach)) return;
-    u128 x = start, e = 0;
-    uint32_t id = 0;
-#pragma unroll 1
-    for (uint32_t j = 0; j < kStageEach; ++j) {
-        bool keeps;
-        const u128 y = drawn(j, &keeps);
-        if (found ? y != 0 && x <= rest : i0 + j == end) e = y, id = i0 + j;
-        x += y;
+    const uint32_t end = (sm.last & (kWeighs - 1)) - 1, by = found ? sm.id : (end - first) / kStageEach;
+    const uint32_t id = first + kStageEach * by + t;
+    const u128 e = drawn(by, t, sm.stage[by * kStageStride + t]);
+    Halves h = halve(e);
+    h.lo = row_incl_scan_u64(h.lo), h.hi = row_incl_scan_u64(h.hi);
+    const u128 upto = join(h);
+    if (found ? upto > sm.want && upto - e <= sm.want : id == end) {
+        a.o.tokens[r] = id;
+        if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(e) / to_double(kept)));
+        if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(any ? st.count_l + sm.n : st.live);
     }
-    a.o.tokens[r] = id;
-    if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(e) / to_double(kept)));
-    if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(any ? st.count_l + sm.n : st.live);
 }
 static_assert(kBins <= kRowThreads && kMaxSlices <= 64, "a thread to a bin, a lane to a slice");
 
