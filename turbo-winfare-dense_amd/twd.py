@@ -730,36 +730,64 @@ class LMHead:
 F32, BF16, F16 = 0, 1, 2
 
 
+_torch_types: dict = {}  # torch dtype -> TWD_F32, TWD_BF16, TWD_F16
+
+
 def _type_of(t, what: str) -> int:
-    import torch
-    code = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}.get(t.dtype)
+    if not _torch_types:
+        import torch
+        _torch_types.update({torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16})
+    code = _torch_types.get(t.dtype)
     if code is None:
         raise ValueError(f"{what} must be float32, bfloat16 or float16, not {t.dtype}")
     return code
 
 
+class _Here:
+    """No change of device."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_here = _Here()
+
+
 def _on_device(*tensors):
     """A guard that makes the tensors' one device the current one for the call."""
     import torch
-    dev = tensors[0].device
+    dev = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"tensors on {dev} and {t.device} in one call")
-    if dev.type != "cuda":
-        raise ValueError(f"device tensors are needed, not tensors on {dev}")
-    return torch.cuda.device(dev)
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"tensors on {tensors[0].device} and {t.device} in one call")
+    if dev < 0:
+        raise ValueError(f"device tensors are needed, not tensors on {tensors[0].device}")
+    return _here if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+
+
+def _stream_on(t, stream=None):
+    """The stream given, or the current one of the tensor's device (which the guard made the current device)."""
+    if stream is not None:
+        return stream
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a tenth of the time of current_stream()
+    return raw(t.get_device()) if raw is not None else torch.cuda.current_stream(t.device).cuda_stream
 
 
 def _matrix(t, what: str):
     """(rows, cols, row stride) of a 2-D tensor whose columns are adjacent."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError(f"{what} must be two-dimensional with adjacent columns")
-    return t.shape[0], t.shape[1], t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    return shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1]
 
 
 def _buffer(t, shape, dtype, what: str):
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {tuple(shape)}")
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {dtype} tensor of shape {shape}")
     return t
 
 
@@ -772,11 +800,14 @@ def mx_quantize(x, codes=None, scales=None, stream=None):
     with _on_device(x, codes, scales):
         if codes is None:
             codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
+        else:
+            _buffer(codes, (rows, cols // 2), torch.uint8, "codes")
         if scales is None:
             scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
-        _buffer(codes, (rows, cols // 2), torch.uint8, "codes")
-        _buffer(scales, (rows, cols // 32), torch.uint8, "scales")
-        _check(lib.twd_mx_quantize(_ptr(x), kind, rows, cols, stride, _ptr(codes), _ptr(scales), _stream(stream)))
+        else:
+            _buffer(scales, (rows, cols // 32), torch.uint8, "scales")
+        _check(lib.twd_mx_quantize(x.data_ptr(), kind, rows, cols, stride, codes.data_ptr(), scales.data_ptr(),
+                                   _stream_on(x, stream)))
     return codes, scales
 
 
@@ -789,12 +820,12 @@ def mx_dequantize(codes, scales, dtype=None, out=None, stream=None):
     with _on_device(codes, scales, out):
         if out is None:
             out = torch.empty(rows, 2 * half, dtype=dtype or torch.bfloat16, device=codes.device)
-        elif tuple(out.shape) != (rows, 2 * half) or (dtype is not None and out.dtype != dtype):
+        elif out.shape != (rows, 2 * half) or (dtype is not None and out.dtype != dtype):
             raise ValueError(f"out must be of shape {(rows, 2 * half)} and of dtype, where that is given")
         kind = _type_of(out, "out")
         _, _, stride = _matrix(out, "out")
-        _check(lib.twd_mx_dequantize(_ptr(codes), _ptr(scales), rows, 2 * half, _ptr(out), kind, stride,
-                                     _stream(stream)))
+        _check(lib.twd_mx_dequantize(codes.data_ptr(), scales.data_ptr(), rows, 2 * half, out.data_ptr(), kind, stride,
+                                     _stream_on(codes, stream)))
     return out
 
 
@@ -811,8 +842,8 @@ class MxHead:
         _buffer(scales, (vocab, half // 16), torch.uint8, "scales")
         h = C.c_void_p()
         with _on_device(codes, scales):
-            _check(lib.twd_mxhead_create(_ptr(codes), _ptr(scales), vocab, 2 * half, softcap, _stream(stream),
-                                         C.byref(h)))
+            _check(lib.twd_mxhead_create(_ptr(codes), _ptr(scales), vocab, 2 * half, softcap,
+                                         _stream_on(codes, stream), C.byref(h)))
         self.handle = h
         self.device = codes.device
         self.vocab, self.d_model, self.softcap = vocab, 2 * half, softcap
@@ -841,7 +872,7 @@ class MxHead:
         import torch
         if out is None:
             out = torch.empty(rows, self.vocab, dtype=torch.float32, device=self.device)
-        if tuple(out.shape) != (rows, self.vocab):
+        if out.shape != (rows, self.vocab):
             raise ValueError(f"out must be of shape {(rows, self.vocab)}")
         return out, _type_of(out, "out"), _matrix(out, "out")[2]
 
@@ -854,8 +885,8 @@ class MxHead:
             raise ValueError(f"hidden must be bfloat16 [rows, {self.d_model}]")
         with _on_device(hidden, out):
             out, kind, out_stride = self._out(rows, out)
-            _check(lib.twd_mxhead_logits(self.handle, _ptr(hidden), rows, stride, _ptr(out), kind, out_stride,
-                                         _stream(stream)))
+            _check(lib.twd_mxhead_logits(self.handle, hidden.data_ptr(), rows, stride, out.data_ptr(), kind, out_stride,
+                                         _stream_on(hidden, stream)))
         return out
 
     def logits_mx(self, codes, scales, out=None, stream=None):
@@ -866,8 +897,8 @@ class MxHead:
         _buffer(scales, (rows, self.d_model // 32), torch.uint8, "scales")
         with _on_device(codes, scales, out):
             out, kind, out_stride = self._out(rows, out)
-            _check(lib.twd_mxhead_logits_mx(self.handle, _ptr(codes), _ptr(scales), rows, _ptr(out), kind,
-                                            out_stride, _stream(stream)))
+            _check(lib.twd_mxhead_logits_mx(self.handle, codes.data_ptr(), scales.data_ptr(), rows, out.data_ptr(), kind,
+                                            out_stride, _stream_on(codes, stream)))
         return out
 
 
@@ -902,18 +933,19 @@ class Sampler:
         kind = _type_of(logits, "logits")
         rows, vocab, stride = _matrix(logits, "logits")
         with _on_device(logits, uniform, temperature, top_k, top_p, min_p, tokens, logprobs, kept):
+            one = (rows,)
             for t, what in ((uniform, "uniform"), (temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"),
                             (logprobs, "logprobs")):
                 if t is not None:
-                    _buffer(t, (rows,), torch.float32, what)
+                    _buffer(t, one, torch.float32, what)
             for t, what in ((top_k, "top_k"), (tokens, "tokens"), (kept, "kept")):
                 if t is not None:
-                    _buffer(t, (rows,), torch.int32, what)
+                    _buffer(t, one, torch.int32, what)
             if tokens is None:
                 tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
-            _check(lib.twd_sampler_sample(self.handle, _ptr(logits), kind, vocab, rows, stride, _ptr(temperature),
+            _check(lib.twd_sampler_sample(self.handle, logits.data_ptr(), kind, vocab, rows, stride, _ptr(temperature),
                                           _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(tokens),
-                                          _ptr(logprobs), _ptr(kept), _stream(stream)))
+                                          _ptr(logprobs), _ptr(kept), _stream_on(logits, stream)))
         return tokens
 
 
