@@ -62,15 +62,6 @@ struct Eight<float> {
             for (int i = 0; i < 8; ++i) v[i] = p[i];
         }
     }
-    __device__ static void store(float* p, bool wide, const float* v) {
-        if (wide) {
-            reinterpret_cast<f32x4_t*>(p)[0] = f32x4_t{v[0], v[1], v[2], v[3]};
-            reinterpret_cast<f32x4_t*>(p)[1] = f32x4_t{v[4], v[5], v[6], v[7]};
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) p[i] = v[i];
-        }
-    }
 };
 struct Bf16 {
     uint16_t u;
@@ -106,18 +97,6 @@ struct Eight {
             const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = half_to_f32<T>(q[i]);
-        }
-    }
-    __device__ static void store(T* p, bool wide, const float* v) {
-        if (wide) {
-            u32x4_t a;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) a[i] = f32_to_half<T>(v[2 * i]) | (f32_to_half<T>(v[2 * i + 1]) << 16);
-            *reinterpret_cast<u32x4_t*>(p) = a;
-        } else {
-            uint16_t* q = reinterpret_cast<uint16_t*>(p);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = static_cast<uint16_t>(f32_to_half<T>(v[i]));
         }
     }
 };
@@ -179,28 +158,50 @@ struct DequantArgs {
     const uint8_t* codes;
     const uint8_t* scales;
     uint64_t rows;
-    uint32_t groups;
+    uint32_t pieces;  // of 16 bytes of values in a row
     void* out;
     uint64_t stride;
-    bool wide;
+    bool wide;  // rows start at multiples of 16 bytes
 };
 
 // The magnitude bits c as a float's exponent and first mantissa bit are the element's value times
 // 2^-126 (a subnormal float for 0.5), so one exact product by 2^126 decodes it.
+__device__ __forceinline__ float decode(uint32_t c, float s) {
+    return __uint_as_float(((c & 7u) << 22) | ((c & 8u) << 28)) * 0x1p126f * s;
+}
+
+// A lane writes 16 bytes, so that a wave's store fills whole lines; the pass is bound by them, and they are not
+// read here again.
 template <typename T>
 __global__ __launch_bounds__(kQuantThreads) void mx_dequantize_kernel(DequantArgs a) {
+    constexpr uint32_t kEach = 16 / sizeof(T);
     const uint32_t g = blockIdx.x * kQuantThreads + threadIdx.x;
-    if (g >= a.groups) return;
+    if (g >= a.pieces) return;
     for (uint64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
-        const uint32_t w = reinterpret_cast<const uint32_t*>(a.codes)[r * a.groups + g];
-        const float s = scale_value(a.scales[r * (a.groups / 4) + g / 4]);
-        float v[8];
+        const uint64_t at = r * a.pieces + g;
+        const uint32_t w = kEach == 8 ? reinterpret_cast<const uint32_t*>(a.codes)[at] : reinterpret_cast<const uint16_t*>(a.codes)[at];
+        const float s = scale_value(a.scales[at * kEach / kMxBlock]);
+        float v[kEach];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const uint32_t c = w >> (4 * i);
-            v[i] = __uint_as_float(((c & 7u) << 22) | ((c & 8u) << 28)) * 0x1p126f * s;
+        for (uint32_t i = 0; i < kEach; ++i) v[i] = decode(w >> (4 * i), s);
+        T* out = static_cast<T*>(a.out) + r * a.stride + kEach * g;
+        u32x4_t bits;
+        if constexpr (kEach == 8) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) bits[i] = f32_to_half<T>(v[2 * i]) | (f32_to_half<T>(v[2 * i + 1]) << 16);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) bits[i] = __float_as_uint(v[i]);
         }
-        Eight<T>::store(static_cast<T*>(a.out) + r * a.stride + 8ull * g, a.wide, v);
+        if (a.wide) {
+            __builtin_nontemporal_store(bits, reinterpret_cast<u32x4_t*>(out));
+        } else if constexpr (kEach == 8) {
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) reinterpret_cast<uint16_t*>(out)[i] = static_cast<uint16_t>(bits[i / 2] >> (16 * (i % 2)));
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(out)[i] = bits[i];
+        }
     }
 }
 
@@ -797,11 +798,11 @@ TWD_API int twd_mx_dequantize(const uint8_t* codes, const uint8_t* scales, uint6
     const uint64_t size = type_size(type);
     if (!aligned(out, size)) return fail(TWD_E_INVALID, "twd_mx_dequantize: out is not aligned to its type");
     if (!aligned(codes, 16)) return fail(TWD_E_INVALID, "twd_mx_dequantize: codes must start at a multiple of 16 bytes");
-    DequantArgs a{codes, scales, rows, cols / 8, out, row_stride,
+    DequantArgs a{codes, scales, rows, static_cast<uint32_t>(cols * size / 16), out, row_stride,
                   aligned(out, 16) && (rows == 1 || row_stride * size % 16 == 0)};
     return by_type(type, [&](auto t) -> int {
         mx_dequantize_kernel<decltype(t)>
-            <<<matrix_grid(a.groups, rows), kQuantThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
+            <<<matrix_grid(a.pieces, rows), kQuantThreads, 0, static_cast<hipStream_t>(stream)>>>(a);
         TWD_HIP(hipGetLastError());
         return TWD_OK;
     });
