@@ -531,20 +531,22 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
         }
     };
     f32x4_t acc[4][NT] = {};
-    const u32x4_t* codes = a.codes + g * a.chunks * 256;
-    const uint32_t* scales = a.scales + g * a.quads * 256;
+    const auto codes = make_rsrc(a.codes + g * a.chunks * 256, a.chunks * 4096);
+    const auto scales = make_rsrc(a.scales + g * a.quads * 256, a.quads * 1024);
+    constexpr int kWeights = 0;  // cache policy
     // w, ws: the chunk's codes and the quad's scales; wn, wsn: the next ones, on their way
     u32x4_t w[4], wn[4];
     uint32_t ws[4], wsn[4];
     auto load_codes = [&](uint32_t c) {
-        const uint32_t cn = min(c, a.chunks - 1);
+        const int at = __builtin_amdgcn_readfirstlane(static_cast<int>(min(c, a.chunks - 1) * 4096));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wn[j] = codes[(cn * 4 + j) * 64 + lane];
+        for (int j = 0; j < 4; ++j)
+            wn[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(codes, lane * 16 + 1024 * j, at, kWeights));
     };
     auto load_scales = [&](uint32_t q) {
-        const uint32_t qn = min(q, a.quads - 1);
+        const int at = __builtin_amdgcn_readfirstlane(static_cast<int>(min(q, a.quads - 1) * 1024));
 #pragma unroll
-        for (int j = 0; j < 4; ++j) wsn[j] = scales[(qn * 4 + j) * 64 + lane];
+        for (int j = 0; j < 4; ++j) wsn[j] = __builtin_amdgcn_raw_buffer_load_b32(scales, lane * 4 + 256 * j, at, kWeights);
     };
     // x(n, t): the hidden fragment of tile n and step t
     auto chunk_bf16 = [&](uint32_t c, auto x) {
@@ -605,11 +607,13 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
             if constexpr (MX) fetch_scales(s + 1);
             fetch(s + 1, to);
         }
-        if constexpr (MX)
-            quad_mx(s, 4, [&](int n, uint32_t c) { return x[(c * NT + n) * 64 + lane]; },
-                    [&](int n, uint32_t c) { return xs[(16 * n + r) * 4 + c] >> (8 * kg); });
-        else
-            chunk_bf16(s, [&](int n, int t) { return x[(16 * n + r) * 16 + ((4 * kg + t) ^ r)]; });
+        if (have_group) {  // a wave past the vocabulary only helps with the hidden rows
+            if constexpr (MX)
+                quad_mx(s, 4, [&](int n, uint32_t c) { return x[(c * NT + n) * 64 + lane]; },
+                        [&](int n, uint32_t c) { return xs[(16 * n + r) * 4 + c] >> (8 * kg); });
+            else
+                chunk_bf16(s, [&](int n, int t) { return x[(16 * n + r) * 16 + ((4 * kg + t) ^ r)]; });
+        }
         if constexpr (MX) {
             if (s + 1 < stages) write_scales(to_xs);
         }
@@ -631,7 +635,7 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
         if (s + 1 >= stages) break;
         stage(s + 1, buf1, sc1, buf0, sc0);
     }
-    if (stages * 256 < width) {  // the columns past the last whole stage, straight from memory
+    if (have_group && stages * 256 < width) {  // the columns past the last whole stage, straight from memory
         ahead(stages);
         if constexpr (MX) {
             quad_mx(stages, a.chunks - 4 * stages,
