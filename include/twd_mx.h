@@ -39,7 +39,7 @@ TWD_API int twd_mx_dequantize(const uint8_t* codes, const uint8_t* scales, uint6
  * published in it. The codes and scales (device) are copied into the layout the kernels read and
  * may be freed after the call, which is synchronous. d_model is a multiple of 32, at most 2^20;
  * vocab at most 2^30. Scales above 2^100, and NaN, are rejected with TWD_E_UNSUPPORTED, as
- * twd_head_create rejects such groups. softcap >= 0 (0: none). */
+ * twd_head_create rejects such groups. softcap 0 (none) or in 1e-30..1e30. */
 typedef struct twd_mxhead twd_mxhead;
 TWD_API int twd_mxhead_create(const uint8_t* codes, const uint8_t* scales, uint32_t vocab, uint32_t d_model,
                               float softcap, void* stream, twd_mxhead** out);
@@ -48,8 +48,8 @@ TWD_API int twd_mxhead_info(const twd_mxhead* head, uint32_t* vocab, uint32_t* d
                             uint64_t* device_bytes);
 /* logits[m][v] = softcap(sum_c w[v][c] h[m][c]), 1 to 65,536 rows, summed in fp32; logits_type TWD_F32
  * or TWD_BF16 with logits_stride >= vocab elements between rows. hidden_bf16: rows of d_model bf16
- * values, hidden_stride (a multiple of 8) elements apart, starting at a multiple of 16 bytes; every
- * product is exact. The call keeps no state: calls on one head may overlap, on any streams, and may be
+ * values, hidden_stride (a multiple of 8, at most 2^26) elements apart, starting at a multiple of 16
+ * bytes; every product is exact. The call keeps no state: calls on one head may overlap, on any streams, and may be
  * captured. Asynchronous on `stream`. */
 TWD_API int twd_mxhead_logits(const twd_mxhead* head, const uint16_t* hidden_bf16, uint32_t rows,
                               uint64_t hidden_stride, void* logits, int logits_type, uint64_t logits_stride,

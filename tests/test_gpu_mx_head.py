@@ -107,6 +107,45 @@ def test_normal_rows(vocab, d, rows, cap, mx, out_type):
     head.close()
 
 
+@pytest.mark.parametrize("cap", [1e-30, 0.37, 30.0, 1e30])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_softcap_over_its_whole_range(cap, rows):
+    """The cap of exact sums from far below it to far past it, either sign, within the four half steps that
+    the quotient, the function and the product have: the sums are two bf16 parts of 16-bit values."""
+    t = twd()
+    cap = float(np.float32(cap))
+    x = np.concatenate([[0.0, 1e-3], np.geomspace(0.01, 200.0, 801), np.linspace(0.9, 1.1, 197)]) * cap
+    x[1::2] *= -1
+    bits = x.astype(np.float32).view(np.uint32)
+    z, hi = ((bits & m).astype(np.uint32).view(np.float32) for m in (0xFFFFFF00, 0xFFFF0000))
+    h = np.zeros((1000, 64), np.float32)
+    h[:, 0], h[:, 1] = hi, z - hi
+    codes, scales = np.zeros((5, 32), np.uint8), np.full((5, 2), 127, np.uint8)
+    codes[:, 0] = 0x22  # ones in the first two columns
+    want = cap * np.tanh(z.astype(np.float64) / cap)
+    head = t.MxHead(dev(codes), dev(scales), softcap=cap)
+    hd = dev(h).bfloat16()
+    got = np.concatenate([head.logits(hd[i:i + rows]).double().cpu().numpy() for i in range(0, 1000, rows)])
+    assert (np.abs(got - want[:, None]) <= 4 * 2.0 ** -24 * np.abs(want)[:, None]).all()
+    head.close()
+
+
+@pytest.mark.parametrize("rows,stride", [(3, 1 << 26), (35, (1 << 25) + 8), (66, (1 << 24) + 64)])
+def test_hidden_rows_far_apart(rows, stride):
+    """Rows so far apart that a tile of 128 does not lie within 32-bit offsets; the last reads the last bytes."""
+    import torch
+    t = twd()
+    rng = np.random.default_rng(rows)
+    d = 160
+    codes, scales = random_matrix(rng, 70, d)
+    h = rng.integers(-4, 5, (rows, d)).astype(np.float32)
+    x = torch.zeros((rows - 1) * stride + d, dtype=torch.bfloat16, device="cuda:0").as_strided((rows, d), (stride, 1))
+    x.copy_(dev(h))
+    head = t.MxHead(dev(codes), dev(scales))
+    assert np.array_equal(head.logits(x).double().cpu().numpy(), h.astype(np.float64) @ decode(codes, scales).T)
+    head.close()
+
+
 @pytest.mark.parametrize("rows", [1, 20, 70])
 @pytest.mark.parametrize("mx", [False, True])
 def test_nan_and_inf_rows_stay_theirs(rows, mx):

@@ -69,7 +69,7 @@ def test_head_refusals():
     refused(create(P, P, (1 << 30) + 1, 32, 0.0, None, C.byref(h)), inv, "vocab")
     for d in (0, 16, 40, (1 << 20) + 32):
         refused(create(P, P, 16, d, 0.0, None, C.byref(h)), inv, "d_model")
-    for cap in (-1.0, float("nan"), float("inf")):
+    for cap in (-1.0, float("nan"), float("inf"), 1e-31, 1e31):
         refused(create(P, P, 16, 32, cap, None, C.byref(h)), inv, "softcap")
     refused(create(P + 8, P, 16, 32, 0.0, None, C.byref(h)), inv, "16 bytes")
     assert not h
@@ -132,6 +132,7 @@ def test_refusals_of_live_objects():
     refused(lg(hh, P, 1, 64, P + 2, 0, 20, None), inv, "aligned")
     refused(lg(hh, P, 2, 63, P, 0, 20, None), inv, "hidden rows' stride")
     refused(lg(hh, P, 2, 68, P, 0, 20, None), inv, "hidden rows' stride")
+    refused(lg(hh, P, 2, (1 << 26) + 8, P, 0, 20, None), inv, "hidden rows' stride")
     refused(lmx(hh, P, None, 1, P, 0, 20, None), inv, "null")
     with pytest.raises(ValueError, match="hidden"):
         head.logits(torch.zeros(1, 96, dtype=torch.bfloat16, device="cuda:0"))

@@ -266,6 +266,18 @@ namespace twd {
 
 namespace {
 
+// A softcap's reciprocal and its multiples stay normal numbers.
+constexpr float kMinSoftCap = 1e-30f, kMaxSoftCap = 1e30f;
+
+struct SoftCap {
+    float cap, inv, twice;  // cap (0: none), 1 / cap, 2 log2(e) / cap
+};
+
+SoftCap soft_cap(float cap) {
+    const double c = cap > 0.0f ? cap : 1.0;
+    return SoftCap{cap, static_cast<float>(1.0 / c), static_cast<float>(2.8853900817779268 / c)};
+}
+
 struct MxArgs {
     const u32x4_t* codes;
     const uint32_t* scales;
@@ -275,13 +287,46 @@ struct MxArgs {
     void* out;
     uint64_t out_stride;
     uint32_t vocab, d, chunks, quads, groups, rows;
-    float softcap;
+    SoftCap softcap;
 };
 
 __device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = static_cast<uint16_t>(bf16_bits(v)); }
 
-__device__ __forceinline__ float cap_logit(float v, float cap) { return cap > 0.0f ? cap * tanhf(v / cap) : v; }
+// cap * tanh(v / cap) of N logits. Below the cap it is v + v t^2 r(t^2) with t = v / cap, r the polynomial
+// through (tanh(t)/t - 1)/t^2 at nine Chebyshev nodes of t^2 in 0..1: v itself enters the last sum exactly,
+// so the roundings of t count for less than half (at most 3 * 2^-24 of the result in all, 1.8 seen). Past
+// the cap it is cap - 2 cap / (exp(2 |t|) + 1), where the subtracted part is at most 0.31 of the result
+// (3.6 * 2^-24). A wave takes the second way only if one of its logits needs it. tanhf(v / cap) spent 36
+// instructions on every logit, as much time as the products of a tile of 2,048 columns.
+template <int N>
+__device__ __forceinline__ void cap_logits(float (&y)[N], const SoftCap& c) {
+    if (!(c.cap > 0.0f)) return;
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) top = fmaxf(top, fabsf(y[i]));
+    const bool past = __builtin_amdgcn_ballot_w64(top > c.cap) != 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float v = y[i], t = v * c.inv, t2 = t * t;
+        float p = -4.8467110900674015e-05f;
+        p = fmaf(p, t2, 0.000337689823936671f);
+        p = fmaf(p, t2, -0.0012421574375301295f);
+        p = fmaf(p, t2, 0.00347838643938303f);
+        p = fmaf(p, t2, -0.008826250210404396f);
+        p = fmaf(p, t2, 0.0218625757843256f);
+        p = fmaf(p, t2, -0.05396759510040283f);
+        p = fmaf(p, t2, 0.13333331048488617f);
+        p = fmaf(p, t2, -0.3333333432674408f);
+        float z = fmaf(v * t2, p, v);
+        if (past) {
+            const float e = __builtin_amdgcn_exp2f(fabsf(v) * c.twice);  // past 2^128: 1 / inf is 0
+            const float w = fmaf(-2.0f * c.cap, __builtin_amdgcn_rcpf(e + 1.0f), c.cap);
+            z = fabsf(v) > c.cap ? copysignf(w, v) : z;  // a NaN stays one by the first way
+        }
+        y[i] = z;
+    }
+}
 
 __device__ __forceinline__ i32x8_t mx_operand(u32x4_t v) {  // 4-bit operands fill half the registers
     const i32x4_t x = __builtin_bit_cast(i32x4_t, v);
@@ -427,10 +472,11 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a, ui
         // the team's waves share the sums: element e is hidden row e / 64, vocabulary row e % 64
         for (uint32_t e = quad * 64 + lane; e < a.rows * 64; e += a.quads * 64) {
             const float* p = part + static_cast<uint64_t>(buf * teams + team) * a.quads * cols * 64 + e;
-            float y = p[0];
-            for (uint32_t q = 1; q < a.quads; ++q) y += p[q * cols * 64];
+            float y[1] = {p[0]};
+            for (uint32_t q = 1; q < a.quads; ++q) y[0] += p[q * cols * 64];
+            cap_logits(y, a.softcap);
             const uint64_t v = static_cast<uint64_t>(g) * kMxGroupRows + e % 64;
-            if (v < a.vocab) store_logit(static_cast<Out*>(a.out) + (e / 64) * a.out_stride + v, cap_logit(y, a.softcap));
+            if (v < a.vocab) store_logit(static_cast<Out*>(a.out) + (e / 64) * a.out_stride + v, y[0]);
         }
         buf ^= 1;
     }
@@ -671,7 +717,8 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) y[4 * j + i] = cap_logit(acc[j][n][i], a.softcap);
+            for (int i = 0; i < 4; ++i) y[4 * j + i] = acc[j][n][i];
+        cap_logits(y, a.softcap);
         store_logits(static_cast<Out*>(a.out) + m * a.out_stride + v, y, n_v);
     }
 }
@@ -738,8 +785,10 @@ int launch_typed(const twd_mxhead* h, const MxArgs& a, hipStream_t s) {
         TWD_HIP(hipGetLastError());
         return TWD_OK;
     }
-    if (a.rows <= 32) return launch_tile<MX, 2, Out>(a, s);
-    if (a.rows <= 64) return launch_tile<MX, 4, Out>(a, s);
+    // a tile's hidden rows are read at 32-bit offsets from its first
+    const uint64_t apart = MX ? a.d / 2 : 2 * a.x_stride;
+    if (a.rows <= 32 || apart > 1u << 26) return launch_tile<MX, 2, Out>(a, s);
+    if (a.rows <= 64 || apart > 1u << 25) return launch_tile<MX, 4, Out>(a, s);
     return launch_tile<MX, 8, Out>(a, s);
 }
 
@@ -749,6 +798,7 @@ int launch_logits(const twd_mxhead* h, const MxArgs& a, int out_type, hipStream_
 }
 
 constexpr uint32_t kMxMaxRows = 65536;
+constexpr uint64_t kMxMaxStride = 1ull << 26;  // 32 rows within 4 GiB
 
 int check_logits(const twd_mxhead* h, const void* x, uint32_t rows, const void* logits, int out_type,
                  uint64_t out_stride) {
@@ -821,7 +871,8 @@ TWD_API int twd_mxhead_create(const uint8_t* codes, const uint8_t* scales, uint3
     if (vocab == 0 || vocab > (1u << 30)) return fail(TWD_E_INVALID, "vocab must be in 1..2^30");
     if (d_model == 0 || d_model % kMxBlock != 0 || d_model > (1u << 20))
         return fail(TWD_E_INVALID, "d_model must be a positive multiple of 32, at most 2^20");
-    if (!(softcap >= 0.0f) || softcap > 3.0e38f) return fail(TWD_E_INVALID, "softcap must be finite and >= 0 (0: none)");
+    if (softcap != 0.0f && !(softcap >= kMinSoftCap && softcap <= kMaxSoftCap))
+        return fail(TWD_E_INVALID, "softcap must be 0 (none) or in 1e-30..1e30");
     if (!aligned(codes, 16)) return fail(TWD_E_INVALID, "codes must start at a multiple of 16 bytes");
     const uint32_t chunks = (d_model + kMxChunkK - 1) / kMxChunkK, quads = (chunks + 3) / 4;
     const uint32_t groups = (vocab + kMxGroupRows - 1) / kMxGroupRows;
@@ -885,9 +936,11 @@ TWD_API int twd_mxhead_logits(const twd_mxhead* head, const uint16_t* hidden_bf1
     if (rc) return rc;
     if (rows > 1 && (hidden_stride < head->d || hidden_stride % 8 != 0))
         return fail(TWD_E_INVALID, "the hidden rows' stride must be a multiple of 8 and at least d_model");
+    if (rows > 1 && hidden_stride > kMxMaxStride)
+        return fail(TWD_E_INVALID, "the hidden rows' stride must be at most 2^26 elements");
     if ((rc = check_device(head))) return rc;
     const MxArgs a{head->codes, head->scales, hidden_bf16, nullptr, hidden_stride, logits, logits_stride,
-                   head->vocab, head->d, head->chunks, head->quads, head->groups, rows, head->softcap};
+                   head->vocab, head->d, head->chunks, head->quads, head->groups, rows, soft_cap(head->softcap)};
     return launch_logits<false>(head, a, logits_type, static_cast<hipStream_t>(stream));
 }
 
@@ -899,7 +952,7 @@ TWD_API int twd_mxhead_logits_mx(const twd_mxhead* head, const uint8_t* codes, c
     if (!scales) return fail(TWD_E_INVALID, "null argument");
     if ((rc = check_device(head))) return rc;
     const MxArgs a{head->codes, head->scales, codes, scales, head->d, logits, logits_stride,
-                   head->vocab, head->d, head->chunks, head->quads, head->groups, rows, head->softcap};
+                   head->vocab, head->d, head->chunks, head->quads, head->groups, rows, soft_cap(head->softcap)};
     return launch_logits<true>(head, a, logits_type, static_cast<hipStream_t>(stream));
 }
 
