@@ -542,7 +542,9 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
     };
     auto byte_of = [&](uint32_t i) {
         const uint32_t p = i * kTileWaves + wave;
-        return MX ? 64 * (p / NT) + 16 * kg : 16 * ((lane ^ (4 * p + lane / 16)) % 16);
+        if (MX) return 64 * (p / NT) + 16 * kg;
+        const uint32_t q = (lane ^ (4 * p + lane / 16)) % 16;
+        return 64 * (0x78u >> (2 * (q / 4)) & 3) + 16 * (q % 4);
     };
     const char* x0 = static_cast<const char*>(a.x) + static_cast<uint64_t>(m0) * row_bytes;
     const uint32_t rows_here = min(a.rows - m0, kRows);
@@ -658,7 +660,7 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
                 quad_mx(s, 4, [&](int n, uint32_t c) { return x[(c * NT + n) * 64 + lane]; },
                         [&](int n, uint32_t c) { return xs[(16 * n + r) * 4 + c] >> (8 * kg); });
             else
-                chunk_bf16(s, [&](int n, int t) { return x[(16 * n + r) * 16 + ((4 * kg + t) ^ r)]; });
+                chunk_bf16(s, [&](int n, int t) { return x[(16 * n + r) * 16 + ((4 * (0x9cu >> (2 * kg) & 3) + t) ^ r)]; });
         }
         if constexpr (MX) {
             if (s + 1 < stages) write_scales(to_xs);
