@@ -601,18 +601,31 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
         float f[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(((ws[j] >> (8 * (c % 4))) & 255u) << 23);
+        // two fragments are read from LDS while the two before them are multiplied
+        constexpr int kPairs = NT / 2;
+        bf16x8_t e[4], y[2][2];
+        auto read = [&](int i) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            __builtin_amdgcn_sched_barrier(0);  // one step's operands at a time: more would not fit beside the sums
-            bf16x8_t e[4];
+            for (int k = 0; k < 2; ++k) y[i % 2][k] = __builtin_bit_cast(bf16x8_t, x(2 * (i % kPairs) + k, i / kPairs));
+        };
+        __builtin_amdgcn_sched_barrier(0);
+        read(0);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) e[j] = widen(w[j][t], f[j]);
+        for (int i = 0; i < 4 * kPairs; ++i) {
+            if (i + 1 < 4 * kPairs) read(i + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i % kPairs == 0) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const bf16x8_t y = __builtin_bit_cast(bf16x8_t, x(n, t));
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[j][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e[j], y, acc[j][n], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) e[j] = widen(w[j][i / kPairs], f[j]);
             }
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    f32x4_t& sum = acc[j][2 * (i % kPairs) + k];
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e[j], y[i % 2][k], sum, 0, 0, 0);
+                }
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = wn[j], ws[j] = c % 4 == 3 ? wsn[j] : ws[j];
