@@ -678,9 +678,12 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
         if constexpr (MX) {
             if (s + 1 < stages) write_scales(to_xs);
         }
-        // the next stage's loads into LDS are done before the barrier that hands it over; quantised, the next
-        // chunk's codes, the last four loads issued, may still be on their way
-        __builtin_amdgcn_s_waitcnt(MX ? kVmcnt0 + 4 : kVmcnt0);
+        // the next stage's loads into LDS are done before the barrier that hands it over; where quantised
+        // products were made, the next chunk's codes, the last four loads issued, may still be on their way
+        __builtin_amdgcn_sched_barrier(0);
+        if (MX && have_group) __builtin_amdgcn_s_waitcnt(kVmcnt0 + 4);
+        else __builtin_amdgcn_s_waitcnt(kVmcnt0);
+        __builtin_amdgcn_sched_barrier(0);
     };
     load_codes(0);
     load_scales(0);
