@@ -1,4 +1,4 @@
-"""Sampler.sample against the definition in 64 bits: ids and kept counts have to be equal. Weights carry 38
+"""Sampler.sample against the definition in 64 bits: ids and kept counts have to be equal. Weights carry 37
 bits and sums are exact, so a logprob is off by at most half a step of fp32 and 2^-36."""
 import math
 

@@ -780,7 +780,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     const uint32_t lo = st.lo, hi = st.hi, k = st.k, bin_k = st.bin_k;
     const bool on_list = listed <= kListCap, any = lo <= hi, use_p = st.use_p != 0, need_k = bin_k < kBins;
     auto weight = [&](float l, uint32_t* bin) {
-        const Weight w = weight_of(l, c);
+        const Weight w = weight_of(l, c, a.poly);
         *bin = bin_of(w, top);
         return mass_of(w, *bin, top);
     };
