@@ -56,47 +56,38 @@ __device__ __forceinline__ Scale scale_of(float t) {
     return s;
 }
 
-// The weight's octave floor(z), the eighth of it that z lies in, counted from the top, and the weight's 37 bits.
-// The octave rises with l, and the eighth falls within it.
-struct Weight {
-    double oct;
-    uint32_t sub;
-    uint64_t q;
+// Where a weight lies: floor(8 z), the eighths of its octave counted from 2^0 up. It rises with l.
+__device__ __forceinline__ double place_of(float l, const Scale& c) { return __builtin_floor(static_cast<double>(l) * (8.0 * c.hi)); }
+__device__ __forceinline__ double octave_of(double place) { return __builtin_floor(0.125 * place); }
+
+// 2^(t/8), t in 0..1: the degree-5 polynomial through the Chebyshev nodes (3e-13 relative); and 2^36 times the power
+// of two at the lower end of each eighth of an octave, falling, less 2^-30 of it, so that 8,192 weights stay under 2^50.
+// A kernel that evaluates them for every logit takes the coefficients as an argument, in scalar registers (as literals
+// each would be moved into a register pair before its use), and the eighths in LDS. (One polynomial of degree 9 over the
+// octave instead: 35 instead of 28 instructions a logit, 51 instead of 46 us for the slices of 256 rows of 151,669.)
+constexpr double kRoot = 0x1p36 * (1.0 - 0x1p-30);
+struct WeightTable {
+    double c[6], eighth[8];
 };
+constexpr WeightTable kWeightTable{{0x1.ffffffffff586p-1, 0x1.62e42ff11cbe7p-4, 0x1.ebfbddd2b054ap-9, 0x1.c6b1b1f5de28ap-14,
+                                    0x1.3ae471589a702p-19, 0x1.6d07e00a32dbap-25},
+                                   {0x1.d5818dcfba487p+0 * kRoot, 0x1.ae89f995ad3adp+0 * kRoot, 0x1.8ace5422aa0dbp+0 * kRoot,
+                                    0x1.6a09e667f3bcdp+0 * kRoot, 0x1.4bfdad5362a27p+0 * kRoot, 0x1.306fe0a31b715p+0 * kRoot,
+                                    0x1.172b83c7d517bp+0 * kRoot, 0x1.0000000000000p+0 * kRoot}};
+// The weight's 37 bits, from its place and its eighth of the octave.
 // FAR: |z| may reach 2^45, where neighbouring floats lie more octaves apart than any sum holds and z has no
-// fraction left: the weight is its octave's middle then. A caller that knows better leaves the test out.
-// 2^(36.5 + t) less 2^-30 of it, so that 8,192 of them stay under 2^50; |t| <= 0.5: the degree-9 polynomial
-// through the Chebyshev nodes (2e-14 relative). A kernel that
-// evaluates it for every logit takes the coefficients as an argument, in scalar registers: as literals each
-// would be moved into a register pair before its use.
-constexpr double kRoot = 0x1.6a09e667f3bcdp+36 * (1.0 - 0x1p-30);
-struct Exp2Poly {
-    double c[10];
-};
-constexpr Exp2Poly kExp2Poly{{0x1.000000000003dp+0 * kRoot, 0x1.62e42fefa39f7p-1 * kRoot, 0x1.ebfbdff8149f2p-3 * kRoot,
-                              0x1.c6b08d7044119p-5 * kRoot, 0x1.3b2ab72b175eep-7 * kRoot, 0x1.5d87fe908f88ap-10 * kRoot,
-                              0x1.43088e257f341p-13 * kRoot, 0x1.ffcb76789860fp-17 * kRoot, 0x1.63ef969a64d3cp-20 * kRoot,
-                              0x1.b6571de2f2351p-24 * kRoot}};
+// fraction left: the weight is its eighth's middle then. A caller that knows better leaves the test out.
 template <bool FAR = true>
-__device__ __forceinline__ Weight weight_of(float l, const Scale& c, const Exp2Poly& k = kExp2Poly) {
+__device__ __forceinline__ uint64_t weight_of(float l, double place, double eighth, const Scale& c, const WeightTable& k) {
 #pragma clang fp contract(off)
     const double ld = l;
-    const double zh = ld * c.hi;
-    Weight w;
-    w.oct = __builtin_floor(zh);
-    const double mid = w.oct + 0.5;
-    double t = fma(ld, c.hi, -mid);  // z less the octave's middle, rounded once, so rising with l
-    if (FAR) t = __builtin_fabs(zh) < 0x1p45 ? t : 0.0;
-    const uint32_t sub = static_cast<uint32_t>(fma(t, -8.0, 4.0));
-    w.sub = sub < 7u ? sub : 7u;
-    if (FAR) t = __builtin_fabs(zh) < 0x1p45 ? fma(ld, c.lo, t) : t;
-    else t = fma(ld, c.lo, t);
-    double p = fma(t, k.c[9], k.c[8]);
+    double t = fma(ld, 8.0 * c.lo, fma(ld, 8.0 * c.hi, -place));  // 8 z's fraction
+    if (FAR) t = __builtin_fabs(place) < 0x1p48 ? t : 0.5;
+    double p = fma(t, k.c[5], k.c[4]);
 #pragma unroll
-    for (int i = 7; i >= 0; --i) p = fma(t, p, k.c[i]);
+    for (int i = 3; i >= 0; --i) p = fma(t, p, k.c[i]);
     // + 2^52 leaves the nearest integer in the low mantissa bits
-    w.q = __builtin_bit_cast(uint64_t, p + 0x1p52) & 0xFFFFFFFFFFFFFull;
-    return w;
+    return __builtin_bit_cast(uint64_t, fma(p, eighth, 0x1p52)) & 0xFFFFFFFFFFFFFull;
 }
 
 // floor(f s) and ceil(f s) of a float f in [0, 1) and a sum: f is m 2^-k with a 24-bit m.
@@ -207,7 +198,7 @@ struct SampleArgs {
     SampleParams p;
     SampleOut o;
     SamplerScratch s;
-    Exp2Poly poly;
+    WeightTable table;
 };
 
 // 16 bytes of logits from any address (the hardware splits an unaligned load itself): entries i .. of a row, moved
@@ -247,15 +238,22 @@ __device__ __forceinline__ Vec load_vec(const void* row, uint32_t i, uint32_t vo
 }
 
 // The bin of a weight counted from octave `top`, and its integer in that bin.
-__device__ __forceinline__ uint32_t bin_of(const Weight& w, double top) {
-    const double down = top - w.oct;
-    if (!(down < static_cast<double>(kTailOct + 1))) return kTail;
-    return (static_cast<uint32_t>(down) << 3) + w.sub;
+__device__ __forceinline__ uint32_t bin_of(double place, double top) {
+    const double down = 8.0 * top + 7.0 - place;
+    return down < static_cast<double>(kBins) ? static_cast<uint32_t>(down) : kTail;
 }
-__device__ __forceinline__ uint64_t mass_of(const Weight& w, uint32_t bin, double top) {
-    if (bin != kTail) return w.q;
-    const double deep = top - w.oct - static_cast<double>(kTailOct);
-    return deep < 64.0 ? w.q >> static_cast<int>(deep) : 0;
+__device__ __forceinline__ uint64_t mass_of(uint64_t q, double place, uint32_t bin, double top) {
+    if (bin != kTail) return q;
+    const double deep = top - octave_of(place) - static_cast<double>(kTailOct);
+    return deep < 64.0 ? q >> static_cast<int>(deep) : 0;
+}
+// The two of one logit; eighths: the table's, in LDS.
+__device__ __forceinline__ uint64_t entry_weight(float l, const Scale& c, const WeightTable& k, const double* eighths, double top,
+                                          uint32_t* bin) {
+    const double place = place_of(l, c);
+    const uint32_t e = 7 - static_cast<uint32_t>(place - 8.0 * octave_of(place));
+    *bin = bin_of(place, top);
+    return mass_of(weight_of(l, place, eighths[e & 7], c, k), place, *bin, top);
 }
 // A bin's integer in units of the row's sums.
 __device__ __forceinline__ u128 unit(uint64_t mass, uint32_t bin) {
@@ -340,6 +338,7 @@ constexpr uint32_t kCopies = 4;  // of a slice's bins, by lane, so that a wave's
 template <typename T, bool TINY>
 __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs a) {
     __shared__ uint64_t bins[kBins][kCopies];
+    __shared__ double eighths[8];
     __shared__ uint32_t s_key[kSliceThreads / 64], s_bad[kSliceThreads / 64], s_idx;
     const uint32_t t = threadIdx.x, slice = blockIdx.x, lane = t % 64, wave = t / 64;
     const uint64_t r = blockIdx.y;
@@ -352,6 +351,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
     for (uint32_t j = 0; j < kLoads; ++j) raw[j] = load_vec<T, TINY>(row, i0 + j * kSliceThreads * kVec<T>, a.vocab);
     const float temp = a.p.temperature ? a.p.temperature[r] : 1.0f;
     for (uint32_t i = t; i < kBins * kCopies; i += kSliceThreads) bins[i / kCopies][i % kCopies] = 0;
+    if (t < 8) eighths[t] = a.table.eighth[t];
     if (t == 0) s_idx = ~0u;
     const Scale c = scale_of(temp);
     float best = -INFINITY;
@@ -390,17 +390,17 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
     }
     const bool weigh = live && bad == 0 && temp > 0.0f;  // a row with a NaN or +inf, and a greedy one, needs no weights
     if (weigh) {
-        const double top = weight_of(best, c).oct;
+        const double top = octave_of(place_of(best, c));
         if (__builtin_fabs(top) < 0x1p44) {
             // Nothing branches on an entry's value, and only the counting leaves masked ones out. (An entry so far
             // down that its z holds no fraction shifts to nothing.)
 #pragma unroll
             for (uint32_t j = 0; j < kEach; ++j) {
-                const Weight w = weight_of<false>(v[j], c, a.poly);
-                uint32_t d = static_cast<uint32_t>(top - w.oct);
-                d = d < kTailOct + 63 ? d : kTailOct + 63;
-                const uint32_t b = d << 3 | w.sub;
-                const uint64_t m = w.q >> ((d > kTailOct ? d : kTailOct) - kTailOct);
+                const double place = place_of(v[j], c);
+                const uint32_t b = static_cast<uint32_t>(8.0 * top + 7.0 - place);
+                const uint64_t q = weight_of<false>(v[j], place, eighths[b & 7], c, a.table);
+                const uint32_t d = b >> 3 < kTailOct + 63 ? b >> 3 : kTailOct + 63;
+                const uint64_t m = q >> ((d > kTailOct ? d : kTailOct) - kTailOct);
                 if (v[j] > -INFINITY)
                     atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b < kTail ? b : kTail][lane % kCopies]),
                               static_cast<unsigned long long>(1ull << kCountBit | m));
@@ -410,10 +410,10 @@ __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs
             for (uint32_t i = slice * kSlice + t; i < min(a.vocab, (slice + 1) * kSlice); i += kSliceThreads) {
                 const float l = load_logit<T>(row, i);
                 if (!(l > -INFINITY)) continue;
-                const Weight w = weight_of(l, c);
-                const uint32_t b = bin_of(w, top);
+                uint32_t b;
+                const uint64_t m = entry_weight(l, c, a.table, eighths, top, &b);
                 atomicAdd(reinterpret_cast<unsigned long long*>(&bins[b][lane % kCopies]),
-                          static_cast<unsigned long long>(1ull << kCountBit | mass_of(w, b, top)));
+                          static_cast<unsigned long long>(1ull << kCountBit | m));
             }
         }
     }
@@ -487,7 +487,7 @@ __device__ uint32_t bin_key(uint32_t b, uint32_t above, double top, const Scale&
     if (b >= kTail) return kLeast + 1;
     const double z = top + 1.0 - 0.125 * static_cast<double>(b + 1);
     const uint32_t guess = c.hi > 0.0 ? float_key(static_cast<float>(z / c.hi)) : above;
-    return least_key(guess, above, [&](float l) { return bin_of(weight_of(l, c), top) <= b; });
+    return least_key(guess, above, [&](float l) { return bin_of(place_of(l, c), top) <= b; });
 }
 
 // What every wave of a block learns of its row from the slices' heads.
@@ -530,7 +530,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         return;
     }
     const Scale c = scale_of(temp);
-    const double top = weight_of(rank_value(best), c).oct;
+    const double top = octave_of(place_of(rank_value(best), c));
     const uint32_t shift = slice_shift(head.own, top, c);
 
     // ---- the row's bins. Two threads to a bin, every other slice each: a slice's bin 8 `shift` above it. What lies
@@ -583,7 +583,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
         if (wave == kRowThreads / 64 - 1 && min_p > 0.0f) {
             const uint64_t rank = least_kept(best, min_p, c);
             const float l = rank_value(rank);
-            const uint32_t b = l > -INFINITY ? bin_of(weight_of(l, c), top) : kBins;
+            const uint32_t b = l > -INFINITY ? bin_of(place_of(l, c), top) : kBins;
             if (lane == 0) s_rank_m = rank, s_bin_m = b;
         }
         __syncthreads();
@@ -757,6 +757,7 @@ struct FinishMem {
     unsigned long long slice_lo[kMaxSlices], slice_hi[kMaxSlices];
     ScanMem scan;
     unsigned long long least, most;
+    double eighths[8];
     uint64_t cut;
     u128 sum, base_w, want;
     uint32_t n, base_n, pick, id, last;
@@ -779,13 +780,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     const double top = st.top;
     const uint32_t lo = st.lo, hi = st.hi, k = st.k, bin_k = st.bin_k;
     const bool on_list = listed <= kListCap, any = lo <= hi, use_p = st.use_p != 0, need_k = bin_k < kBins;
-    auto weight = [&](float l, uint32_t* bin) {
-        const Weight w = weight_of(l, c, a.poly);
-        *bin = bin_of(w, top);
-        return mass_of(w, *bin, top);
-    };
+    auto weight = [&](float l, uint32_t* bin) { return entry_weight(l, c, a.table, sm.eighths, top, bin); };
     if (t < kMaxSlices) sm.slice_lo[t] = 0, sm.slice_hi[t] = 0;
     if (t == 0) sm.last = 0, sm.id = ~0u;
+    if (t < 8) sm.eighths[t] = a.table.eighth[t];
+    __syncthreads();
     if (on_list) {
 #pragma unroll 1
         for (uint32_t i = t; i < listed; i += kRowThreads) {
@@ -1125,7 +1124,7 @@ TWD_API int twd_sampler_sample(twd_sampler* sampler, const void* logits, int typ
     if (rc) return rc;
     const SampleArgs args{logits, row_stride, vocab, (vocab + kSlice - 1) / kSlice,
                           SampleParams{temperature, top_k, top_p, min_p, uniform}, SampleOut{tokens, logprobs, kept},
-                          sampler->scratch, kExp2Poly};
+                          sampler->scratch, kWeightTable};
     if (type == TWD_F32)
         launch<float>(args, rows, s);
     else if (type == TWD_BF16)
