@@ -795,7 +795,13 @@ int launch_tile(const MxArgs& a, hipStream_t s) {
 
 template <bool MX, typename Out>
 int launch_typed(const twd_mxhead* h, const MxArgs& a, hipStream_t s) {
-    if (a.rows <= kSmallRows && a.quads <= kSmallWaves) {
+    // Few rows stream (262,144 x 5,376, 1 row: 117 us; as a tile 137). The wider the rows' sums against the quads a
+    // wave reads between two of them, the more the joining costs, which a tile does not have: 8 bf16 rows of
+    // 131,072 x 3,584 took 48 us streamed and 41 as a tile, of 262,144 x 2,048 57 and 53, of 131,072 x 2,880 41 and
+    // 34. A head of less than a tile's block for every compute unit streams on (8 rows of 32,768 x 3,584: 15 us, as a
+    // tile 21), and so do quantised rows (16 of 131,072 x 4,608: 53 and 56 us).
+    const bool tiles = !MX && a.rows > a.quads && a.groups >= kTileWaves * static_cast<uint32_t>(h->cus);
+    if (a.rows <= kSmallRows && a.quads <= kSmallWaves && !tiles) {
         const uint32_t teams = kSmallWaves / a.quads;
         const uint32_t blocks = min((a.groups + teams - 1) / teams, static_cast<uint32_t>(h->cus));
         const uint32_t lds = 2 * teams * a.quads * a.rows * 64 * sizeof(float);
@@ -803,7 +809,9 @@ int launch_typed(const twd_mxhead* h, const MxArgs& a, hipStream_t s) {
         TWD_HIP(hipGetLastError());
         return TWD_OK;
     }
-    // a tile's hidden rows are read at 32-bit offsets from its first
+    // Rows that a tile lacks are multiplied all the same, and every tile widens the weights anew (64 rows of 262,144 x
+    // 5,376: 188 us in one tile of 64, 217 in two of 32; 32 rows: 152 in a tile of 32).
+    // A tile's hidden rows are read at 32-bit offsets from its first.
     const uint64_t apart = MX ? a.d / 2 : 2 * a.x_stride;
     if (a.rows <= 32 || apart > 1u << 26) return launch_tile<MX, 2, Out>(a, s);
     if (a.rows <= 64 || apart > 1u << 25) return launch_tile<MX, 4, Out>(a, s);
