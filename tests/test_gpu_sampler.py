@@ -120,6 +120,17 @@ def test_wide_nuclei_and_flat_rows(vocab, dtype):
     check(dev(a, dtype), [1.0, 1.6] * (n // 2), ks, ps, [0.0] * n, us, tag="flat")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_lists_of_thousands(dtype):
+    """Between 5,000 and 30,000 entries in the eighth of an octave where a limit cuts: the list is read from memory."""
+    rng = np.random.default_rng(7)
+    a = rows_of(rng, 8, 262144, 1.0)
+    ks = [0, 100000, 0, 60000, 131072, 0, 262143, 200000]
+    ps = [0.9, 1.0, 0.8, 0.9, 0.5, 0.95, 0.85, 1.0]
+    us = (rng.integers(0, 1 << 24, 8) / (1 << 24)).tolist()
+    check(dev(a, dtype), [1.0, 1.0, 1.5, 1.5, 2.0, 2.0, 0.8, 0.8], ks, ps, [0.0] * 7 + [0.3], us, tag="thousands")
+
+
 @pytest.mark.parametrize("vocab", [1, 17, 4096, 5000, 100000, 262144])
 def test_equal_logits(vocab):
     """All logits equal, or two values: every cut falls among ties, which go by index."""

@@ -151,7 +151,9 @@ constexpr uint32_t kSlice = 8192;
 constexpr uint32_t kBins = 256;
 constexpr uint32_t kTail = kBins - 1;
 constexpr uint32_t kTailOct = kTail >> 3;
-constexpr uint32_t kListCap = 4096;  // rows with more entries in the deciding bins are read again instead
+// Entries in the deciding bins: up to kNearCap of them are kept in LDS while they are cut, up to kListCap read from the
+// list each time, and more (nearly equal logits) from the row.
+constexpr uint32_t kNearCap = 4096, kListCap = 32768;
 constexpr uint32_t kMaxSlices = 524288 / kSlice;
 // A bin of a slice: its entries' number from bit 50 on, the sum of their weights below.
 constexpr int kCountBit = 50;
@@ -188,9 +190,10 @@ struct SamplerScratch {
     uint64_t* bins;   // [rows][slices][kBins]
     SliceHead* head;  // [rows][slices]
     RowState* state;  // [rows]
-    uint64_t* list;   // [rows][kListCap] ranks
+    uint64_t* list;   // [rows][list_cap] ranks
     u128* under;      // [rows][slices] a slice's sum of the weights in bins under lo
     uint32_t slices;  // of max_vocab
+    uint32_t list_cap;  // kListCap, or all of a smaller vocabulary
 };
 
 struct SampleArgs {
@@ -693,7 +696,7 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArg
     RowState* st = a.s.state + r;
     const uint32_t listed = st->listed, k0 = st->key[0], k1 = st->key[1], k2 = st->key[2], k3 = st->key[3];
     const uint32_t most = static_cast<uint32_t>(a.s.head[r * a.s.slices + slice].best >> 32);
-    if (listed == 0 || listed > kListCap) return;
+    if (listed == 0 || listed > a.s.list_cap) return;
     const bool two = k2 < k3 && k2 < k0;  // a bin_k past lo .. hi
     if (most < (two ? k2 : k0)) return;   // all of the slice lies below
     if (t == 0) s_n = 0;
@@ -740,13 +743,14 @@ __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArg
             const uint32_t to = at + __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(in[j][e] >> 32),
                                                               __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(in[j][e]), 0));
             // the bins' own numbers say how many come: the list holds them all
-            if ((in[j][e] >> lane & 1) != 0 && to < kListCap)
-                a.s.list[r * kListCap + to] = rank_key(load_logit<T>(v[j].w, e), v[j].first + e);
+            if ((in[j][e] >> lane & 1) != 0 && to < a.s.list_cap)
+                a.s.list[r * a.s.list_cap + to] = rank_key(load_logit<T>(v[j].w, e), v[j].first + e);
             at += static_cast<uint32_t>(__builtin_popcountll(in[j][e]));
         }
     }
 }
 
+constexpr uint32_t kFarAhead = 4;         // entries on their way where they come from memory
 constexpr uint32_t kSmall = 64;           // entries that are ranked against each other directly
 constexpr uint32_t kParts = kRowThreads;  // parts that a range of ranks is cut into
 constexpr uint32_t kStageEach = kSlice / kRowThreads, kStageStride = kStageEach + 1;  // a thread's entries, an odd way apart
@@ -754,8 +758,8 @@ constexpr uint32_t kStageEach = kSlice / kRowThreads, kStageStride = kStageEach 
 struct FinishMem {
     union {
         struct {
-            uint64_t rank[kListCap];
-            uint64_t weight[kListCap];  // its bin above bit 48, the weight below
+            uint64_t rank[kNearCap];
+            uint64_t weight[kNearCap];  // its bin above bit 48, the weight below
         };
         float stage[kRowThreads * kStageStride];
     };
@@ -792,52 +796,71 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     const Scale c = scale_of(temp);
     const double top = st.top;
     const uint32_t lo = st.lo, hi = st.hi, k = st.k, bin_k = st.bin_k;
-    const bool on_list = listed <= kListCap, any = lo <= hi, use_p = st.use_p != 0, need_k = bin_k < kBins;
+    const bool near = listed <= kNearCap, on_list = listed <= a.s.list_cap, any = lo <= hi, use_p = st.use_p != 0, need_k = bin_k < kBins;
     auto weight = [&](float l, uint32_t* bin) { return entry_weight(l, c, a.table, sm.eighths, top, bin); };
     if (t < kMaxSlices) sm.slice_lo[t] = 0, sm.slice_hi[t] = 0;
     if (t == 0) sm.last = 0, sm.id = ~0u;
     if (t < 8) sm.eighths[t] = a.table.eighth[t];
     __syncthreads();
-    if (on_list) {
+    const uint64_t* list = a.s.list + r * a.s.list_cap;
+    if (near) {
 #pragma unroll 1
         for (uint32_t i = t; i < listed; i += kRowThreads) {
-            const uint64_t rank = a.s.list[r * kListCap + i];
+            const uint64_t rank = list[i];
             uint32_t b;
             const uint64_t m = weight(rank_value(rank), &b);
             sm.rank[i] = rank, sm.weight[i] = static_cast<uint64_t>(b) << 48 | m;
         }
     }
-    // f(rank, bin, weight) of every entry in the row's bins b0 .. b1: from the list, or, where equal or nearly
-    // equal logits are too many for it, from the row. (A thread meets the same entries of the list each time.)
-    auto members = [&](uint32_t b0, uint32_t b1, auto f) {
+    // f(rank, bin, weight) of every entry in the row's bins lo .. hi, or, of_k, in bin_k: those whose keys the bins'
+    // bound. (A thread meets the same entries in LDS each time.)
+    auto members = [&](bool of_k, auto f) {
+        const uint32_t key0 = st.key[of_k ? 2 : 0], key1 = st.key[of_k ? 3 : 1];
+        auto in = [&](uint64_t rank) {
+            const uint32_t key = static_cast<uint32_t>(rank >> 32);
+            return key >= key0 && key < key1;
+        };
+        if (near) {
+#pragma unroll 1
+            for (uint32_t i = t; i < listed; i += kRowThreads) {
+                const uint64_t rank = sm.rank[i], x = sm.weight[i];
+                if (in(rank)) f(rank, static_cast<uint32_t>(x >> 48), x & 0xFFFFFFFFFFFFull);
+            }
+            return;
+        }
         const uint32_t end = on_list ? listed : a.vocab;
+        auto get = [&](uint32_t i) -> uint64_t {  // (key 0 lies below every entry's)
+            if (i >= end) return 0;
+            return on_list ? list[i] : rank_key(load_logit<T>(row, i), i);
+        };
+        uint64_t ahead[kFarAhead];
+#pragma unroll
+        for (uint32_t j = 0; j < kFarAhead; ++j) ahead[j] = get(t + j * kRowThreads);
 #pragma unroll 1
         for (uint32_t i = t; i < end; i += kRowThreads) {
-            uint64_t rank, m;
-            uint32_t b;
-            if (on_list) {
-                const uint64_t x = sm.weight[i];
-                rank = sm.rank[i], b = static_cast<uint32_t>(x >> 48), m = x & 0xFFFFFFFFFFFFull;
-            } else {
-                const float l = load_logit<T>(row, i);
-                if (!(l > -INFINITY)) continue;
-                rank = rank_key(l, i), m = weight(l, &b);
+            const uint64_t rank = ahead[0];
+#pragma unroll
+            for (uint32_t j = 0; j + 1 < kFarAhead; ++j) ahead[j] = ahead[j + 1];
+            ahead[kFarAhead - 1] = get(i + kFarAhead * kRowThreads);
+            if (in(rank)) {
+                uint32_t b;
+                const uint64_t m = weight(rank_value(rank), &b);
+                f(rank, b, m);
             }
-            if (b >= b0 && b <= b1) f(rank, b, m);
         }
     };
-    // Among the entries of bins b0 .. b1, `have` of them, ranks r0 .. r1, with base_n entries of sum base_w before
+    // Among the entries of bins lo .. hi, or of bin_k, `have` of them, ranks r0 .. r1, with base_n entries of sum base_w before
     // them: the rank of the one that brings the number to n, or the sum to w (by_sum); 0 where none does. *sum:
     // the sum with it. While they are many, the range of their ranks is cut into parts and the part that holds it
     // kept.
-    auto select = [&](uint32_t b0, uint32_t b1, uint32_t have, uint64_t r0, uint64_t r1, uint32_t base_n, u128 base_w,
+    auto select = [&](bool of_k, uint32_t have, uint64_t r0, uint64_t r1, uint32_t base_n, u128 base_w,
                       bool by_sum, uint32_t n, u128 w, u128* sum) {
         for (bool first = true;; first = false) {
             __syncthreads();
             if (t == 0) sm.n = 0, sm.least = ~0ull, sm.most = 0, sm.cut = 0, sm.sum = 0, sm.pick = kParts;
             if (have <= kSmall) {
                 __syncthreads();
-                members(b0, b1, [&](uint64_t k, uint32_t b, uint64_t m) {
+                members(of_k, [&](uint64_t k, uint32_t b, uint64_t m) {
                     if (k < r0 || k > r1) return;
                     const uint32_t at = atomicAdd(&sm.n, 1u);
                     if (at < kSmall) sm.small[at] = k, sm.small_w[at] = unit(m, b);
@@ -867,7 +890,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
             __syncthreads();
             if (!first) {  // equal logits: their ranks fill little of the range
                 uint64_t least = ~0ull, most = 0;
-                members(b0, b1, [&](uint64_t k, uint32_t, uint64_t) {
+                members(of_k, [&](uint64_t k, uint32_t, uint64_t) {
                     if (k < r0 || k > r1) return;
                     least = k < least ? k : least, most = k > most ? k : most;
                 });
@@ -880,7 +903,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
             }
             const uint64_t range = r1 - r0;
             const int sft = range < kParts ? 0 : 55 - __builtin_clzll(range);  // range >> sft < 512
-            members(b0, b1, [&](uint64_t k, uint32_t b, uint64_t m) {
+            members(of_k, [&](uint64_t k, uint32_t b, uint64_t m) {
                 if (k < r0 || k > r1) return;
                 const uint32_t d = kParts - 1 - static_cast<uint32_t>((k - r0) >> sft);  // falling
                 const Halves x = halve(unit(m, b));
@@ -942,7 +965,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
         if (for_k || by_sum == 0 || want > 0) {
             const uint32_t key0 = st.key[for_k ? 2 : 0], key1 = st.key[for_k ? 3 : 1];
             u128 with;
-            x = select(for_k ? bin_k : lo, for_k ? bin_k : hi, for_k ? st.in_k : st.in_l, static_cast<uint64_t>(key0) << 32,
+            x = select(for_k, for_k ? st.in_k : st.in_l, static_cast<uint64_t>(key0) << 32,
                        (static_cast<uint64_t>(key1) << 32) - 1, for_k ? st.count_k : st.count_l, for_k ? st.below_k : st.below_l,
                        by_sum != 0, k, want, &with);
             if (by_sum == 0) sum = with;
@@ -956,7 +979,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     if (t == 0) sm.n = 0;
     __syncthreads();
     if (any) {
-        members(lo, hi, [&](uint64_t k, uint32_t b, uint64_t m) {
+        members(false, [&](uint64_t k, uint32_t b, uint64_t m) {
             if (k < cut) return;
             const Halves x = halve(unit(m, b));
             const uint32_t slice = rank_index(k) / kSlice;
@@ -1080,7 +1103,8 @@ TWD_API int twd_sampler_create(uint32_t max_vocab, uint32_t max_rows, twd_sample
     if (!s) return fail(TWD_E_INVALID, "out of host memory");
     s->max_vocab = max_vocab, s->max_rows = max_rows, s->device = dev;
     const uint64_t slices = (max_vocab + kSlice - 1) / kSlice, rows = max_rows;
-    const uint64_t bins = rows * slices * kBins * sizeof(uint64_t), list = rows * kListCap * sizeof(uint64_t);
+    const uint32_t cap = static_cast<uint32_t>(slices) * kSlice < kListCap ? static_cast<uint32_t>(slices) * kSlice : kListCap;
+    const uint64_t bins = rows * slices * kBins * sizeof(uint64_t), list = rows * cap * sizeof(uint64_t);
     const uint64_t under = rows * slices * sizeof(u128), states = rows * sizeof(RowState);
     const uint64_t heads = rows * slices * sizeof(SliceHead);
     hipError_t e = hipSuccess;
@@ -1104,6 +1128,7 @@ TWD_API int twd_sampler_create(uint32_t max_vocab, uint32_t max_rows, twd_sample
     s->scratch.state = reinterpret_cast<RowState*>(at), at += states;
     s->scratch.head = reinterpret_cast<SliceHead*>(at);
     s->scratch.slices = static_cast<uint32_t>(slices);
+    s->scratch.list_cap = cap;
     *out = s;
     return TWD_OK;
 }
