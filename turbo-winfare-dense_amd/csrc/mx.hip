@@ -369,10 +369,12 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, uint3
 
 // ---- up to 16 hidden rows: the weights stream past rows held in registers ---------------------------
 //
-// Bound by the read of the head. The waves of a team split d_model by quads: a wave keeps its quad of the
+// Bound by the read of the head. The waves of a block split d_model by quads: a wave keeps its quad of the
 // hidden rows in registers for the whole launch and streams its quad of one group after another, kRing
-// chunks (4 KB each) ahead of the arithmetic. The teams' sums over the quads meet in LDS, two buffers in
-// turn, so that one barrier a group is enough and no load waits at it. One row of 262,144 x 5,376: 117 us,
+// chunks (4 KB each) ahead of the arithmetic. The sums over the quads meet in LDS, two buffers in turn, so
+// that one barrier a group is enough and no load waits at it. Where d_model has few quads, several blocks
+// share a compute unit (as one block of several groups, 32,003 x 2,048 left a third of the units idle: 10.5 us
+// instead of 8.6). One row of 262,144 x 5,376: 117 us,
 // 6.4 TB/s, of the 6.7 that a pure read reaches (a first, simple kernel took 193);
 // 7 quantised rows of 151,669 x 3,584: 47 us, 6.2 TB/s; one row of 32,003 x 2,048: 11.6 us, where a wave's first
 // bytes and the end of the launch are half of it.
@@ -381,11 +383,10 @@ constexpr uint32_t kSmallWaves = 12;  // 168 registers each
 constexpr uint32_t kRing = 4;
 
 template <bool MX, typename Out>
-__global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a, uint32_t teams, uint32_t cols) {
-    extern __shared__ float part[];  // [2][team][quad][cols][64]
+__global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a) {
+    extern __shared__ float part[];  // [2][quad][row][64]
     const uint32_t lane = threadIdx.x % 64, kg = lane / 16, r = lane % 16;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-    const uint32_t team = wave / a.quads, quad = wave % a.quads;
+    const uint32_t quad = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t blocks = a.d / kMxBlock;
     const uint32_t here = min(4u, a.chunks - 4 * quad);  // chunks of this wave
 
@@ -406,14 +407,14 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a, ui
         }
     }
 
-    const uint32_t step = gridDim.x * teams;
     // Buffer loads: the base in scalar registers, one lane offset for all. Past the quad's end (the last quad)
     // the last chunk comes again, whose hidden columns are zero.
+    // A group past the last has no bytes, so nothing is read of it.
     auto codes_of = [&](uint32_t g) {
-        return make_rsrc(a.codes + (static_cast<uint64_t>(g) * a.chunks + 4 * quad) * 256, here * 4096);
+        return make_rsrc(a.codes + (static_cast<uint64_t>(g) * a.chunks + 4 * quad) * 256, g < a.groups ? here * 4096 : 0);
     };
     auto scales_of = [&](uint32_t g) {
-        return make_rsrc(a.scales + (static_cast<uint64_t>(g) * a.quads + quad) * 256, 1024);
+        return make_rsrc(a.scales + (static_cast<uint64_t>(g) * a.quads + quad) * 256, g < a.groups ? 1024 : 0);
     };
     auto load_codes = [&](const __amdgpu_buffer_rsrc_t& at, uint32_t c, u32x4_t (&to)[4]) {
         const int chunk = static_cast<int>(min(c, here - 1) * 4096);
@@ -427,9 +428,8 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a, ui
     };
     u32x4_t w[kRing][4];
     uint32_t ws[4];
-    const uint32_t last = a.groups - 1, g0 = min(blockIdx.x * teams + team, last);
     {
-        const auto codes = codes_of(g0), scales = scales_of(g0);
+        const auto codes = codes_of(blockIdx.x), scales = scales_of(blockIdx.x);
 #pragma unroll
         for (uint32_t c = 0; c < kRing; ++c) {
             load_codes(codes, c, w[c]);
@@ -438,10 +438,8 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a, ui
         }
     }
     uint32_t buf = 0;
-    // every wave of the block takes the same number of turns
-    for (uint32_t base = blockIdx.x * teams; base < a.groups; base += step) {
-        const uint32_t g = base + team, next = min(g + step, last);
-        const auto codes = codes_of(next), scales = scales_of(next);
+    for (uint32_t g = blockIdx.x; g < a.groups; g += gridDim.x) {
+        const auto codes = codes_of(g + gridDim.x), scales = scales_of(g + gridDim.x);
         f32x4_t acc[4] = {};
         uint32_t s[4];
 #pragma unroll
@@ -469,17 +467,17 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a, ui
             if (c == 0) load_scales(scales, ws);
             __builtin_amdgcn_sched_barrier(0);
         }
-        float* mine = part + (static_cast<uint64_t>(buf * teams + team) * a.quads + quad) * cols * 64;
-        if (r < cols) {
+        float* mine = part + (buf * a.quads + quad) * a.rows * 64;
+        if (r < a.rows) {
 #pragma unroll
             for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4_t*>(mine + r * 64 + 16 * kg + 4 * j) = acc[j];
         }
         lds_barrier();
-        // the team's waves share the sums: element e is hidden row e / 64, vocabulary row e % 64
+        // the waves share the sums: element e is hidden row e / 64, vocabulary row e % 64
         for (uint32_t e = quad * 64 + lane; e < a.rows * 64; e += a.quads * 64) {
-            const float* p = part + static_cast<uint64_t>(buf * teams + team) * a.quads * cols * 64 + e;
+            const float* p = part + buf * a.quads * a.rows * 64 + e;
             float y[1] = {p[0]};
-            for (uint32_t q = 1; q < a.quads; ++q) y[0] += p[q * cols * 64];
+            for (uint32_t q = 1; q < a.quads; ++q) y[0] += p[q * a.rows * 64];
             cap_logits(y, a.softcap);
             const uint64_t v = static_cast<uint64_t>(g) * kMxGroupRows + e % 64;
             if (v < a.vocab) store_logit(static_cast<Out*>(a.out) + (e / 64) * a.out_stride + v, y[0]);
@@ -814,10 +812,9 @@ int launch_typed(const twd_mxhead* h, const MxArgs& a, hipStream_t s) {
     // tile 21), and so do quantised rows (16 of 131,072 x 4,608: 53 and 56 us).
     const bool tiles = !MX && a.rows > a.quads && a.groups >= kTileWaves * static_cast<uint32_t>(h->cus);
     if (a.rows <= kSmallRows && a.quads <= kSmallWaves && !tiles) {
-        const uint32_t teams = kSmallWaves / a.quads;
-        const uint32_t blocks = min((a.groups + teams - 1) / teams, static_cast<uint32_t>(h->cus));
-        const uint32_t lds = 2 * teams * a.quads * a.rows * 64 * sizeof(float);
-        mx_small_kernel<MX, Out><<<blocks, teams * a.quads * 64, lds, s>>>(a, teams, a.rows);
+        const uint32_t blocks = min(a.groups, kSmallWaves / a.quads * static_cast<uint32_t>(h->cus));
+        const uint32_t lds = 2 * a.quads * a.rows * 64 * sizeof(float);
+        mx_small_kernel<MX, Out><<<blocks, a.quads * 64, lds, s>>>(a);
         TWD_HIP(hipGetLastError());
         return TWD_OK;
     }
