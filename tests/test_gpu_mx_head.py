@@ -16,7 +16,7 @@ SHAPES = [  # vocab, d_model, rows
     (1, 32, 1), (15, 32, 1), (16, 128, 1), (17, 160, 2), (1000, 1024, 1), (1003, 2080, 3), (517, 5376, 1),
     (4099, 2048, 1), (777, 5376, 7), (640, 2880, 8), (333, 3584, 15), (65, 4096, 16), (131, 1056, 17),
     (1029, 512, 33), (300, 5376, 64), (259, 2880, 65), (515, 640, 129), (1031, 416, 300), (96, 8224, 5),
-    (70, 17440, 2), (33, 17440, 40), (2050, 96, 1025), (65600, 544, 9), (65540, 160, 2),
+    (70, 17440, 2), (33, 17440, 40), (2050, 96, 1025), (98400, 544, 9), (98310, 160, 2),
 ]
 
 

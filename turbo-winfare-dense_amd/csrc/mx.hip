@@ -376,7 +376,7 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, uint3
 // share a compute unit (as one block of several groups, 32,003 x 2,048 left a third of the units idle: 10.5 us
 // instead of 8.6). One row of 262,144 x 5,376: 117 us,
 // 6.4 TB/s, of the 6.7 that a pure read reaches (a first, simple kernel took 193);
-// 7 quantised rows of 151,669 x 3,584: 47 us, 6.2 TB/s; one row of 32,003 x 2,048: 11.6 us, where a wave's first
+// 7 quantised rows of 151,669 x 3,584: 47 us, 6.2 TB/s; one row of 32,003 x 2,048: 8.3 us, where a wave's first
 // bytes and the end of the launch are half of it.
 constexpr uint32_t kSmallRows = 16;
 constexpr uint32_t kSmallWaves = 12;  // 168 registers each
@@ -805,12 +805,12 @@ int launch_tile(const MxArgs& a, hipStream_t s) {
 
 template <bool MX, typename Out>
 int launch_typed(const twd_mxhead* h, const MxArgs& a, hipStream_t s) {
-    // Few rows stream (262,144 x 5,376, 1 row: 117 us; as a tile 137). The wider the rows' sums against the quads a
-    // wave reads between two of them, the more the joining costs, which a tile does not have: 8 bf16 rows of
-    // 131,072 x 3,584 took 48 us streamed and 41 as a tile, of 262,144 x 2,048 57 and 53, of 131,072 x 2,880 41 and
-    // 34. A head of less than a tile's block for every compute unit streams on (8 rows of 32,768 x 3,584: 15 us, as a
-    // tile 21), and so do quantised rows (16 of 131,072 x 4,608: 53 and 56 us).
-    const bool tiles = !MX && a.rows > a.quads && a.groups >= kTileWaves * static_cast<uint32_t>(h->cus);
+    // Few rows stream (262,144 x 5,376, 1 row: 116 us; as a tile 137). The more rows there are to the quads whose sums
+    // are joined, the more the joining costs, which a tile does not have: 8 bf16 rows of 131,072 x 2,880 took 42 us
+    // streamed and 34 as a tile, of 98,304 x 3,584 35 and 32, 16 of 262,144 x 1,024 34 and 31; but 12 of 262,144 x
+    // 5,376, whose quads fill a compute unit, 131 and 139, and 8 of 65,536 x 2,048, one tile's block to a unit, 16 and
+    // 21. Quantised rows, fewer bytes each, stream as fast or faster.
+    const bool tiles = !MX && a.rows > a.quads && a.quads <= 8 && a.groups >= 6 * static_cast<uint32_t>(h->cus);
     if (a.rows <= kSmallRows && a.quads <= kSmallWaves && !tiles) {
         const uint32_t blocks = min(a.groups, kSmallWaves / a.quads * static_cast<uint32_t>(h->cus));
         const uint32_t lds = 2 * a.quads * a.rows * 64 * sizeof(float);
