@@ -492,7 +492,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a) {
 // through LDS, loaded there without registers one stage ahead into the other of two buffers. A stage is a
 // chunk of bf16 rows (256 bytes a row) or a quad of quantised ones (4 x 64 bytes a row and 16 scales).
 //
-// Bound by the matrix instructions and the socket's power: 1,023 bf16 rows of 65,537 x 2,880 in 326 us, 1,185
+// Bound by the matrix instructions and the socket's power: 1,023 bf16 rows of 65,537 x 2,880 in 313 us, 1,233
 // TFLOP/s (a large library product: 1,237), 2,048 quantised rows of 262,144 x 5,376 in 1,980 us, 2,915 TFLOP/s
 // (3,008). 64 bf16 rows of 262,144 x 5,376 take 189 us, 90 and 26 more for every 16 rows, at a clock of 1.9 of 2.4
 // GHz: the energy of the reads and of the products adds up. Codes two chunks ahead, or stages of two chunks, changed
@@ -611,9 +611,12 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
         float f[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = __uint_as_float(((ws[j] >> (8 * (c % 4))) & 255u) << 23);
-        // two fragments are read from LDS while the two before them are multiplied
-        constexpr int kPairs = NT / 2;
-        bf16x8_t e[4], y[2][2];
+        // Two fragments are read from LDS while the two before them are multiplied, and tiles of 128 rows widen a part
+        // of the next step's codes beside them (1,023 rows: 326 to 313 us). Smaller tiles have no registers for it:
+        // 64 rows would leave two waves to a SIMD instead of three (of 196,608 x 5,376: 161 instead of 145 us).
+        constexpr bool kWidenAhead = NT == 8;
+        constexpr int kPairs = NT / 2, kWiden = 4 / kPairs;
+        bf16x8_t e[kWidenAhead ? 2 : 1][4], y[2][2];
         auto read = [&](int i) {
 #pragma unroll
             for (int k = 0; k < 2; ++k) y[i % 2][k] = __builtin_bit_cast(bf16x8_t, x(2 * (i % kPairs) + k, i / kPairs));
@@ -624,16 +627,21 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
         for (int i = 0; i < 4 * kPairs; ++i) {
             if (i + 1 < 4 * kPairs) read(i + 1);
             __builtin_amdgcn_sched_barrier(0);
-            if (i % kPairs == 0) {
+            const int t = i / kPairs;
+            if (kWidenAhead ? i == 0 : i % kPairs == 0) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) e[j] = widen(w[j][i / kPairs], f[j]);
+                for (int j = 0; j < 4; ++j) e[0][j] = widen(w[j][t], f[j]);
+            }
+            if (kWidenAhead && t < 3) {
+#pragma unroll
+                for (int j = i % kPairs * kWiden; j < (i % kPairs + 1) * kWiden; ++j) e[kWidenAhead ? (t + 1) % 2 : 0][j] = widen(w[j][t + 1], f[j]);
             }
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     f32x4_t& sum = acc[j][2 * (i % kPairs) + k];
-                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e[j], y[i % 2][k], sum, 0, 0, 0);
+                    sum = __builtin_amdgcn_mfma_f32_16x16x32_bf16(e[kWidenAhead ? t % 2 : 0][j], y[i % 2][k], sum, 0, 0, 0);
                 }
             __builtin_amdgcn_sched_barrier(0);
         }
