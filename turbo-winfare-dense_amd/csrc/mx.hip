@@ -492,31 +492,34 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a) {
 // through LDS, loaded there without registers one stage ahead into the other of two buffers. A stage is a
 // chunk of bf16 rows (256 bytes a row) or a quad of quantised ones (4 x 64 bytes a row and 16 scales).
 //
-// Bound by the matrix instructions and the socket's power: 1,023 bf16 rows of 65,537 x 2,880 in 313 us, 1,233
-// TFLOP/s (a large library product: 1,237), 2,048 quantised rows of 262,144 x 5,376 in 1,980 us, 2,915 TFLOP/s
-// (3,008). 64 bf16 rows of 262,144 x 5,376 take 189 us, 90 and 26 more for every 16 rows, at a clock of 1.9 of 2.4
-// GHz: the energy of the reads and of the products adds up. Codes two chunks ahead, or stages of two chunks, changed
-// none of these by more than a run to run does (64 rows: 194 and 198; 1,023: 325 and 321).
+// From 128 rows on bound by the matrix instructions, whose clock follows the socket's power (1,024 rows of 262,144 x
+// 5,376: 1,360 TFLOP/s, 1,577 where all weights are zero): 1,023 bf16 rows of 65,537 x 2,880 in 313 to 325 us from
+// card to card, 1,188 to 1,233 TFLOP/s (a large library product: 1,237), 2,048 quantised rows of 262,144 x 5,376 in
+// 1,970 to 2,000 us, 2,890 to 2,930 TFLOP/s (3,008). 64 bf16 rows of 262,144 x 5,376 take 176 us, whatever the data:
+// 112 are the reads of the head, with its codes served by an L2 it would be 127, without the logits' stores 156.
+// Codes two chunks ahead, stages of two chunks and two blocks to a compute unit instead of three did not bring the two
+// together (within 3%).
 constexpr uint32_t kTileWaves = 4;
 constexpr int kVmcnt0 = 0x0F70;  // s_waitcnt vmcnt(0), no other counter
 
 typedef __attribute__((address_space(3))) void lds_void;
 
 template <typename Out>
-__device__ __forceinline__ void store_logits(Out* p, const float* y, uint32_t n) {  // n of 16
-    if (n >= 16) {
-        if constexpr (sizeof(Out) == 4) {
-            __builtin_memcpy(p, y, 64);
-        } else {
-            uint32_t w[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] = bf16_bits(y[2 * i]) | (bf16_bits(y[2 * i + 1]) << 16);
-            __builtin_memcpy(p, w, 32);
-        }
+struct Sixteen {
+    Out e[16 / sizeof(Out)];
+};
+
+// 16 bytes of logits at any alignment, n of them at most; they are not read here again.
+template <typename Out>
+__device__ __forceinline__ void store_logits(Out* p, u32x4_t v, uint32_t n) {
+    constexpr uint32_t kEach = 16 / sizeof(Out);
+    typedef u32x4_t __attribute__((aligned(2))) any_place_t;
+    if (n >= kEach) {
+        __builtin_nontemporal_store(v, reinterpret_cast<any_place_t*>(p));
     } else {
 #pragma unroll
-        for (uint32_t i = 0; i < 16; ++i)
-            if (i < n) store_logit(p + i, y[i]);
+        for (uint32_t i = 0; i < kEach; ++i)
+            if (i < n) p[i] = __builtin_bit_cast(Sixteen<Out>, v).e[i];
     }
 }
 
@@ -742,20 +745,47 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
             });
         }
     }
-    const uint64_t v = g * kMxGroupRows + 16 * kg;
-    if (!have_group || v >= a.vocab) return;
-    const uint32_t n_v = v + 16 <= a.vocab ? 16u : a.vocab - static_cast<uint32_t>(v);
+    // A lane's 16 logits of a row are a quarter of the wave's 64: they change places in LDS, so that a store fills
+    // whole lines (64 rows of 262,144 x 5,376: 192 us with stores of a lane's own 16, 184 with whole lines, 176 with
+    // whole lines past the caches).
+    __syncthreads();  // nobody reads the hidden rows any more
+    if (!have_group) return;
+    constexpr uint32_t kPieces = 4 * sizeof(Out), kOwn = kPieces / 4, kEach = 16 / sizeof(Out);  // of 16 bytes: of a row, of a lane
+    u32x4_t* const mine = (wave < 2 ? buf0 : buf1) + wave % 2 * (kStage / 2);
+    auto place = [&](uint32_t row, uint32_t piece) {
+        const uint32_t p = kPieces == 16 ? 4 * (0x9cu >> (2 * (piece / 4)) & 3) + piece % 4 : piece;
+        return row * kPieces + (p ^ row % kPieces);
+    };
+    const uint64_t v = g * kMxGroupRows + kEach * (lane % kPieces);
+    const uint32_t n_v = v < a.vocab ? static_cast<uint32_t>(min<uint64_t>(a.vocab - v, kEach)) : 0u;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-        const uint32_t m = m0 + 16 * n + r;
-        if (m >= a.rows) continue;
         float y[16];
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i) y[4 * j + i] = acc[j][n][i];
         cap_logits(y, a.softcap);
-        store_logits(static_cast<Out*>(a.out) + m * a.out_stride + v, y, n_v);
+#pragma unroll
+        for (uint32_t k = 0; k < kOwn; ++k) {
+            u32x4_t w;
+            if constexpr (sizeof(Out) == 4) {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) w[i] = __float_as_uint(y[4 * k + i]);
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) w[i] = bf16_bits(y[8 * k + 2 * i]) | (bf16_bits(y[8 * k + 2 * i + 1]) << 16);
+            }
+            mine[place(r, kOwn * kg + k)] = w;
+        }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (uint32_t k = 0; k < kOwn; ++k) {
+            const uint32_t row = k * (64 / kPieces) + lane / kPieces, m = m0 + 16 * n + row;
+            const u32x4_t w = mine[place(row, lane % kPieces)];
+            if (m < a.rows) store_logits(static_cast<Out*>(a.out) + m * a.out_stride + v, w, n_v);
+        }
+        __builtin_amdgcn_wave_barrier();
     }
 }
 
