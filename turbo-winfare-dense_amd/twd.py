@@ -756,25 +756,37 @@ class _Here:
 _here = _Here()
 
 
+_device_now = None  # the current device's number
+_stream_now = None  # the handle of a device's current stream
+
+
+def _bind_torch():
+    """torch's own lookups where it has them: a tenth of the time of current_stream(), half of current_device()'s."""
+    global _device_now, _stream_now
+    import torch
+    _stream_now = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    _device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
 def _on_device(*tensors):
     """A guard that makes the tensors' one device the current one for the call."""
-    import torch
     dev = tensors[0].get_device()
     for t in tensors:
         if t is not None and t.get_device() != dev:
             raise ValueError(f"tensors on {tensors[0].device} and {t.device} in one call")
     if dev < 0:
         raise ValueError(f"device tensors are needed, not tensors on {tensors[0].device}")
-    return _here if torch.cuda.current_device() == dev else torch.cuda.device(dev)
+    if _device_now is None:
+        _bind_torch()
+    if _device_now() == dev:
+        return _here
+    import torch
+    return torch.cuda.device(dev)
 
 
 def _stream_on(t, stream=None):
     """The stream given, or the current one of the tensor's device (which the guard made the current device)."""
-    if stream is not None:
-        return stream
-    import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # a tenth of the time of current_stream()
-    return raw(t.get_device()) if raw is not None else torch.cuda.current_stream(t.device).cuda_stream
+    return _stream_now(t.get_device()) if stream is None else stream
 
 
 def _matrix(t, what: str):
