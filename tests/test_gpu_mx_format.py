@@ -163,3 +163,18 @@ def test_captured_on_another_stream():
         assert torch.equal(c, codes) and torch.equal(sc, scales), rep
         assert torch.equal(t.mx_dequantize(c, sc), out), rep
     del g
+
+
+def test_rows_more_than_4_gib_apart():
+    import torch
+    t = twd()
+    x = np.random.default_rng(8).standard_normal((2, 64)).astype(np.float32)
+    far = (1 << 31) + 8
+    buf = torch.empty(far + 64, dtype=torch.bfloat16, device="cuda:0")
+    v = buf.as_strided((2, 64), (far, 1))
+    v.copy_(torch.from_numpy(x))
+    want = quantize_ref(v.double().cpu().numpy())
+    codes, scales = t.mx_quantize(v)
+    assert np.array_equal(codes.cpu().numpy(), want[0]) and np.array_equal(scales.cpu().numpy(), want[1])
+    t.mx_dequantize(codes, scales, out=v)
+    assert np.array_equal(v.double().cpu().numpy(), values_ref(*want))

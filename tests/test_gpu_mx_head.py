@@ -146,6 +146,21 @@ def test_hidden_rows_far_apart(rows, stride):
     head.close()
 
 
+@pytest.mark.parametrize("rows", [3, 40])
+def test_logits_more_than_4_gib_apart(rows):
+    import torch
+    t = twd()
+    rng = np.random.default_rng(rows)
+    codes, scales = random_matrix(rng, 70, 288)
+    h = rng.integers(-4, 5, (rows, 288)).astype(np.float32)
+    far = ((1 << 32) + 4096) // 2 // (rows - 1) + 1
+    out = torch.empty((rows - 1) * far + 70, dtype=torch.bfloat16, device="cuda:0").as_strided((rows, 70), (far, 1))
+    head = t.MxHead(dev(codes), dev(scales))
+    want = torch.from_numpy(h.astype(np.float64) @ decode(codes, scales).T).to(torch.bfloat16)
+    assert torch.equal(head.logits(dev(h).bfloat16(), out=out).cpu(), want)
+    head.close()
+
+
 @pytest.mark.parametrize("rows", [1, 20, 70])
 @pytest.mark.parametrize("mx", [False, True])
 def test_nan_and_inf_rows_stay_theirs(rows, mx):

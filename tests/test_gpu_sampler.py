@@ -143,6 +143,15 @@ def test_equal_logits(vocab):
     check(dev(a), [1.0] * 10, ks, ps, [0.0, 0, 1.0, 0, 0, 0, 1.0, 0.5, 0.25, 0.25], us, tag="equal")
 
 
+def test_rows_more_than_4_gib_apart():
+    import torch
+    rng = np.random.default_rng(9)
+    far, vocab = (1 << 30) + 5, 20000
+    v = torch.empty(far + vocab, device="cuda:0").as_strided((2, vocab), (far, 1))
+    v.copy_(torch.from_numpy(rows_of(rng, 2, vocab)))
+    check(v, [0.7, 1.2], [0, 300], [0.9, 0.8], [0.0, 0.01], [0.3, 0.8], tag="far")
+
+
 def test_masks():
     """Rows of -inf but for a few entries, one or none; masks of the type's lowest value; NaN and +inf."""
     rng = np.random.default_rng(5)
