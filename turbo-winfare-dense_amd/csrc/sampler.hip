@@ -274,6 +274,11 @@ struct Halves {
 __device__ __forceinline__ Halves halve(u128 x) {
     return Halves{static_cast<uint64_t>(x) & ((uint64_t{1} << kHalf) - 1), static_cast<uint64_t>(x >> kHalf)};
 }
+// halve(unit(q, bin)) of one weight, without 128-bit shifts.
+__device__ __forceinline__ Halves unit_halves(uint64_t q, uint32_t bin) {
+    static_assert(kSumShift == kHalf + 1 && kTailOct < kHalf, "no bit of a weight is lost");
+    return Halves{(q << (kSumShift - (bin >> 3))) & ((uint64_t{1} << kHalf) - 1), (q << 1) >> (bin >> 3)};
+}
 __device__ __forceinline__ u128 join(const Halves& h) { return (static_cast<u128>(h.hi) << kHalf) + h.lo; }
 __device__ __forceinline__ uint64_t wave_incl_scan_u64(uint64_t x) {
     x += dpp_move<0x111>(uint64_t{0}, x);
@@ -776,10 +781,10 @@ struct FinishMem {
     uint32_t n, base_n, pick, id, last;
 };
 
-// One block to a row: 9.6 us for one row, the slowest of 64 takes 21 and of 256 bf16 rows (2,000 listed entries of a
-// few values each) 31. About half goes to the cuts, a round of adding up by parts after another, a quarter to the
-// weights of the one slice that the draw falls in (11,900 cycles where all of it is kept; vector units). 1,024
-// threads: 13.7 us for one row, 39 for 256.
+// One block to a row: 9.7 us for one row, the slowest of 64 takes 19 and of 256 bf16 rows (2,000 listed entries of a
+// few values each) 29. About half goes to the cuts, a round of adding up by parts after another, a quarter to the
+// weights of the one slice that the draw falls in, where all of it is kept (vector units of one compute unit; with sums
+// of 128 bits instead of halves there and in the rounds 21 and 31 us). 1,024 threads: 13.7 us for one row, 39 for 256.
 template <typename T, bool TINY>
 __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a) {
     extern __shared__ char finish_mem[];
@@ -906,7 +911,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
             members(of_k, [&](uint64_t k, uint32_t b, uint64_t m) {
                 if (k < r0 || k > r1) return;
                 const uint32_t d = kParts - 1 - static_cast<uint32_t>((k - r0) >> sft);  // falling
-                const Halves x = halve(unit(m, b));
+                const Halves x = unit_halves(m, b);
                 // Equal logits meet in one part: while a wave's first entry has company, the lanes that hold its part
                 // and its weight add up as one.
                 bool todo = true;
@@ -981,7 +986,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     if (any) {
         members(false, [&](uint64_t k, uint32_t b, uint64_t m) {
             if (k < cut) return;
-            const Halves x = halve(unit(m, b));
+            const Halves x = unit_halves(m, b);
             const uint32_t slice = rank_index(k) / kSlice;
             atomicAdd(&sm.slice_lo[slice], static_cast<unsigned long long>(x.lo));
             atomicAdd(&sm.slice_hi[slice], static_cast<unsigned long long>(x.hi));
@@ -1015,26 +1020,27 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     }
     __syncthreads();
     constexpr uint32_t kWeighs = 1u << 20;  // above every index
-    // the weight of entry j of thread `by`, where it is kept
-    auto drawn = [&](uint32_t by, uint32_t j, float l) -> u128 {
-        if (!(l > -INFINITY) || rank_key(l, first + kStageEach * by + j) < cut) return 0;
-        uint32_t b;
-        const uint64_t m = weight(l, &b);
-        return unit(m, b);
+    // the weight of entry j of thread `by`, 0 where it is not kept
+    auto kept_at = [&](uint32_t by, uint32_t j, float l) {
+        return l > -INFINITY && rank_key(l, first + kStageEach * by + j) >= cut;
     };
     const float floor_l = key_float(static_cast<uint32_t>(cut >> 32));  // (NaN for no cut: nothing lies below it)
-    u128 run = 0;
+    Halves sums{0, 0};
     uint32_t last = 0;
 #pragma unroll 1
     for (uint32_t j = 0; j < kStageEach; ++j) {
         const float l = sm.stage[t * kStageStride + j];
         if (__ballot(l > -INFINITY && !(l < floor_l)) == 0) continue;
-        const u128 e = drawn(t, j, l);
+        const bool in = kept_at(t, j, l);
+        uint32_t b;
+        const uint64_t m = weight(l, &b);
+        const Halves x = unit_halves(in ? m : 0, b);
+        sums.lo += x.lo, sums.hi += x.hi;
         const uint32_t i = first + kStageEach * t + j;
-        if (l > -INFINITY && rank_key(l, i) >= cut) last = e != 0 ? (i + 1) | kWeighs : (last > kWeighs ? last : i + 1);
-        run += e;
+        if (in) last = m != 0 ? (i + 1) | kWeighs : (last > kWeighs ? last : i + 1);
     }
-    const u128 mine = run;
+    const u128 mine = join(sums);
+    u128 run = mine;
     last = wave_reduce(last, 0u, [](uint32_t p, uint32_t q) { return p > q ? p : q; });
     if (lane == 0 && last != 0) atomicMax(&sm.last, last);
     u128 ignored;
@@ -1049,8 +1055,11 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     const bool found = sm.id != ~0u;
     const uint32_t end = (sm.last & (kWeighs - 1)) - 1, by = found ? sm.id : (end - first) / kStageEach;
     const uint32_t id = first + kStageEach * by + t;
-    const u128 e = drawn(by, t, sm.stage[by * kStageStride + t]);
-    Halves h = halve(e);
+    const float l = sm.stage[by * kStageStride + t];
+    uint32_t b;
+    const uint64_t m = weight(l, &b);
+    Halves h = unit_halves(kept_at(by, t, l) ? m : 0, b);
+    const u128 e = join(h);
     h.lo = row_incl_scan_u64(h.lo), h.hi = row_incl_scan_u64(h.hi);
     const u128 upto = join(h);
     if (found ? upto > sm.want && upto - e <= sm.want : id == end) {
