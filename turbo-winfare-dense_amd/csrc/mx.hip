@@ -493,9 +493,9 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a) {
 // chunk of bf16 rows (256 bytes a row) or a quad of quantised ones (4 x 64 bytes a row and 16 scales).
 //
 // From 128 rows on bound by the matrix instructions, whose clock follows the socket's power (1,024 rows of 262,144 x
-// 5,376: 1,360 TFLOP/s, 1,577 where all weights are zero): 1,023 bf16 rows of 65,537 x 2,880 in 313 to 325 us from
-// card to card, 1,188 to 1,233 TFLOP/s (a large library product: 1,237), 2,048 quantised rows of 262,144 x 5,376 in
-// 1,970 to 2,000 us, 2,890 to 2,930 TFLOP/s (3,008). 64 bf16 rows of 262,144 x 5,376 take 176 us, whatever the data:
+// 5,376: 1,360 TFLOP/s, 1,577 where all weights are zero): 1,023 bf16 rows of 65,537 x 2,880 in 313 to 331 us from
+// card to card, 1,165 to 1,233 TFLOP/s (a large library product: 1,237), 2,048 quantised rows of 262,144 x 5,376 in
+// 1,966 to 2,051 us, 2,815 to 2,936 TFLOP/s (3,008). 64 bf16 rows of 262,144 x 5,376 take 176 us, whatever the data:
 // 112 are the reads of the head, with its codes served by an L2 it would be 127, without the logits' stores 156.
 // Codes two chunks ahead, stages of two chunks and two blocks to a compute unit instead of three did not bring the two
 // together (within 3%).
