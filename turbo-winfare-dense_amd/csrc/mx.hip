@@ -594,7 +594,7 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
     f32x4_t acc[4][NT] = {};
     const auto codes = make_rsrc(a.codes + g * a.chunks * 256, a.chunks * 4096);
     const auto scales = make_rsrc(a.scales + g * a.quads * 256, a.quads * 1024);
-    constexpr int kWeights = 0;  // cache policy
+    constexpr int kWeights = 0;  // cached: the tiles of other hidden rows read them again from the L2
     // w, ws: the chunk's codes and the quad's scales; wn, wsn: the next ones, on their way
     u32x4_t w[4], wn[4];
     uint32_t ws[4], wsn[4];
