@@ -173,6 +173,10 @@ def _load() -> C.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built; run __graft_entry__.build() "
                           "(or python turbo-winfare-dense_amd/build.py) first")
+    try:  # torch first: the library then binds to its HIP runtime, where it would bring a second one along
+        import torch  # noqa: F401
+    except ImportError:  # the host-side calls need no torch
+        pass
     lib = C.CDLL(LIB_PATH)
     for name, (res, args) in _SIGS.items():
         fn = getattr(lib, name)
