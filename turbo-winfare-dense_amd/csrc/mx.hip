@@ -353,6 +353,7 @@ __device__ __forceinline__ bf16x8_t widen(uint32_t w, float s) {
     e[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
     return __builtin_bit_cast(bf16x8_t, e);
 }
+// The scale of byte c as the conversion reads it, by its exponent field alone: 0 is 2^-127 there.
 __device__ __forceinline__ float scale_float(uint32_t word, int c) { return __uint_as_float(((word >> (8 * c)) & 255u) << 23); }
 
 // A barrier that waits for the wave's LDS accesses only: loads on their way into registers stay in flight.
