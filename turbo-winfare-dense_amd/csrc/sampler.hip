@@ -9,9 +9,11 @@
 //
 // Arithmetic. Sums decide, so they may not depend on the order in which threads add: weights are
 // fixed-point numbers and sums are integers. With z = l log2(e) / T (formed in two doubles), a weight is
-// 2^floor(z) times the fraction's power of two, rounded to 37 bits (2^-37 relative); sums are held in 128
-// bits whose unit is 2^-77 of the largest weight's octave, so nothing above that is dropped. Every decision
-// is then an exact comparison of integers, and equal logits have equal weights.
+// 2^floor(z) times the fraction's power of two, rounded to 37 bits (2^-37 relative). Sums are held in 128
+// bits, in units of 2^-77 of the largest weight's octave. Weights from 31 octaves under that one on lose their
+// bits below 2^-67 of it, and what lies 67 or more octaves down weighs nothing: 524,288 such weights are at most 2^-47 of a
+// row's sum, where a draw's own steps are 2^-24. Every decision is then an exact comparison of integers, and
+// equal logits have equal weights.
 #include <hip/hip_runtime.h>
 
 #include <cmath>
@@ -151,6 +153,10 @@ constexpr uint32_t kSlice = 8192;
 constexpr uint32_t kBins = 256;
 constexpr uint32_t kTail = kBins - 1;
 constexpr uint32_t kTailOct = kTail >> 3;
+// From this octave on a weight (37 bits, 36 where it is least) may be nothing in the last bin's unit. It counts as nothing
+// everywhere then: in its own sum as in its slice's, whose entries add up before they are shifted and would leave
+// a sum that none of them has.
+constexpr uint32_t kNothingOct = kTailOct + 36;
 // Entries in the deciding bins: up to kNearCap of them are kept in LDS while they are cut, up to kListCap read from the
 // list each time, and more (nearly equal logits) from the row.
 constexpr uint32_t kNearCap = 4096, kListCap = 32768;
@@ -250,7 +256,7 @@ __device__ __forceinline__ uint32_t bin_of(double place, double top) {
 __device__ __forceinline__ uint64_t mass_of(uint64_t q, double place, uint32_t bin, double top) {
     if (bin != kTail) return q;
     const double deep = top - octave_of(place) - static_cast<double>(kTailOct);
-    return deep < 64.0 ? q >> static_cast<int>(deep) : 0;
+    return deep < static_cast<double>(kNothingOct - kTailOct) ? q >> static_cast<int>(deep) : 0;
 }
 // The two of one logit; eighths: the table's, in LDS.
 __device__ __forceinline__ uint64_t entry_weight(float l, const Scale& c, const WeightTable& k, const double* eighths, double top,
@@ -451,10 +457,12 @@ __device__ __forceinline__ uint32_t row_bin(uint32_t b, uint32_t shift, uint32_t
     return kTail;
 }
 constexpr uint32_t kNoSlice = 255;  // the shift of a slice whose bins are not written
+constexpr uint32_t kFarSlice = 128;  // and of one that lies too deep: its entries count, and every sum is shifted to nothing
+static_assert(kFarSlice - kTailOct >= 64, "row_bin's shift");
 __device__ __forceinline__ uint32_t slice_shift(const SliceHead& h, double top, const Scale& c) {
     if (h.weighed == 0) return kNoSlice;
     const double d = top - __builtin_floor(static_cast<double>(rank_value(h.best)) * c.hi);
-    return d < 128.0 ? static_cast<uint32_t>(d) : 128u;
+    return d < static_cast<double>(kNothingOct) ? static_cast<uint32_t>(d) : kFarSlice;
 }
 
 // The least key at which `yes` holds, by a wave: it holds from there up to `above`, where it is taken to hold.
