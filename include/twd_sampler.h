@@ -28,8 +28,8 @@ extern "C" {
  * holds a NaN or +inf logit or no entry above -inf, and one whose T, top_p, min_p or uniform is NaN,
  * gives TWD_TOKEN_DEGENERATE, a NaN logprob and 0 kept.
  *
- * Sums are integers (weights of 37 bits; a weight 67 octaves under the largest, of a logit about 46.4 T
- * below it, and less counts as nothing in them), so results do not depend on the launch, the batch or
+ * Sums are integers (weights of 37 bits; a weight under 2^-66 of the largest, of a logit 45.7 T and more
+ * below it, may count as nothing in them), so results do not depend on the launch, the batch or
  * the run. logits are rows of `type` with row_stride elements between them, at any alignment of that
  * type, and stay as they are. A sampler holds the scratch of up to max_rows (4,096) rows of up to
  * max_vocab (524,288) entries, about 330 KB a row of 262,144; its calls are ordered across streams as a

@@ -46,3 +46,14 @@ def test_least_positive_draws_take_an_id_with_weight(depth):
             want = z[tok[m]] - math.log(np.exp(z).sum())
             assert abs(float(lp[m]) - want) <= 2.0 ** -24 * abs(want) + 2.0 ** -36, (depth, u, m)
     sam.close()
+
+
+@pytest.mark.parametrize("depth", [5.0, 20.0, 23.0, 30.0, 36.0, 40.0, 44.0])
+@pytest.mark.parametrize("temp", [1.0, 0.3])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_logprobs_of_deep_ids(depth, temp, dtype):
+    """A draw of 0 takes the first id, whose logprob is as near as any other's."""
+    rows = np.stack([stairs([depth, 8.0, 0.0, 3.0], temp), stairs([depth, depth, depth, 0.0], temp),
+                     stairs([0.0, depth, 2.0, depth], temp)])
+    rows[1, ::5] = -np.inf  # the first id and others masked
+    check(dev(rows, dtype), [temp] * 3, None, None, None, [0.0, 0.0, 0.0], tag=("deep", depth))

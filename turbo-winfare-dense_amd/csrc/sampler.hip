@@ -11,8 +11,8 @@
 // fixed-point numbers and sums are integers. With z = l log2(e) / T (formed in two doubles), a weight is
 // 2^floor(z) times the fraction's power of two, rounded to 37 bits (2^-37 relative). Sums are held in 128
 // bits, in units of 2^-77 of the largest weight's octave. Weights from 31 octaves under that one on lose their
-// bits below 2^-67 of it, and what lies 67 or more octaves down weighs nothing: 524,288 such weights are at most 2^-47 of a
-// row's sum, where a draw's own steps are 2^-24. Every decision is then an exact comparison of integers, and
+// bits below 2^-67 of it, and what lies 67 or more octaves below it weighs nothing (so less than 2^-66 of the largest): 524,288
+// such weights are at most 2^-47 of a row's sum, where a draw's own steps are 2^-24. Every decision is then an exact comparison of integers, and
 // equal logits have equal weights.
 #include <hip/hip_runtime.h>
 
@@ -1072,7 +1072,15 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     const u128 upto = join(h);
     if (found ? upto > sm.want && upto - e <= sm.want : id == end) {
         a.o.tokens[r] = id;
-        if (a.o.logprobs) a.o.logprobs[r] = static_cast<float>(log(to_double(e) / to_double(kept)));
+        if (a.o.logprobs) {
+            double p = log(to_double(e) / to_double(kept));
+            if (b == kTail) {  // a weight that has lost bits: from the logit, counted from the largest
+                const float best = rank_value(st.best);
+                const uint64_t q = weight(best, &b);
+                p = (static_cast<double>(l) - best) / temp + log(to_double(unit(q, b)) / to_double(kept));
+            }
+            a.o.logprobs[r] = static_cast<float>(p);
+        }
         if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(any ? st.count_l + sm.n : st.live);
     }
 }
