@@ -29,11 +29,12 @@ extern "C" {
  * gives TWD_TOKEN_DEGENERATE, a NaN logprob and 0 kept.
  *
  * Sums are integers (weights of 37 bits; a weight under 2^-66 of the largest, of a logit 45.7 T and more
- * below it, may count as nothing in them), so results do not depend on the launch, the batch or
- * the run. logits are rows of `type` with row_stride elements between them, at any alignment of that
- * type, and stay as they are. A sampler holds the scratch of up to max_rows (4,096) rows of up to
- * max_vocab (524,288) entries, about 330 KB a row of 262,144; its calls are ordered across streams as a
- * selector's are, and replays of captured calls are ordered by the caller. Asynchronous on `stream`. */
+ * below it, may count as nothing in them, but for a draw of 0, which takes the first kept id down to
+ * 745 T below), so results do not depend on the launch, the batch or the run. logits are rows of `type`
+ * with row_stride elements between them, at any alignment of that type, and stay as they are. A sampler
+ * holds the scratch of up to max_rows (4,096) rows of up to max_vocab (524,288) entries, about 330 KB a
+ * row of 262,144; its calls are ordered across streams as a selector's are, and replays of captured
+ * calls are ordered by the caller. Asynchronous on `stream`. */
 typedef struct twd_sampler twd_sampler;
 TWD_API int twd_sampler_create(uint32_t max_vocab, uint32_t max_rows, twd_sampler** out);
 TWD_API void twd_sampler_destroy(twd_sampler* sampler);

@@ -1,4 +1,6 @@
-"""Draws where kept ids lie far under the largest logit, down to weights that the sums no longer hold."""
+"""Draws where kept ids lie far under the largest logit, down to weights that the sums no longer hold: a draw of 0
+takes the first kept id as the definition in 64 bits does, a draw of 1 never one without weight, and a logprob is
+as near for these as for any other."""
 import math
 
 import numpy as np
@@ -57,3 +59,31 @@ def test_logprobs_of_deep_ids(depth, temp, dtype):
                      stairs([0.0, depth, 2.0, depth], temp)])
     rows[1, ::5] = -np.inf  # the first id and others masked
     check(dev(rows, dtype), [temp] * 3, None, None, None, [0.0, 0.0, 0.0], tag=("deep", depth))
+
+
+@pytest.mark.parametrize("depth", [5.0, 20.0, 23.0, 30.0, 36.0, 40.0, 44.0, 46.0, 48.0, 50.0, 53.0, 55.0, 100.0, 700.0])
+@pytest.mark.parametrize("temp", [1.0, 0.3])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16", "float16"])
+def test_draw_of_zero_takes_the_first_kept_id(depth, temp, dtype):
+    rows = np.stack([stairs([depth, 8.0, 0.0, 3.0], temp), stairs([depth, depth, depth, 0.0], temp),
+                     stairs([0.0, depth, 2.0, depth], temp)])
+    rows[1, ::5] = -np.inf  # the first id and others masked
+    for us in ([0.0, 0.0, 0.0], [-0.0, -1.0, -math.inf]):
+        check(dev(rows, dtype), [temp] * 3, None, None, None, us, tag=("zero", depth))
+
+
+def test_masks_of_the_lowest_value_are_not_drawn():
+    """Ids whose weight is 0 in 64 bits too, before and behind the live ones."""
+    a = np.full((4, 3 * SLICE + 7), np.finfo(np.float32).min, np.float32)
+    a[0, 100] = a[1, SLICE + 5] = a[2, 3 * SLICE + 6] = 1.0
+    a[3, [SLICE, 2 * SLICE]] = [-1.0, 4.0]
+    for u in (0.0, -1.0, 0.5, 1.0):
+        check(dev(a), [0.7] * 4, None, None, None, [u] * 4, tag=("lowest", u))
+
+
+@pytest.mark.parametrize("k,p,mp", [(3, 1.0, 0.0), (SLICE + 100, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.1), (0, 1.0, 1e-12),
+                                    (0, 1.0, 1e-30), (2 * SLICE, 0.999, 1e-20)])
+def test_draw_of_zero_under_limits(k, p, mp):
+    rows = np.stack([stairs([50.0, 8.0, 0.0, 3.0], 1.0), stairs([40.0, 28.0, 0.0, 27.0], 1.0),
+                     stairs([12.0, 0.0, 50.0, 52.0], 1.0)])
+    check(dev(rows), [1.0] * 3, [k] * 3, [p] * 3, [mp] * 3, [0.0] * 3, tag=("limits", k, p, mp))

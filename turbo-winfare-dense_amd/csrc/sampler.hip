@@ -1008,7 +1008,21 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     u128 w = own;
     block_scan<kMaxSlices / 64>(n, w, &n_all, &kept, sm.scan);
     const u128 want = u < 1.0f ? part_of(u, kept, false) : kept - 1;  // the first running sum past this is drawn
-    if (t < a.slices && w > want && w - own <= want) sm.pick = t, sm.want = want - (w - own);
+    // A draw of 0 takes the first kept id, however little it weighs: the first slice whose largest rank is kept, and
+    // there the first kept entry. What even a double holds nothing of (exp of less than -745.14, 1,075 octaves) weighs nothing.
+    const bool at_zero = !(u > 0.0f);
+    const float largest = rank_value(st.best);
+    auto positive = [&](float l) { return (static_cast<double>(l) - largest) * c.hi > -1075.0; };
+    if (at_zero) {
+        static_assert(kMaxSlices == 64, "a wave's lanes are the slices");
+        if (t < kMaxSlices) {
+            const uint64_t rank = t < a.slices ? a.s.head[r * a.s.slices + t].best : 0;
+            const uint64_t in = __ballot(rank != 0 && rank >= cut && positive(rank_value(rank)));
+            if (t == 0) sm.pick = static_cast<uint32_t>(__builtin_ctzll(in)), sm.want = 0;  // (the row's largest is one)
+        }
+    } else if (t < a.slices && w > want && w - own <= want) {
+        sm.pick = t, sm.want = want - (w - own);
+    }
     __syncthreads();
     const uint32_t first = sm.pick * kSlice;
     const u128 rest = sm.want;
@@ -1028,7 +1042,12 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     }
     __syncthreads();
     constexpr uint32_t kWeighs = 1u << 20;  // above every index
-    // the weight of entry j of thread `by`, 0 where it is not kept
+    // what entry j of thread `by` counts for in the walk: its weight, or, for a draw of 0, anything at all
+    auto counts_for = [&](float l, uint32_t* bin) {
+        if (!at_zero) return weight(l, bin);
+        *bin = 0;
+        return positive(l) ? uint64_t{1} : 0;
+    };
     auto kept_at = [&](uint32_t by, uint32_t j, float l) {
         return l > -INFINITY && rank_key(l, first + kStageEach * by + j) >= cut;
     };
@@ -1041,7 +1060,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
         if (__ballot(l > -INFINITY && !(l < floor_l)) == 0) continue;
         const bool in = kept_at(t, j, l);
         uint32_t b;
-        const uint64_t m = weight(l, &b);
+        const uint64_t m = counts_for(l, &b);
         const Halves x = unit_halves(in ? m : 0, b);
         sums.lo += x.lo, sums.hi += x.hi;
         const uint32_t i = first + kStageEach * t + j;
@@ -1065,7 +1084,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     const uint32_t id = first + kStageEach * by + t;
     const float l = sm.stage[by * kStageStride + t];
     uint32_t b;
-    const uint64_t m = weight(l, &b);
+    const uint64_t m = counts_for(l, &b);
     Halves h = unit_halves(kept_at(by, t, l) ? m : 0, b);
     const u128 e = join(h);
     h.lo = row_incl_scan_u64(h.lo), h.hi = row_incl_scan_u64(h.hi);
@@ -1073,12 +1092,13 @@ __global__ __launch_bounds__(kRowThreads) void sample_finish_kernel(SampleArgs a
     if (found ? upto > sm.want && upto - e <= sm.want : id == end) {
         a.o.tokens[r] = id;
         if (a.o.logprobs) {
-            double p = log(to_double(e) / to_double(kept));
+            uint64_t q = weight(l, &b);
+            double p = 0.0;
             if (b == kTail) {  // a weight that has lost bits: from the logit, counted from the largest
-                const float best = rank_value(st.best);
-                const uint64_t q = weight(best, &b);
-                p = (static_cast<double>(l) - best) / temp + log(to_double(unit(q, b)) / to_double(kept));
+                p = (static_cast<double>(l) - largest) / temp;
+                q = weight(largest, &b);
             }
+            p += log(to_double(unit(q, b)) / to_double(kept));
             a.o.logprobs[r] = static_cast<float>(p);
         }
         if (a.o.kept) a.o.kept[r] = static_cast<int32_t>(any ? st.count_l + sm.n : st.live);
