@@ -793,6 +793,23 @@ def _stream_on(t, stream=None):
     return _stream_now(t.get_device()) if stream is None else stream
 
 
+def _made(make, shape, dtype, device, stream):
+    """A tensor that the call itself makes, with torch's `make`, from the pool of the stream that the call goes to:
+    its memory may still be read or written by earlier work of that stream, but by no other's. The current
+    stream, where the caller may use it once that stream's work is ordered before, is recorded with it."""
+    import torch
+    if _stream_now is None:
+        _bind_torch()
+    index = device.index
+    if stream is None or stream == _stream_now(index):
+        return make(shape, dtype=dtype, device=device)
+    there = torch.cuda.ExternalStream(stream, index) if stream else torch.cuda.default_stream(index)
+    with torch.cuda.stream(there):
+        t = make(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(index))
+    return t
+
+
 def _matrix(t, what: str):
     """(rows, cols, row stride) of a 2-D tensor whose columns are adjacent."""
     shape, stride = t.shape, t.stride()
@@ -815,11 +832,11 @@ def mx_quantize(x, codes=None, scales=None, stream=None):
     rows, cols, stride = _matrix(x, "x")
     with _on_device(x, codes, scales):
         if codes is None:
-            codes = torch.empty(rows, cols // 2, dtype=torch.uint8, device=x.device)
+            codes = _made(torch.empty, (rows, cols // 2), torch.uint8, x.device, stream)
         else:
             _buffer(codes, (rows, cols // 2), torch.uint8, "codes")
         if scales is None:
-            scales = torch.empty(rows, cols // 32, dtype=torch.uint8, device=x.device)
+            scales = _made(torch.empty, (rows, cols // 32), torch.uint8, x.device, stream)
         else:
             _buffer(scales, (rows, cols // 32), torch.uint8, "scales")
         _check(lib.twd_mx_quantize(x.data_ptr(), kind, rows, cols, stride, codes.data_ptr(), scales.data_ptr(),
@@ -835,7 +852,7 @@ def mx_dequantize(codes, scales, dtype=None, out=None, stream=None):
     _buffer(scales, (rows, half // 16), torch.uint8, "scales")
     with _on_device(codes, scales, out):
         if out is None:
-            out = torch.empty(rows, 2 * half, dtype=dtype or torch.bfloat16, device=codes.device)
+            out = _made(torch.empty, (rows, 2 * half), dtype or torch.bfloat16, codes.device, stream)
         elif out.shape != (rows, 2 * half) or (dtype is not None and out.dtype != dtype):
             raise ValueError(f"out must be of shape {(rows, 2 * half)} and of dtype, where that is given")
         kind = _type_of(out, "out")
@@ -884,10 +901,10 @@ class MxHead:
         except Exception:
             pass
 
-    def _out(self, rows: int, out):
+    def _out(self, rows: int, out, stream):
         import torch
         if out is None:
-            out = torch.empty(rows, self.vocab, dtype=torch.float32, device=self.device)
+            out = _made(torch.empty, (rows, self.vocab), torch.float32, self.device, stream)
         if out.shape != (rows, self.vocab):
             raise ValueError(f"out must be of shape {(rows, self.vocab)}")
         return out, _type_of(out, "out"), _matrix(out, "out")[2]
@@ -900,7 +917,7 @@ class MxHead:
         if d != self.d_model or hidden.dtype not in (torch.bfloat16, torch.int16):
             raise ValueError(f"hidden must be bfloat16 [rows, {self.d_model}]")
         with _on_device(hidden, out):
-            out, kind, out_stride = self._out(rows, out)
+            out, kind, out_stride = self._out(rows, out, stream)
             _check(lib.twd_mxhead_logits(self.handle, hidden.data_ptr(), rows, stride, out.data_ptr(), kind, out_stride,
                                          _stream_on(hidden, stream)))
         return out
@@ -912,7 +929,7 @@ class MxHead:
         _buffer(codes, (rows, self.d_model // 2), torch.uint8, "codes")
         _buffer(scales, (rows, self.d_model // 32), torch.uint8, "scales")
         with _on_device(codes, scales, out):
-            out, kind, out_stride = self._out(rows, out)
+            out, kind, out_stride = self._out(rows, out, stream)
             _check(lib.twd_mxhead_logits_mx(self.handle, codes.data_ptr(), scales.data_ptr(), rows, out.data_ptr(), kind,
                                             out_stride, _stream_on(codes, stream)))
         return out
@@ -958,7 +975,7 @@ class Sampler:
                 if t is not None:
                     _buffer(t, one, torch.int32, what)
             if tokens is None:
-                tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+                tokens = _made(torch.empty, (rows,), torch.int32, logits.device, stream)
             _check(lib.twd_sampler_sample(self.handle, logits.data_ptr(), kind, vocab, rows, stride, _ptr(temperature),
                                           _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(tokens),
                                           _ptr(logprobs), _ptr(kept), _stream_on(logits, stream)))
