@@ -210,6 +210,35 @@ def _stream(stream=None) -> int | None:
     return torch.cuda.current_stream().cuda_stream
 
 
+_device_now = None  # the current device's number
+_stream_now = None  # the handle of a device's current stream
+
+
+def _bind_torch():
+    """torch's own lookups where it has them: a tenth of the time of current_stream(), half of current_device()'s."""
+    global _device_now, _stream_now
+    import torch
+    _stream_now = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
+    _device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+
+
+def _made(make, shape, dtype, device, stream):
+    """A tensor that the call itself makes, with torch's `make`, from the pool of the stream that the call goes to:
+    its memory may still be read or written by earlier work of that stream, but by no other's. The current
+    stream, where the caller may use it once that stream's work is ordered before, is recorded with it."""
+    import torch
+    if _stream_now is None:
+        _bind_torch()
+    index = device.index
+    if stream is None or stream == _stream_now(index):
+        return make(shape, dtype=dtype, device=device)
+    there = torch.cuda.ExternalStream(stream, index) if stream else torch.cuda.default_stream(index)
+    with torch.cuda.stream(there):
+        t = make(shape, dtype=dtype, device=device)
+    t.record_stream(torch.cuda.current_stream(index))
+    return t
+
+
 # ---- sampling.hpp mirror --------------------------------------------------------------------------
 
 @dataclasses.dataclass
@@ -284,7 +313,7 @@ class Selector:
         import torch
         rows, vocab = logits.shape
         if tokens is None:
-            tokens = torch.empty(rows, dtype=torch.int32, device=logits.device)
+            tokens = _made(torch.empty, (rows,), torch.int32, logits.device, stream)
         arr = _params_array(params)
         if logits.stride(1) != 1:
             raise ValueError("logit rows must be contiguous")
@@ -298,7 +327,7 @@ class Selector:
         import torch
         rows, vocab = logits.shape
         if result is None:
-            result = torch.zeros(VERIFY_WORDS, dtype=torch.int32, device=logits.device)
+            result = _made(torch.zeros, (VERIFY_WORDS,), torch.int32, logits.device, stream)
         if logits.stride(1) != 1:
             raise ValueError("logit rows must be contiguous")
         stride = logits.stride(0) if rows > 1 else vocab
@@ -323,7 +352,7 @@ class Selector:
         rows, vocab = logits.shape
         if result is None:
             import torch
-            result = torch.zeros(VERIFY_WORDS, dtype=torch.int32, device=logits.device)
+            result = _made(torch.zeros, (VERIFY_WORDS,), torch.int32, logits.device, stream)
         if logits.stride(1) != 1:
             raise ValueError("logit rows must be contiguous")
         for r in draft_rows:
@@ -349,7 +378,7 @@ def probe_expf(x, out=None, stream=None):
     """The draft verify's device expf over a float32 device tensor (twd_probe_expf)."""
     import torch
     if out is None:
-        out = torch.empty_like(x)
+        out = _made(lambda *_, **__: torch.empty_like(x), x.shape, x.dtype, x.device, stream)
     _check(lib.twd_probe_expf(_ptr(x), _ptr(out), x.numel(), _stream(stream)))
     return out
 
@@ -358,7 +387,7 @@ def probe_exp(x, out=None, stream=None):
     """The sampled shortlist's device exp(double) over a float64 device tensor (twd_probe_exp)."""
     import torch
     if out is None:
-        out = torch.empty_like(x)
+        out = _made(lambda *_, **__: torch.empty_like(x), x.shape, x.dtype, x.device, stream)
     _check(lib.twd_probe_exp(_ptr(x), _ptr(out), x.numel(), _stream(stream)))
     return out
 
@@ -646,7 +675,7 @@ class LMHead:
         import torch
         rows = hidden.shape[0]
         if out is None:
-            out = torch.empty(rows, self.vocab, dtype=torch.float32, device=hidden.device)
+            out = _made(torch.empty, (rows, self.vocab), torch.float32, hidden.device, stream)
         _check(lib.twd_head_logits(self.handle, _ptr(hidden), rows, _ptr(out), _stream(stream)))
         return out
 
@@ -654,7 +683,7 @@ class LMHead:
         import torch
         rows = hidden.shape[0]
         if tokens is None:
-            tokens = torch.empty(rows, dtype=torch.int32, device=hidden.device)
+            tokens = _made(torch.empty, (rows,), torch.int32, hidden.device, stream)
         _check(lib.twd_head_greedy(self.handle, _ptr(hidden), rows, _ptr(logits), _ptr(tokens),
                                    _stream(stream)))
         return tokens
@@ -664,9 +693,9 @@ class LMHead:
         import torch
         rows = hidden.shape[0]
         if logits is None:
-            logits = torch.empty(rows, self.vocab, dtype=torch.float32, device=hidden.device)
+            logits = _made(torch.empty, (rows, self.vocab), torch.float32, hidden.device, stream)
         if tokens is None:
-            tokens = torch.empty(rows, dtype=torch.int32, device=hidden.device)
+            tokens = _made(torch.empty, (rows,), torch.int32, hidden.device, stream)
         arr = _params_array(params)
         _check(lib.twd_head_sample(self.handle, _ptr(hidden), rows, arr, _ptr(history),
                                    _ptr(logits), _ptr(tokens), _stream(stream)))
@@ -676,7 +705,7 @@ class LMHead:
         import torch
         rows = hidden.shape[0]
         if result is None:
-            result = torch.zeros(VERIFY_WORDS, dtype=torch.int32, device=hidden.device)
+            result = _made(torch.zeros, (VERIFY_WORDS,), torch.int32, hidden.device, stream)
         nd = 0 if drafts is None else drafts.numel()
         _check(lib.twd_head_verify_greedy(self.handle, _ptr(hidden), rows, _ptr(drafts), nd,
                                           _ptr(logits), _ptr(result), _stream(stream)))
@@ -688,7 +717,7 @@ class LMHead:
         import torch
         rows = x.shape[0]
         if out is None:
-            out = torch.empty(rows, self.vocab, dtype=torch.float32, device=x.device)
+            out = _made(torch.empty, (rows, self.vocab), torch.float32, x.device, stream)
         _check(lib.twd_head_logits_rmsnorm(self.handle, _ptr(x), _ptr(norm_weight), eps, rows,
                                            _ptr(out), _stream(stream)))
         return out
@@ -697,7 +726,7 @@ class LMHead:
         import torch
         rows = x.shape[0]
         if tokens is None:
-            tokens = torch.empty(rows, dtype=torch.int32, device=x.device)
+            tokens = _made(torch.empty, (rows,), torch.int32, x.device, stream)
         _check(lib.twd_head_greedy_rmsnorm(self.handle, _ptr(x), _ptr(norm_weight), eps, rows,
                                            _ptr(logits), _ptr(tokens), _stream(stream)))
         return tokens
@@ -707,7 +736,7 @@ class LMHead:
         import torch
         rows = x.shape[0]
         if result is None:
-            result = torch.zeros(VERIFY_WORDS, dtype=torch.int32, device=x.device)
+            result = _made(torch.zeros, (VERIFY_WORDS,), torch.int32, x.device, stream)
         nd = 0 if drafts is None else drafts.numel()
         _check(lib.twd_head_verify_greedy_rmsnorm(self.handle, _ptr(x), _ptr(norm_weight), eps,
                                                   rows, _ptr(drafts), nd, _ptr(logits),
@@ -719,9 +748,9 @@ class LMHead:
         import torch
         rows = x.shape[0]
         if logits is None:
-            logits = torch.empty(rows, self.vocab, dtype=torch.float32, device=x.device)
+            logits = _made(torch.empty, (rows, self.vocab), torch.float32, x.device, stream)
         if tokens is None:
-            tokens = torch.empty(rows, dtype=torch.int32, device=x.device)
+            tokens = _made(torch.empty, (rows,), torch.int32, x.device, stream)
         arr = _params_array(params)
         _check(lib.twd_head_sample_rmsnorm(self.handle, _ptr(x), _ptr(norm_weight), eps, rows, arr,
                                            _ptr(history), _ptr(logits), _ptr(tokens),
@@ -760,18 +789,6 @@ class _Here:
 _here = _Here()
 
 
-_device_now = None  # the current device's number
-_stream_now = None  # the handle of a device's current stream
-
-
-def _bind_torch():
-    """torch's own lookups where it has them: a tenth of the time of current_stream(), half of current_device()'s."""
-    global _device_now, _stream_now
-    import torch
-    _stream_now = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda d: torch.cuda.current_stream(d).cuda_stream)
-    _device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
-
-
 def _on_device(*tensors):
     """A guard that makes the tensors' one device the current one for the call."""
     dev = tensors[0].get_device()
@@ -791,23 +808,6 @@ def _on_device(*tensors):
 def _stream_on(t, stream=None):
     """The stream given, or the current one of the tensor's device (which the guard made the current device)."""
     return _stream_now(t.get_device()) if stream is None else stream
-
-
-def _made(make, shape, dtype, device, stream):
-    """A tensor that the call itself makes, with torch's `make`, from the pool of the stream that the call goes to:
-    its memory may still be read or written by earlier work of that stream, but by no other's. The current
-    stream, where the caller may use it once that stream's work is ordered before, is recorded with it."""
-    import torch
-    if _stream_now is None:
-        _bind_torch()
-    index = device.index
-    if stream is None or stream == _stream_now(index):
-        return make(shape, dtype=dtype, device=device)
-    there = torch.cuda.ExternalStream(stream, index) if stream else torch.cuda.default_stream(index)
-    with torch.cuda.stream(there):
-        t = make(shape, dtype=dtype, device=device)
-    t.record_stream(torch.cuda.current_stream(index))
-    return t
 
 
 def _matrix(t, what: str):
