@@ -34,7 +34,11 @@ extern "C" {
  * with row_stride elements between them, at any alignment of that type, and stay as they are. A sampler
  * holds the scratch of up to max_rows (4,096) rows of up to max_vocab (524,288) entries, about 330 KB a
  * row of 262,144; its calls are ordered across streams as a selector's are, and replays of captured
- * calls are ordered by the caller. Asynchronous on `stream`. */
+ * calls are ordered by the caller. Asynchronous on `stream`.
+ *
+ * A row of 262,144 takes some 30 us, 64 of them under 60. A row of which more than 32,768 entries lie in the
+ * eighth of an octave of weight where a limit cuts takes 1 to 4 ms, and its batch with it: equal logits under any
+ * limit, or T so high that the weights are nearly equal (T = +inf with a limit among them). */
 typedef struct twd_sampler twd_sampler;
 TWD_API int twd_sampler_create(uint32_t max_vocab, uint32_t max_rows, twd_sampler** out);
 TWD_API void twd_sampler_destroy(twd_sampler* sampler);

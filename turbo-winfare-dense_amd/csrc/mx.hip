@@ -375,9 +375,9 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, uint3
 // chunks (4 KB each) ahead of the arithmetic. The sums over the quads meet in LDS, two buffers in turn, so
 // that one barrier a group is enough and no load waits at it. Where d_model has few quads, several blocks
 // share a compute unit (as one block of several groups, 32,003 x 2,048 left a third of the units idle: 10.5 us
-// instead of 8.6). One row of 262,144 x 5,376: 117 us,
-// 6.4 TB/s, of the 6.7 that a pure read reaches (a first, simple kernel took 193);
-// 7 quantised rows of 151,669 x 3,584: 47 us, 6.2 TB/s; one row of 32,003 x 2,048: 8.3 us, where a wave's first
+// instead of 8.6). One row of 262,144 x 5,376: 115 to 117 us,
+// 6.4 to 6.5 TB/s, of the 6.7 that a pure read reaches (a first, simple kernel took 193);
+// 7 quantised rows of 151,669 x 3,584: 46 us, 6.3 TB/s; one row of 32,003 x 2,048: 7.7 to 8.3 us, where a wave's first
 // bytes and the end of the launch are half of it.
 constexpr uint32_t kSmallRows = 16;
 constexpr uint32_t kSmallWaves = 12;  // 168 registers each
@@ -493,13 +493,16 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a) {
 // through LDS, loaded there without registers one stage ahead into the other of two buffers. A stage is a
 // chunk of bf16 rows (256 bytes a row) or a quad of quantised ones (4 x 64 bytes a row and 16 scales).
 //
-// From 128 rows on bound by the matrix instructions, whose clock follows the socket's power (1,024 rows of 262,144 x
-// 5,376: 1,360 TFLOP/s, 1,577 where all weights are zero): 1,023 bf16 rows of 65,537 x 2,880 in 313 to 331 us from
-// card to card, 1,165 to 1,233 TFLOP/s (a large library product: 1,237), 2,048 quantised rows of 262,144 x 5,376 in
-// 1,966 to 2,051 us, 2,815 to 2,936 TFLOP/s (3,008). 64 bf16 rows of 262,144 x 5,376 take 176 us, whatever the data:
-// 112 are the reads of the head, with its codes served by an L2 it would be 127, without the logits' stores 156.
-// Codes two chunks ahead, stages of two chunks and two blocks to a compute unit instead of three did not bring the two
-// together (within 3%).
+// Times are medians over hundreds of calls in a row, from card to card. From 128 bf16 rows on bound by the matrix
+// instructions, whose clock follows the socket's power: 1,023 rows of 65,537 x 2,880 in 313 to 331 us, 1,165 to 1,233
+// TFLOP/s (a large library product: 1,237), with the matrix units busy in 65% of the cycles at 1.6 GHz (1,024 rows of
+// 262,144 x 5,376: 1,360 TFLOP/s, 1,577 where all weights are zero). Quantised rows do not keep them busy: 2,048 of 262,144
+// x 5,376 take 1,966 to 2,051 us, 2,815 to 2,936 TFLOP/s (3,008), with the matrix units busy in 32% of the cycles, at 2.1
+// GHz, vector instructions issued in 41%, 9 TB/s out of the L2s; the two waves of a SIMD wait for loads and barriers in
+// 26% of their time and to issue in 43%, and do not cover each other's waits. 64 bf16 rows of 262,144 x 5,376 take 176 to
+// 183 us, whatever the data: 112 are the reads of the head; on the card where it took 176, 127 with its codes
+// served by an L2 and 156 without the logits' stores. Codes two chunks ahead, stages of two chunks and two blocks to a
+// compute unit instead of three did not bring reads and products together (within 3%).
 constexpr uint32_t kTileWaves = 4;
 constexpr int kVmcnt0 = 0x0F70;  // s_waitcnt vmcnt(0), no other counter
 
@@ -844,11 +847,13 @@ int launch_tile(const MxArgs& a, hipStream_t s) {
 
 template <bool MX, typename Out>
 int launch_typed(const twd_mxhead* h, const MxArgs& a, hipStream_t s) {
-    // Few rows stream (262,144 x 5,376, 1 row: 116 us; as a tile 137). The more rows there are to the quads whose sums
-    // are joined, the more the joining costs, which a tile does not have: 8 bf16 rows of 131,072 x 2,880 took 42 us
-    // streamed and 34 as a tile, of 98,304 x 3,584 35 and 32, 16 of 262,144 x 1,024 34 and 31; but 12 of 262,144 x
-    // 5,376, whose quads fill a compute unit, 131 and 139, and 8 of 65,536 x 2,048, one tile's block to a unit, 16 and
-    // 21. Quantised rows, fewer bytes each, stream as fast or faster.
+    // Few rows stream (262,144 x 5,376, 1 row: 116 us; as a tile 134). The more rows there are to the quads whose sums
+    // are joined, the more the joining costs, which a tile does not have: 8 bf16 rows of 131,072 x 2,880 take 42 us
+    // streamed and 34 as a tile, of 98,304 x 3,584 35 and 32, 16 of 262,144 x 1,024 33 and 29; but 12 of 262,144 x
+    // 5,376, whose quads fill a compute unit, 132 and 136, and 8 of 65,536 x 2,048, one tile's block to a unit, 16 and
+    // 21. Quantised rows, fewer bytes each, stream as fast or faster (16 of 131,072 x 2,880: 37 and 34). The rule
+    // misses the better side where they lie close (8 rows of 131,072 x 2,048: 28 and 30, taken as a tile) and past 8 quads (16
+    // rows of 131,072 x 4,608: 64 and 57, of 65,536 x 5,376: 39 and 33, both streamed).
     const bool tiles = !MX && a.rows > a.quads && a.quads <= 8 && a.groups >= 6 * static_cast<uint32_t>(h->cus);
     if (a.rows <= kSmallRows && a.quads <= kSmallWaves && !tiles) {
         const uint32_t blocks = min(a.groups, kSmallWaves / a.quads * static_cast<uint32_t>(h->cus));
@@ -858,7 +863,8 @@ int launch_typed(const twd_mxhead* h, const MxArgs& a, hipStream_t s) {
         return TWD_OK;
     }
     // Rows that a tile lacks are multiplied all the same, and every tile widens the weights anew (64 rows of 262,144 x
-    // 5,376: 188 us in one tile of 64, 217 in two of 32; 32 rows: 152 in a tile of 32).
+    // 5,376: 180 us in one tile of 64, 195 in two of 32; 32 rows: 139 in a tile of 32, 170 in one of 64; 128 rows: 304 in
+    // one tile, 303 in two, quantised 179 and 202).
     // A tile's hidden rows are read at 32-bit offsets from its first.
     const uint64_t apart = MX ? a.d / 2 : 2 * a.x_stride;
     if (a.rows <= 32 || apart > 1u << 26) return launch_tile<MX, 2, Out>(a, s);

@@ -143,8 +143,8 @@ constexpr uint32_t kLogitBytes<float> = 4;
 //   collect  every slice: its entries in those bins, onto the row's list
 //   finish   per row: the cuts among the listed entries, and the draw
 //
-// (limits, collect and finish as one block per row measured 78 us instead of 43 us for 64 rows of 262,144: one
-// compute unit reads a row at 30 GB/s or so where all of them read it in 8 us.)
+// (limits, collect and finish as one block per row measured 78 us where the three, now 38, took 43 us for 64 rows of
+// 262,144: one compute unit reads a row at 30 GB/s or so where all of them read it in 8 us.)
 // A bin is an eighth of an octave of weight. A slice counts from its own largest octave down (its row's is
 // not known yet), 256 bins to a slice, the last one for all that lies deeper; octaves are absolute, so the
 // slices' bins line up. A bin's entries share an octave, so its sum of 37-bit weights is one integer; the
@@ -158,7 +158,8 @@ constexpr uint32_t kTailOct = kTail >> 3;
 // a sum that none of them has.
 constexpr uint32_t kNothingOct = kTailOct + 36;
 // Entries in the deciding bins: up to kNearCap of them are kept in LDS while they are cut, up to kListCap read from the
-// list each time, and more (nearly equal logits) from the row.
+// list each time, and more (nearly equal logits, or nearly equal weights under a high temperature) from the row, by the
+// row's one block: 0.9 to 3.9 ms for 262,144 entries.
 constexpr uint32_t kNearCap = 4096, kListCap = 32768;
 constexpr uint32_t kMaxSlices = 524288 / kSlice;
 // A bin of a slice: its entries' number from bit 50 on, the sum of their weights below.
@@ -352,8 +353,8 @@ constexpr uint32_t kSliceThreads = 512;
 constexpr uint32_t kCopies = 4;  // of a slice's bins, by lane, so that a wave's equal bins meet less often
 
 // Bound by its arithmetic: 28 instructions a logit, 18 of them in doubles, and 10 more for the largest rank; 64 rows of
-// 262,144 fp32 logits in 22 us (3.1 TB/s), 256 of 151,669 in bf16 in 45, where the vector units are busy all the
-// time; one row in 5.5. More copies of the bins, or four and eight entries at once, changed nothing.
+// 262,144 fp32 logits in 20 to 22 us (3.1 to 3.4 TB/s), 256 of 151,669 in bf16 in 40 to 45, where the vector units are
+// busy all the time; one row in 5.5. More copies of the bins, or four and eight entries at once, changed nothing.
 template <typename T, bool TINY>
 __global__ __launch_bounds__(kSliceThreads) void sample_slices_kernel(SampleArgs a) {
     __shared__ uint64_t bins[kBins][kCopies];
@@ -527,7 +528,7 @@ __device__ __forceinline__ RowHead read_heads(const SampleArgs& a, uint64_t r) {
 }
 
 // A chain of dependent steps in one block to a row (heads, bins, a scan, the cuts, their keys): 9.4 us for one row,
-// 10.2 for 256.
+// 10.0 for 256.
 __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a) {
     __shared__ uint64_t mass[kRowThreads], s_rank_m;
     __shared__ uint32_t count[kRowThreads], counts[kBins], found[3], s_key[4], s_bin_m, s_tail_n;
@@ -699,7 +700,7 @@ __global__ __launch_bounds__(kRowThreads) void sample_limits_kernel(SampleArgs a
     }
 }
 
-// A second look at the logits, of the slices alone whose largest may decide: 4.2 us for one row, 9.5 for 64 rows of
+// A second look at the logits, of the slices alone whose largest may decide: 4.2 us for one row, 8.7 for 64 rows of
 // 262,144 fp32 logits, 24 for 256 of 151,669 in bf16 (most of the logits, 3.2 TB/s).
 template <typename T, bool TINY>
 __global__ __launch_bounds__(kSliceThreads) void sample_collect_kernel(SampleArgs a) {
@@ -789,7 +790,7 @@ struct FinishMem {
     uint32_t n, base_n, pick, id, last;
 };
 
-// One block to a row: 9.7 us for one row, the slowest of 64 takes 19 and of 256 bf16 rows (2,000 listed entries of a
+// One block to a row: 9.8 us for one row, the slowest of 64 takes 19 and of 256 bf16 rows (2,000 listed entries of a
 // few values each) 29. About half goes to the cuts, a round of adding up by parts after another, a quarter to the
 // weights of the one slice that the draw falls in, where all of it is kept (vector units of one compute unit; with sums
 // of 128 bits instead of halves there and in the rounds 21 and 31 us). 1,024 threads: 13.7 us for one row, 39 for 256.
