@@ -1,6 +1,7 @@
 """Tensors that a call makes for itself when it is given another stream than the current one: they come from that
 stream's pool and are not handed out again while either stream may use them."""
-import numpy as np
+import ctypes
+
 import pytest
 
 from helpers import twd
@@ -135,3 +136,15 @@ def test_captured_calls_make_their_tensors_in_the_graph(mx):
         torch.cuda.synchronize()
         assert torch.equal(a, want) and torch.equal(b, want), rep
     del g
+
+
+def test_stream_handles_as_ctypes_pointers(mx):
+    import torch
+    t, head, x, _ = mx
+    want = head.logits(x)
+    s = torch.cuda.Stream()
+    for handle in (s.cuda_stream, None):
+        torch.cuda.synchronize()
+        got = head.logits(x, stream=ctypes.c_void_p(handle))
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

@@ -232,7 +232,8 @@ def _made(make, shape, dtype, device, stream):
     index = device.index
     if stream is None or stream == _stream_now(index):
         return make(shape, dtype=dtype, device=device)
-    there = torch.cuda.ExternalStream(stream, index) if stream else torch.cuda.default_stream(index)
+    handle = getattr(stream, "value", stream)  # an integer, or a ctypes.c_void_p of one
+    there = torch.cuda.ExternalStream(handle, index) if handle else torch.cuda.default_stream(index)
     with torch.cuda.stream(there):
         t = make(shape, dtype=dtype, device=device)
     t.record_stream(torch.cuda.current_stream(index))
