@@ -8,4 +8,5 @@ from .twd import *  # noqa: F401,F403
 from .twd import (LMHead, Selector, SamplingParams, SpeculativeCoordinator, RowParams,  # noqa: F401
                   apply_repetition_penalty, sample_token, seed_for, splitmix64,
                   validate_sampling, uniform_from_seed, generate_head, head_bytes, decode_verify,
-                  TwdError, G4DenseFormatError, LIB_PATH, MxHead, Sampler, mx_quantize, mx_dequantize)
+                  TwdError, G4DenseFormatError, LIB_PATH, MxHead, Sampler, mx_quantize, mx_dequantize,
+                  HeadLoss)

@@ -17,15 +17,17 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB = os.path.join(HERE, "libtwd_head.so")
 SOURCES = ["csrc/head.hip", "csrc/select.hip", "csrc/verify.hip", "csrc/host.cpp", "csrc/g4dense_api.cpp",
-           "csrc/container.cpp", "csrc/generator.cpp", "csrc/probe.hip", "csrc/mx.hip", "csrc/sampler.hip"]
+           "csrc/container.cpp", "csrc/generator.cpp", "csrc/probe.hip", "csrc/mx.hip", "csrc/sampler.hip",
+           "csrc/loss.hip"]
 ARCH = os.environ.get("TWD_OFFLOAD_ARCH", "gfx950")
 
 # Packed-fp32 VALU forms are kept out of the code object: hipcc would otherwise pair fp32 adds
 # and multiplies into v_pk_* instructions on its own. MFMA results stay in ordinary VGPRs: the
 # head kernels read every accumulator back on the VALU, and accumulation registers would cost
 # a copy per read.
-DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-                "-mllvm", "-amdgpu-mfma-vgpr-form"]
+DEVICE_FLAGS = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+VGPR_SUMS = ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+ACCUMULATORS = {"csrc/loss.hip"}  # a wave's 256 sums of a tile fill the accumulation registers
 COMMON = ["-O3", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-Wall",
           f"--offload-arch={ARCH}", "-I" + os.path.join(ROOT, "include"),
           "-I" + os.path.join(HERE, "csrc")]
@@ -41,6 +43,8 @@ def hipcc() -> str:
 def _compile(src: str, out_dir: str) -> str:
     obj = os.path.join(out_dir, os.path.basename(src) + ".o")
     cmd = [hipcc(), "-x", "hip", "-c", os.path.join(HERE, src), "-o", obj] + COMMON + DEVICE_FLAGS
+    if src not in ACCUMULATORS:
+        cmd += VGPR_SUMS
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src}:\n{res.stderr}")

@@ -164,6 +164,12 @@ _SIGS = {
     "twd_sampler_destroy": (None, [_vp]),
     "twd_sampler_sample": (C.c_int, [_vp, _vp, C.c_int, _u32, _u32, _u64, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                      _vp, _vp]),
+    "twd_headloss_create": (C.c_int, [_u32, _u32, _u32, _f32, C.c_int, C.POINTER(_vp)]),
+    "twd_headloss_destroy": (None, [_vp]),
+    "twd_headloss_info": (C.c_int, [_vp, C.POINTER(_u64)]),
+    "twd_headloss_forward": (C.c_int, [_vp, _vp, _u32, _u64, _vp, _u64, _vp, _vp, _vp, _vp]),
+    "twd_headloss_backward": (C.c_int, [_vp, _vp, _u32, _u64, _vp, _u64, _vp, _vp, _vp, _vp, _u64, _vp, C.c_int, _u64,
+                                        C.c_int, _vp]),
     "twd_probe_read_bandwidth": (C.c_int, [_vp, _u64, _u32, _u32, _vp, C.POINTER(_f32),
                                            C.POINTER(_u64)]),
 }
@@ -981,6 +987,100 @@ class Sampler:
                                           _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(tokens),
                                           _ptr(logprobs), _ptr(kept), _stream_on(logits, stream)))
         return tokens
+
+
+# ---- the vocabulary matrix in training ----------------------------------------------------------------
+
+class HeadLoss:
+    """Scratch for a bf16 head's softmax cross entropy and its gradients, without the logits being kept
+    (twd_headloss)."""
+
+    def __init__(self, max_rows: int, vocab: int, d_model: int, softcap: float = 0.0, backward: bool = True):
+        """backward=False: the forward pass alone, which needs far less scratch."""
+        self.handle = None
+        h = C.c_void_p()
+        _check(lib.twd_headloss_create(max_rows, vocab, d_model, softcap, 1 if backward else 0, C.byref(h)))
+        self.handle = h
+        self.max_rows, self.vocab, self.d_model, self.softcap = max_rows, vocab, d_model, softcap
+        n = _u64()
+        _check(lib.twd_headloss_info(h, C.byref(n)))
+        self.nbytes = n.value
+
+    def close(self):
+        if self.handle:
+            lib.twd_headloss_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def _inputs(self, hidden, weight, targets):
+        import torch
+        rows, d, stride = _matrix(hidden, "hidden")
+        if d != self.d_model or hidden.dtype != torch.bfloat16:
+            raise ValueError(f"hidden must be bfloat16 [rows, {self.d_model}]")
+        vocab, d, w_stride = _matrix(weight, "weight")
+        if vocab != self.vocab or d != self.d_model or weight.dtype != torch.bfloat16:
+            raise ValueError(f"weight must be bfloat16 [{self.vocab}, {self.d_model}]")
+        _buffer(targets, (rows,), torch.int32, "targets")
+        return rows, stride, w_stride
+
+    def forward(self, hidden, weight, targets, losses=None, lse=None, stream=None):
+        """(losses, lse), float32 [rows], of bfloat16 hidden rows [rows, d_model], a head's bfloat16 weights [vocab,
+        d_model] and int32 targets [rows] (twd_headloss_forward): -losses are the targets' log-probabilities. A
+        target outside the vocabulary (-100) leaves its row out."""
+        import torch
+        rows, stride, w_stride = self._inputs(hidden, weight, targets)
+        with _on_device(hidden, weight, targets, losses, lse):
+            made = []
+            for t, what in ((losses, "losses"), (lse, "lse")):
+                made.append(_made(torch.empty, (rows,), torch.float32, hidden.device, stream) if t is None
+                            else _buffer(t, (rows,), torch.float32, what))
+            losses, lse = made
+            _check(lib.twd_headloss_forward(self.handle, hidden.data_ptr(), rows, stride, weight.data_ptr(), w_stride,
+                                            targets.data_ptr(), losses.data_ptr(), lse.data_ptr(),
+                                            _stream_on(hidden, stream)))
+        return losses, lse
+
+    def backward(self, hidden, weight, targets, lse, grad=None, d_hidden=None, d_weight=None, accumulate=False,
+                 need=(True, True), stream=None):
+        """(d_hidden, d_weight): the gradients of sum(grad * losses) from the forward pass's inputs and lse
+        (twd_headloss_backward); grad is float32 [rows], all ones where not given. d_hidden is bfloat16 [rows, d_model],
+        d_weight bfloat16 or float32 [vocab, d_model] (bfloat16 where none is given), added to with accumulate. need says
+        which of the two are wanted; the other is not computed and comes back as None."""
+        import torch
+        rows, stride, w_stride = self._inputs(hidden, weight, targets)
+        if accumulate and need[1] and d_weight is None:
+            raise ValueError("accumulate needs a d_weight to add to")
+        with _on_device(hidden, weight, targets, lse, grad, d_hidden, d_weight):
+            _buffer(lse, (rows,), torch.float32, "lse")
+            if grad is not None:
+                _buffer(grad, (rows,), torch.float32, "grad")
+            h_stride = v_stride = kind = 0
+            if not need[0]:
+                d_hidden = None
+            else:
+                if d_hidden is None:
+                    d_hidden = _made(torch.empty, (rows, self.d_model), torch.bfloat16, hidden.device, stream)
+                elif d_hidden.shape != (rows, self.d_model) or d_hidden.dtype != torch.bfloat16:
+                    raise ValueError(f"d_hidden must be bfloat16 {(rows, self.d_model)}")
+                h_stride = _matrix(d_hidden, "d_hidden")[2]
+            if not need[1]:
+                d_weight = None
+            else:
+                if d_weight is None:
+                    d_weight = _made(torch.empty, (self.vocab, self.d_model), torch.bfloat16, hidden.device, stream)
+                elif d_weight.shape != (self.vocab, self.d_model):
+                    raise ValueError(f"d_weight must be of shape {(self.vocab, self.d_model)}")
+                v_stride, kind = _matrix(d_weight, "d_weight")[2], _type_of(d_weight, "d_weight")
+            _check(lib.twd_headloss_backward(self.handle, hidden.data_ptr(), rows, stride, weight.data_ptr(), w_stride,
+                                             targets.data_ptr(), lse.data_ptr(), _ptr(grad), _ptr(d_hidden), h_stride,
+                                             _ptr(d_weight), kind, v_stride, 1 if accumulate else 0,
+                                             _stream_on(hidden, stream)))
+        return d_hidden, d_weight
 
 
 def probe_read_bandwidth(buf, waves: int = 32768, launches: int = 50, stream=None):
