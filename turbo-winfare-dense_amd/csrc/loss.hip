@@ -31,7 +31,7 @@ struct LossRows {
     float* grad;
     float* lse;
     float* hit;     // the target's logit
-    uint16_t* h;    // [m][d, zeros up to a multiple of 128]
+    uint16_t* h;    // [m][d]
 };
 
 struct GatherArgs {
@@ -43,8 +43,7 @@ struct GatherArgs {
     const float* lse_in;  // backward
     float* losses;        // forward
     float* lse_out;       // forward
-    uint32_t rows, vocab;
-    uint32_t pieces, h_pieces;  // of 16 bytes in a row, and in a gathered one, which ends in zeros
+    uint32_t rows, vocab, pieces;  // of 16 bytes in a row
 };
 
 constexpr uint32_t kGatherRows = 8;
@@ -67,8 +66,8 @@ __global__ __launch_bounds__(256) void loss_gather_kernel(GatherArgs a) {
             continue;
         }
         const u32x4_t* from = reinterpret_cast<const u32x4_t*>(a.hidden + r * a.stride);
-        u32x4_t* to = reinterpret_cast<u32x4_t*>(a.r.h) + static_cast<uint64_t>(m) * a.h_pieces;
-        for (uint32_t i = t; i < a.h_pieces; i += 256) to[i] = i < a.pieces ? from[i] : u32x4_t{0, 0, 0, 0};
+        u32x4_t* to = reinterpret_cast<u32x4_t*>(a.r.h) + static_cast<uint64_t>(m) * a.pieces;
+        for (uint32_t i = t; i < a.pieces; i += 256) to[i] = from[i];
         if (t == 0) {
             a.r.at[m] = r;
             a.r.target[m] = a.targets[r];
@@ -88,16 +87,23 @@ struct LogitArgs {
     TileGrid grid;
     float2* part;         // forward: [tile][stride] largest logit and sum of exponentials
     uint16_t* dz;         // backward: [m][dz_stride], from v0 on
-    uint16_t* dzt;        // [v - v0][dzt_stride]
-    uint32_t part_stride, dz_stride, dzt_stride;
+    uint32_t part_stride, dz_stride;
 };
 
-template <typename Tile>
-constexpr int kWavesPerEu = Tile::kStage * 16 * 4 > 81920 ? 1 : 2;
+// By rows, or with the second operand turned.
+using Tile64 = ProductTile<2, 2, 4, 1, 4, false, false>;
+using Tile128 = ProductTile<4, 2, 2, 2, 4, false, false>;
+using Tile256 = ProductTile<4, 4, 2, 2, 4, false, false>;
+using TileHidden = ProductTile<4, 4, 2, 2, 4, false, true>;
+using TileWeight = ProductTile<4, 4, 2, 2, 4, true, true>;
 
-template <typename Tile, int TA, int TB, int GA, int GB, bool GRAD>
+template <typename Tile>
+constexpr int kWavesPerEu = (3 * Tile::kPieces + Tile::kLast) * 16 > 81920 ? 1 : 2;
+
+template <typename Tile, bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_logits_kernel(LogitArgs a) {
-    __shared__ u32x4_t s0[Tile::kStage], s1[Tile::kStage], s2[Tile::kStage], s3[Tile::kStage];
+    constexpr int TA = Tile::kTA, TB = Tile::kTB, GA = Tile::kGA, GB = Tile::kGB;
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kLast];
     TileAt at;
     if (!tile_of_block(a.grid, &at)) return;
     const uint32_t count = *a.r.count, m0 = at.b * Tile::kB, v_tile = a.v0 + at.a * Tile::kA;
@@ -106,67 +112,83 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     Tile::template sums<false>(s0, s1, s2, s3, a.weight, a.hidden, v_tile, m0, a.d, acc);
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
     const uint32_t v_lane = v_tile + 32 * TA * wa + 4 * (lane / 32);
+    const bool whole = v_tile + Tile::kA <= a.vocab;
     float2* joint = reinterpret_cast<float2*>(s0);  // [wa][kB]
-#pragma unroll
-    for (int tb = 0; tb < TB; ++tb) {
+    each<TB>([&](auto tb) {
         const uint32_t in = 32 * (TB * wb + tb) + lane % 32, m = m0 + in;
         const bool live = m < count;
-        const int32_t target = live ? a.r.target[m] : -1;
+        const uint32_t target = live ? static_cast<uint32_t>(a.r.target[m]) : ~0u;
+        // square ta's logits, and which of them is the target's, if one is
+        auto logits = [&](auto ta, float (&y)[16]) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) y[i] = acc[ta][tb][i];
+            cap_logits(y, a.softcap);
+        };
+        auto in_lane = [](int i) { return 8u * (i / 4) + i % 4; };
+        auto at_target = [&](auto ta, auto&& f) {
+            const uint32_t off = target - (v_lane + 32 * ta);
+            if (__builtin_amdgcn_ballot_w64(off < 32) == 0) return;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) f(i, off == in_lane(i));
+        };
         if constexpr (!GRAD) {
-            float top = -INFINITY, sum = 0.0f;
-#pragma unroll
-            for (int ta = 0; ta < TA; ++ta) {  // sixteen at a time against the largest so far
+            float top = -INFINITY, sum = 0.0f, hit = 0.0f;
+            each<TA>([&](auto ta) {  // sixteen at a time against the largest so far
                 float y[16], most = top;
+                logits(ta, y);
+                at_target(ta, [&](int i, bool is) { hit = is ? y[i] : hit; });
+                if (!whole) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] = acc[ta][tb][i];
-                cap_logits(y, a.softcap);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t v = v_lane + 32 * ta + 8 * (i / 4) + i % 4;
-                    if (static_cast<int32_t>(v) == target) a.r.hit[m] = y[i];
-                    y[i] = v < a.vocab ? y[i] : -INFINITY;
-                    most = fmaxf(most, y[i]);
+                    for (int i = 0; i < 16; ++i) y[i] = v_lane + 32 * ta + in_lane(i) < a.vocab ? y[i] : -INFINITY;
                 }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) most = fmaxf(most, y[i]);
                 const float ref = most > -INFINITY ? most * kLog2e : 0.0f;  // nothing of the vocabulary yet: no infinity less itself
                 sum *= __builtin_amdgcn_exp2f(fmaf(top, kLog2e, -ref));
 #pragma unroll
                 for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(y[i], kLog2e, -ref));
                 top = most;
-            }
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            const uint32_t off = target - v_lane;
+            if (off < 32 * TA && off % 8 < 4) a.r.hit[m] = hit;
             const float other_top = __shfl_xor(top, 32), other_sum = __shfl_xor(sum, 32);
             const float both = fmaxf(top, other_top), ref = both > -INFINITY ? both : 0.0f;
             sum = sum * __builtin_amdgcn_exp2f((top - ref) * kLog2e) + other_sum * __builtin_amdgcn_exp2f((other_top - ref) * kLog2e);
             if (lane < 32) joint[wa * Tile::kB + in] = make_float2(both, sum);
         } else {
-            const float lse = live ? a.r.lse[m] : 0.0f, grad = live ? a.r.grad[m] : 0.0f;
+            const float lse = live ? a.r.lse[m] * -kLog2e : 0.0f, grad = live ? a.r.grad[m] : 0.0f;
+            store_rows<TA, uint16_t>((wave < 2 ? s0 : s1) + wave % 2 * (TA * 128),
+                [&](auto ta) {
+                    float y[16];
+                    f32x16_t dz;
+                    logits(ta, y);
 #pragma unroll
-            for (int ta = 0; ta < TA; ++ta) {
-                float y[16];
+                    for (int i = 0; i < 16; ++i) dz[i] = __builtin_amdgcn_exp2f(fmaf(y[i], kLog2e, lse));
+                    at_target(ta, [&](int i, bool is) { dz[i] = is ? dz[i] - 1.0f : dz[i]; });
+                    if (a.softcap.cap > 0.0f) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) y[i] = acc[ta][tb][i];
-                cap_logits(y, a.softcap);
-                uint32_t e[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const uint32_t v = v_lane + 32 * ta + 8 * (i / 4) + i % 4;
-                    float p = __builtin_amdgcn_exp2f((y[i] - lse) * kLog2e);
-                    if (static_cast<int32_t>(v) == target) p -= 1.0f;
-                    const float c = y[i] * a.softcap.inv;
-                    if (a.softcap.cap > 0.0f) p *= fmaf(-c, c, 1.0f);
-                    e[i] = live && v < a.vocab ? bf16_bits(p * grad) : 0u;
-                    const uint32_t row = v - a.v0;
-                    if (m < a.dzt_stride) a.dzt[static_cast<uint64_t>(row) * a.dzt_stride + m] = static_cast<uint16_t>(e[i]);
-                }
-                if (m < a.dzt_stride) {
-#pragma unroll
-                    for (int i = 0; i < 16; i += 4) {
-                        const u32x2_t w = {e[i] | e[i + 1] << 16, e[i + 2] | e[i + 3] << 16};
-                        *reinterpret_cast<u32x2_t*>(a.dz + static_cast<uint64_t>(m) * a.dz_stride + (v_lane - a.v0) + 32 * ta + 2 * i) = w;
+                        for (int i = 0; i < 16; ++i) {
+                            const float c = y[i] * a.softcap.inv;
+                            dz[i] *= fmaf(-c, c, 1.0f);
+                        }
                     }
-                }
-            }
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dz[i] *= grad;
+                    if (!whole) {  // past the vocabulary the products read zeros
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) dz[i] = v_lane + 32 * ta + in_lane(i) < a.vocab ? dz[i] : 0.0f;
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                    return dz;
+                },
+                [&](uint32_t row, uint32_t col, u32x4_t w) {
+                    const uint32_t m_row = m0 + 32 * (TB * wb + tb) + row;
+                    if (m_row < count)
+                        *reinterpret_cast<u32x4_t*>(a.dz + static_cast<uint64_t>(m_row) * a.dz_stride + (v_tile - a.v0) + 32 * TA * wa + col) = w;
+                });
         }
-    }
+    });
     if constexpr (!GRAD) {
         __syncthreads();
         for (uint32_t in = threadIdx.x; in < Tile::kB && m0 + in < count; in += kProductThreads) {
@@ -228,74 +250,50 @@ __global__ __launch_bounds__(kJoinThreads) void loss_join_kernel(JoinArgs a) {
     }
 }
 
-// A matrix's columns as rows: out[c][r] = in[r0 + r][c], 64 x 64 at a time; rows from `rows` on read as zero.
-struct TurnArgs {
-    const uint16_t* in;
-    uint64_t stride;
-    uint32_t rows, cols;
-    const uint32_t* count;  // where given, the rows
-    uint16_t* out;
-    uint32_t out_stride, out_cols;  // out_cols: a multiple of 8
-};
-
-__global__ __launch_bounds__(256) void loss_turn_kernel(TurnArgs a) {
-    __shared__ uint16_t tile[64][72];
-    const uint32_t rows = a.count ? *a.count : a.rows;
-    const uint32_t r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, t = threadIdx.x;
-    for (uint32_t i = t; i < 64 * 8; i += 256) {
-        const uint32_t r = i / 8, c = i % 8 * 8;
-        u32x4_t w = {0, 0, 0, 0};
-        if (r0 + r < rows && c0 + c < a.cols) w = *reinterpret_cast<const u32x4_t*>(a.in + (r0 + r) * a.stride + c0 + c);
-        *reinterpret_cast<u32x4_t*>(&tile[r][c]) = w;
-    }
-    __syncthreads();
-    for (uint32_t i = t; i < 64 * 8; i += 256) {
-        const uint32_t c = i / 8, r = i % 8 * 8;
-        if (c0 + c >= a.cols || r0 + r >= a.out_cols) continue;
-        u32x4_t w;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) w[j] = tile[r + 2 * j][c] | static_cast<uint32_t>(tile[r + 2 * j + 1][c]) << 16;
-        *reinterpret_cast<u32x4_t*>(a.out + static_cast<uint64_t>(c0 + c) * a.out_stride + r0 + r) = w;
-    }
-}
-
 struct GradArgs {
     const uint32_t* count;
     Operand a, b;
-    uint32_t k, k_part;      // columns, and those of a part of the sum
-    uint32_t rows, cols;     // of the result
-    bool by_count;           // d_weight: k is the count's; d_hidden: rows are
+    uint32_t k, k_part;    // of the product, and of a part of its sum
+    uint32_t rows, cols;   // of the result
     TileGrid grid;
     void* out;
-    uint64_t stride, part;   // between the result's rows, and its parts
+    uint64_t stride, part; // between the result's rows, and its parts
     bool add;
 };
 
-__device__ __forceinline__ void put4(float* p, f32x4_t v, bool add) {
-    if (add) v += *reinterpret_cast<const f32x4_t*>(p);
-    *reinterpret_cast<f32x4_t*>(p) = v;
+// 16 bytes of a result, on top of what is there.
+__device__ __forceinline__ u32x4_t added(u32x4_t w, u32x4_t old, float) {
+    return __builtin_bit_cast(u32x4_t, __builtin_bit_cast(f32x4_t, w) + __builtin_bit_cast(f32x4_t, old));
 }
-__device__ __forceinline__ void put4(uint16_t* p, f32x4_t v, bool add) {
-    if (add) {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p);
-        v[0] += bf16_lo(w[0]), v[1] += bf16_hi(w[0]), v[2] += bf16_lo(w[1]), v[3] += bf16_hi(w[1]);
-    }
-    *reinterpret_cast<u32x2_t*>(p) = u32x2_t{bf16_bits(v[0]) | bf16_bits(v[1]) << 16, bf16_bits(v[2]) | bf16_bits(v[3]) << 16};
+__device__ __forceinline__ u32x4_t added(u32x4_t w, u32x4_t old, uint16_t) {
+    u32x4_t sum;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = bf16_pair(bf16_lo(w[i]) + bf16_lo(old[i]), bf16_hi(w[i]) + bf16_hi(old[i]));
+    return sum;
 }
 
-template <typename Tile, int TA, int TB, int GA, int GB, typename Out>
+// d_weight = dz^T H (BY_COUNT: k runs over the rows that count) or a piece's part of d_hidden = dz W.
+template <typename Tile, typename Out, bool BY_COUNT>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_grad_kernel(GradArgs a) {
-    __shared__ u32x4_t s0[Tile::kStage], s1[Tile::kStage], s2[Tile::kStage], s3[Tile::kStage];
+    constexpr int TA = Tile::kTA, TB = Tile::kTB, GB = Tile::kGB;
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kLast];
     TileAt at;
     if (!tile_of_block(a.grid, &at)) return;
     const uint32_t count = *a.count, a0 = at.a * Tile::kA, b0 = at.b * Tile::kB;
-    if (!a.by_count && a0 >= count) return;
-    const uint32_t k_all = a.by_count ? (count + 127) / 128 * 128 : a.k;
-    const uint32_t k0 = min(at.part * a.k_part, k_all), k = min(k_all - k0, a.k_part);
+    if (!BY_COUNT && a0 >= count) return;
+    Operand x = a.a, y = a.b;
+    uint32_t k;
+    if constexpr (BY_COUNT) {
+        k = x.rows = y.rows = count;
+    } else {
+        const uint32_t k0 = min(at.part * a.k_part, a.k);
+        k = min(a.k - k0, a.k_part);
+        x.rows = count;
+        x.p += k0, x.cols = (k + 7) / 8 * 8;  // dz is zero past the vocabulary
+        y.p += k0 * y.stride, y.rows = k;
+    }
     f32x16_t acc[TA][TB];
     if (k > 0) {
-        Operand x = a.a, y = a.b;
-        x.p += k0, y.p += k0;
         Tile::template sums<true>(s0, s1, s2, s3, x, y, a0, b0, k, acc);
     } else {
 #pragma unroll
@@ -303,21 +301,19 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
             for (int j = 0; j < TB; ++j) acc[i][j] = f32x16_t{};
     }
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
+    const uint32_t wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
+    const uint32_t rows = BY_COUNT ? a.rows : count;
     Out* const out = static_cast<Out*>(a.out) + at.part * a.part;
-#pragma unroll
-    for (int ta = 0; ta < TA; ++ta) {
-        const uint32_t row = a0 + 32 * (TA * wa + ta) + lane % 32;
-        if (row >= a.rows) continue;
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                const uint32_t col = b0 + 32 * (TB * wb + tb) + 2 * i + 4 * (lane / 32);
-                const f32x4_t v = {acc[ta][tb][i], acc[ta][tb][i + 1], acc[ta][tb][i + 2], acc[ta][tb][i + 3]};
-                if (col < a.cols) put4(out + row * a.stride + col, v, a.add);
-            }
-    }
+    each<TA>([&](auto ta) {
+        store_rows<TB, Out>((wave < 2 ? s0 : s1) + wave % 2 * (TB * 64 * sizeof(Out)), [&](auto tb) { return acc[ta][tb]; },
+            [&](uint32_t row, uint32_t col, u32x4_t w) {
+                const uint32_t r = a0 + 32 * (TA * wa + ta) + row, c = b0 + 32 * TB * wb + col;
+                if (r >= rows || c >= a.cols) return;
+                u32x4_t* const p = reinterpret_cast<u32x4_t*>(out + r * a.stride + c);
+                if (a.add) w = added(w, *p, Out{});
+                *p = w;
+            });
+    });
 }
 
 struct SpreadArgs {
@@ -342,39 +338,35 @@ __global__ __launch_bounds__(256) void loss_spread_kernel(SpreadArgs a) {
         const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.part + p * a.part_size + static_cast<uint64_t>(b) * a.d + c);
         lo += from[0], hi += from[1];
     }
-    const u32x4_t w = {bf16_bits(lo[0]) | bf16_bits(lo[1]) << 16, bf16_bits(lo[2]) | bf16_bits(lo[3]) << 16,
-                       bf16_bits(hi[0]) | bf16_bits(hi[1]) << 16, bf16_bits(hi[2]) | bf16_bits(hi[3]) << 16};
+    const u32x4_t w = {bf16_pair(lo[0], lo[1]), bf16_pair(lo[2], lo[3]), bf16_pair(hi[0], hi[1]), bf16_pair(hi[2], hi[3])};
     *reinterpret_cast<u32x4_t*>(a.out + a.r.at[b] * a.stride + c) = w;
 }
 
 uint32_t div_up(uint64_t x, uint32_t y) { return static_cast<uint32_t>((x + y - 1) / y); }
 uint32_t round_up(uint32_t x, uint32_t y) { return div_up(x, y) * y; }
 
+constexpr uint32_t kVocabTile = 256;  // vocabulary rows of every tile of logits
 constexpr uint32_t kLossMaxRows = 65536, kLossMaxVocab = 1u << 24;
-constexpr uint32_t kRowPad = 128;
 
 // How a backward pass over `rows` rows is cut.
 struct BackPlan {
-    uint32_t m;       // rows, rounded up: dzt's stride
-    uint32_t piece;   // vocabulary rows at a time, a multiple of 256
-    uint32_t parts;   // of d_hidden's sums
-    uint64_t dz, wt, part;  // elements of dz (and of dzt), of the turned weights and of all parts
+    uint32_t piece;     // vocabulary rows at a time, a multiple of 256
+    uint32_t parts;     // of d_hidden's sums
+    uint64_t dz, part;  // elements of dz and of all parts
 };
 
 BackPlan back_plan(uint32_t rows, uint32_t vocab, uint32_t d) {
     BackPlan p{};
-    p.m = round_up(rows, kRowPad);
     const uint32_t all = round_up(vocab, 256);
-    uint32_t most = static_cast<uint32_t>((1ull << 27) / p.m) / 256 * 256;
-    most = most < 32768 ? most : 32768;
+    uint32_t most = static_cast<uint32_t>((1ull << 27) / rows) / 256 * 256;
+    most = most < 65536 ? most : 65536;
     most = most > 256 ? most : 256;
     p.piece = round_up(div_up(all, div_up(all, most)), 256);
-    const uint32_t tiles = div_up(p.m, 256) * div_up(d, 256);
+    const uint32_t tiles = div_up(rows, 256) * div_up(d, 256);
     const uint32_t want = div_up(512, tiles), can = div_up(p.piece, 1024);
     p.parts = want < can ? want : can;
-    p.dz = static_cast<uint64_t>(p.m) * p.piece;
-    p.wt = static_cast<uint64_t>(d) * p.piece;
-    p.part = static_cast<uint64_t>(p.parts) * p.m * d;
+    p.dz = static_cast<uint64_t>(rows) * p.piece;
+    p.part = static_cast<uint64_t>(p.parts) * rows * d;
     return p;
 }
 
@@ -388,14 +380,11 @@ struct twd_headloss {
     twd::StreamOrder order;
     twd::LossRows r;
     float2* part;      // forward
-    uint16_t* ht;      // backward: [d][m]
-    uint16_t* dz;      // [m][piece]
-    uint16_t* dzt;     // [piece][m]
-    uint16_t* wt;      // [d][piece]
+    uint16_t* dz;      // backward: [m][piece]
     float* dh;         // [part][m][d]
     void* block;       // the one allocation behind them
     uint64_t bytes;
-    uint32_t max_rows, vocab, d, d_pad;  // d_pad: a multiple of 128
+    uint32_t max_rows, vocab, d;
     float softcap;
     bool backward;
     int device;
@@ -406,40 +395,31 @@ namespace twd {
 namespace {
 
 template <bool GRAD>
-int launch_logits(const twd_headloss* l, LogitArgs a, uint32_t rows, uint32_t vocab_rows, hipStream_t s) {
-    auto go = [&](auto tile, auto ta, auto tb, auto ga, auto gb) -> int {
+int launch_logits(LogitArgs a, uint32_t rows, uint32_t vocab_rows, hipStream_t s) {
+    auto go = [&](auto tile) -> int {
         using Tile = decltype(tile);
+        static_assert(Tile::kA == kVocabTile, "the tiles' parts");
         a.grid = TileGrid{div_up(vocab_rows, Tile::kA), div_up(rows, Tile::kB), 1};
-        loss_logits_kernel<Tile, ta(), tb(), ga(), gb(), GRAD><<<a.grid.blocks(), kProductThreads, 0, s>>>(a);
+        loss_logits_kernel<Tile, GRAD><<<a.grid.blocks(), kProductThreads, 0, s>>>(a);
         TWD_HIP(hipGetLastError());
         return TWD_OK;
     };
-    using std::integral_constant;
-    if (!GRAD && rows <= 64)  // dz is written for whole steps of 128 rows
-        return go(ProductTile<2, 2, 4, 1>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 1>{});
-    if (rows <= 128)
-        return go(ProductTile<4, 2, 2, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
-    return go(ProductTile<4, 4, 2, 2>{}, integral_constant<int, 4>{}, integral_constant<int, 4>{}, integral_constant<int, 2>{}, integral_constant<int, 2>{});
+    if (rows <= 64) return go(Tile64{});
+    if (rows <= 128) return go(Tile128{});
+    return go(Tile256{});
 }
 
-template <typename Out>
+template <typename Tile, typename Out, bool BY_COUNT>
 int launch_grad(GradArgs a, hipStream_t s) {
-    using Tile = ProductTile<4, 4, 2, 2>;
     a.grid = TileGrid{div_up(a.rows, Tile::kA), div_up(a.cols, Tile::kB), a.grid.parts};
-    loss_grad_kernel<Tile, 4, 4, 2, 2, Out><<<a.grid.blocks(), kProductThreads, 0, s>>>(a);
+    loss_grad_kernel<Tile, Out, BY_COUNT><<<a.grid.blocks(), kProductThreads, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
 
 int launch_gather(const twd_headloss* l, GatherArgs a, hipStream_t s) {
-    a.r = l->r, a.vocab = l->vocab, a.pieces = l->d / 8, a.h_pieces = l->d_pad / 8;
+    a.r = l->r, a.vocab = l->vocab, a.pieces = l->d / 8;
     loss_gather_kernel<<<div_up(a.rows, kGatherRows), 256, 0, s>>>(a);
-    TWD_HIP(hipGetLastError());
-    return TWD_OK;
-}
-
-int launch_turn(TurnArgs a, hipStream_t s) {
-    loss_turn_kernel<<<dim3(div_up(a.out_cols, 64), div_up(a.cols, 64)), 256, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -447,11 +427,11 @@ int launch_turn(TurnArgs a, hipStream_t s) {
 int forward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, hipStream_t s) {
     if (const int rc = launch_gather(l, g, s)) return rc;
     LogitArgs a{};
-    a.r = l->r, a.weight = weight, a.hidden = Operand{l->r.h, l->d_pad, g.rows};
+    a.r = l->r, a.weight = weight, a.hidden = Operand{l->r.h, l->d, g.rows, l->d};
     a.d = l->d, a.vocab = l->vocab, a.softcap = soft_cap(l->softcap), a.part = l->part, a.part_stride = g.rows;
-    if (const int rc = launch_logits<false>(l, a, g.rows, l->vocab, s)) return rc;
+    if (const int rc = launch_logits<false>(a, g.rows, l->vocab, s)) return rc;
     loss_join_kernel<<<div_up(g.rows, kJoinRows), kJoinThreads, 0, s>>>(
-        JoinArgs{l->r, l->part, div_up(l->vocab, 256), g.rows, g.losses, g.lse_out});
+        JoinArgs{l->r, l->part, div_up(l->vocab, kVocabTile), g.rows, g.losses, g.lse_out});
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -469,36 +449,32 @@ int backward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, 
     const BackPlan p = back_plan(g.rows, l->vocab, l->d);
     int rc = launch_gather(l, g, s);
     if (rc) return rc;
-    if (o.d_weight && (rc = launch_turn(TurnArgs{l->r.h, l->d_pad, 0, l->d, l->r.count, l->ht, p.m, p.m}, s))) return rc;
     for (uint32_t v0 = 0; v0 < l->vocab; v0 += p.piece) {
-        const uint32_t here = l->vocab - v0 < p.piece ? l->vocab - v0 : p.piece, k = round_up(here, 128);
+        const uint32_t here = l->vocab - v0 < p.piece ? l->vocab - v0 : p.piece;
+        const Operand h{l->r.h, l->d, g.rows, l->d}, w{weight.p + v0 * weight.stride, weight.stride, here, l->d};
         LogitArgs a{};
-        a.r = l->r, a.weight = weight, a.hidden = Operand{l->r.h, l->d_pad, g.rows};
-        a.d = l->d, a.vocab = l->vocab, a.v0 = v0, a.softcap = soft_cap(l->softcap);
-        a.dz = l->dz, a.dzt = l->dzt, a.dz_stride = p.piece, a.dzt_stride = p.m;
-        if ((rc = launch_logits<true>(l, a, g.rows, here, s))) return rc;
+        a.r = l->r, a.weight = weight, a.hidden = h;
+        a.d = l->d, a.vocab = l->vocab, a.v0 = v0, a.softcap = soft_cap(l->softcap), a.dz = l->dz, a.dz_stride = p.piece;
+        if ((rc = launch_logits<true>(a, g.rows, here, s))) return rc;
         if (o.d_weight) {
             GradArgs b{};
-            b.count = l->r.count, b.a = Operand{l->dzt, p.m, here}, b.b = Operand{l->ht, p.m, l->d};
-            b.k_part = p.m, b.rows = here, b.cols = l->d, b.by_count = true, b.grid.parts = 1;
-            b.stride = o.d_weight_stride, b.add = o.add;
-            const uint64_t size = o.type == TWD_F32 ? 4 : 2;
-            b.out = static_cast<char*>(o.d_weight) + v0 * o.d_weight_stride * size;
-            if ((rc = o.type == TWD_F32 ? launch_grad<float>(b, s) : launch_grad<uint16_t>(b, s))) return rc;
+            b.count = l->r.count, b.a = Operand{l->dz, p.piece, g.rows, p.piece}, b.b = h;
+            b.rows = here, b.cols = l->d, b.grid.parts = 1, b.stride = o.d_weight_stride, b.add = o.add;
+            b.out = static_cast<char*>(o.d_weight) + v0 * o.d_weight_stride * (o.type == TWD_F32 ? 4 : 2);
+            rc = o.type == TWD_F32 ? launch_grad<TileWeight, float, true>(b, s) : launch_grad<TileWeight, uint16_t, true>(b, s);
+            if (rc) return rc;
         }
         if (o.d_hidden) {
-            const TurnArgs t{weight.p + v0 * weight.stride, weight.stride, here, l->d, nullptr, l->wt, p.piece, k};
-            if ((rc = launch_turn(t, s))) return rc;
             GradArgs b{};
-            b.count = l->r.count, b.a = Operand{l->dz, p.piece, p.m}, b.b = Operand{l->wt, p.piece, l->d};
-            b.k = k, b.k_part = round_up(div_up(k, p.parts), 128), b.rows = p.m, b.cols = l->d, b.grid.parts = p.parts;
-            b.out = l->dh, b.stride = l->d, b.part = static_cast<uint64_t>(p.m) * l->d, b.add = v0 > 0;
-            if ((rc = launch_grad<float>(b, s))) return rc;
+            b.count = l->r.count, b.a = Operand{l->dz, p.piece, g.rows, here}, b.b = w;
+            b.k = here, b.k_part = round_up(div_up(here, p.parts), 128), b.rows = g.rows, b.cols = l->d, b.grid.parts = p.parts;
+            b.out = l->dh, b.stride = l->d, b.part = static_cast<uint64_t>(g.rows) * l->d, b.add = v0 > 0;
+            if ((rc = launch_grad<TileHidden, float, false>(b, s))) return rc;
         }
     }
     if (!o.d_hidden) return TWD_OK;
     loss_spread_kernel<<<dim3(g.rows, div_up(l->d, 2048)), 256, 0, s>>>(
-        SpreadArgs{l->r, g.targets, l->dh, p.parts, g.rows, l->vocab, l->d, static_cast<uint64_t>(p.m) * l->d, o.d_hidden, o.d_hidden_stride});
+        SpreadArgs{l->r, g.targets, l->dh, p.parts, g.rows, l->vocab, l->d, static_cast<uint64_t>(g.rows) * l->d, o.d_hidden, o.d_hidden_stride});
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -548,12 +524,11 @@ TWD_API int twd_headloss_create(uint32_t max_rows, uint32_t vocab, uint32_t d_mo
     TWD_HIP(hipGetDevice(&dev));
     twd_headloss* l = new (std::nothrow) twd_headloss{};
     if (!l) return fail(TWD_E_INVALID, "out of host memory");
-    l->max_rows = max_rows, l->vocab = vocab, l->d = d_model, l->d_pad = round_up(d_model, 128), l->softcap = softcap, l->backward = backward != 0, l->device = dev;
-    uint64_t dz = 0, wt = 0, part = 0;
-    const uint32_t m = round_up(max_rows, kRowPad);
-    for (uint32_t rows = kRowPad; l->backward && rows <= m; rows += kRowPad) {  // the most that any number of rows takes
+    l->max_rows = max_rows, l->vocab = vocab, l->d = d_model, l->softcap = softcap, l->backward = backward != 0, l->device = dev;
+    uint64_t dz = 0, part = 0;
+    for (uint32_t rows = 1; l->backward && rows <= max_rows; ++rows) {  // the most that any number of rows takes
         const BackPlan p = back_plan(rows, vocab, d_model);
-        dz = p.dz > dz ? p.dz : dz, wt = p.wt > wt ? p.wt : wt, part = p.part > part ? p.part : part;
+        dz = p.dz > dz ? p.dz : dz, part = p.part > part ? p.part : part;
     }
     char* at = nullptr;
     uint64_t size = 0;
@@ -564,18 +539,15 @@ TWD_API int twd_headloss_create(uint32_t max_rows, uint32_t vocab, uint32_t d_mo
     auto lay_out = [&] {
         size = 0;
         take(l->r.count, 1);
-        take(l->r.at, m);
-        take(l->r.target, m);
-        take(l->r.grad, m);
-        take(l->r.lse, m);
-        take(l->r.hit, m);
-        take(l->r.h, static_cast<uint64_t>(m) * l->d_pad);
-        take(l->part, static_cast<uint64_t>(div_up(vocab, 256)) * max_rows);
+        take(l->r.at, max_rows);
+        take(l->r.target, max_rows);
+        take(l->r.grad, max_rows);
+        take(l->r.lse, max_rows);
+        take(l->r.hit, max_rows);
+        take(l->r.h, static_cast<uint64_t>(max_rows) * d_model);
+        take(l->part, static_cast<uint64_t>(div_up(vocab, kVocabTile)) * max_rows);
         if (!l->backward) return;
-        take(l->ht, static_cast<uint64_t>(m) * d_model);
         take(l->dz, dz);
-        take(l->dzt, dz);
-        take(l->wt, wt);
         take(l->dh, part);
     };
     lay_out();
@@ -616,7 +588,7 @@ TWD_API int twd_headloss_forward(twd_headloss* l, const uint16_t* hidden_bf16, u
     GatherArgs g{};
     g.hidden = hidden_bf16, g.stride = hidden_stride, g.targets = targets, g.losses = losses, g.lse_out = lse, g.rows = rows;
     if ((rc = order_before(l->order, s))) return rc;
-    if ((rc = forward(l, g, Operand{weight_bf16, weight_stride, l->vocab}, s))) return rc;
+    if ((rc = forward(l, g, Operand{weight_bf16, weight_stride, l->vocab, l->d}, s))) return rc;
     return order_after(l->order, s);
 }
 
@@ -640,7 +612,7 @@ TWD_API int twd_headloss_backward(twd_headloss* l, const uint16_t* hidden_bf16, 
     g.hidden = hidden_bf16, g.stride = hidden_stride, g.targets = targets, g.grad = grad, g.lse_in = lse, g.rows = rows;
     const BackOut o{d_hidden_bf16, d_hidden_stride, d_weight, d_weight_type, d_weight_stride, accumulate != 0};
     if ((rc = order_before(l->order, s))) return rc;
-    if ((rc = backward(l, g, Operand{weight_bf16, weight_stride, l->vocab}, o, s))) return rc;
+    if ((rc = backward(l, g, Operand{weight_bf16, weight_stride, l->vocab, l->d}, o, s))) return rc;
     return order_after(l->order, s);
 }
 

@@ -1,11 +1,15 @@
-// A tile of the product of two bf16 matrices along their rows, C[a][b] = sum_k A[a][k] B[b][k], summed in fp32: the
-// core of the head's loss and its gradients. The caller brings what happens to the tile's sums.
+// A tile of the product of two bf16 matrices, C[a][b] = sum_k A(a, k) B(b, k), summed in fp32: the core of the head's loss
+// and its gradients. The caller brings what happens to the tile's sums.
 //
-// Four waves share a tile of kA x kB; a wave holds TA x TB squares of 32 x 32. Both operands go through LDS in stages of
-// 32 columns, loaded there without registers, three stages ahead into four buffers; a stage's barrier stands between
-// its two steps of 16 columns, so that the second step's products cover the reads of the next stage's first
-// fragments. In LDS a row's four pieces of 16 bytes change places with its number, so that eight rows' reads of one
-// piece meet different banks.
+// Four waves share a tile of kA x kB; a wave holds TA x TB squares of 32 x 32. Both operands go through LDS in stages of 32
+// of k, loaded there without registers, into BUFS buffers in turn; a stage's barrier stands between its two steps of 16, so
+// that the second step's products cover the reads of the next stage's first fragments. What lies outside an operand is read
+// as zero by the buffer loads' range check.
+//
+// An operand lies in memory by rows of k ([a][k]), or turned ([k][a]). By rows, its stage in LDS is [a][4 pieces of 16 bytes],
+// a row's pieces exchanged by its number, so that eight rows' reads of one piece meet different banks. Turned, it is [k][a],
+// a row's pieces of 32 bytes exchanged by k: four rows' reads of one piece meet different banks, and the reads turn 4 (k) x
+// 16 (a) elements over sixteen lanes.
 #pragma once
 
 #include "twd_internal.h"
@@ -15,129 +19,196 @@ namespace twd {
 
 namespace {
 
-// Operands: rows at a multiple of 16 bytes, strides in elements, multiples of 8 and at most kMaxProductStride (a tile's rows
-// lie within 32-bit offsets).
+// Starts at a multiple of 16 bytes; the stride between rows in elements, a multiple of 8 and at most kMaxProductStride (what
+// a stage reads lies within 32-bit offsets).
 struct Operand {
     const uint16_t* p;
     uint64_t stride;
-    uint32_t rows;  // rows past the last read the last
+    uint32_t rows;  // [a][k]: a; [k][a]: k
+    uint32_t cols;  // [a][k]: k; [k][a]: a; a multiple of 8, as a load of 16 bytes lies inside the range or out of it
 };
 constexpr uint64_t kMaxProductStride = 1ull << 22;
 
 constexpr uint32_t kStageK = 32;
 constexpr uint32_t kProductThreads = 256;
 
-template <int TA, int TB, int GA, int GB>
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
+
+// One operand's part of a stage: ROWS of a, T fragments to a wave.
+template <uint32_t ROWS, int T, bool TURNED>
+struct ProductSide {
+    static constexpr uint32_t kLoads = ROWS / 64;                       // of 1 KB, each wave's
+    static constexpr uint32_t kLines = TURNED ? 512 / ROWS : 16;        // rows in memory of a load
+    static constexpr uint32_t kPerLine = 64 / kLines;                   // lanes, of 16 bytes
+    Operand x;
+    uint32_t first;   // of a
+    uint32_t line;    // bytes between rows in memory
+    uint32_t off[kLoads];
+    uint32_t column;  // by rows: this lane's byte in a stage
+    __amdgpu_buffer_rsrc_t rsrc;
+    uint32_t wave, at;  // at: where this lane's fragments lie in the stage (by rows: pieces; turned: bytes)
+
+    __device__ __forceinline__ ProductSide(const Operand& o, uint32_t a0, uint32_t wave_, uint32_t share) : x(o), first(a0), wave(wave_) {
+        const uint32_t lane = threadIdx.x % 64, in = lane / kPerLine, piece = lane % kPerLine;
+        line = static_cast<uint32_t>(2 * x.stride);
+        if constexpr (TURNED) {
+#pragma unroll
+            for (uint32_t j = 0; j < kLoads; ++j) {
+                const uint32_t row = kLines * (wave * kLoads + j) + in;
+                off[j] = row * line + 32 * ((piece / 2) ^ (row % 4)) + 16 * (piece % 2);
+            }
+            const uint32_t g = lane / 16, j = lane % 16;
+            at = (8 * (g / 2) + j / 4) * (2 * ROWS) + 32 * ((2 * T * share + g % 2) ^ (j / 4)) + 8 * (j % 4);
+        } else {
+            column = 16 * (piece ^ (lane / 8 % 4));
+#pragma unroll
+            for (uint32_t j = 0; j < kLoads; ++j) off[j] = (16 * (wave * kLoads + j) + in) * line + column;
+            const uint32_t here = min(x.rows - first, ROWS);
+            rsrc = make_rsrc(x.p + first * x.stride, (here - 1) * line + 2 * x.cols);
+            at = (32 * T * share + lane % 32) * 4;
+        }
+    }
+    // Loads first .. last - 1 of a stage into its buffer.
+    __device__ __forceinline__ void load(uint32_t stage, u32x4_t* to, uint32_t from, uint32_t last) {
+        if (from >= last) return;
+        if constexpr (TURNED) {
+            const uint32_t k = stage * kStageK, left = k < x.rows ? min(x.rows - k, kStageK) : 0;
+            const auto r = make_rsrc(x.p + k * x.stride + first, left ? (left - 1) * line + 2 * (x.cols - first) : 0);
+#pragma unroll
+            for (uint32_t j = from; j < last; ++j)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + (wave * kLoads + j) * 64), 16, static_cast<int>(off[j]), 0, 0, 0);
+        } else {
+            const uint32_t byte = stage * (2 * kStageK);
+            const uint32_t go = byte + column < 2 * x.cols ? byte : 0x80000000u;  // beyond any range
+#pragma unroll
+            for (uint32_t j = from; j < last; ++j)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + (wave * kLoads + j) * 64), 16,
+                                                         static_cast<int>(off[j] + go), 0, 0, 0);
+        }
+    }
+    __device__ __forceinline__ bf16x8_t read(const u32x4_t* from, int step, int t) const {
+        if constexpr (TURNED) {
+            // fragment t's two pieces of 32 bytes: t's bits change the piece number's alone above the lowest, which g % 2 sets
+            const char* p = reinterpret_cast<const char*>(from) + (at ^ (64 * t)) + 16 * step * (2 * ROWS);
+            const i16x4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)p);
+            const i16x4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4_t*)(p + 4 * (2 * ROWS)));
+            return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        } else {
+            const uint32_t lane = threadIdx.x % 64;
+            return __builtin_bit_cast(bf16x8_t, from[at + 128 * t + ((2 * step + lane / 32) ^ (lane / 2 % 4))]);
+        }
+    }
+};
+
+template <int TA, int TB, int GA, int GB, int BUFS, bool TURNED_A, bool TURNED_B>
 struct ProductTile {
     static_assert(GA * GB == 4, "four waves");
+    static_assert(BUFS == 3 || BUFS == 4, "buffers");
+    static constexpr int kTA = TA, kTB = TB, kGA = GA, kGB = GB;
     static constexpr uint32_t kA = 32 * TA * GA, kB = 32 * TB * GB;
-    static constexpr uint32_t kStage = (kA + kB) * 4;                    // 16-byte pieces
-    static constexpr uint32_t kLoadsA = kA / 64, kLoadsB = kB / 64;      // of 16 rows, each wave's
-    static constexpr uint32_t kLoads = kLoadsA + kLoadsB;
-    static constexpr uint32_t kAhead = 2 * kLoads;                       // a wave's loads of two stages
+    static constexpr uint32_t kPieces = (kA + kB) * 4;  // of 16 bytes in a buffer
+    static constexpr uint32_t kLast = BUFS == 4 ? kPieces : 1;
+    static constexpr uint32_t kLoadsA = kA / 64, kLoads = kLoadsA + kB / 64;
+    static constexpr uint32_t kAhead = (BUFS - 2) * kLoads;  // a wave's loads that need not have arrived at a stage's end
 
-    static __host__ __device__ constexpr uint32_t padded(uint32_t k) { return (k + 127) / 128 * 128; }
-
-    // sum(ta, tb) is the square of A rows a0 + 32 (TA wa + ta) .. and B rows b0 + 32 (TB wb + tb) ..; lane l's element i is
-    // the one of B row l % 32 and A row 8 (i / 4) + 4 (l / 32) + i % 4, or with SWAP the other way round. k: a positive
-    // multiple of 32, taken up to a multiple of 128: there B's rows hold zeros, and A's are read from their start again, so
-    // that nothing but A's own row meets them.
+    // sum(ta, tb) is the square of A's a0 + 32 (TA wa + ta) .. and B's b0 + 32 (TB wb + tb) ..; lane l's element i is the one of
+    // B's l % 32 and A's 8 (i / 4) + 4 (l / 32) + i % 4, or with SWAP the other way round. s3 is the fourth buffer, if any.
     template <bool SWAP>
     static __device__ __forceinline__ void sums(u32x4_t* s0, u32x4_t* s1, u32x4_t* s2, u32x4_t* s3, const Operand& A,
                                                 const Operand& B, uint32_t a0, uint32_t b0, uint32_t k,
                                                 f32x16_t (&acc)[TA][TB]) {
-        const uint32_t lane = threadIdx.x % 64;
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        const uint32_t wa = wave / GB, wb = wave % GB;
-        const uint32_t rows_a = min(A.rows - a0, kA), rows_b = min(B.rows - b0, kB);
-        const uint32_t bytes_a = static_cast<uint32_t>(2 * A.stride), bytes_b = static_cast<uint32_t>(2 * B.stride);
-        const auto ra = make_rsrc(A.p + a0 * A.stride, (rows_a - 1) * bytes_a + 2 * k);
-        const auto rb = make_rsrc(B.p + b0 * B.stride, (rows_b - 1) * bytes_b + 2 * padded(k));
-        // lane l of a load brings the piece that belongs to place l % 4 of row l / 4
-        const uint32_t row = lane / 4, piece = (lane % 4) ^ (lane / 8 % 4);
-        uint32_t off_a[kLoadsA], off_b[kLoadsB];
-#pragma unroll
-        for (uint32_t j = 0; j < kLoadsA; ++j) off_a[j] = min(16 * (wave * kLoadsA + j) + row, rows_a - 1) * bytes_a + 16 * piece;
-#pragma unroll
-        for (uint32_t j = 0; j < kLoadsB; ++j) off_b[j] = min(16 * (wave * kLoadsB + j) + row, rows_b - 1) * bytes_b + 16 * piece;
-        const uint32_t stages = padded(k) / kStageK;
-        // past the last stage it comes again, into a buffer that is not read any more
+        ProductSide<kA, TA, TURNED_A> x(A, a0, wave, wave / GB);
+        ProductSide<kB, TB, TURNED_B> y(B, b0, wave, wave % GB);
+        // whole turns of the buffers; past the operands' ends stages are zero
+        const uint32_t turns = (k + BUFS * kStageK - 1) / (BUFS * kStageK);
         auto load = [&](uint32_t stage, u32x4_t* to, uint32_t first, uint32_t last) {
-            const uint32_t at = __builtin_amdgcn_readfirstlane(min(stage, stages - 1) * (2 * kStageK));
-            const uint32_t at_a = at + 16 * piece < 2 * k ? at : 0u;
-#pragma unroll
-            for (uint32_t j = first; j < last; ++j) {
-                if (j < kLoadsA)
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, (lds_void*)(to + (wave * kLoadsA + j) * 64), 16,
-                                                             static_cast<int>(off_a[j] + at_a), 0, 0, 0);
-                else
-                    __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, (lds_void*)(to + kA * 4 + (wave * kLoadsB + j - kLoadsA) * 64), 16,
-                                                             static_cast<int>(off_b[j - kLoadsA]), static_cast<int>(at), 0, 0);
-            }
+            x.load(stage, to, min(first, kLoadsA), min(last, kLoadsA));
+            y.load(stage, to + kA * 4, max(first, kLoadsA) - kLoadsA, max(last, kLoadsA) - kLoadsA);
         };
-        const uint32_t r = lane % 32, h = lane / 32, turn = r / 2 % 4;
-        const uint32_t at_a = (32 * TA * wa + r) * 4, at_b = kA * 4 + (32 * TB * wb + r) * 4;
         bf16x8_t fa[2][TA], fb[2][TB];
-        auto read_a = [&](const u32x4_t* from, int step, int t) {
-            fa[step][t] = __builtin_bit_cast(bf16x8_t, from[at_a + 128 * t + ((2 * step + h) ^ turn)]);
-        };
-        auto read_b = [&](const u32x4_t* from, int step, int t) {
-            fb[step][t] = __builtin_bit_cast(bf16x8_t, from[at_b + 128 * t + ((2 * step + h) ^ turn)]);
-        };
-        auto product = [&](int step, int ta, int tb) {
-            acc[ta][tb] = SWAP ? __builtin_amdgcn_mfma_f32_32x32x16_bf16(fb[step][tb], fa[step][ta], acc[ta][tb], 0, 0, 0)
-                               : __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa[step][ta], fb[step][tb], acc[ta][tb], 0, 0, 0);
-        };
-        // One step's products, with the next step's reads (from, to_step) spread among them.
+        constexpr int kProducts = TA * TB, kReads = TA + TB;
+        // One step's products, with the next step's reads and some loads spread among them.
         auto step = [&](int now, const u32x4_t* from, int next, auto more) {
-            constexpr int kProducts = TA * TB, kReads = TA + TB;
 #pragma unroll
             for (int i = 0; i < kProducts; ++i) {
 #pragma unroll
                 for (int j = i * kReads / kProducts; j < (i + 1) * kReads / kProducts; ++j) {
-                    if (j < TA) read_a(from, next, j);
-                    else read_b(from, next, j - TA);
+                    if (j < TA) fa[next][j] = x.read(from, next, j);
+                    else fb[next][j - TA] = y.read(from + kA * 4, next, j - TA);
                 }
                 more(i);
-                product(now, i / TB, i % TB);
+                f32x16_t& sum = acc[i / TB][i % TB];
+                const bf16x8_t p = fa[now][i / TB], q = fb[now][i % TB];
+                sum = SWAP ? __builtin_amdgcn_mfma_f32_32x32x16_bf16(q, p, sum, 0, 0, 0)
+                           : __builtin_amdgcn_mfma_f32_32x32x16_bf16(p, q, sum, 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
         auto nothing = [](int) {};
         auto stage = [&](uint32_t i, u32x4_t* now, const u32x4_t* next) {
             step(0, now, 1, nothing);
-            // this stage is read, and the next has arrived: of the loads only two stages' may still be on their way
+            // this stage has been read, and the next has arrived
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_waitcnt(0x0070 | (kAhead & 15) | (kAhead >> 4) << 14);
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
-            constexpr int kProducts = TA * TB;
-            step(1, next, 0, [&](int n) { load(i + 4, now, n * kLoads / kProducts, (n + 1) * kLoads / kProducts); });
+            step(1, next, 0, [&](int n) { load(i + BUFS, now, n * kLoads / kProducts, (n + 1) * kLoads / kProducts); });
         };
         load(0, s0, 0, kLoads);
         load(1, s1, 0, kLoads);
         load(2, s2, 0, kLoads);
-        load(3, s3, 0, kLoads);
+        if constexpr (BUFS == 4) load(3, s3, 0, kLoads);
 #pragma unroll
         for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < TB; ++j) acc[i][j] = f32x16_t{};
-        __builtin_amdgcn_s_waitcnt(0x0F70);  // once a tile: everything (the first stage would do)
+        constexpr uint32_t kFirst = (BUFS - 1) * kLoads;
+        __builtin_amdgcn_s_waitcnt(0x0F70 | (kFirst & 15) | (kFirst >> 4) << 14);
         __syncthreads();
 #pragma unroll
-        for (int t = 0; t < TA; ++t) read_a(s0, 0, t);
+        for (int t = 0; t < TA; ++t) fa[0][t] = x.read(s0, 0, t);
 #pragma unroll
-        for (int t = 0; t < TB; ++t) read_b(s0, 0, t);
-        for (uint32_t i = 0; i < stages; i += 4) {
+        for (int t = 0; t < TB; ++t) fb[0][t] = y.read(s0 + kA * 4, 0, t);
+        for (uint32_t i = 0; i < turns * BUFS; i += BUFS) {
             stage(i, s0, s1);
             stage(i + 1, s1, s2);
-            stage(i + 2, s2, s3);
-            stage(i + 3, s3, s0);
+            stage(i + 2, s2, BUFS == 4 ? s3 : s0);
+            if constexpr (BUFS == 4) stage(i + 3, s3, s0);
         }
         __builtin_amdgcn_s_waitcnt(kVmcnt0);  // the buffers may be used for something else
         __syncthreads();
     }
 };
+
+// Squares side by side, as a lane holds them (its row l % 32; columns 8 (i / 4) + 4 (l / 32) + i % 4 of each), change places
+// in the wave's own part of LDS, so that whole lines are stored: squares(n) gives a lane's sixteen of square n, put(row,
+// col, 16 bytes) takes them in rows. `mine`: 32 rows of 32 N columns.
+template <int N, typename Out, typename Squares, typename Put>
+__device__ __forceinline__ void store_rows(u32x4_t* mine, Squares squares, Put put) {
+    constexpr uint32_t kEach = 16 / sizeof(Out), kRow = 32 * N / kEach, kTurn = kRow < 16 ? kRow : 16;
+    const uint32_t lane = threadIdx.x % 64, r = lane % 32, h = lane / 32;
+    auto place = [&](uint32_t row, uint32_t piece) { return row * kRow + (piece ^ row % kTurn); };
+    each<N>([&](auto n) {
+        const auto square = squares(n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4_t v = {square[4 * i], square[4 * i + 1], square[4 * i + 2], square[4 * i + 3]};
+            if constexpr (sizeof(Out) == 4)
+                mine[place(r, 8 * n + 2 * i + h)] = __builtin_bit_cast(u32x4_t, v);
+            else
+                reinterpret_cast<u32x2_t*>(mine + place(r, 4 * n + i))[h] = u32x2_t{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+        }
+    });
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (uint32_t i = 0; i < 32 * kRow / 64; ++i) {
+        const uint32_t row = i * (64 / kRow) + lane / kRow, piece = lane % kRow;
+        put(row, piece * kEach, mine[place(row, piece)]);
+    }
+    __builtin_amdgcn_wave_barrier();
+}
 
 // Which tile a block takes: blocks go to the XCDs in turn, and each XCD takes a contiguous stretch of the tiles, ordered
 // so that a few rows of tiles along A meet up to eight along B at a time: what an XCD's blocks read at once stays in its

@@ -5,6 +5,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace twd {
 
 namespace {
@@ -22,6 +24,21 @@ __device__ __forceinline__ uint32_t bf16_bits(float v) {
     const uint32_t u = __float_as_uint(v);
     if (v != v) return (u >> 16) | 0x40u;
     return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
+}
+
+// Two floats as bf16 in a word, each rounded to nearest even (NaN stays NaN), in one instruction.
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, bf16x2_t{static_cast<__bf16>(lo), static_cast<__bf16>(hi)});
+}
+
+// f(0) .. f(N - 1), the numbers known to the compiler: for sums in registers, which have no index.
+template <int N, typename F>
+__device__ __forceinline__ void each(F&& f) {
+    if constexpr (N > 0) {
+        each<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
 }
 
 template <typename T>
