@@ -95,7 +95,7 @@ using Tile64 = ProductTile<2, 2, 4, 1, 4, false, false>;
 using Tile128 = ProductTile<4, 2, 2, 2, 4, false, false>;
 using Tile256 = ProductTile<4, 4, 2, 2, 4, false, false>;
 using TileHidden = ProductTile<4, 4, 2, 2, 4, false, true>;
-using TileWeight = ProductTile<4, 4, 2, 2, 4, true, true>;
+using TileWeight = ProductTile<4, 2, 2, 2, 3, true, true>;
 
 template <typename Tile>
 constexpr int kWavesPerEu = (3 * Tile::kPieces + Tile::kLast) * 16 > 81920 ? 1 : 2;
@@ -362,9 +362,14 @@ BackPlan back_plan(uint32_t rows, uint32_t vocab, uint32_t d) {
     most = most < 65536 ? most : 65536;
     most = most > 256 ? most : 256;
     p.piece = round_up(div_up(all, div_up(all, most)), 256);
-    const uint32_t tiles = div_up(rows, 256) * div_up(d, 256);
-    const uint32_t want = div_up(512, tiles), can = div_up(p.piece, 1024);
-    p.parts = want < can ? want : can;
+    // d_hidden has few tiles: its sums are cut into the parts, of at least 1,024 columns, that fill the units best, the
+    // fewest of those (2,048 rows of 5,376: 168 tiles in 3 parts, two full rounds)
+    const uint64_t tiles = static_cast<uint64_t>(div_up(rows, 256)) * div_up(d, 256), can = div_up(p.piece, 1024);
+    p.parts = 1;
+    for (uint32_t n = 2; n <= can && n <= 16; ++n) {
+        const uint64_t now = (tiles * n + 255) / 256 * p.parts, best = (tiles * p.parts + 255) / 256 * n;
+        if (20 * now < 19 * best) p.parts = n;
+    }
     p.dz = static_cast<uint64_t>(rows) * p.piece;
     p.part = static_cast<uint64_t>(p.parts) * rows * d;
     return p;

@@ -7,9 +7,9 @@
 // as zero by the buffer loads' range check.
 //
 // An operand lies in memory by rows of k ([a][k]), or turned ([k][a]). By rows, its stage in LDS is [a][4 pieces of 16 bytes],
-// a row's pieces exchanged by its number, so that eight rows' reads of one piece meet different banks. Turned, it is [k][a],
-// a row's pieces of 32 bytes exchanged by k: four rows' reads of one piece meet different banks, and the reads turn 4 (k) x
-// 16 (a) elements over sixteen lanes.
+// a row's pieces exchanged by a / 4, so that sixteen rows' reads of one piece meet different banks (of 64). Turned, it is
+// [k][a], a row's pieces of 32 bytes exchanged by k: four rows' reads of two pieces meet different banks, and the reads turn
+// 4 (k) x 16 (a) elements over sixteen lanes.
 #pragma once
 
 #include "twd_internal.h"
@@ -56,12 +56,12 @@ struct ProductSide {
 #pragma unroll
             for (uint32_t j = 0; j < kLoads; ++j) {
                 const uint32_t row = kLines * (wave * kLoads + j) + in;
-                off[j] = row * line + 32 * ((piece / 2) ^ (row % 4)) + 16 * (piece % 2);
+                off[j] = row * line + 32 * ((piece / 2) ^ 2 * (row % 4)) + 16 * (piece % 2);
             }
             const uint32_t g = lane / 16, j = lane % 16;
-            at = (8 * (g / 2) + j / 4) * (2 * ROWS) + 32 * ((2 * T * share + g % 2) ^ (j / 4)) + 8 * (j % 4);
+            at = (8 * (g / 2) + j / 4) * (2 * ROWS) + 32 * ((2 * T * share + g % 2) ^ 2 * (j / 4)) + 8 * (j % 4);
         } else {
-            column = 16 * (piece ^ (lane / 8 % 4));
+            column = 16 * (piece ^ (lane / 16 % 4));
 #pragma unroll
             for (uint32_t j = 0; j < kLoads; ++j) off[j] = (16 * (wave * kLoads + j) + in) * line + column;
             const uint32_t here = min(x.rows - first, ROWS);
@@ -96,7 +96,7 @@ struct ProductSide {
             return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             const uint32_t lane = threadIdx.x % 64;
-            return __builtin_bit_cast(bf16x8_t, from[at + 128 * t + ((2 * step + lane / 32) ^ (lane / 2 % 4))]);
+            return __builtin_bit_cast(bf16x8_t, from[at + 128 * t + ((2 * step + lane / 32) ^ (lane / 4 % 4))]);
         }
     }
 };
