@@ -91,19 +91,19 @@ struct LogitArgs {
 };
 
 // By rows, or with the second operand turned.
-using Tile64 = ProductTile<2, 2, 4, 1, 4, false, false>;
-using Tile128 = ProductTile<4, 2, 2, 2, 4, false, false>;
-using Tile256 = ProductTile<4, 4, 2, 2, 4, false, false>;
-using TileHidden = ProductTile<4, 4, 2, 2, 4, false, true>;
-using TileWeight = ProductTile<4, 2, 2, 2, 3, true, true>;
+using Tile64 = ProductTile<2, 2, 4, 1, 64, 2, false, false>;
+using Tile128 = ProductTile<4, 2, 2, 2, 64, 3, false, false>;
+using Tile256 = ProductTile<4, 4, 2, 2, 64, 2, false, false>;
+using TileHidden = ProductTile<4, 4, 2, 2, 64, 2, false, true>;
+using TileWeight = ProductTile<4, 2, 2, 2, 32, 3, true, true>;
 
 template <typename Tile>
-constexpr int kWavesPerEu = (3 * Tile::kPieces + Tile::kLast) * 16 > 81920 ? 1 : 2;
+constexpr int kWavesPerEu = Tile::kBytes > 81920 ? 1 : 2;
 
 template <typename Tile, bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_logits_kernel(LogitArgs a) {
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GA = Tile::kGA, GB = Tile::kGB;
-    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kLast];
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
     TileAt at;
     if (!tile_of_block(a.grid, &at)) return;
     const uint32_t count = *a.r.count, m0 = at.b * Tile::kB, v_tile = a.v0 + at.a * Tile::kA;
@@ -276,7 +276,7 @@ __device__ __forceinline__ u32x4_t added(u32x4_t w, u32x4_t old, uint16_t) {
 template <typename Tile, typename Out, bool BY_COUNT>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_grad_kernel(GradArgs a) {
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GB = Tile::kGB;
-    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kLast];
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
     TileAt at;
     if (!tile_of_block(a.grid, &at)) return;
     const uint32_t count = *a.count, a0 = at.a * Tile::kA, b0 = at.b * Tile::kB;

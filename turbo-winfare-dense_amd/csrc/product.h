@@ -1,15 +1,15 @@
 // A tile of the product of two bf16 matrices, C[a][b] = sum_k A(a, k) B(b, k), summed in fp32: the core of the head's loss
 // and its gradients. The caller brings what happens to the tile's sums.
 //
-// Four waves share a tile of kA x kB; a wave holds TA x TB squares of 32 x 32. Both operands go through LDS in stages of 32
-// of k, loaded there without registers, into BUFS buffers in turn; a stage's barrier stands between its two steps of 16, so
-// that the second step's products cover the reads of the next stage's first fragments. What lies outside an operand is read
-// as zero by the buffer loads' range check.
+// Four waves share a tile of kA x kB; a wave holds TA x TB squares of 32 x 32. Both operands go through LDS in stages of K of
+// k, loaded there without registers, into BUFS buffers in turn; a stage's barrier stands before its last step of 16, so that
+// this step's products cover the reads of the next stage's first fragments. What lies outside an operand is read as zero by
+// the buffer loads' range check.
 //
-// An operand lies in memory by rows of k ([a][k]), or turned ([k][a]). By rows, its stage in LDS is [a][4 pieces of 16 bytes],
-// a row's pieces exchanged by a / 4, so that sixteen rows' reads of one piece meet different banks (of 64). Turned, it is
-// [k][a], a row's pieces of 32 bytes exchanged by k: four rows' reads of two pieces meet different banks, and the reads turn
-// 4 (k) x 16 (a) elements over sixteen lanes.
+// An operand lies in memory by rows of k ([a][k]), or turned ([k][a]). By rows, its stage in LDS is [a][K / 8 pieces of 16
+// bytes], a row's pieces exchanged by its number, so that sixteen rows' reads of one piece meet different banks (of 64).
+// Turned, it is [k][a], a row's pieces of 32 bytes exchanged by k: four rows' reads of two pieces meet different banks, and
+// the reads turn 4 (k) x 16 (a) elements over sixteen lanes.
 #pragma once
 
 #include "twd_internal.h"
@@ -29,23 +29,22 @@ struct Operand {
 };
 constexpr uint64_t kMaxProductStride = 1ull << 22;
 
-constexpr uint32_t kStageK = 32;
 constexpr uint32_t kProductThreads = 256;
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
-// One operand's part of a stage: ROWS of a, T fragments to a wave.
-template <uint32_t ROWS, int T, bool TURNED>
+// One operand's part of a stage: ROWS of a, K of k, T fragments to a wave.
+template <uint32_t ROWS, uint32_t K, int T, bool TURNED>
 struct ProductSide {
-    static constexpr uint32_t kLoads = ROWS / 64;                       // of 1 KB, each wave's
-    static constexpr uint32_t kLines = TURNED ? 512 / ROWS : 16;        // rows in memory of a load
+    static constexpr uint32_t kLoads = ROWS * K / 2048;                 // of 1 KB, each wave's
+    static constexpr uint32_t kLines = 512 / (TURNED ? ROWS : K);       // rows in memory of a load
     static constexpr uint32_t kPerLine = 64 / kLines;                   // lanes, of 16 bytes
     Operand x;
     uint32_t first;   // of a
     uint32_t line;    // bytes between rows in memory
     uint32_t off[kLoads];
-    uint32_t column;  // by rows: this lane's byte in a stage
+    uint32_t column;  // by rows: this lane's byte in a stage, or with bit 6 the other way, in every second load
     __amdgpu_buffer_rsrc_t rsrc;
     uint32_t wave, at;  // at: where this lane's fragments lie in the stage (by rows: pieces; turned: bytes)
 
@@ -61,30 +60,33 @@ struct ProductSide {
             const uint32_t g = lane / 16, j = lane % 16;
             at = (8 * (g / 2) + j / 4) * (2 * ROWS) + 32 * ((2 * T * share + g % 2) ^ 2 * (j / 4)) + 8 * (j % 4);
         } else {
-            column = 16 * (piece ^ (lane / 16 % 4));
+            // rows four apart (two, of 64 columns) read the same banks: those exchange their pieces
+            column = 16 * (piece ^ (K == 64 ? lane / 16 : lane / 16 % 4));
 #pragma unroll
-            for (uint32_t j = 0; j < kLoads; ++j) off[j] = (16 * (wave * kLoads + j) + in) * line + column;
+            for (uint32_t j = 0; j < kLoads; ++j) off[j] = (kLines * (wave * kLoads + j) + in) * line + column_of(j);
             const uint32_t here = min(x.rows - first, ROWS);
             rsrc = make_rsrc(x.p + first * x.stride, (here - 1) * line + 2 * x.cols);
-            at = (32 * T * share + lane % 32) * 4;
+            at = (32 * T * share + lane % 32) * (K / 8);
         }
     }
-    // Loads first .. last - 1 of a stage into its buffer.
+    __device__ __forceinline__ uint32_t column_of(uint32_t j) const { return K == 64 && j % 2 ? column ^ 64 : column; }
+    // Loads from .. last - 1 of a stage into its buffer.
     __device__ __forceinline__ void load(uint32_t stage, u32x4_t* to, uint32_t from, uint32_t last) {
         if (from >= last) return;
         if constexpr (TURNED) {
-            const uint32_t k = stage * kStageK, left = k < x.rows ? min(x.rows - k, kStageK) : 0;
+            const uint32_t k = stage * K, left = k < x.rows ? min(x.rows - k, K) : 0;
             const auto r = make_rsrc(x.p + k * x.stride + first, left ? (left - 1) * line + 2 * (x.cols - first) : 0);
 #pragma unroll
             for (uint32_t j = from; j < last; ++j)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + (wave * kLoads + j) * 64), 16, static_cast<int>(off[j]), 0, 0, 0);
         } else {
-            const uint32_t byte = stage * (2 * kStageK);
-            const uint32_t go = byte + column < 2 * x.cols ? byte : 0x80000000u;  // beyond any range
+            const uint32_t byte = stage * (2 * K);
 #pragma unroll
-            for (uint32_t j = from; j < last; ++j)
+            for (uint32_t j = from; j < last; ++j) {
+                const uint32_t go = byte + column_of(j) < 2 * x.cols ? byte : 0x80000000u;  // beyond any range
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + (wave * kLoads + j) * 64), 16,
                                                          static_cast<int>(off[j] + go), 0, 0, 0);
+            }
         }
     }
     __device__ __forceinline__ bf16x8_t read(const u32x4_t* from, int step, int t) const {
@@ -96,36 +98,40 @@ struct ProductSide {
             return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
         } else {
             const uint32_t lane = threadIdx.x % 64;
-            return __builtin_bit_cast(bf16x8_t, from[at + 128 * t + ((2 * step + lane / 32) ^ (lane / 4 % 4))]);
+            const uint32_t turn = K == 64 ? lane / 2 % 8 : lane / 4 % 4;
+            return __builtin_bit_cast(bf16x8_t, from[at + 4 * K * t + ((2 * step + lane / 32) ^ turn)]);
         }
     }
 };
 
-template <int TA, int TB, int GA, int GB, int BUFS, bool TURNED_A, bool TURNED_B>
+template <int TA, int TB, int GA, int GB, uint32_t K, uint32_t BUFS, bool TURNED_A, bool TURNED_B>
 struct ProductTile {
     static_assert(GA * GB == 4, "four waves");
-    static_assert(BUFS == 3 || BUFS == 4, "buffers");
+    static_assert(BUFS >= 2 && BUFS <= 4, "buffers");
+    static_assert(K == 32 || K == 64, "a stage");
     static constexpr int kTA = TA, kTB = TB, kGA = GA, kGB = GB;
     static constexpr uint32_t kA = 32 * TA * GA, kB = 32 * TB * GB;
-    static constexpr uint32_t kPieces = (kA + kB) * 4;  // of 16 bytes in a buffer
-    static constexpr uint32_t kLast = BUFS == 4 ? kPieces : 1;
-    static constexpr uint32_t kLoadsA = kA / 64, kLoads = kLoadsA + kB / 64;
+    static constexpr uint32_t kPieces = (kA + kB) * K / 8, kPiecesA = kA * K / 8;  // of 16 bytes in a buffer
+    static constexpr uint32_t kPieces2 = BUFS > 2 ? kPieces : 1, kPieces3 = BUFS > 3 ? kPieces : 1;
+    static constexpr uint32_t kBytes = BUFS * kPieces * 16;
+    static constexpr uint32_t kLoadsA = kA * K / 2048, kLoads = kPieces / 256;
     static constexpr uint32_t kAhead = (BUFS - 2) * kLoads;  // a wave's loads that need not have arrived at a stage's end
 
     // sum(ta, tb) is the square of A's a0 + 32 (TA wa + ta) .. and B's b0 + 32 (TB wb + tb) ..; lane l's element i is the one of
-    // B's l % 32 and A's 8 (i / 4) + 4 (l / 32) + i % 4, or with SWAP the other way round. s3 is the fourth buffer, if any.
+    // B's l % 32 and A's 8 (i / 4) + 4 (l / 32) + i % 4, or with SWAP the other way round. s2 and s3 are the third and
+    // fourth buffer, if any.
     template <bool SWAP>
     static __device__ __forceinline__ void sums(u32x4_t* s0, u32x4_t* s1, u32x4_t* s2, u32x4_t* s3, const Operand& A,
                                                 const Operand& B, uint32_t a0, uint32_t b0, uint32_t k,
                                                 f32x16_t (&acc)[TA][TB]) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        ProductSide<kA, TA, TURNED_A> x(A, a0, wave, wave / GB);
-        ProductSide<kB, TB, TURNED_B> y(B, b0, wave, wave % GB);
+        ProductSide<kA, K, TA, TURNED_A> x(A, a0, wave, wave / GB);
+        ProductSide<kB, K, TB, TURNED_B> y(B, b0, wave, wave % GB);
         // whole turns of the buffers; past the operands' ends stages are zero
-        const uint32_t turns = (k + BUFS * kStageK - 1) / (BUFS * kStageK);
+        const uint32_t turns = (k + BUFS * K - 1) / (BUFS * K);
         auto load = [&](uint32_t stage, u32x4_t* to, uint32_t first, uint32_t last) {
             x.load(stage, to, min(first, kLoadsA), min(last, kLoadsA));
-            y.load(stage, to + kA * 4, max(first, kLoadsA) - kLoadsA, max(last, kLoadsA) - kLoadsA);
+            y.load(stage, to + kPiecesA, max(first, kLoadsA) - kLoadsA, max(last, kLoadsA) - kLoadsA);
         };
         bf16x8_t fa[2][TA], fb[2][TB];
         constexpr int kProducts = TA * TB, kReads = TA + TB;
@@ -135,31 +141,32 @@ struct ProductTile {
             for (int i = 0; i < kProducts; ++i) {
 #pragma unroll
                 for (int j = i * kReads / kProducts; j < (i + 1) * kReads / kProducts; ++j) {
-                    if (j < TA) fa[next][j] = x.read(from, next, j);
-                    else fb[next][j - TA] = y.read(from + kA * 4, next, j - TA);
+                    if (j < TA) fa[next % 2][j] = x.read(from, next, j);
+                    else fb[next % 2][j - TA] = y.read(from + kPiecesA, next, j - TA);
                 }
                 more(i);
                 f32x16_t& sum = acc[i / TB][i % TB];
-                const bf16x8_t p = fa[now][i / TB], q = fb[now][i % TB];
+                const bf16x8_t p = fa[now % 2][i / TB], q = fb[now % 2][i % TB];
                 sum = SWAP ? __builtin_amdgcn_mfma_f32_32x32x16_bf16(q, p, sum, 0, 0, 0)
                            : __builtin_amdgcn_mfma_f32_32x32x16_bf16(p, q, sum, 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto nothing = [](int) {};
         auto stage = [&](uint32_t i, u32x4_t* now, const u32x4_t* next) {
-            step(0, now, 1, nothing);
+            constexpr int kSteps = K / 16;
+#pragma unroll
+            for (int s = 0; s < kSteps - 1; ++s) step(s, now, s + 1, [](int) {});
             // this stage has been read, and the next has arrived
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_waitcnt(0x0070 | (kAhead & 15) | (kAhead >> 4) << 14);
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
-            step(1, next, 0, [&](int n) { load(i + BUFS, now, n * kLoads / kProducts, (n + 1) * kLoads / kProducts); });
+            step(kSteps - 1, next, 0, [&](int n) { load(i + BUFS, now, n * kLoads / kProducts, (n + 1) * kLoads / kProducts); });
         };
         load(0, s0, 0, kLoads);
         load(1, s1, 0, kLoads);
-        load(2, s2, 0, kLoads);
-        if constexpr (BUFS == 4) load(3, s3, 0, kLoads);
+        if constexpr (BUFS > 2) load(2, s2, 0, kLoads);
+        if constexpr (BUFS > 3) load(3, s3, 0, kLoads);
 #pragma unroll
         for (int i = 0; i < TA; ++i)
 #pragma unroll
@@ -170,12 +177,12 @@ struct ProductTile {
 #pragma unroll
         for (int t = 0; t < TA; ++t) fa[0][t] = x.read(s0, 0, t);
 #pragma unroll
-        for (int t = 0; t < TB; ++t) fb[0][t] = y.read(s0 + kA * 4, 0, t);
+        for (int t = 0; t < TB; ++t) fb[0][t] = y.read(s0 + kPiecesA, 0, t);
         for (uint32_t i = 0; i < turns * BUFS; i += BUFS) {
             stage(i, s0, s1);
-            stage(i + 1, s1, s2);
-            stage(i + 2, s2, BUFS == 4 ? s3 : s0);
-            if constexpr (BUFS == 4) stage(i + 3, s3, s0);
+            stage(i + 1, s1, BUFS > 2 ? s2 : s0);
+            if constexpr (BUFS > 2) stage(i + 2, s2, BUFS > 3 ? s3 : s0);
+            if constexpr (BUFS > 3) stage(i + 3, s3, s0);
         }
         __builtin_amdgcn_s_waitcnt(kVmcnt0);  // the buffers may be used for something else
         __syncthreads();
