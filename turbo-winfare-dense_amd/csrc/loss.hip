@@ -93,23 +93,26 @@ struct LogitArgs {
 // By rows, or with the second operand turned.
 using Tile64 = ProductTile<2, 2, 4, 1, 64, 2, false, false>;
 using Tile128 = ProductTile<4, 2, 2, 2, 64, 3, false, false>;
-using Tile256 = ProductTile<4, 4, 2, 2, 64, 2, false, false>;
+using Tile256 = ProductTile<4, 4, 2, 2, 64, 2, false, false, true>;
 using TileHidden = ProductTile<4, 4, 2, 2, 64, 2, false, true>;
 using TileWeight = ProductTile<4, 2, 2, 2, 32, 3, true, true>;
 
 template <typename Tile>
-constexpr int kWavesPerEu = Tile::kBytes > 81920 ? 1 : 2;
+constexpr int kWavesPerEu = Tile::kBytes > 81920 ? 1 : 2;  // blocks to a unit
 
 template <typename Tile, bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_logits_kernel(LogitArgs a) {
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GA = Tile::kGA, GB = Tile::kGB;
     __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
+    __shared__ uint32_t sink[Tile::kSink];
     TileAt at;
     if (!tile_of_block(a.grid, &at)) return;
     const uint32_t count = *a.r.count, m0 = at.b * Tile::kB, v_tile = a.v0 + at.a * Tile::kA;
     if (m0 >= count) return;
+    Operand w = a.weight;  // the piece's rows
+    w.p += a.v0 * w.stride, w.rows -= a.v0;
     f32x16_t acc[TA][TB];
-    Tile::template sums<false>(s0, s1, s2, s3, a.weight, a.hidden, v_tile, m0, a.d, acc);
+    Tile::template sums<false>(s0, s1, s2, s3, sink, w, a.hidden, at, a.d, acc);
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
     const uint32_t v_lane = v_tile + 32 * TA * wa + 4 * (lane / 32);
     const bool whole = v_tile + Tile::kA <= a.vocab;
@@ -277,6 +280,7 @@ template <typename Tile, typename Out, bool BY_COUNT>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_grad_kernel(GradArgs a) {
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GB = Tile::kGB;
     __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
+    __shared__ uint32_t sink[Tile::kSink];
     TileAt at;
     if (!tile_of_block(a.grid, &at)) return;
     const uint32_t count = *a.count, a0 = at.a * Tile::kA, b0 = at.b * Tile::kB;
@@ -294,7 +298,7 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     }
     f32x16_t acc[TA][TB];
     if (k > 0) {
-        Tile::template sums<true>(s0, s1, s2, s3, x, y, a0, b0, k, acc);
+        Tile::template sums<true>(s0, s1, s2, s3, sink, x, y, at, k, acc);
     } else {
 #pragma unroll
         for (int i = 0; i < TA; ++i)

@@ -29,6 +29,29 @@ struct Operand {
 };
 constexpr uint64_t kMaxProductStride = 1ull << 22;
 
+// Which tile a block takes: blocks go to the XCDs in turn, and each XCD takes a contiguous stretch of the tiles, ordered
+// so that a few rows of tiles along A meet up to eight along B at a time: what an XCD's blocks read at once stays in its
+// L2.
+struct TileGrid {
+    uint32_t na, nb, parts;  // tiles along A and B, and parts of the sum
+    __host__ __device__ uint32_t tiles() const { return na * nb * parts; }
+    __host__ __device__ uint32_t blocks() const { return (tiles() + 7) / 8 * 8; }
+};
+struct TileAt {
+    uint32_t a, b, part;
+    uint32_t share, who;  // the blocks that read the same rows of A at once, and which of them this is
+};
+__device__ __forceinline__ bool tile_of_block(const TileGrid& g, TileAt* at) {
+    const uint32_t id = blockIdx.x % 8 * (g.blocks() / 8) + blockIdx.x / 8;
+    if (id >= g.tiles()) return false;
+    const uint32_t each = g.na * g.nb, in = id % each;
+    at->part = id / each;
+    const uint32_t group = in / (8 * g.na), left = in - group * 8 * g.na, width = min(8u, g.nb - 8 * group);
+    at->a = left / width, at->b = 8 * group + left % width;
+    at->share = width, at->who = left % width;
+    return true;
+}
+
 constexpr uint32_t kProductThreads = 256;
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
@@ -89,6 +112,14 @@ struct ProductSide {
             }
         }
     }
+    // Brings the lines of a stage by rows to the L2, each of `share` blocks that read them its part: one word of a line into
+    // LDS, where nobody reads it.
+    __device__ __forceinline__ void touch(uint32_t stage, uint32_t* sink, uint32_t share, uint32_t who) {
+        static_assert(!TURNED && ROWS == kProductThreads && K == 64, "a line to a thread");
+        const uint32_t byte = stage * (2 * K), id = threadIdx.x;
+        const uint32_t at_byte = id % share == who && byte < 2 * x.cols ? id * line + byte : 0x80000000u;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(sink + 64 * wave), 4, static_cast<int>(at_byte), 0, 0, 0);
+    }
     __device__ __forceinline__ bf16x8_t read(const u32x4_t* from, int step, int t) const {
         if constexpr (TURNED) {
             // fragment t's two pieces of 32 bytes: t's bits change the piece number's alone above the lowest, which g % 2 sets
@@ -104,7 +135,10 @@ struct ProductSide {
     }
 };
 
-template <int TA, int TB, int GA, int GB, uint32_t K, uint32_t BUFS, bool TURNED_A, bool TURNED_B>
+// Where several blocks read the same rows of A from memory at once, TOUCH brings its lines to the L2 three stages ahead: the
+// loads into LDS, of which one stage is on its way, then seldom wait for memory (2,048 x 65,536 x 5,376: 1,285 TFLOP/s without,
+// 1,329 with it; all zeros, where the clock is not held by the power, 1,527 and 1,857; of B's lines too: 1,183).
+template <int TA, int TB, int GA, int GB, uint32_t K, uint32_t BUFS, bool TURNED_A, bool TURNED_B, bool TOUCH = false>
 struct ProductTile {
     static_assert(GA * GB == 4, "four waves");
     static_assert(BUFS >= 2 && BUFS <= 4, "buffers");
@@ -114,19 +148,20 @@ struct ProductTile {
     static constexpr uint32_t kPieces = (kA + kB) * K / 8, kPiecesA = kA * K / 8;  // of 16 bytes in a buffer
     static constexpr uint32_t kPieces2 = BUFS > 2 ? kPieces : 1, kPieces3 = BUFS > 3 ? kPieces : 1;
     static constexpr uint32_t kBytes = BUFS * kPieces * 16;
+    static constexpr uint32_t kSink = TOUCH ? kProductThreads : 1;
     static constexpr uint32_t kLoadsA = kA * K / 2048, kLoads = kPieces / 256;
-    static constexpr uint32_t kAhead = (BUFS - 2) * kLoads;  // a wave's loads that need not have arrived at a stage's end
+    static constexpr uint32_t kAhead = (BUFS - 2) * kLoads + (TOUCH ? BUFS - 1 : 0);  // a wave's loads that need not have arrived at a stage's end
 
-    // sum(ta, tb) is the square of A's a0 + 32 (TA wa + ta) .. and B's b0 + 32 (TB wb + tb) ..; lane l's element i is the one of
-    // B's l % 32 and A's 8 (i / 4) + 4 (l / 32) + i % 4, or with SWAP the other way round. s2 and s3 are the third and
-    // fourth buffer, if any.
+    // sum(ta, tb) is the square of A's kA at.a + 32 (TA wa + ta) .. and B's kB at.b + 32 (TB wb + tb) ..; lane l's element i is
+    // the one of B's l % 32 and A's 8 (i / 4) + 4 (l / 32) + i % 4, or with SWAP the other way round. s2 and s3 are the third and
+    // fourth buffer, if any; sink: kSink words.
     template <bool SWAP>
-    static __device__ __forceinline__ void sums(u32x4_t* s0, u32x4_t* s1, u32x4_t* s2, u32x4_t* s3, const Operand& A,
-                                                const Operand& B, uint32_t a0, uint32_t b0, uint32_t k,
+    static __device__ __forceinline__ void sums(u32x4_t* s0, u32x4_t* s1, u32x4_t* s2, u32x4_t* s3, uint32_t* sink,
+                                                const Operand& A, const Operand& B, const TileAt& at, uint32_t k,
                                                 f32x16_t (&acc)[TA][TB]) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        ProductSide<kA, K, TA, TURNED_A> x(A, a0, wave, wave / GB);
-        ProductSide<kB, K, TB, TURNED_B> y(B, b0, wave, wave % GB);
+        ProductSide<kA, K, TA, TURNED_A> x(A, at.a * kA, wave, wave / GB);
+        ProductSide<kB, K, TB, TURNED_B> y(B, at.b * kB, wave, wave % GB);
         // whole turns of the buffers; past the operands' ends stages are zero
         const uint32_t turns = (k + BUFS * K - 1) / (BUFS * K);
         auto load = [&](uint32_t stage, u32x4_t* to, uint32_t first, uint32_t last) {
@@ -152,26 +187,40 @@ struct ProductTile {
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        auto stage = [&](uint32_t i, u32x4_t* now, const u32x4_t* next) {
-            constexpr int kSteps = K / 16;
+        // A stage's loads are spread over the steps: in one burst they fill the queue to memory, and the wave's products wait
+        // behind them (the same product: 1,166 and 1,285 TFLOP/s).
+        constexpr uint32_t kSteps = K / 16, kSpread = kSteps > 2 ? kSteps - 1 : kSteps;
+        auto part = [&](uint32_t stage, u32x4_t* to, uint32_t p, int n) {
+            if (p >= kSpread) return;
+            const uint32_t lo = kLoads * p / kSpread, hi = kLoads * (p + 1) / kSpread;
+            load(stage, to, lo + (hi - lo) * n / kProducts, lo + (hi - lo) * (n + 1) / kProducts);
+        };
+        auto stage = [&](uint32_t i, u32x4_t* before, u32x4_t* now, const u32x4_t* next) {
 #pragma unroll
-            for (int s = 0; s < kSteps - 1; ++s) step(s, now, s + 1, [](int) {});
+            for (uint32_t s = 0; s < kSteps - 1; ++s)
+                step(s, now, s + 1, [&](int n) {
+                    part(i - 1 + BUFS, before, s + 1, n);
+                    if constexpr (TOUCH) {
+                        if (s == kSteps - 2 && n == kProducts - 1) x.touch(i + BUFS + 1, sink, at.share, at.who);
+                    }
+                });
             // this stage has been read, and the next has arrived
             __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_waitcnt(0x0070 | (kAhead & 15) | (kAhead >> 4) << 14);
             __builtin_amdgcn_s_barrier();
             __builtin_amdgcn_sched_barrier(0);
-            step(kSteps - 1, next, 0, [&](int n) { load(i + BUFS, now, n * kLoads / kProducts, (n + 1) * kLoads / kProducts); });
+            step(kSteps - 1, next, 0, [&](int n) { part(i + BUFS, now, 0, n); });
         };
+        u32x4_t* const last = BUFS == 2 ? s1 : BUFS == 3 ? s2 : s3;
         load(0, s0, 0, kLoads);
-        load(1, s1, 0, kLoads);
-        if constexpr (BUFS > 2) load(2, s2, 0, kLoads);
-        if constexpr (BUFS > 3) load(3, s3, 0, kLoads);
+        if constexpr (BUFS > 2) load(1, s1, 0, kLoads);
+        if constexpr (BUFS > 3) load(2, s2, 0, kLoads);
+        load(BUFS - 1, last, 0, kLoads / kSpread);
 #pragma unroll
         for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < TB; ++j) acc[i][j] = f32x16_t{};
-        constexpr uint32_t kFirst = (BUFS - 1) * kLoads;
+        constexpr uint32_t kFirst = (BUFS - 2) * kLoads + kLoads / kSpread;
         __builtin_amdgcn_s_waitcnt(0x0F70 | (kFirst & 15) | (kFirst >> 4) << 14);
         __syncthreads();
 #pragma unroll
@@ -179,10 +228,10 @@ struct ProductTile {
 #pragma unroll
         for (int t = 0; t < TB; ++t) fb[0][t] = y.read(s0 + kPiecesA, 0, t);
         for (uint32_t i = 0; i < turns * BUFS; i += BUFS) {
-            stage(i, s0, s1);
-            stage(i + 1, s1, BUFS > 2 ? s2 : s0);
-            if constexpr (BUFS > 2) stage(i + 2, s2, BUFS > 3 ? s3 : s0);
-            if constexpr (BUFS > 3) stage(i + 3, s3, s0);
+            stage(i, last, s0, s1);
+            stage(i + 1, s0, s1, BUFS > 2 ? s2 : s0);
+            if constexpr (BUFS > 2) stage(i + 2, s1, s2, BUFS > 3 ? s3 : s0);
+            if constexpr (BUFS > 3) stage(i + 3, s2, s3, s0);
         }
         __builtin_amdgcn_s_waitcnt(kVmcnt0);  // the buffers may be used for something else
         __syncthreads();
@@ -215,27 +264,6 @@ __device__ __forceinline__ void store_rows(u32x4_t* mine, Squares squares, Put p
         put(row, piece * kEach, mine[place(row, piece)]);
     }
     __builtin_amdgcn_wave_barrier();
-}
-
-// Which tile a block takes: blocks go to the XCDs in turn, and each XCD takes a contiguous stretch of the tiles, ordered
-// so that a few rows of tiles along A meet up to eight along B at a time: what an XCD's blocks read at once stays in its
-// L2.
-struct TileGrid {
-    uint32_t na, nb, parts;  // tiles along A and B, and parts of the sum
-    __host__ __device__ uint32_t tiles() const { return na * nb * parts; }
-    __host__ __device__ uint32_t blocks() const { return (tiles() + 7) / 8 * 8; }
-};
-struct TileAt {
-    uint32_t a, b, part;
-};
-__device__ __forceinline__ bool tile_of_block(const TileGrid& g, TileAt* at) {
-    const uint32_t id = blockIdx.x % 8 * (g.blocks() / 8) + blockIdx.x / 8;
-    if (id >= g.tiles()) return false;
-    const uint32_t each = g.na * g.nb, in = id % each;
-    at->part = id / each;
-    const uint32_t group = in / (8 * g.na), left = in - group * 8 * g.na, width = min(8u, g.nb - 8 * group);
-    at->a = left / width, at->b = 8 * group + left % width;
-    return true;
 }
 
 }  // namespace
