@@ -44,14 +44,14 @@ struct GatherArgs {
     float* losses;        // forward
     float* lse_out;       // forward
     uint32_t rows, vocab, pieces;  // of 16 bytes in a row
+    uint32_t each;                 // rows of a block
 };
 
-constexpr uint32_t kGatherRows = 8;
 
 // A block counts the rows before its own that count, then brings its own to their places.
 __global__ __launch_bounds__(256) void loss_gather_kernel(GatherArgs a) {
     __shared__ uint32_t wave_sum[4];
-    const uint32_t r0 = blockIdx.x * kGatherRows, t = threadIdx.x;
+    const uint32_t r0 = blockIdx.x * a.each, t = threadIdx.x;
     auto counts = [&](uint32_t r) { return static_cast<uint32_t>(a.targets[r]) < a.vocab; };
     uint32_t before = 0;
     for (uint32_t r = t; r < r0; r += 256) before += counts(r) ? 1u : 0u;
@@ -59,7 +59,7 @@ __global__ __launch_bounds__(256) void loss_gather_kernel(GatherArgs a) {
     if (t % 64 == 0) wave_sum[t / 64] = before;
     __syncthreads();
     uint32_t m = wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3];
-    const uint32_t last = min(r0 + kGatherRows, a.rows);
+    const uint32_t last = min(r0 + a.each, a.rows);
     for (uint32_t r = r0; r < last; ++r) {
         if (!counts(r)) {
             if (t == 0 && a.losses) a.losses[r] = 0.0f, a.lse_out[r] = 0.0f;
@@ -82,20 +82,40 @@ struct LogitArgs {
     LossRows r;
     Operand weight, hidden;
     uint32_t d, vocab;
-    uint32_t v0;          // the piece's first vocabulary row
+    uint32_t v0, here;    // the piece's first vocabulary row, and its rows
     SoftCap softcap;
-    TileGrid grid;
     float2* part;         // forward: [tile][stride] largest logit and sum of exponentials
     uint16_t* dz;         // backward: [m][dz_stride], from v0 on
     uint32_t part_stride, dz_stride;
 };
 
 // By rows, or with the second operand turned.
-using Tile64 = ProductTile<2, 2, 4, 1, 64, 2, false, false>;
-using Tile128 = ProductTile<4, 2, 2, 2, 64, 3, false, false>;
-using Tile256 = ProductTile<4, 4, 2, 2, 64, 2, false, false, true>;
-using TileHidden = ProductTile<4, 4, 2, 2, 64, 2, false, true>;
+using TileFew = ProductTile<1, 2, 4, 1, 64, 3, false, false>;
+using TileNarrow = ProductTile<2, 2, 4, 1, 64, 2, false, false>;
+using TileWide = ProductTile<4, 4, 2, 2, 64, 2, false, false, true>;
+using TileHidden = ProductTile<4, 4, 2, 2, 32, 4, false, true>;
 using TileWeight = ProductTile<4, 2, 2, 2, 32, 3, true, true>;
+
+// Which tiles of logits are wide (256 rows) and which narrow (64): of the rows that count, whole wide tiles, and a last one
+// where that saves narrow ones; and of these tiles, whole rounds of the units, and a last one likewise. Narrow tiles are
+// two to a unit and take some 0.35 of a wide one's time.
+constexpr uint32_t kVocabTile = 256;  // vocabulary rows of a wide or narrow tile
+static_assert(TileWide::kA == kVocabTile && TileNarrow::kA == kVocabTile && TileNarrow::kB * 4 == TileWide::kB, "quarters");
+constexpr uint32_t kFewRows = 64, kMostNarrow = 128, kRound = 256;
+struct WideTiles {
+    TileGrid grid;   // of wide tiles
+    uint32_t wide;   // those that are taken as wide ones, the first in order
+    uint32_t rest;   // rows past the wide tiles'
+    __device__ uint32_t narrow() const { return (grid.tiles() - wide) * 4 + grid.na * ((rest + 63) / 64); }
+};
+__device__ __forceinline__ WideTiles wide_tiles(uint32_t count, uint32_t na) {
+    WideTiles w;
+    w.rest = count % 256 <= kMostNarrow ? count % 256 : 0;
+    w.grid = TileGrid{na, (count - w.rest + 255) / 256, 1};
+    const uint32_t left = w.grid.tiles() % kRound;
+    w.wide = w.grid.tiles() - (left <= kMostNarrow ? left : 0);
+    return w;
+}
 
 template <typename Tile>
 constexpr int kWavesPerEu = Tile::kBytes > 81920 ? 1 : 2;  // blocks to a unit
@@ -106,11 +126,32 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
     __shared__ uint32_t sink[Tile::kSink];
     TileAt at;
-    if (!tile_of_block(a.grid, &at)) return;
-    const uint32_t count = *a.r.count, m0 = at.b * Tile::kB, v_tile = a.v0 + at.a * Tile::kA;
+    const uint32_t count = *a.r.count, na = (a.here + Tile::kA - 1) / Tile::kA;
+    if constexpr (Tile::kA != kVocabTile) {  // few rows: one tile along them
+        const uint32_t id = stretched(na);
+        if (id >= na) return;
+        at = TileAt{id, 0, 0, 1, 0};
+    } else {
+        const WideTiles t = wide_tiles(count, na);
+        const uint32_t tiles = Tile::kB == 256 ? t.wide : t.narrow(), id = stretched(tiles);
+        if (id >= tiles) return;
+        if constexpr (Tile::kB == 256) {
+            at = tile_at(t.grid, id);
+        } else {
+            const uint32_t quarters = (t.grid.tiles() - t.wide) * 4;
+            if (id < quarters) {
+                at = tile_at(t.grid, t.wide + id / 4);
+                at.b = 4 * at.b + id % 4;
+            } else {
+                const uint32_t wide = (t.rest + 63) / 64;
+                at = TileAt{(id - quarters) / wide, 4 * t.grid.nb + (id - quarters) % wide, 0, 1, 0};
+            }
+        }
+    }
+    const uint32_t m0 = at.b * Tile::kB, v_tile = a.v0 + at.a * Tile::kA;
     if (m0 >= count) return;
     Operand w = a.weight;  // the piece's rows
-    w.p += a.v0 * w.stride, w.rows -= a.v0;
+    w.p += a.v0 * w.stride, w.rows = a.here;
     f32x16_t acc[TA][TB];
     Tile::template sums<false>(s0, s1, s2, s3, sink, w, a.hidden, at, a.d, acc);
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
@@ -253,14 +294,23 @@ __global__ __launch_bounds__(kJoinThreads) void loss_join_kernel(JoinArgs a) {
     }
 }
 
+// d_hidden has few tiles: its sums are cut into the parts, of at least 1,024 columns, that fill the units best, the fewest
+// of those (2,048 rows of 5,376: 168 tiles in 3 parts, two full rounds).
+__host__ __device__ inline uint32_t hidden_parts(uint32_t rows, uint32_t d, uint32_t piece) {
+    const uint64_t tiles = static_cast<uint64_t>((rows + 255) / 256) * ((d + 255) / 256);
+    uint32_t best = 1;
+    for (uint32_t n = 2; n <= 16 && n <= (piece + 1023) / 1024; ++n)
+        if (20 * ((tiles * n + 255) / 256 * best) < 19 * ((tiles * best + 255) / 256 * n)) best = n;
+    return best;
+}
+
 struct GradArgs {
     const uint32_t* count;
     Operand a, b;
-    uint32_t k, k_part;    // of the product, and of a part of its sum
+    uint32_t k, piece;     // d_hidden: of this product, and of the first
     uint32_t rows, cols;   // of the result
-    TileGrid grid;
     void* out;
-    uint64_t stride, part; // between the result's rows, and its parts
+    uint64_t stride;       // between the result's rows; the parts of d_hidden follow one another
     bool add;
 };
 
@@ -281,17 +331,20 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GB = Tile::kGB;
     __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
     __shared__ uint32_t sink[Tile::kSink];
-    TileAt at;
-    if (!tile_of_block(a.grid, &at)) return;
-    const uint32_t count = *a.count, a0 = at.a * Tile::kA, b0 = at.b * Tile::kB;
-    if (!BY_COUNT && a0 >= count) return;
+    const uint32_t count = *a.count, rows = BY_COUNT ? a.rows : count;
+    const uint32_t parts = BY_COUNT ? 1 : hidden_parts(count, a.cols, a.piece);
+    const TileGrid grid{(rows + Tile::kA - 1) / Tile::kA, (a.cols + Tile::kB - 1) / Tile::kB, parts};
+    const uint32_t id = stretched(grid.tiles());
+    if (id >= grid.tiles()) return;
+    const TileAt at = tile_at(grid, id);
+    const uint32_t a0 = at.a * Tile::kA, b0 = at.b * Tile::kB;
     Operand x = a.a, y = a.b;
     uint32_t k;
     if constexpr (BY_COUNT) {
         k = x.rows = y.rows = count;
     } else {
-        const uint32_t k0 = min(at.part * a.k_part, a.k);
-        k = min(a.k - k0, a.k_part);
+        const uint32_t k_part = ((a.k + parts - 1) / parts + 127) / 128 * 128, k0 = min(at.part * k_part, a.k);
+        k = min(a.k - k0, k_part);
         x.rows = count;
         x.p += k0, x.cols = (k + 7) / 8 * 8;  // dz is zero past the vocabulary
         y.p += k0 * y.stride, y.rows = k;
@@ -306,8 +359,7 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
             for (int j = 0; j < TB; ++j) acc[i][j] = f32x16_t{};
     }
     const uint32_t wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
-    const uint32_t rows = BY_COUNT ? a.rows : count;
-    Out* const out = static_cast<Out*>(a.out) + at.part * a.part;
+    Out* const out = static_cast<Out*>(a.out) + at.part * (rows * a.stride);
     each<TA>([&](auto ta) {
         store_rows<TB, Out>((wave < 2 ? s0 : s1) + wave % 2 * (TB * 64 * sizeof(Out)), [&](auto tb) { return acc[ta][tb]; },
             [&](uint32_t row, uint32_t col, u32x4_t w) {
@@ -324,8 +376,7 @@ struct SpreadArgs {
     LossRows r;
     const int32_t* targets;
     const float* part;   // [part][m][d]
-    uint32_t parts, rows, vocab, d;
-    uint64_t part_size;
+    uint32_t piece, vocab, d;
     uint16_t* out;
     uint64_t stride;
 };
@@ -336,10 +387,12 @@ __global__ __launch_bounds__(256) void loss_spread_kernel(SpreadArgs a) {
     if (c >= a.d) return;
     // a block writes row `at[b]` from sum b, and row b if it is left out
     if (static_cast<uint32_t>(a.targets[b]) >= a.vocab) *reinterpret_cast<u32x4_t*>(a.out + b * a.stride + c) = u32x4_t{0, 0, 0, 0};
-    if (b >= *a.r.count) return;
+    const uint32_t count = *a.r.count;
+    if (b >= count) return;
+    const uint32_t parts = hidden_parts(count, a.d, a.piece);
     f32x4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-    for (uint32_t p = 0; p < a.parts; ++p) {
-        const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.part + p * a.part_size + static_cast<uint64_t>(b) * a.d + c);
+    for (uint32_t p = 0; p < parts; ++p) {
+        const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.part + (static_cast<uint64_t>(p) * count + b) * a.d + c);
         lo += from[0], hi += from[1];
     }
     const u32x4_t w = {bf16_pair(lo[0], lo[1]), bf16_pair(lo[2], lo[3]), bf16_pair(hi[0], hi[1]), bf16_pair(hi[2], hi[3])};
@@ -349,34 +402,16 @@ __global__ __launch_bounds__(256) void loss_spread_kernel(SpreadArgs a) {
 uint32_t div_up(uint64_t x, uint32_t y) { return static_cast<uint32_t>((x + y - 1) / y); }
 uint32_t round_up(uint32_t x, uint32_t y) { return div_up(x, y) * y; }
 
-constexpr uint32_t kVocabTile = 256;  // vocabulary rows of every tile of logits
 constexpr uint32_t kLossMaxRows = 65536, kLossMaxVocab = 1u << 24;
 
-// How a backward pass over `rows` rows is cut.
-struct BackPlan {
-    uint32_t piece;     // vocabulary rows at a time, a multiple of 256
-    uint32_t parts;     // of d_hidden's sums
-    uint64_t dz, part;  // elements of dz and of all parts
-};
-
-BackPlan back_plan(uint32_t rows, uint32_t vocab, uint32_t d) {
-    BackPlan p{};
+// dz holds a piece of the vocabulary: up to 65,536 of it, 2^27 values with all rows (256 MB), a multiple of 256.
+uint32_t most_of_piece(uint32_t rows) {
+    const uint32_t most = static_cast<uint32_t>((1ull << 27) / rows) / 256 * 256;
+    return most < 256 ? 256 : most < 65536 ? most : 65536;
+}
+uint32_t piece_of(uint32_t rows, uint32_t vocab) {  // pieces alike
     const uint32_t all = round_up(vocab, 256);
-    uint32_t most = static_cast<uint32_t>((1ull << 27) / rows) / 256 * 256;
-    most = most < 65536 ? most : 65536;
-    most = most > 256 ? most : 256;
-    p.piece = round_up(div_up(all, div_up(all, most)), 256);
-    // d_hidden has few tiles: its sums are cut into the parts, of at least 1,024 columns, that fill the units best, the
-    // fewest of those (2,048 rows of 5,376: 168 tiles in 3 parts, two full rounds)
-    const uint64_t tiles = static_cast<uint64_t>(div_up(rows, 256)) * div_up(d, 256), can = div_up(p.piece, 1024);
-    p.parts = 1;
-    for (uint32_t n = 2; n <= can && n <= 16; ++n) {
-        const uint64_t now = (tiles * n + 255) / 256 * p.parts, best = (tiles * p.parts + 255) / 256 * n;
-        if (20 * now < 19 * best) p.parts = n;
-    }
-    p.dz = static_cast<uint64_t>(rows) * p.piece;
-    p.part = static_cast<uint64_t>(p.parts) * rows * d;
-    return p;
+    return round_up(div_up(all, div_up(all, most_of_piece(rows))), 256);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -404,31 +439,36 @@ namespace twd {
 namespace {
 
 template <bool GRAD>
-int launch_logits(LogitArgs a, uint32_t rows, uint32_t vocab_rows, hipStream_t s) {
-    auto go = [&](auto tile) -> int {
-        using Tile = decltype(tile);
-        static_assert(Tile::kA == kVocabTile, "the tiles' parts");
-        a.grid = TileGrid{div_up(vocab_rows, Tile::kA), div_up(rows, Tile::kB), 1};
-        loss_logits_kernel<Tile, GRAD><<<a.grid.blocks(), kProductThreads, 0, s>>>(a);
+int launch_logits(const LogitArgs& a, uint32_t rows, hipStream_t s) {
+    if (rows <= kFewRows) {
+        loss_logits_kernel<TileFew, GRAD><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a);
         TWD_HIP(hipGetLastError());
         return TWD_OK;
-    };
-    if (rows <= 64) return go(Tile64{});
-    if (rows <= 128) return go(Tile128{});
-    return go(Tile256{});
+    }
+    // as many blocks as any number of rows that count needs
+    const uint32_t na = div_up(a.here, kVocabTile);
+    if (rows > kMostNarrow) {
+        loss_logits_kernel<TileWide, GRAD><<<blocks_for(na * div_up(rows, 256)), kProductThreads, 0, s>>>(a);
+        TWD_HIP(hipGetLastError());
+    }
+    const uint32_t narrow = (rows > kMostNarrow ? 4 * kMostNarrow : 0) + na * div_up(rows < kMostNarrow ? rows : kMostNarrow, 64);
+    loss_logits_kernel<TileNarrow, GRAD><<<blocks_for(narrow), kProductThreads, 0, s>>>(a);
+    TWD_HIP(hipGetLastError());
+    return TWD_OK;
 }
 
 template <typename Tile, typename Out, bool BY_COUNT>
-int launch_grad(GradArgs a, hipStream_t s) {
-    a.grid = TileGrid{div_up(a.rows, Tile::kA), div_up(a.cols, Tile::kB), a.grid.parts};
-    loss_grad_kernel<Tile, Out, BY_COUNT><<<a.grid.blocks(), kProductThreads, 0, s>>>(a);
+int launch_grad(const GradArgs& a, uint32_t most_tiles, hipStream_t s) {
+    const uint64_t nb = div_up(a.cols, Tile::kB), tiles = BY_COUNT ? nb * div_up(a.rows, Tile::kA) : most_tiles;
+    loss_grad_kernel<Tile, Out, BY_COUNT><<<blocks_for(static_cast<uint32_t>(tiles)), kProductThreads, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
 
 int launch_gather(const twd_headloss* l, GatherArgs a, hipStream_t s) {
     a.r = l->r, a.vocab = l->vocab, a.pieces = l->d / 8;
-    loss_gather_kernel<<<div_up(a.rows, kGatherRows), 256, 0, s>>>(a);
+    a.each = div_up(a.rows, 4096);  // a block counts all targets before its own: not too many of them
+    loss_gather_kernel<<<div_up(a.rows, a.each), 256, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -437,10 +477,10 @@ int forward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, h
     if (const int rc = launch_gather(l, g, s)) return rc;
     LogitArgs a{};
     a.r = l->r, a.weight = weight, a.hidden = Operand{l->r.h, l->d, g.rows, l->d};
-    a.d = l->d, a.vocab = l->vocab, a.softcap = soft_cap(l->softcap), a.part = l->part, a.part_stride = g.rows;
-    if (const int rc = launch_logits<false>(a, g.rows, l->vocab, s)) return rc;
+    a.d = l->d, a.vocab = a.here = l->vocab, a.softcap = soft_cap(l->softcap), a.part = l->part, a.part_stride = g.rows;
+    if (const int rc = launch_logits<false>(a, g.rows, s)) return rc;
     loss_join_kernel<<<div_up(g.rows, kJoinRows), kJoinThreads, 0, s>>>(
-        JoinArgs{l->r, l->part, div_up(l->vocab, kVocabTile), g.rows, g.losses, g.lse_out});
+        JoinArgs{l->r, l->part, div_up(l->vocab, g.rows <= kFewRows ? TileFew::kA : kVocabTile), g.rows, g.losses, g.lse_out});
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -455,35 +495,40 @@ struct BackOut {
 };
 
 int backward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, const BackOut& o, hipStream_t s) {
-    const BackPlan p = back_plan(g.rows, l->vocab, l->d);
+    const uint32_t piece = piece_of(g.rows, l->vocab);
     int rc = launch_gather(l, g, s);
     if (rc) return rc;
-    for (uint32_t v0 = 0; v0 < l->vocab; v0 += p.piece) {
-        const uint32_t here = l->vocab - v0 < p.piece ? l->vocab - v0 : p.piece;
+    uint32_t most_tiles = 0;  // of d_hidden's product, for any number of rows that count
+    for (uint32_t n = 1; n <= div_up(g.rows, TileHidden::kA); ++n) {
+        const uint32_t tiles = n * div_up(l->d, TileHidden::kB) * hidden_parts(n * TileHidden::kA, l->d, piece);
+        most_tiles = tiles > most_tiles ? tiles : most_tiles;
+    }
+    for (uint32_t v0 = 0; v0 < l->vocab; v0 += piece) {
+        const uint32_t here = l->vocab - v0 < piece ? l->vocab - v0 : piece;
         const Operand h{l->r.h, l->d, g.rows, l->d}, w{weight.p + v0 * weight.stride, weight.stride, here, l->d};
         LogitArgs a{};
         a.r = l->r, a.weight = weight, a.hidden = h;
-        a.d = l->d, a.vocab = l->vocab, a.v0 = v0, a.softcap = soft_cap(l->softcap), a.dz = l->dz, a.dz_stride = p.piece;
-        if ((rc = launch_logits<true>(a, g.rows, here, s))) return rc;
+        a.d = l->d, a.vocab = l->vocab, a.v0 = v0, a.here = here, a.softcap = soft_cap(l->softcap), a.dz = l->dz, a.dz_stride = piece;
+        if ((rc = launch_logits<true>(a, g.rows, s))) return rc;
         if (o.d_weight) {
             GradArgs b{};
-            b.count = l->r.count, b.a = Operand{l->dz, p.piece, g.rows, p.piece}, b.b = h;
-            b.rows = here, b.cols = l->d, b.grid.parts = 1, b.stride = o.d_weight_stride, b.add = o.add;
+            b.count = l->r.count, b.a = Operand{l->dz, piece, g.rows, piece}, b.b = h;
+            b.rows = here, b.cols = l->d, b.stride = o.d_weight_stride, b.add = o.add;
             b.out = static_cast<char*>(o.d_weight) + v0 * o.d_weight_stride * (o.type == TWD_F32 ? 4 : 2);
-            rc = o.type == TWD_F32 ? launch_grad<TileWeight, float, true>(b, s) : launch_grad<TileWeight, uint16_t, true>(b, s);
+            rc = o.type == TWD_F32 ? launch_grad<TileWeight, float, true>(b, 0, s) : launch_grad<TileWeight, uint16_t, true>(b, 0, s);
             if (rc) return rc;
         }
         if (o.d_hidden) {
             GradArgs b{};
-            b.count = l->r.count, b.a = Operand{l->dz, p.piece, g.rows, here}, b.b = w;
-            b.k = here, b.k_part = round_up(div_up(here, p.parts), 128), b.rows = g.rows, b.cols = l->d, b.grid.parts = p.parts;
-            b.out = l->dh, b.stride = l->d, b.part = static_cast<uint64_t>(g.rows) * l->d, b.add = v0 > 0;
-            if ((rc = launch_grad<TileHidden, float, false>(b, s))) return rc;
+            b.count = l->r.count, b.a = Operand{l->dz, piece, g.rows, here}, b.b = w;
+            b.k = here, b.piece = piece, b.cols = l->d;
+            b.out = l->dh, b.stride = l->d, b.add = v0 > 0;
+            if ((rc = launch_grad<TileHidden, float, false>(b, most_tiles, s))) return rc;
         }
     }
     if (!o.d_hidden) return TWD_OK;
     loss_spread_kernel<<<dim3(g.rows, div_up(l->d, 2048)), 256, 0, s>>>(
-        SpreadArgs{l->r, g.targets, l->dh, p.parts, g.rows, l->vocab, l->d, static_cast<uint64_t>(g.rows) * l->d, o.d_hidden, o.d_hidden_stride});
+        SpreadArgs{l->r, g.targets, l->dh, piece, l->vocab, l->d, o.d_hidden, o.d_hidden_stride});
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -534,10 +579,11 @@ TWD_API int twd_headloss_create(uint32_t max_rows, uint32_t vocab, uint32_t d_mo
     twd_headloss* l = new (std::nothrow) twd_headloss{};
     if (!l) return fail(TWD_E_INVALID, "out of host memory");
     l->max_rows = max_rows, l->vocab = vocab, l->d = d_model, l->softcap = softcap, l->backward = backward != 0, l->device = dev;
-    uint64_t dz = 0, part = 0;
-    for (uint32_t rows = 1; l->backward && rows <= max_rows; ++rows) {  // the most that any number of rows takes
-        const BackPlan p = back_plan(rows, vocab, d_model);
-        dz = p.dz > dz ? p.dz : dz, part = p.part > part ? p.part : part;
+    uint64_t dz = 0, part = 0;  // the most that any number of rows, and of those that count, takes
+    for (uint32_t rows = 1; l->backward && rows <= max_rows; ++rows) {
+        const uint64_t n = static_cast<uint64_t>(rows) * piece_of(rows, vocab);
+        const uint64_t m = static_cast<uint64_t>(rows) * d_model * hidden_parts(rows, d_model, most_of_piece(rows));
+        dz = n > dz ? n : dz, part = m > part ? m : part;
     }
     char* at = nullptr;
     uint64_t size = 0;
@@ -554,7 +600,9 @@ TWD_API int twd_headloss_create(uint32_t max_rows, uint32_t vocab, uint32_t d_mo
         take(l->r.lse, max_rows);
         take(l->r.hit, max_rows);
         take(l->r.h, static_cast<uint64_t>(max_rows) * d_model);
-        take(l->part, static_cast<uint64_t>(div_up(vocab, kVocabTile)) * max_rows);
+        const uint64_t many = static_cast<uint64_t>(div_up(vocab, kVocabTile)) * max_rows;
+        const uint64_t few = static_cast<uint64_t>(div_up(vocab, TileFew::kA)) * (max_rows < kFewRows ? max_rows : kFewRows);
+        take(l->part, many > few ? many : few);
         if (!l->backward) return;
         take(l->dz, dz);
         take(l->dh, part);

@@ -35,21 +35,21 @@ constexpr uint64_t kMaxProductStride = 1ull << 22;
 struct TileGrid {
     uint32_t na, nb, parts;  // tiles along A and B, and parts of the sum
     __host__ __device__ uint32_t tiles() const { return na * nb * parts; }
-    __host__ __device__ uint32_t blocks() const { return (tiles() + 7) / 8 * 8; }
 };
 struct TileAt {
     uint32_t a, b, part;
     uint32_t share, who;  // the blocks that read the same rows of A at once, and which of them this is
 };
-__device__ __forceinline__ bool tile_of_block(const TileGrid& g, TileAt* at) {
-    const uint32_t id = blockIdx.x % 8 * (g.blocks() / 8) + blockIdx.x / 8;
-    if (id >= g.tiles()) return false;
+__host__ __device__ inline uint32_t blocks_for(uint32_t tiles) { return (tiles + 7) / 8 * 8; }
+// This block's number among `tiles`, or one past them.
+__device__ __forceinline__ uint32_t stretched(uint32_t tiles) {
+    const uint32_t each = (tiles + 7) / 8, in = blockIdx.x / 8;
+    return in < each ? blockIdx.x % 8 * each + in : tiles;
+}
+__device__ __forceinline__ TileAt tile_at(const TileGrid& g, uint32_t id) {
     const uint32_t each = g.na * g.nb, in = id % each;
-    at->part = id / each;
     const uint32_t group = in / (8 * g.na), left = in - group * 8 * g.na, width = min(8u, g.nb - 8 * group);
-    at->a = left / width, at->b = 8 * group + left % width;
-    at->share = width, at->who = left % width;
-    return true;
+    return TileAt{left / width, 8 * group + left % width, id / each, width, left % width};
 }
 
 constexpr uint32_t kProductThreads = 256;
