@@ -91,69 +91,42 @@ struct LogitArgs {
 
 // By rows, or with the second operand turned.
 using TileFew = ProductTile<1, 2, 4, 1, 64, 3, false, false>;
-using TileNarrow = ProductTile<2, 2, 4, 1, 64, 2, false, false>;
 using TileWide = ProductTile<4, 4, 2, 2, 64, 2, false, false, true>;
+using TileMiddle = ProductTile<4, 2, 2, 2, 64, 2, false, false, true>;
+using TileQuarter = ProductTile<2, 2, 4, 1, 64, 3, false, false, true>;
 using TileHidden = ProductTile<4, 4, 2, 2, 32, 4, false, true>;
 using TileWeight = ProductTile<4, 2, 2, 2, 32, 3, true, true>;
 
-// Which tiles of logits are wide (256 rows) and which narrow (64): of the rows that count, whole wide tiles, and a last one
-// where that saves narrow ones; and of these tiles, whole rounds of the units, and a last one likewise. Narrow tiles are
-// two to a unit and take some 0.35 of a wide one's time.
-constexpr uint32_t kVocabTile = 256;  // vocabulary rows of a wide or narrow tile
-static_assert(TileWide::kA == kVocabTile && TileNarrow::kA == kVocabTile && TileNarrow::kB * 4 == TileWide::kB, "quarters");
-constexpr uint32_t kFewRows = 64, kMostNarrow = 128, kRound = 256;
-struct WideTiles {
-    TileGrid grid;   // of wide tiles
-    uint32_t wide;   // those that are taken as wide ones, the first in order
-    uint32_t rest;   // rows past the wide tiles'
-    __device__ uint32_t narrow() const { return (grid.tiles() - wide) * 4 + grid.na * ((rest + 63) / 64); }
+// Tiles of logits are of 256 vocabulary rows by 256 hidden rows, or by 128 where no more count. (Narrower tiles for the last
+// hidden rows do not pay: a stage waits for memory as long as a wide one's. 823 rows of 65,537 x 2,880 with 55 in tiles of 64:
+// 437 us.) The few tiles past whole rounds of the units are cut into four and follow in a launch of their own, so that a
+// last round of up to kMostCut costs less than a round (1,023 rows: 459 and 403 us).
+constexpr uint32_t kVocabTile = 256, kRound = 256, kMostCut = 64, kFewRows = 64;
+static_assert(TileWide::kA == kVocabTile && TileMiddle::kA == kVocabTile && TileQuarter::kA == kVocabTile, "one width");
+struct LogitTiles {
+    TileGrid grid;
+    uint32_t cut;  // of the last tiles
 };
-__device__ __forceinline__ WideTiles wide_tiles(uint32_t count, uint32_t na) {
-    WideTiles w;
-    w.rest = count % 256 <= kMostNarrow ? count % 256 : 0;
-    w.grid = TileGrid{na, (count - w.rest + 255) / 256, 1};
-    const uint32_t left = w.grid.tiles() % kRound;
-    w.wide = w.grid.tiles() - (left <= kMostNarrow ? left : 0);
-    return w;
+__device__ __forceinline__ LogitTiles logit_tiles(uint32_t count, uint32_t na) {
+    const TileGrid g{na, (count + 255) / 256, 1};
+    const uint32_t left = g.tiles() % kRound;
+    return LogitTiles{g, count > 128 && left <= kMostCut ? left : 0};
 }
 
 template <typename Tile>
 constexpr int kWavesPerEu = Tile::kBytes > 81920 ? 1 : 2;  // blocks to a unit
 
+// The tile of vocabulary rows kA va .. and hidden rows m0 ..
 template <typename Tile, bool GRAD>
-__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_logits_kernel(LogitArgs a) {
+__device__ __forceinline__ void logits_tile(const LogitArgs& a, uint32_t count, uint32_t va, uint32_t m0, uint32_t share, uint32_t who,
+                                            u32x4_t* s0, u32x4_t* s1, u32x4_t* s2, u32x4_t* s3, uint32_t* sink) {
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GA = Tile::kGA, GB = Tile::kGB;
-    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
-    __shared__ uint32_t sink[Tile::kSink];
-    TileAt at;
-    const uint32_t count = *a.r.count, na = (a.here + Tile::kA - 1) / Tile::kA;
-    if constexpr (Tile::kA != kVocabTile) {  // few rows: one tile along them
-        const uint32_t id = stretched(na);
-        if (id >= na) return;
-        at = TileAt{id, 0, 0, 1, 0};
-    } else {
-        const WideTiles t = wide_tiles(count, na);
-        const uint32_t tiles = Tile::kB == 256 ? t.wide : t.narrow(), id = stretched(tiles);
-        if (id >= tiles) return;
-        if constexpr (Tile::kB == 256) {
-            at = tile_at(t.grid, id);
-        } else {
-            const uint32_t quarters = (t.grid.tiles() - t.wide) * 4;
-            if (id < quarters) {
-                at = tile_at(t.grid, t.wide + id / 4);
-                at.b = 4 * at.b + id % 4;
-            } else {
-                const uint32_t wide = (t.rest + 63) / 64;
-                at = TileAt{(id - quarters) / wide, 4 * t.grid.nb + (id - quarters) % wide, 0, 1, 0};
-            }
-        }
-    }
-    const uint32_t m0 = at.b * Tile::kB, v_tile = a.v0 + at.a * Tile::kA;
-    if (m0 >= count) return;
-    Operand w = a.weight;  // the piece's rows
+    const uint32_t v_tile = a.v0 + va * Tile::kA;
+    Operand w = a.weight, h = a.hidden;  // the piece's rows, and those from m0 on
     w.p += a.v0 * w.stride, w.rows = a.here;
+    h.p += m0 * h.stride, h.rows = count - m0;
     f32x16_t acc[TA][TB];
-    Tile::template sums<false>(s0, s1, s2, s3, sink, w, a.hidden, at, a.d, acc);
+    Tile::template sums<false>(s0, s1, s2, s3, sink, w, h, TileAt{va, 0, 0, share, who}, a.d, acc);
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
     const uint32_t v_lane = v_tile + 32 * TA * wa + 4 * (lane / 32);
     const bool whole = v_tile + Tile::kA <= a.vocab;
@@ -244,9 +217,45 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
                 p.y = p.y * __builtin_amdgcn_exp2f((p.x - ref) * kLog2e) + q.y * __builtin_amdgcn_exp2f((q.x - ref) * kLog2e);
                 p.x = top;
             }
-            a.part[static_cast<uint64_t>(at.a) * a.part_stride + m0 + in] = p;
+            a.part[static_cast<uint64_t>(va) * a.part_stride + m0 + in] = p;
         }
     }
+}
+
+template <bool GRAD>
+__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_logits_kernel(LogitArgs a) {
+    __shared__ u32x4_t s0[TileWide::kPieces], s1[TileWide::kPieces];
+    __shared__ uint32_t sink[TileWide::kSink];
+    const uint32_t count = *a.r.count;
+    const LogitTiles t = logit_tiles(count, (a.here + kVocabTile - 1) / kVocabTile);
+    const uint32_t tiles = t.grid.tiles() - t.cut, id = stretched(tiles);
+    if (id >= tiles) return;
+    const TileAt at = tile_at(t.grid, id);
+    if (count > 128) logits_tile<TileWide, GRAD>(a, count, at.a, 256 * at.b, at.share, at.who, s0, s1, nullptr, nullptr, sink);
+    else logits_tile<TileMiddle, GRAD>(a, count, at.a, 0, 1, 0, s0, s1, nullptr, nullptr, sink);
+}
+
+template <bool GRAD>
+__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_quarters_kernel(LogitArgs a) {
+    using Tile = TileQuarter;
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces];
+    __shared__ uint32_t sink[Tile::kSink];
+    const uint32_t count = *a.r.count;
+    const LogitTiles t = logit_tiles(count, (a.here + kVocabTile - 1) / kVocabTile);
+    const uint32_t id = stretched(4 * t.cut);
+    if (id >= 4 * t.cut) return;
+    const TileAt at = tile_at(t.grid, t.grid.tiles() - t.cut + id / 4);
+    const uint32_t m0 = 256 * at.b + 64 * (id % 4);
+    if (m0 < count) logits_tile<Tile, GRAD>(a, count, at.a, m0, 4, id % 4, s0, s1, s2, nullptr, sink);
+}
+
+// Few rows: bound by the read of the weights.
+template <bool GRAD>
+__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_few_kernel(LogitArgs a) {
+    using Tile = TileFew;
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces];
+    const uint32_t count = *a.r.count, tiles = (a.here + Tile::kA - 1) / Tile::kA, id = stretched(tiles);
+    if (id < tiles && count > 0) logits_tile<Tile, GRAD>(a, count, id, 0, 1, 0, s0, s1, s2, nullptr, nullptr);
 }
 
 struct JoinArgs {
@@ -441,18 +450,12 @@ namespace {
 template <bool GRAD>
 int launch_logits(const LogitArgs& a, uint32_t rows, hipStream_t s) {
     if (rows <= kFewRows) {
-        loss_logits_kernel<TileFew, GRAD><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a);
+        loss_few_kernel<GRAD><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a);
+    } else {  // as many blocks as any number of rows that count needs
+        loss_logits_kernel<GRAD><<<blocks_for(div_up(a.here, kVocabTile) * div_up(rows, 256)), kProductThreads, 0, s>>>(a);
         TWD_HIP(hipGetLastError());
-        return TWD_OK;
+        loss_quarters_kernel<GRAD><<<4 * kMostCut, kProductThreads, 0, s>>>(a);
     }
-    // as many blocks as any number of rows that count needs
-    const uint32_t na = div_up(a.here, kVocabTile);
-    if (rows > kMostNarrow) {
-        loss_logits_kernel<TileWide, GRAD><<<blocks_for(na * div_up(rows, 256)), kProductThreads, 0, s>>>(a);
-        TWD_HIP(hipGetLastError());
-    }
-    const uint32_t narrow = (rows > kMostNarrow ? 4 * kMostNarrow : 0) + na * div_up(rows < kMostNarrow ? rows : kMostNarrow, 64);
-    loss_logits_kernel<TileNarrow, GRAD><<<blocks_for(narrow), kProductThreads, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
