@@ -170,6 +170,12 @@ _SIGS = {
     "twd_headloss_forward": (C.c_int, [_vp, _vp, _u32, _u64, _vp, _u64, _vp, _vp, _vp, _vp]),
     "twd_headloss_backward": (C.c_int, [_vp, _vp, _u32, _u64, _vp, _u64, _vp, _vp, _vp, _vp, _u64, _vp, C.c_int, _u64,
                                         C.c_int, _vp]),
+    "twd_embed": (C.c_int, [_vp, C.c_int, _u32, _u32, _u64, _vp, _u32, _f32, _vp, C.c_int, _u64, _vp]),
+    "twd_embedgrad_create": (C.c_int, [_u32, _u32, C.POINTER(_vp)]),
+    "twd_embedgrad_destroy": (None, [_vp]),
+    "twd_embedgrad_info": (C.c_int, [_vp, C.POINTER(_u64)]),
+    "twd_embedgrad_run": (C.c_int, [_vp, _vp, C.c_int, _u32, _u32, _u64, _vp, _f32, _vp, C.c_int, _u32, _u64, C.c_int,
+                                    _vp]),
     "twd_probe_read_bandwidth": (C.c_int, [_vp, _u64, _u32, _u32, _vp, C.POINTER(_f32),
                                            C.POINTER(_u64)]),
 }
@@ -1081,6 +1087,66 @@ class HeadLoss:
                                              _ptr(d_weight), kind, v_stride, 1 if accumulate else 0,
                                              _stream_on(hidden, stream)))
         return d_hidden, d_weight
+
+
+def embed(table, ids, scale: float = 1.0, out=None, dtype=None, stream=None):
+    """Rows of a float32, bfloat16 or float16 table [vocab, d_model] by int32 ids [n] of the device, times scale
+    (twd_embed), in out's type, or `dtype`, or the table's. An id outside the vocabulary (-1) gives a row of zeros."""
+    import torch
+    kind = _type_of(table, "table")
+    vocab, d, stride = _matrix(table, "table")
+    n = ids.shape[0]
+    _buffer(ids, (n,), torch.int32, "ids")
+    with _on_device(table, ids, out):
+        if out is None:
+            out = _made(torch.empty, (n, d), dtype or table.dtype, table.device, stream)
+        elif out.shape != (n, d) or (dtype is not None and out.dtype != dtype):
+            raise ValueError(f"out must be of shape {(n, d)} and of dtype, where that is given")
+        _check(lib.twd_embed(table.data_ptr(), kind, vocab, d, stride, ids.data_ptr(), n, scale, out.data_ptr(),
+                             _type_of(out, "out"), _matrix(out, "out")[2], _stream_on(table, stream)))
+    return out
+
+
+class EmbedGrad:
+    """Scratch for the embedding lookup's gradient by sorted ids (twd_embedgrad)."""
+
+    def __init__(self, max_ids: int, max_d_model: int):
+        self.handle = None
+        h = C.c_void_p()
+        _check(lib.twd_embedgrad_create(max_ids, max_d_model, C.byref(h)))
+        self.handle = h
+        self.max_ids, self.max_d_model = max_ids, max_d_model
+        n = _u64()
+        _check(lib.twd_embedgrad_info(h, C.byref(n)))
+        self.nbytes = n.value
+
+    def close(self):
+        if self.handle:
+            lib.twd_embedgrad_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def run(self, d_rows, ids, d_table, scale: float = 1.0, accumulate: bool = False, stream=None):
+        """d_table [vocab, d_model] from the gradients d_rows [n, d_model] of the rows looked up by int32 ids [n]
+        (twd_embedgrad_run), each in any of the three floating types: every row is written, or with accumulate only
+        those that have an id are added to. Ids outside the vocabulary have no part in it."""
+        import torch
+        kind, out_kind = _type_of(d_rows, "d_rows"), _type_of(d_table, "d_table")
+        n, d, stride = _matrix(d_rows, "d_rows")
+        vocab, width, out_stride = _matrix(d_table, "d_table")
+        if width != d:
+            raise ValueError(f"d_table must have d_rows' {d} columns")
+        _buffer(ids, (n,), torch.int32, "ids")
+        with _on_device(d_table, d_rows, ids):
+            _check(lib.twd_embedgrad_run(self.handle, d_rows.data_ptr(), kind, n, d, stride, ids.data_ptr(), scale,
+                                         d_table.data_ptr(), out_kind, vocab, out_stride, 1 if accumulate else 0,
+                                         _stream_on(d_table, stream)))
+        return d_table
 
 
 def probe_read_bandwidth(buf, waves: int = 32768, launches: int = 50, stream=None):
