@@ -9,4 +9,4 @@ from .twd import (LMHead, Selector, SamplingParams, SpeculativeCoordinator, RowP
                   apply_repetition_penalty, sample_token, seed_for, splitmix64,
                   validate_sampling, uniform_from_seed, generate_head, head_bytes, decode_verify,
                   TwdError, G4DenseFormatError, LIB_PATH, MxHead, Sampler, mx_quantize, mx_dequantize,
-                  HeadLoss, embed, EmbedGrad)
+                  HeadLoss, embed, EmbedGrad, Fp8Head, fp8_quantize)

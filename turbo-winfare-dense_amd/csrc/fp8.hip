@@ -1,0 +1,571 @@
+// 8-bit floating point with a scale for each block of 128: rows and weights to the format, and the LM head's product with
+// weights held in it.
+//
+// An element is an e4m3 code; hidden rows have an fp32 scale for each 128 columns, weights one for each 128 x 128. The product
+// of 128 columns runs on the 8-bit matrix instructions, whose sums are then multiplied by the two scales and added up in fp32.
+#include <hip/hip_runtime.h>
+
+#include <new>
+#include <string>
+
+#include "product.h"
+#include "twd_fp8.h"
+#include "twd_internal.h"
+#include "vocab_core.h"
+
+namespace twd {
+
+namespace {
+
+constexpr uint32_t kBlock = 128;
+constexpr float kTop = 448.0f, kLeastScale = 0x1p-126f;
+
+// ---- to the format --------------------------------------------------------------------------------------
+
+// x / s to the nearest float, but where the quotient lies between two floats, to the one with an odd mantissa: rounding
+// that to fewer bits is rounding the quotient itself. The remainder's sign says on which side it lies; where it would be
+// below the normal numbers, both are brought up first.
+__device__ __forceinline__ float quotient(float x, float s) {
+    const float up_by = s < 0x1p-64f ? 0x1p64f : 1.0f;
+    x *= up_by, s *= up_by;
+    const float q = x / s, left = fmaf(-q, s, x);
+    const uint32_t u = __float_as_uint(q);
+    const bool up = (left > 0.0f) != (x < 0.0f);  // the quotient is larger in magnitude
+    const bool move = left != 0.0f && (u & 1u) == 0;
+    return __uint_as_float(move ? (up ? u + 1 : u - 1) : u);
+}
+
+__device__ __forceinline__ float scale_of(uint32_t top) {  // of the largest magnitude's bits
+    const float s = fmaxf(__uint_as_float(top) / kTop, kLeastScale);
+    return top >= 0x7F800000u ? __builtin_nanf("") : s;
+}
+
+__device__ __forceinline__ u32x2_t codes_of(const float (&v)[8], float s) {
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) q[i] = quotient(v[i], s);
+    u32x2_t w;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        int c = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
+        c = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], c, true);
+        w[i] = s != s ? 0u : static_cast<uint32_t>(c);
+    }
+    return w;
+}
+
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t largest(const float (&v)[8]) {  // magnitudes order as their bits do, NaN above all
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = larger(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return top;
+}
+__device__ __forceinline__ uint32_t largest_of_sixteen(uint32_t top) {  // lanes
+    top = larger(top, dpp_move<0xB1>(top, top));
+    top = larger(top, dpp_move<0x4E>(top, top));
+    top = larger(top, dpp_move<0x141>(top, top));
+    return larger(top, dpp_move<0x140>(top, top));
+}
+
+struct QuantArgs {
+    const void* x;
+    uint64_t stride;
+    uint64_t rows;
+    uint32_t blocks;  // of 128 columns
+    uint8_t* codes;
+    float* scales;
+    bool wide;  // rows start at multiples of 16 bytes
+};
+
+// Eight columns to a lane, sixteen lanes to a scale.
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_rows_kernel(QuantArgs a) {
+    const uint32_t g = blockIdx.x * 256 + threadIdx.x, b = g / 16;
+    if (b >= a.blocks) return;
+    for (uint64_t r = blockIdx.y; r < a.rows; r += gridDim.y) {
+        float v[8];
+        Eight<T>::load(static_cast<const T*>(a.x) + r * a.stride + 8ull * g, a.wide, v);
+        const float s = scale_of(largest_of_sixteen(largest(v)));
+        reinterpret_cast<u32x2_t*>(a.codes)[(r * a.blocks) * 16 + g] = codes_of(v, s);
+        if (g % 16 == 0) a.scales[r * a.blocks + b] = s;
+    }
+}
+
+// A block to 128 x 128.
+template <typename T>
+__global__ __launch_bounds__(256) void fp8_weights_kernel(QuantArgs a) {
+    __shared__ uint32_t tops[4];
+    const uint32_t t = threadIdx.x, b = blockIdx.y, in = t % 16;
+    const uint64_t r0 = static_cast<uint64_t>(blockIdx.x) * kBlock;
+    float v[8][8] = {};
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const uint64_t r = r0 + 16 * i + t / 16;
+        if (r < a.rows) Eight<T>::load(static_cast<const T*>(a.x) + r * a.stride + kBlock * b + 8 * in, a.wide, v[i]);
+        top = larger(top, largest(v[i]));
+    }
+    top = wave_reduce(top, 0u, [](uint32_t x, uint32_t y) { return larger(x, y); });
+    if (t % 64 == 0) tops[t / 64] = top;
+    __syncthreads();
+    const float s = scale_of(larger(larger(tops[0], tops[1]), larger(tops[2], tops[3])));
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        const uint64_t r = r0 + 16 * i + t / 16;
+        if (r < a.rows) reinterpret_cast<u32x2_t*>(a.codes)[(r * a.blocks + b) * 16 + in] = codes_of(v[i], s);
+    }
+    if (t == 0) a.scales[blockIdx.x * static_cast<uint64_t>(a.blocks) + b] = s;
+}
+
+// ---- the head's layout in HBM ---------------------------------------------------------------------
+//
+// A group is 64 vocabulary rows, four tiles of 16; a chunk is 128 columns. Codes are [group][chunk][tile][half][lane] 16 bytes:
+// lane 16 kg + r's two halves are row r's columns 32 kg .. 32 kg + 31 of the chunk, as the 16 x 16 x 128 instruction takes
+// them; two tiles' lanes of two kg's are an operand of a 32 x 32 x 64 one. A wave's load moves contiguous memory either
+// way. Rows past the vocabulary are zero codes. Scales stay [group / 2][chunk].
+constexpr uint32_t kGroupRows = 64;
+constexpr uint32_t kUnit = 512;  // 16-byte pieces of a group's chunk
+
+__global__ __launch_bounds__(256) void fp8_repack_kernel(const uint8_t* __restrict__ codes, uint32_t vocab, uint32_t d,
+                                                        u32x4_t* __restrict__ out) {
+    const uint32_t lane = threadIdx.x % 64, tile = threadIdx.x / 64, kg = lane / 16, chunks = d / kBlock;
+    const uint64_t group = blockIdx.x, row = group * kGroupRows + 16 * tile + lane % 16;
+    for (uint32_t c = 0; c < chunks; ++c)
+#pragma unroll
+        for (uint32_t h = 0; h < 2; ++h) {
+            u32x4_t w = {0, 0, 0, 0};
+            if (row < vocab) w = *reinterpret_cast<const u32x4_t*>(codes + row * d + kBlock * c + 32 * kg + 16 * h);
+            out[(group * chunks + c) * kUnit + (2 * tile + h) * 64 + lane] = w;
+        }
+}
+
+__global__ __launch_bounds__(256) void fp8_check_kernel(const float* scales, float* kept, uint64_t n, uint32_t* bad) {
+    for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
+        const float s = scales[i];
+        if (!(s >= 0.0f && s <= 0x1p100f)) *bad = 1;
+        kept[i] = s;
+    }
+}
+
+struct Fp8Args {
+    const u32x4_t* codes;
+    const float* scales;
+    const uint8_t* x;
+    const float* xs;
+    void* out;
+    uint64_t out_stride;
+    uint32_t vocab, d, chunks, groups, rows;
+    SoftCap softcap;
+};
+
+__device__ __forceinline__ i32x8_t operand(u32x4_t lo, u32x4_t hi) {
+    return __builtin_bit_cast(i32x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+// ---- up to 16 hidden rows: the weights stream past rows held in registers ---------------------------
+//
+// Bound by the read of the head. The waves of a block split d_model by quads of chunks; a wave keeps its quad of the hidden
+// rows in registers and streams its quad of one group after another, kAhead chunks (8 KB each) ahead of the arithmetic. The
+// sums over the quads meet in LDS, two buffers in turn.
+constexpr uint32_t kSmallRows = 16;
+constexpr uint32_t kSmallWaves = 12;
+constexpr uint32_t kAhead = 2;
+
+template <typename Out>
+__global__ __launch_bounds__(kSmallWaves * 64) void fp8_small_kernel(Fp8Args a) {
+    extern __shared__ float part[];  // [2][quad][row][64]
+    const uint32_t lane = threadIdx.x % 64, kg = lane / 16, r = lane % 16, quads = (a.chunks + 3) / 4;
+    const uint32_t quad = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t here = min(4u, a.chunks - 4 * quad);
+    i32x8_t x[4];
+    float xs[4];
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) {
+        u32x4_t lo = {0, 0, 0, 0}, hi = lo;
+        xs[c] = 0.0f;
+        if (c < here && r < a.rows) {
+            const u32x4_t* p = reinterpret_cast<const u32x4_t*>(a.x + static_cast<uint64_t>(r) * a.d + kBlock * (4 * quad + c) + 32 * kg);
+            lo = p[0], hi = p[1];
+            xs[c] = a.xs[static_cast<uint64_t>(r) * a.chunks + 4 * quad + c];
+        }
+        x[c] = operand(lo, hi);
+    }
+    // a group past the last has no bytes, so nothing is read of it; past the quad's end the last chunk comes again, whose
+    // products count for nothing
+    auto codes_of_group = [&](uint32_t g) {
+        return make_rsrc(a.codes + (static_cast<uint64_t>(g) * a.chunks + 4 * quad) * kUnit, g < a.groups ? here * kUnit * 16 : 0);
+    };
+    auto scales_of_group = [&](uint32_t g) {
+        return make_rsrc(a.scales + static_cast<uint64_t>(g / 2) * a.chunks + 4 * quad, g < a.groups ? here * 4 : 0);
+    };
+    u32x4_t w[kAhead][8];
+    float ws[4];
+    auto load_codes = [&](const __amdgpu_buffer_rsrc_t& at, uint32_t c, u32x4_t (&to)[8]) {
+        const int chunk = static_cast<int>(min(c, here - 1) * (kUnit * 16));
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            to[j] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(at, lane * 16 + 1024 * j, chunk, kStreamed));
+    };
+    auto load_scales = [&](const __amdgpu_buffer_rsrc_t& at, float (&to)[4]) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) to[c] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(at, 0, 4 * c, 0));
+    };
+    auto codes = codes_of_group(blockIdx.x);
+    load_scales(scales_of_group(blockIdx.x), ws);
+#pragma unroll
+    for (uint32_t c = 0; c < kAhead; ++c) {
+        load_codes(codes, c, w[c]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    uint32_t buf = 0;
+    for (uint32_t g = blockIdx.x; g < a.groups; g += gridDim.x) {
+        const auto next = codes_of_group(g + gridDim.x);
+        float f[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f[c] = xs[c] * ws[c];
+        f32x4_t acc[4] = {};
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (uint32_t c = 0; c < 4; ++c) {
+            f32x4_t sum[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                sum[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w[c % kAhead][2 * j], w[c % kAhead][2 * j + 1]), x[c], f32x4_t{}, 0, 0, 0, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (c == 0) load_scales(scales_of_group(g + gridDim.x), ws);
+            if (c + kAhead < 4) load_codes(codes, c + kAhead, w[c % kAhead]);
+            else load_codes(next, c + kAhead - 4, w[c % kAhead]);
+            __builtin_amdgcn_sched_barrier(0);
+            if (c < here) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[j][i] = fmaf(sum[j][i], f[c], acc[j][i]);
+            }
+        }
+        codes = next;
+        // a lane's sums are of hidden row r and the group's rows 16 j + 4 kg + i
+        float* mine = part + (buf * quads + quad) * a.rows * 64;
+        if (r < a.rows) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4_t*>(mine + r * 64 + 16 * j + 4 * kg) = acc[j];
+        }
+        lds_barrier();
+        for (uint32_t e = quad * 64 + lane; e < a.rows * 64; e += quads * 64) {
+            const float* p = part + buf * quads * a.rows * 64 + e;
+            float y[1] = {p[0]};
+            for (uint32_t q = 1; q < quads; ++q) y[0] += p[q * a.rows * 64];
+            cap_logits(y, a.softcap);
+            const uint64_t v = static_cast<uint64_t>(g) * kGroupRows + e % 64;
+            if (v < a.vocab) store_logit(static_cast<Out*>(a.out) + (e / 64) * a.out_stride + v, y[0]);
+        }
+        buf ^= 1;
+    }
+}
+
+// ---- more hidden rows: tiles of 256 vocabulary rows by 32 NS hidden rows -----------------------------
+//
+// Four waves, a group of weights each, read straight from memory a chunk ahead; the hidden rows' chunk goes through LDS,
+// loaded there without registers one chunk ahead into the other of two buffers.
+constexpr uint32_t kTileWaves = 4;
+
+template <int NS, typename Out>
+__global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void fp8_tile_kernel(Fp8Args a) {
+    constexpr uint32_t kRows = 32 * NS;
+    constexpr uint32_t kStage = kRows * 8;  // 16-byte pieces
+    constexpr uint32_t kSpace = kStage > 1024 ? kStage : 1024;  // two waves' logits change places in a buffer
+    __shared__ u32x4_t buf0[kSpace], buf1[kSpace];
+    const uint32_t lane = threadIdx.x % 64, h = lane / 32, r = lane % 32;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t row_tiles = (a.rows + kRows - 1) / kRows, stretches = (a.groups + kTileWaves - 1) / kTileWaves;
+    const uint32_t xcd = blockIdx.x % 8, turn = blockIdx.x / 8;
+    const uint32_t stretch_up = turn / row_tiles * 8 + xcd;
+    if (stretch_up >= stretches) return;
+    const uint32_t stretch = stretches - 1 - stretch_up;
+    const uint32_t m0 = turn % row_tiles * kRows;
+    const uint32_t group = stretch * kTileWaves + wave;
+    const bool have_group = group < a.groups;
+    const uint64_t g = min(group, a.groups - 1);
+    const uint32_t rows_here = min(a.rows - m0, kRows);
+
+    // eight rows of 128 bytes to a load; a row's pieces change places with its number, so that sixteen rows' reads of one
+    // piece meet different banks
+    const auto rsrc = make_rsrc(a.x + static_cast<uint64_t>(m0) * a.d, rows_here * a.d);
+    auto fetch = [&](uint32_t c, u32x4_t* to) {
+        const uint32_t at = c * kBlock;
+#pragma unroll
+        for (uint32_t i = 0; i < NS; ++i) {
+            const uint32_t p = i * kTileWaves + wave, row = 8 * p + lane / 8, piece = (lane % 8) ^ (row / 2 % 8);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + p * 64), 16, static_cast<int>(row * a.d + 16 * piece + at), 0, 0, 0);
+        }
+    };
+    const auto codes = make_rsrc(a.codes + g * a.chunks * kUnit, a.chunks * (kUnit * 16));
+    const auto scales = make_rsrc(a.scales + g / 2 * a.chunks, a.chunks * 4);
+    // square j, step s, half: rows 32 j + r, columns 32 (2 s + h) + 16 half of the chunk
+    const uint32_t w_off = 16 * ((r / 16) * 128 + h * 16 + r % 16);
+    u32x4_t w[8], wn[8];
+    float ws, wsn, xs[NS], xsn[NS];
+    auto load_codes = [&](uint32_t c) {
+        const int at = __builtin_amdgcn_readfirstlane(static_cast<int>(min(c, a.chunks - 1) * (kUnit * 16)));
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+                    wn[4 * j + 2 * s + half] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(codes, w_off + 4096 * j + 512 * s + 1024 * half, at, 0));
+    };
+    const float* xs_at[NS];
+#pragma unroll
+    for (int n = 0; n < NS; ++n) xs_at[n] = a.xs + static_cast<uint64_t>(min(m0 + 32 * n + r, a.rows - 1)) * a.chunks;
+    auto load_scales = [&](uint32_t c) {
+        const uint32_t at = min(c, a.chunks - 1);
+        wsn = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(scales, 0, static_cast<int>(4 * at), 0));
+#pragma unroll
+        for (int n = 0; n < NS; ++n) xsn[n] = xs_at[n][at];
+    };
+    f32x16_t acc[2][NS];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int n = 0; n < NS; ++n) acc[j][n] = f32x16_t{};
+    auto turn_over = [&] {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = wn[i];
+        ws = wsn;
+#pragma unroll
+        for (int n = 0; n < NS; ++n) xs[n] = xsn[n];
+    };
+    auto chunk = [&](uint32_t c, const u32x4_t* x, u32x4_t* to) {
+        __syncthreads();  // chunk c has arrived, and nobody reads the other buffer
+        load_codes(c + 1);
+        load_scales(c + 1);
+        if (c + 1 < a.chunks) fetch(c + 1, to);
+        __builtin_amdgcn_sched_barrier(0);
+        if (have_group) {
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+                i32x8_t y[2];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) {
+                    const uint32_t row = 32 * n + r, p = 2 * (2 * s + h);
+                    y[s] = operand(x[row * 8 + (p ^ (r / 2 % 8))], x[row * 8 + ((p + 1) ^ (r / 2 % 8))]);
+                }
+                const float f = xs[n] * ws;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    f32x16_t sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w[4 * j], w[4 * j + 1]), y[0], f32x16_t{}, 0, 0, 0, 0, 0, 0);
+                    sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w[4 * j + 2], w[4 * j + 3]), y[1], sum, 0, 0, 0, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) acc[j][n][i] = fmaf(sum[i], f, acc[j][n][i]);
+                }
+            }
+        }
+        turn_over();
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(kVmcnt0);  // the next chunk's loads into LDS are done before the barrier that hands it over
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    load_codes(0);
+    load_scales(0);
+    fetch(0, buf0);
+    turn_over();
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    for (uint32_t c = 0; c < a.chunks; c += 2) {
+        chunk(c, buf0, buf1);
+        if (c + 1 >= a.chunks) break;
+        chunk(c + 1, buf1, buf0);
+    }
+    __syncthreads();  // nobody reads the hidden rows any more
+    if (!have_group) return;
+    constexpr uint32_t kOf = 16 / sizeof(Out);
+    each<NS>([&](auto n) {
+        store_rows<2, Out>((wave < 2 ? buf0 : buf1) + wave % 2 * 512,
+            [&](auto j) {
+                float y[16];
+                f32x16_t z;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] = acc[j][n][i];
+                cap_logits(y, a.softcap);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] = y[i];
+                return z;
+            },
+            [&](uint32_t row, uint32_t col, u32x4_t v) {
+                const uint32_t m = m0 + 32 * n + row;
+                const uint64_t at = g * kGroupRows + col;
+                if (m < a.rows && at < a.vocab)
+                    store_logits(static_cast<Out*>(a.out) + m * a.out_stride + at, v, static_cast<uint32_t>(min<uint64_t>(a.vocab - at, kOf)));
+            });
+    });
+}
+
+bool fp8_aligned(const void* p, uint64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+}  // namespace
+
+}  // namespace twd
+
+struct twd_fp8head {
+    uint32_t vocab, d, chunks, groups;
+    float softcap;
+    int device, cus;
+    twd::u32x4_t* codes;
+    float* scales;
+    uint64_t bytes;
+};
+
+namespace twd {
+
+namespace {
+
+template <int NS, typename Out>
+int launch_tile(const Fp8Args& a, hipStream_t s) {
+    const uint32_t row_tiles = (a.rows + 32 * NS - 1) / (32 * NS), stretches = (a.groups + kTileWaves - 1) / kTileWaves;
+    const uint64_t blocks = static_cast<uint64_t>((stretches + 7) / 8) * 8 * row_tiles;
+    if (blocks > 0xFFFFFFull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
+    fp8_tile_kernel<NS, Out><<<static_cast<uint32_t>(blocks), kTileWaves * 64, 0, s>>>(a);
+    TWD_HIP(hipGetLastError());
+    return TWD_OK;
+}
+
+template <typename Out>
+int launch_logits(const twd_fp8head* h, const Fp8Args& a, hipStream_t s) {
+    const uint32_t quads = (a.chunks + 3) / 4;
+    if (a.rows <= kSmallRows && quads <= kSmallWaves) {
+        const uint32_t blocks = min(a.groups, kSmallWaves / quads * static_cast<uint32_t>(h->cus));
+        fp8_small_kernel<Out><<<blocks, quads * 64, 2 * quads * a.rows * 64 * sizeof(float), s>>>(a);
+        TWD_HIP(hipGetLastError());
+        return TWD_OK;
+    }
+    if (a.rows <= 32) return launch_tile<1, Out>(a, s);
+    if (a.rows <= 64) return launch_tile<2, Out>(a, s);
+    return launch_tile<4, Out>(a, s);
+}
+
+}  // namespace
+
+}  // namespace twd
+
+using namespace twd;
+
+extern "C" {
+
+TWD_API int twd_fp8_quantize(const void* x, int type, uint64_t rows, uint32_t cols, uint64_t row_stride, uint32_t block_rows,
+                             uint8_t* codes, float* scales, void* stream) {
+    clear_error();
+    if (!x || !codes || !scales) return fail(TWD_E_INVALID, "null argument");
+    if (type != TWD_F32 && type != TWD_BF16 && type != TWD_F16) return fail(TWD_E_INVALID, "type must be TWD_F32, TWD_BF16 or TWD_F16");
+    if (rows == 0) return fail(TWD_E_INVALID, "twd_fp8_quantize: no rows");
+    if (cols == 0 || cols % kBlock != 0 || cols > (1u << 20))
+        return fail(TWD_E_INVALID, "twd_fp8_quantize: columns must be a positive multiple of 128, at most 2^20");
+    if (rows > 1 && row_stride < cols) return fail(TWD_E_INVALID, "twd_fp8_quantize: the row stride is below cols");
+    if (block_rows != 1 && block_rows != kBlock) return fail(TWD_E_INVALID, "block_rows must be 1 or 128");
+    if (block_rows == kBlock && rows > (1ull << 30)) return fail(TWD_E_INVALID, "twd_fp8_quantize: too many rows");
+    const uint64_t size = type == TWD_F32 ? 4 : 2;
+    if (!fp8_aligned(x, size) || !fp8_aligned(scales, 4)) return fail(TWD_E_INVALID, "twd_fp8_quantize: x or scales are not aligned to their type");
+    if (!fp8_aligned(codes, 16)) return fail(TWD_E_INVALID, "twd_fp8_quantize: codes must start at a multiple of 16 bytes");
+    const QuantArgs a{x, row_stride, rows, cols / kBlock, codes, scales, fp8_aligned(x, 16) && (rows == 1 || row_stride * size % 16 == 0)};
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    auto go = [&](auto t) {
+        using T = decltype(t);
+        if (block_rows == 1)
+            fp8_rows_kernel<T><<<dim3((a.blocks * 16 + 255) / 256, static_cast<uint32_t>(rows < 65535 ? rows : 65535)), 256, 0, s>>>(a);
+        else
+            fp8_weights_kernel<T><<<dim3(static_cast<uint32_t>((rows + kBlock - 1) / kBlock), a.blocks), 256, 0, s>>>(a);
+    };
+    if (type == TWD_F32) go(float{});
+    else if (type == TWD_BF16) go(Bf16{});
+    else go(Fp16{});
+    TWD_HIP(hipGetLastError());
+    return TWD_OK;
+}
+
+TWD_API int twd_fp8head_create(const uint8_t* codes, const float* scales, uint32_t vocab, uint32_t d_model, float softcap,
+                               void* stream, twd_fp8head** out) {
+    clear_error();
+    if (!out) return fail(TWD_E_INVALID, "null argument");
+    *out = nullptr;
+    if (!codes || !scales) return fail(TWD_E_INVALID, "null argument");
+    if (vocab == 0 || vocab > (1u << 30)) return fail(TWD_E_INVALID, "vocab must be in 1..2^30");
+    if (d_model == 0 || d_model % kBlock != 0 || d_model > (1u << 20))
+        return fail(TWD_E_INVALID, "d_model must be a positive multiple of 128, at most 2^20");
+    if (softcap != 0.0f && !(softcap >= kMinSoftCap && softcap <= kMaxSoftCap))
+        return fail(TWD_E_INVALID, "softcap must be 0 (none) or in 1e-30..1e30");
+    if (!fp8_aligned(codes, 16) || !fp8_aligned(scales, 4)) return fail(TWD_E_INVALID, "codes must start at a multiple of 16 bytes, scales of 4");
+    const uint32_t chunks = d_model / kBlock, groups = (vocab + kGroupRows - 1) / kGroupRows;
+    const uint64_t n_scales = static_cast<uint64_t>((vocab + kBlock - 1) / kBlock) * chunks;
+    const uint64_t code_bytes = static_cast<uint64_t>(groups) * chunks * kUnit * 16, scale_bytes = (n_scales * 4 + 15) / 16 * 16;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    int dev = 0, cus = 0;
+    TWD_HIP(hipGetDevice(&dev));
+    TWD_HIP(hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev));
+    constexpr int kMost = 2 * kSmallWaves * kSmallRows * 64 * sizeof(float);
+    TWD_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fp8_small_kernel<float>), hipFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    TWD_HIP(hipFuncSetAttribute(reinterpret_cast<const void*>(fp8_small_kernel<uint16_t>), hipFuncAttributeMaxDynamicSharedMemorySize, kMost));
+    void* mem = nullptr;
+    TWD_HIP(hipMalloc(&mem, code_bytes + scale_bytes + 16));
+    u32x4_t* kept_codes = static_cast<u32x4_t*>(mem);
+    float* kept_scales = reinterpret_cast<float*>(static_cast<uint8_t*>(mem) + code_bytes);
+    uint32_t* bad_dev = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(mem) + code_bytes + scale_bytes);
+    uint32_t bad = 0;
+    hipError_t e = hipMemsetAsync(bad_dev, 0, sizeof(bad), s);
+    if (e == hipSuccess) {
+        fp8_check_kernel<<<256, 256, 0, s>>>(scales, kept_scales, n_scales, bad_dev);
+        fp8_repack_kernel<<<groups, 256, 0, s>>>(codes, vocab, d_model, kept_codes);
+        e = hipGetLastError();
+    }
+    if (e == hipSuccess) e = hipMemcpyAsync(&bad, bad_dev, sizeof(bad), hipMemcpyDeviceToHost, s);
+    if (e == hipSuccess) e = hipStreamSynchronize(s);
+    twd_fp8head* h = nullptr;
+    if (e == hipSuccess && !bad)
+        h = new (std::nothrow) twd_fp8head{vocab, d_model, chunks, groups, softcap, dev, cus, kept_codes, kept_scales, code_bytes + scale_bytes};
+    if (!h) {
+        (void)hipFree(mem);
+        if (e != hipSuccess) return hip_fail(e, "repacking the head");
+        if (bad) return fail(TWD_E_UNSUPPORTED, "a block scale is negative, above 2^100 or NaN");
+        return fail(TWD_E_INVALID, "out of host memory");
+    }
+    *out = h;
+    return TWD_OK;
+}
+
+TWD_API void twd_fp8head_destroy(twd_fp8head* head) {
+    if (!head) return;
+    (void)hipFree(head->codes);
+    delete head;
+}
+
+TWD_API int twd_fp8head_info(const twd_fp8head* head, uint32_t* vocab, uint32_t* d_model, float* softcap,
+                             uint64_t* device_bytes) {
+    clear_error();
+    if (!head) return fail(TWD_E_INVALID, "null head");
+    if (vocab) *vocab = head->vocab;
+    if (d_model) *d_model = head->d;
+    if (softcap) *softcap = head->softcap;
+    if (device_bytes) *device_bytes = head->bytes;
+    return TWD_OK;
+}
+
+TWD_API int twd_fp8head_logits(const twd_fp8head* head, const uint8_t* codes, const float* scales, uint32_t rows,
+                               void* logits, int logits_type, uint64_t logits_stride, void* stream) {
+    clear_error();
+    if (!head) return fail(TWD_E_INVALID, "null head");
+    if (!codes || !scales || !logits) return fail(TWD_E_INVALID, "null argument");
+    if (rows == 0 || rows > 65536u) return fail(TWD_E_INVALID, "rows must be in 1..65536");
+    if (logits_type != TWD_F32 && logits_type != TWD_BF16) return fail(TWD_E_INVALID, "logits must be fp32 or bf16");
+    if (logits_stride < head->vocab) return fail(TWD_E_INVALID, "the logits' row stride is below vocab");
+    if (!fp8_aligned(codes, 16)) return fail(TWD_E_INVALID, "hidden codes must start at a multiple of 16 bytes");
+    if (!fp8_aligned(scales, 4) || !fp8_aligned(logits, logits_type == TWD_F32 ? 4 : 2))
+        return fail(TWD_E_INVALID, "scales or logits are not aligned to their type");
+    int dev = 0;
+    TWD_HIP(hipGetDevice(&dev));
+    if (dev != head->device) return fail(TWD_E_INVALID, "the head lives on another device than the current one");
+    const Fp8Args a{head->codes, head->scales, codes, scales, logits, logits_stride, head->vocab, head->d, head->chunks,
+                    head->groups, rows, soft_cap(head->softcap)};
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    return logits_type == TWD_F32 ? launch_logits<float>(head, a, s) : launch_logits<uint16_t>(head, a, s);
+}
+
+}  // extern "C"

@@ -214,9 +214,6 @@ struct MxArgs {
     SoftCap softcap;
 };
 
-__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
-__device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = static_cast<uint16_t>(bf16_bits(v)); }
-
 __device__ __forceinline__ i32x8_t mx_operand(u32x4_t v) {  // 4-bit operands fill half the registers
     const i32x4_t x = __builtin_bit_cast(i32x4_t, v);
     return __builtin_shufflevector(x, x, 0, 1, 2, 3, -1, -1, -1, -1);
@@ -378,25 +375,6 @@ __global__ __launch_bounds__(kSmallWaves * 64) void mx_small_kernel(MxArgs a) {
 // served by an L2 and 156 without the logits' stores. Codes two chunks ahead, stages of two chunks and two blocks to a
 // compute unit instead of three did not bring reads and products together (within 3%).
 constexpr uint32_t kTileWaves = 4;
-
-template <typename Out>
-struct Sixteen {
-    Out e[16 / sizeof(Out)];
-};
-
-// 16 bytes of logits at any alignment, n of them at most; they are not read here again.
-template <typename Out>
-__device__ __forceinline__ void store_logits(Out* p, u32x4_t v, uint32_t n) {
-    constexpr uint32_t kEach = 16 / sizeof(Out);
-    typedef u32x4_t __attribute__((aligned(2))) any_place_t;
-    if (n >= kEach) {
-        __builtin_nontemporal_store(v, reinterpret_cast<any_place_t*>(p));
-    } else {
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i)
-            if (i < n) p[i] = __builtin_bit_cast(Sixteen<Out>, v).e[i];
-    }
-}
 
 template <bool MX, int NT, typename Out>
 __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void mx_tile_kernel(MxArgs a) {

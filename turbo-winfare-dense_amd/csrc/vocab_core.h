@@ -142,6 +142,28 @@ __device__ __forceinline__ void cap_logits(float (&y)[N], const SoftCap& c) {
     }
 }
 
+__device__ __forceinline__ void store_logit(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store_logit(uint16_t* p, float v) { *p = static_cast<uint16_t>(bf16_bits(v)); }
+
+template <typename Out>
+struct Sixteen {
+    Out e[16 / sizeof(Out)];
+};
+
+// 16 bytes of logits at any alignment, n of them at most; they are not read here again.
+template <typename Out>
+__device__ __forceinline__ void store_logits(Out* p, u32x4_t v, uint32_t n) {
+    constexpr uint32_t kEach = 16 / sizeof(Out);
+    typedef u32x4_t __attribute__((aligned(2))) any_place_t;
+    if (n >= kEach) {
+        __builtin_nontemporal_store(v, reinterpret_cast<any_place_t*>(p));
+    } else {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i)
+            if (i < n) p[i] = __builtin_bit_cast(Sixteen<Out>, v).e[i];
+    }
+}
+
 // A barrier that waits for the wave's LDS accesses only: loads on their way into registers stay in flight.
 __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");

@@ -176,6 +176,11 @@ _SIGS = {
     "twd_embedgrad_info": (C.c_int, [_vp, C.POINTER(_u64)]),
     "twd_embedgrad_run": (C.c_int, [_vp, _vp, C.c_int, _u32, _u32, _u64, _vp, _f32, _vp, C.c_int, _u32, _u64, C.c_int,
                                     _vp]),
+    "twd_fp8_quantize": (C.c_int, [_vp, C.c_int, _u64, _u32, _u64, _u32, _vp, _vp, _vp]),
+    "twd_fp8head_create": (C.c_int, [_vp, _vp, _u32, _u32, _f32, _vp, C.POINTER(_vp)]),
+    "twd_fp8head_destroy": (None, [_vp]),
+    "twd_fp8head_info": (C.c_int, [_vp, C.POINTER(_u32), C.POINTER(_u32), C.POINTER(_f32), C.POINTER(_u64)]),
+    "twd_fp8head_logits": (C.c_int, [_vp, _vp, _vp, _u32, _vp, C.c_int, _u64, _vp]),
     "twd_probe_read_bandwidth": (C.c_int, [_vp, _u64, _u32, _u32, _vp, C.POINTER(_f32),
                                            C.POINTER(_u64)]),
 }
@@ -993,6 +998,94 @@ class Sampler:
                                           _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(uniform), _ptr(tokens),
                                           _ptr(logprobs), _ptr(kept), _stream_on(logits, stream)))
         return tokens
+
+
+# ---- 8-bit floating point with a scale for each block of 128 ------------------------------------------
+
+def fp8_quantize(x, block_rows: int = 1, codes=None, scales=None, stream=None):
+    """Rows of a float32, bfloat16 or float16 device tensor [rows, cols], cols a multiple of 128, in 8-bit floating point
+    (twd_fp8_quantize): (codes uint8 [rows, cols] of e4m3, scales float32). A scale is for 128 columns of a row [rows, cols /
+    128], or with block_rows=128, as weights are held, for 128 x 128 [rows / 128 rounded up, cols / 128]."""
+    import torch
+    kind = _type_of(x, "x")
+    rows, cols, stride = _matrix(x, "x")
+    if block_rows not in (1, 128):
+        raise ValueError("block_rows must be 1 or 128")
+    shape = ((rows + block_rows - 1) // block_rows, cols // 128)
+    with _on_device(x, codes, scales):
+        if codes is None:
+            codes = _made(torch.empty, (rows, cols), torch.uint8, x.device, stream)
+        else:
+            _buffer(codes, (rows, cols), torch.uint8, "codes")
+        if scales is None:
+            scales = _made(torch.empty, shape, torch.float32, x.device, stream)
+        else:
+            _buffer(scales, shape, torch.float32, "scales")
+        _check(lib.twd_fp8_quantize(x.data_ptr(), kind, rows, cols, stride, block_rows, codes.data_ptr(),
+                                    scales.data_ptr(), _stream_on(x, stream)))
+    return codes, scales
+
+
+class Fp8Head:
+    """An LM head in 8-bit floating point with a scale for each 128 x 128, resident in HBM (twd_fp8head)."""
+
+    def __init__(self, codes, scales, softcap: float = 0.0, stream=None):
+        """codes uint8 (or float8_e4m3fn) [vocab, d_model] and scales float32 [vocab / 128 rounded up, d_model / 128] on
+        the device; they may be freed afterwards."""
+        import torch
+        self.handle = None
+        vocab, d, _ = _matrix(codes, "codes")
+        if codes.dtype == torch.float8_e4m3fn:
+            codes = codes.view(torch.uint8)
+        _buffer(codes, (vocab, d), torch.uint8, "codes")
+        _buffer(scales, ((vocab + 127) // 128, d // 128), torch.float32, "scales")
+        h = C.c_void_p()
+        with _on_device(codes, scales):
+            _check(lib.twd_fp8head_create(_ptr(codes), _ptr(scales), vocab, d, softcap, _stream_on(codes, stream),
+                                          C.byref(h)))
+        self.handle = h
+        self.device = codes.device
+        self.vocab, self.d_model, self.softcap = vocab, d, softcap
+        n = _u64()
+        _check(lib.twd_fp8head_info(h, None, None, None, C.byref(n)))
+        self.nbytes = n.value
+
+    @classmethod
+    def from_weights(cls, w, softcap: float = 0.0, stream=None) -> "Fp8Head":
+        """Quantises float32, bfloat16 or float16 weights [vocab, d_model] (fp8_quantize)."""
+        codes, scales = fp8_quantize(w, 128, stream=stream)
+        return cls(codes, scales, softcap, stream)
+
+    def close(self):
+        if self.handle:
+            lib.twd_fp8head_destroy(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    def logits_fp8(self, codes, scales, out=None, stream=None):
+        """Logits of hidden rows that fp8_quantize brought into the format too, in out's float32 or bfloat16 (float32 where
+        none is given)."""
+        import torch
+        rows = codes.shape[0]
+        _buffer(codes, (rows, self.d_model), torch.uint8, "codes")
+        _buffer(scales, (rows, self.d_model // 128), torch.float32, "scales")
+        with _on_device(codes, scales, out):
+            if out is None:
+                out = _made(torch.empty, (rows, self.vocab), torch.float32, self.device, stream)
+            if out.shape != (rows, self.vocab):
+                raise ValueError(f"out must be of shape {(rows, self.vocab)}")
+            _check(lib.twd_fp8head_logits(self.handle, codes.data_ptr(), scales.data_ptr(), rows, out.data_ptr(),
+                                          _type_of(out, "out"), _matrix(out, "out")[2], _stream_on(codes, stream)))
+        return out
+
+    def logits(self, hidden, out=None, stream=None):
+        """Logits of float32, bfloat16 or float16 hidden rows [rows, d_model], quantised on the way."""
+        return self.logits_fp8(*fp8_quantize(hidden, stream=stream), out=out, stream=stream)
 
 
 # ---- the vocabulary matrix in training ----------------------------------------------------------------
