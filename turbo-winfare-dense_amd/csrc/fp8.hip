@@ -401,6 +401,143 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
     });
 }
 
+// ---- many hidden rows: tiles of 256 x 256 -------------------------------------------------------------
+//
+// Eight waves, 64 vocabulary rows by 128 hidden rows each, two to a SIMD: one's scaling covers the other's matrix
+// instructions. Weights and hidden rows both go through LDS, a chunk of each loaded there without registers one ahead into
+// the other of two buffers; the weights' lines are brought to the L2 three chunks ahead.
+constexpr uint32_t kWideThreads = 512;
+constexpr uint32_t kWideStage = 4 * kUnit + 256 * 8;  // 16-byte pieces: four groups' chunk, 256 hidden rows'
+
+template <typename Out>
+__global__ __launch_bounds__(kWideThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_wide_kernel(Fp8Args a) {
+    __shared__ u32x4_t buf0[kWideStage], buf1[kWideStage];
+    __shared__ float sc0[512], sc1[512];  // hidden row m's scale at 64 (m / 32) + m % 32
+    __shared__ uint32_t sink[kWideThreads];
+    const TileGrid grid{(a.groups + 3) / 4, (a.rows + 255) / 256, 1};
+    const uint32_t id = stretched(grid.tiles());
+    if (id >= grid.tiles()) return;
+    const TileAt at = tile_at(grid, id);
+    const uint32_t lane = threadIdx.x % 64, h = lane / 32, r = lane % 32;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), va = wave % 4, mb = wave / 4;
+    const uint32_t m0 = 256 * at.b, rows_here = min(a.rows - m0, 256u), g0 = 4 * at.a, groups_here = min(a.groups - g0, 4u);
+    const uint32_t group_bytes = a.chunks * (kUnit * 16);
+    // past the last group or row there is nothing: zeros
+    const auto codes = make_rsrc(a.codes + static_cast<uint64_t>(g0) * a.chunks * kUnit, groups_here * group_bytes);
+    const auto hidden = make_rsrc(a.x + static_cast<uint64_t>(m0) * a.d, rows_here * a.d);
+    const auto scales = make_rsrc(a.xs + static_cast<uint64_t>(m0) * a.chunks, rows_here * a.chunks * 4);
+    const auto weight_scales = make_rsrc(a.scales + static_cast<uint64_t>((g0 + va) / 2) * a.chunks, va < groups_here ? a.chunks * 4 : 0);
+    constexpr uint32_t kLoads = 10;
+    uint32_t w_off = 4 * wave / 8 * group_bytes + 4 * wave % 8 * 1024 + lane * 16, x_off[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        const uint32_t row = 8 * (4 * wave + i) + lane / 8;
+        x_off[i] = row * a.d + 16 * ((lane % 8) ^ (row / 2 % 8));
+    }
+    const uint32_t s_off = lane < 32 ? (32 * wave + lane) * a.chunks * 4 : 0x80000000u;
+    const uint32_t t_off = threadIdx.x < 256 && threadIdx.x % at.share == at.who ? threadIdx.x / 64 * group_bytes + threadIdx.x % 64 * 128 : 0x80000000u;
+    // load i of a chunk; past the last chunk none
+    auto fetch = [&](uint32_t i, uint32_t c, u32x4_t* to, float* sc) {
+        if (i < 4) {
+            const uint32_t o = c < a.chunks ? w_off + 1024 * i + c * (kUnit * 16) : 0x80000000u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(codes, (lds_void*)(to + (4 * wave + i) * 64), 16, static_cast<int>(o), 0, 0, 0);
+        } else if (i < 8) {
+            const uint32_t o = c < a.chunks ? x_off[i - 4] + c * kBlock : 0x80000000u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(hidden, (lds_void*)(to + 4 * kUnit + (4 * wave + i - 4) * 64), 16, static_cast<int>(o), 0, 0, 0);
+        } else if (i == 8) {
+            const uint32_t o = c < a.chunks ? s_off + 4 * c : 0x80000000u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(scales, (lds_void*)(sc + 64 * wave), 4, static_cast<int>(o), 0, 0, 0);
+        } else {
+            const uint32_t o = c + 2 < a.chunks ? t_off + (c + 2) * (kUnit * 16) : 0x80000000u;
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(codes, (lds_void*)(sink + 64 * wave), 4, static_cast<int>(o), 0, 0, 0);
+        }
+    };
+    f32x16_t acc[2][4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) acc[j][n] = f32x16_t{};
+    const uint32_t w_at = va * kUnit + r / 16 * 128 + h * 16 + r % 16, x_at = 4 * kUnit + (128 * mb + r) * 8;
+    auto weight_scale = [&](uint32_t c) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(weight_scales, c < a.chunks ? static_cast<int>(4 * c) : -4, 0, 0));
+    };
+    float ws_next = weight_scale(0);
+    auto chunk = [&](uint32_t c, const u32x4_t* from, const float* sc, u32x4_t* to, float* to_sc) {
+        const float ws = ws_next;
+        ws_next = weight_scale(c + 1);
+        float f[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) f[n] = sc[64 * (4 * mb + n) + r];
+        i32x8_t w[2][2], y[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) w[j][s] = operand(from[w_at + 256 * j + 32 * s], from[w_at + 256 * j + 32 * s + 64]);
+        auto read = [&](int n) {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                const uint32_t p = 2 * (2 * s + h);
+                y[s] = operand(from[x_at + 256 * n + (p ^ (r / 2 % 8))], from[x_at + 256 * n + ((p + 1) ^ (r / 2 % 8))]);
+            }
+        };
+        read(0);
+        f32x16_t sum[2];
+#pragma unroll
+        for (int q = 0; q <= 8; ++q) {  // square q's products, and the scaling of the one before
+            const int n = q / 2, j = q % 2;
+            if (q < 8) {
+#pragma unroll
+                for (uint32_t i = kLoads * q / 8; i < kLoads * (q + 1) / 8; ++i) fetch(i, c + 1, to, to_sc);
+                sum[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[j][0], y[0], f32x16_t{}, 0, 0, 0, 0, 0, 0);
+                sum[j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(w[j][1], y[1], sum[j], 0, 0, 0, 0, 0, 0);
+                if (j == 1 && n < 3) read(n + 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (q > 0) {
+                const int m = (q - 1) / 2, k = (q - 1) % 2;
+                if (k == 0) f[m] *= ws;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) acc[k][m][i] = fmaf(sum[k][i], f[m], acc[k][m][i]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0070 | 1);  // all but the last load, of the lines ahead
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#pragma unroll
+    for (uint32_t i = 0; i < kLoads; ++i) fetch(i, 0, buf0, sc0);
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    __syncthreads();
+    for (uint32_t c = 0; c < a.chunks; c += 2) {
+        chunk(c, buf0, sc0, buf1, sc1);
+        chunk(c + 1, buf1, sc1, buf0, sc0);  // past the last chunk: zeros
+    }
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    __syncthreads();
+    if (va >= groups_here) return;
+    constexpr uint32_t kOf = 16 / sizeof(Out);
+    each<4>([&](auto n) {
+        store_rows<2, Out>((wave < 4 ? buf0 : buf1) + wave % 4 * 512,
+            [&](auto j) {
+                float y[16];
+                f32x16_t z;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) y[i] = acc[j][n][i];
+                cap_logits(y, a.softcap);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) z[i] = y[i];
+                return z;
+            },
+            [&](uint32_t row, uint32_t col, u32x4_t v) {
+                const uint32_t m = m0 + 128 * mb + 32 * n + row;
+                const uint64_t at_v = static_cast<uint64_t>(g0 + va) * kGroupRows + col;
+                if (m < a.rows && at_v < a.vocab)
+                    store_logits(static_cast<Out*>(a.out) + m * a.out_stride + at_v, v, static_cast<uint32_t>(min<uint64_t>(a.vocab - at_v, kOf)));
+            });
+    });
+}
+
 bool fp8_aligned(const void* p, uint64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 }  // namespace
@@ -441,7 +578,12 @@ int launch_logits(const twd_fp8head* h, const Fp8Args& a, hipStream_t s) {
     }
     if (a.rows <= 32) return launch_tile<1, Out>(a, s);
     if (a.rows <= 64) return launch_tile<2, Out>(a, s);
-    return launch_tile<4, Out>(a, s);
+    if (a.rows <= 128) return launch_tile<4, Out>(a, s);
+    const uint64_t tiles = static_cast<uint64_t>((a.groups + 3) / 4) * ((a.rows + 255) / 256);
+    if (tiles > 0x7FFFFFull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
+    fp8_wide_kernel<Out><<<blocks_for(static_cast<uint32_t>(tiles)), kWideThreads, 0, s>>>(a);
+    TWD_HIP(hipGetLastError());
+    return TWD_OK;
 }
 
 }  // namespace
