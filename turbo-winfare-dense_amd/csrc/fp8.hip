@@ -163,6 +163,28 @@ __device__ __forceinline__ i32x8_t operand(u32x4_t lo, u32x4_t hi) {
     return __builtin_bit_cast(i32x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
+// The 8-bit matrix instructions align a step's products to the largest of them before they add, which costs some of the
+// bits: sums of 128 normal products are off by 1.4e-5 of their spread (in bf16, exact products added in fp32: 1e-8). That is
+// far inside a bf16 logit's half step, 2^-8 of itself, and is taken there; for fp32 logits both operands are widened to bf16,
+// which holds every e4m3 value, and multiplied at half the rate. Eight elements of two words:
+__device__ __forceinline__ bf16x8_t widened(uint32_t lo, uint32_t hi) {
+    u32x4_t e;
+    e[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
+    e[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, true));
+    e[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, false));
+    e[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.0f, true));
+    return __builtin_bit_cast(bf16x8_t, e);
+}
+struct Wide32 {  // a lane's 32 elements
+    bf16x8_t e[4];
+};
+__device__ __forceinline__ Wide32 widened(i32x8_t v) {
+    Wide32 w;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w.e[i] = widened(static_cast<uint32_t>(v[2 * i]), static_cast<uint32_t>(v[2 * i + 1]));
+    return w;
+}
+
 // ---- up to 16 hidden rows: the weights stream past rows held in registers ---------------------------
 //
 // Bound by the read of the head. The waves of a block split d_model by quads of chunks; a wave keeps its quad of the hidden
@@ -178,7 +200,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void fp8_small_kernel(Fp8Args a) 
     const uint32_t lane = threadIdx.x % 64, kg = lane / 16, r = lane % 16, quads = (a.chunks + 3) / 4;
     const uint32_t quad = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t here = min(4u, a.chunks - 4 * quad);
-    i32x8_t x[4];
+    u32x4_t x[4][2];
     float xs[4];
 #pragma unroll
     for (uint32_t c = 0; c < 4; ++c) {
@@ -189,7 +211,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void fp8_small_kernel(Fp8Args a) 
             lo = p[0], hi = p[1];
             xs[c] = a.xs[static_cast<uint64_t>(r) * a.chunks + 4 * quad + c];
         }
-        x[c] = operand(lo, hi);
+        x[c][0] = lo, x[c][1] = hi;
     }
     // a group past the last has no bytes, so nothing is read of it; past the quad's end the last chunk comes again, whose
     // products count for nothing
@@ -228,11 +250,19 @@ __global__ __launch_bounds__(kSmallWaves * 64) void fp8_small_kernel(Fp8Args a) 
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (uint32_t c = 0; c < 4; ++c) {
-            f32x4_t sum[4];
+            f32x4_t sum[4] = {};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                sum[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(operand(w[c % kAhead][2 * j], w[c % kAhead][2 * j + 1]), x[c], f32x4_t{}, 0, 0, 0, 0, 0, 0);
-            __builtin_amdgcn_sched_barrier(0);
+            for (int t = 0; t < 4; ++t) {
+                u32x2_t in = {x[c][t / 2][t % 2 * 2], x[c][t / 2][t % 2 * 2 + 1]};
+                asm volatile("; widened anew for every group: held widened, the rows would not fit" : "+v"(in));
+                const bf16x8_t y = widened(in[0], in[1]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const u32x4_t& v = w[c % kAhead][2 * j + t / 2];
+                    sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widened(v[t % 2 * 2], v[t % 2 * 2 + 1]), y, sum[j], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);  // a quarter's widened codes at a time
+            }
             if (c == 0) load_scales(scales_of_group(g + gridDim.x), ws);
             if (c + kAhead < 4) load_codes(codes, c + kAhead, w[c % kAhead]);
             else load_codes(next, c + kAhead - 4, w[c % kAhead]);
@@ -344,6 +374,13 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
         if (c + 1 < a.chunks) fetch(c + 1, to);
         __builtin_amdgcn_sched_barrier(0);
         if (have_group) {
+            Wide32 e[2][2];
+            if constexpr (sizeof(Out) == 4) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) e[j][s] = widened(operand(w[4 * j + 2 * s], w[4 * j + 2 * s + 1]));
+            }
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
                 i32x8_t y[2];
@@ -353,6 +390,22 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
                     y[s] = operand(x[row * 8 + (p ^ (r / 2 % 8))], x[row * 8 + ((p + 1) ^ (r / 2 % 8))]);
                 }
                 const float f = xs[n] * ws;
+                if constexpr (sizeof(Out) == 4) {
+                    f32x16_t sum[2] = {};
+#pragma unroll
+                    for (int s = 0; s < 2; ++s) {
+                        const Wide32 z = widened(y[s]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j)
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) sum[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e[j][s].e[t], z.e[t], sum[j], 0, 0, 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) acc[j][n][i] = fmaf(sum[j][i], f, acc[j][n][i]);
+                    continue;
+                }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     f32x16_t sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w[4 * j], w[4 * j + 1]), y[0], f32x16_t{}, 0, 0, 0, 0, 0, 0);
@@ -578,12 +631,16 @@ int launch_logits(const twd_fp8head* h, const Fp8Args& a, hipStream_t s) {
     }
     if (a.rows <= 32) return launch_tile<1, Out>(a, s);
     if (a.rows <= 64) return launch_tile<2, Out>(a, s);
-    if (a.rows <= 128) return launch_tile<4, Out>(a, s);
-    const uint64_t tiles = static_cast<uint64_t>((a.groups + 3) / 4) * ((a.rows + 255) / 256);
-    if (tiles > 0x7FFFFFull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
-    fp8_wide_kernel<Out><<<blocks_for(static_cast<uint32_t>(tiles)), kWideThreads, 0, s>>>(a);
-    TWD_HIP(hipGetLastError());
-    return TWD_OK;
+    if constexpr (sizeof(Out) == 4) {
+        return launch_tile<2, Out>(a, s);  // widened, 128 rows leave no registers
+    } else {
+        if (a.rows <= 128) return launch_tile<4, Out>(a, s);
+        const uint64_t tiles = static_cast<uint64_t>((a.groups + 3) / 4) * ((a.rows + 255) / 256);
+        if (tiles > 0x7FFFFFull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
+        fp8_wide_kernel<Out><<<blocks_for(static_cast<uint32_t>(tiles)), kWideThreads, 0, s>>>(a);
+        TWD_HIP(hipGetLastError());
+        return TWD_OK;
+    }
 }
 
 }  // namespace
