@@ -20,33 +20,39 @@ constexpr uint32_t kSpan = kEmbedThreads * kEach;         // elements of a block
 // of a step for lane t; otherwise a wave's accesses are, element t + 256 i.
 __device__ __forceinline__ uint32_t element(bool wide, uint32_t t, uint32_t i) { return wide ? kEach * t + i : t + kEmbedThreads * i; }
 
-template <typename T>
-__device__ __forceinline__ float widened(const T* p);
-template <>
-__device__ __forceinline__ float widened(const float* p) { return *p; }
-template <>
-__device__ __forceinline__ float widened(const Bf16* p) { return half_to_f32<Bf16>(p->u); }
-template <>
-__device__ __forceinline__ float widened(const Fp16* p) { return static_cast<float>(p->h); }
-
 __device__ __forceinline__ void put(float* p, float v) { *p = v; }
 __device__ __forceinline__ void put(Bf16* p, float v) { p->u = static_cast<uint16_t>(f32_to_half<Bf16>(v)); }
 __device__ __forceinline__ void put(Fp16* p, float v) { p->h = static_cast<_Float16>(v); }
 
-// The lane's eight of a row from element `base` on; zero past its d.
+// The lane's eight of a row from element `base` on, as they lie in memory; zero past its d.
 template <typename T>
-__device__ __forceinline__ void load_eight(const T* row, bool wide, uint32_t base, uint32_t d, float (&v)[kEach]) {
-    const uint32_t t = threadIdx.x, first = base + kEach * t;
-    if (wide && first + kEach <= d) {
-        Eight<T>::load(row + first, true, v);
-        return;
-    }
+struct Raw {
+    static constexpr uint32_t kWords = kEach * sizeof(T) / 16;
+    u32x4_t w[kWords];
+
+    __device__ __forceinline__ void load(const T* row, bool wide, uint32_t base, uint32_t d) {
+        const uint32_t t = threadIdx.x, first = base + kEach * t;
+        if (wide && first + kEach <= d) {
 #pragma unroll
-    for (uint32_t i = 0; i < kEach; ++i) {
-        const uint32_t e = base + element(wide, t, i);
-        v[i] = e < d ? widened(row + e) : 0.0f;
+            for (uint32_t i = 0; i < kWords; ++i) w[i] = reinterpret_cast<const u32x4_t*>(row + first)[i];
+            return;
+        }
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t e = base + element(wide, t, i);
+            if constexpr (sizeof(T) == 4) {
+                w[i / 4][i % 4] = e < d ? __float_as_uint(row[e]) : 0u;
+            } else {
+                const uint32_t bits = e < d ? reinterpret_cast<const uint16_t*>(row)[e] : 0u;
+                w[0][i / 2] = i % 2 == 0 ? bits : w[0][i / 2] | bits << 16;
+            }
+        }
     }
-}
+    __device__ __forceinline__ float operator[](uint32_t i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(w[i / 4][i % 4]);
+        else return half_to_f32<T>(i % 2 == 0 ? w[0][i / 2] & 0xFFFFu : w[0][i / 2] >> 16);
+    }
+};
 
 template <typename T>
 __device__ __forceinline__ void store_eight(T* row, bool wide, uint32_t base, uint32_t d, const float (&v)[kEach]) {
@@ -90,17 +96,18 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedArgs a) {
     const bool wide = a.wide_in && a.wide_out, live = id < a.vocab;
     const In* row = static_cast<const In*>(a.table) + (live ? id : 0) * a.table_stride;
     Out* out = static_cast<Out*>(a.out) + blockIdx.x * a.out_stride;
-    float v[STEPS][kEach] = {};
+    Raw<In> x[STEPS];
     const uint32_t base = blockIdx.y * STEPS * kSpan;
 #pragma unroll
     for (int s = 0; s < STEPS; ++s)
-        if (live && base + s * kSpan < a.d) load_eight(row, wide, base + s * kSpan, a.d, v[s]);
+        if (live && base + s * kSpan < a.d) x[s].load(row, wide, base + s * kSpan, a.d);
 #pragma unroll
     for (int s = 0; s < STEPS; ++s) {
         if (base + s * kSpan >= a.d) break;
+        float v[kEach];
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) v[s][i] = live ? v[s][i] * a.scale : 0.0f;
-        store_eight(out, wide, base + s * kSpan, a.d, v[s]);
+        for (uint32_t i = 0; i < kEach; ++i) v[i] = live ? x[s][i] * a.scale : 0.0f;
+        store_eight(out, wide, base + s * kSpan, a.d, v);
     }
 }
 
@@ -109,8 +116,9 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedArgs a) {
 // Ids are sorted with their places (equal ids by rising place), lists of kList in LDS first; then each entry's place in
 // the whole is its own in its list and, by bisection, the number of smaller ones in every other. Runs of equal ids are
 // summed by a block each; of a long run, the stretches of kPiece entries at multiples of kPiece are summed before, so that
-// no block adds up more than 2 kPiece - 2 rows and a part for each kPiece, whatever the ids.
+// no block adds up more than 2 kPiece - 1 rows and a part for each kPiece, whatever the ids.
 constexpr uint32_t kList = 2048, kListThreads = 1024;
+constexpr uint32_t kFillEach = 4;  // pieces of 16 bytes that a thread clears
 constexpr uint32_t kPiece = 32;
 constexpr uint32_t kNoId = 0xFFFFFFFFu;  // outside the vocabulary: sorted last
 
@@ -120,23 +128,32 @@ struct SortArgs {
     uint64_t* listed;  // sorted lists of id (high), place (low)
     uint32_t* id;      // sorted
     uint32_t* place;
-    u32x4_t* fill;     // d_table's bytes to clear, 16 at a time; null: none
-    uint64_t fills;
-    uint8_t* edge[2];  // and those before and after
-    uint32_t edge_bytes[2];
 };
 
-// The first blocks sort a list each; the others clear d_table meanwhile, which takes longer.
-__global__ __launch_bounds__(kListThreads) void embed_sort_kernel(SortArgs a) {
+// d_table's bytes to clear, 16 at a time, a share of them by the blocks that follow a launch's own: clearing takes longer
+// than everything before the runs, which it hides.
+struct Fill {
+    u32x4_t* at;
+    uint64_t n;
+    uint8_t* edge[2];  // bytes before and after, with the first share
+    uint32_t edge_bytes[2];
+};
+__device__ __forceinline__ void clear_share(const Fill& f, uint32_t block) {
+    const uint32_t t = threadIdx.x, threads = blockDim.x;
+    const uint64_t from = static_cast<uint64_t>(block) * kFillEach * threads + t;
+#pragma unroll
+    for (uint32_t i = 0; i < kFillEach; ++i)
+        if (from + i * threads < f.n) f.at[from + i * threads] = u32x4_t{0, 0, 0, 0};
+    if (block == 0)
+        for (int e = 0; e < 2; ++e)
+            if (t < f.edge_bytes[e]) f.edge[e][t] = 0;
+}
+
+__global__ __launch_bounds__(kListThreads) void embed_sort_kernel(SortArgs a, Fill f) {
     __shared__ uint64_t key[kList];
     const uint32_t t = threadIdx.x;
     if (blockIdx.x >= a.lists) {
-        const uint64_t step = static_cast<uint64_t>(gridDim.x - a.lists) * kListThreads;
-        for (uint64_t i = static_cast<uint64_t>(blockIdx.x - a.lists) * kListThreads + t; i < a.fills; i += step)
-            __builtin_nontemporal_store(u32x4_t{0, 0, 0, 0}, a.fill + i);
-        if (blockIdx.x == a.lists)
-            for (int e = 0; e < 2; ++e)
-                if (t < a.edge_bytes[e]) a.edge[e][t] = 0;
+        clear_share(f, blockIdx.x - a.lists);
         return;
     }
     const uint32_t first = blockIdx.x * kList, here = min(a.n - first, kList);
@@ -164,7 +181,12 @@ __global__ __launch_bounds__(kListThreads) void embed_sort_kernel(SortArgs a) {
     }
 }
 
-__global__ __launch_bounds__(256) void embed_merge_kernel(SortArgs a) {
+__global__ __launch_bounds__(256) void embed_merge_kernel(SortArgs a, Fill f) {
+    const uint32_t own_blocks = (a.n + 255) / 256;
+    if (blockIdx.x >= own_blocks) {
+        clear_share(f, blockIdx.x - own_blocks);
+        return;
+    }
     const uint32_t at = blockIdx.x * 256 + threadIdx.x;
     if (at >= a.n) return;
     const uint64_t key = a.listed[at];
@@ -199,78 +221,95 @@ struct RunArgs {
 
 __host__ __device__ inline uint64_t part_stride(uint32_t d) { return (d + 7ull) / 8 * 8; }
 
-// The sum of the rows of entries from .. to - 1, eight loads on their way at a time.
+// Adds the rows of entries from .. to - 1, several on their way at a time; `places`: lane l's is that of entry from + l.
 template <typename In>
-__device__ __forceinline__ void add_rows(const RunArgs& a, uint32_t from, uint32_t to, uint32_t base, float (&sum)[kEach]) {
-    constexpr uint32_t kAtOnce = 8;
-    for (uint32_t i = from; i < to; i += kAtOnce) {
-        float v[kAtOnce][kEach] = {};
+__device__ __forceinline__ void add_some(const RunArgs& a, uint32_t n, uint32_t places, uint32_t base, float (&sum)[kEach]) {
+    constexpr uint32_t kAtOnce = sizeof(In) == 4 ? 4 : 8;
+    for (uint32_t i = 0; i < n; i += kAtOnce) {
+        Raw<In> x[kAtOnce];
 #pragma unroll
         for (uint32_t j = 0; j < kAtOnce; ++j)
-            if (i + j < to) load_eight(static_cast<const In*>(a.rows) + a.place[i + j] * a.rows_stride, a.wide, base, a.d, v[j]);
+            if (i + j < n) {
+                const uint32_t place = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(places), static_cast<int>(i + j)));
+                x[j].load(static_cast<const In*>(a.rows) + place * a.rows_stride, a.wide, base, a.d);
+            }
 #pragma unroll
         for (uint32_t j = 0; j < kAtOnce; ++j)
-            if (i + j < to) {
+            if (i + j < n) {
 #pragma unroll
-                for (uint32_t e = 0; e < kEach; ++e) sum[e] += v[j][e];
+                for (uint32_t e = 0; e < kEach; ++e) sum[e] += x[j][e];
             }
     }
+}
+template <typename In>
+__device__ __forceinline__ void add_rows(const RunArgs& a, uint32_t from, uint32_t to, uint32_t base, float (&sum)[kEach]) {
+    static_assert(kPiece <= 64, "a lane to each place");
+    if (from >= to) return;
+    const uint32_t at = from + threadIdx.x % 64;
+    add_some<In>(a, to - from, at < to ? a.place[at] : 0u, base, sum);
 }
 
 // The parts of long runs: of each stretch of kPiece entries that all have one id.
 template <typename In>
-__global__ __launch_bounds__(kEmbedThreads) void embed_parts_kernel(RunArgs a) {
-    const uint32_t first = blockIdx.x * kPiece, base = blockIdx.y * kSpan;
+__global__ __launch_bounds__(kEmbedThreads) void embed_parts_kernel(RunArgs a, uint32_t steps, Fill f) {
+    const uint32_t own = a.n / kPiece * steps;
+    if (blockIdx.x >= own) {
+        clear_share(f, blockIdx.x - own);
+        return;
+    }
+    const uint32_t piece = blockIdx.x / steps, first = piece * kPiece, base = blockIdx.x % steps * kSpan;
     const uint32_t id = a.id[first];
-    if (id == kNoId || first + kPiece > a.n || a.id[first + kPiece - 1] != id) return;
+    if (id == kNoId || a.id[first + kPiece - 1] != id) return;
     float sum[kEach] = {};
     add_rows<In>(a, first, first + kPiece, base, sum);
-    store_eight(a.part + blockIdx.x * part_stride(a.d), a.wide, base, a.d, sum);
+    store_eight(a.part + piece * part_stride(a.d), a.wide, base, a.d, sum);
 }
 
-// A block to each run (that of its first entry) and step of columns.
+// A block to each run (that of its first entry) and step of columns. Most runs are short: ids and places of 64 entries come
+// at once, and rows after them.
 template <typename In, typename Out>
 __global__ __launch_bounds__(kEmbedThreads) void embed_runs_kernel(RunArgs a) {
-    const uint32_t first = blockIdx.x, base = blockIdx.y * kSpan;
-    const uint32_t id = a.id[first];
-    if (id == kNoId || (first > 0 && a.id[first - 1] == id)) return;
-    // the run's end: within the next 64 entries, or by a search in 64 places at a time of what follows
-    const uint32_t lane = threadIdx.x % 64;
-    uint32_t last = first + static_cast<uint32_t>(__popcll(__ballot(first + 1 + lane < a.n && a.id[first + 1 + lane] == id)));
-    if (last == first + 64) {
-        uint32_t past = a.n;  // `last` has the id, `past` does not
+    const uint32_t first = blockIdx.x, base = blockIdx.y * kSpan, lane = threadIdx.x % 64;
+    const bool in = first + lane < a.n;
+    const uint32_t ids = in ? a.id[first + lane] : kNoId, places = in ? a.place[first + lane] : 0u;
+    const uint32_t before = first > 0 ? a.id[first - 1] : kNoId;
+    const uint32_t id = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(ids)));
+    if (id == kNoId || before == id) return;
+    const uint32_t near = static_cast<uint32_t>(__popcll(__ballot(ids == id)));  // sorted: the first ones
+    float sum[kEach] = {};
+    if (near < 2 * kPiece) {  // (a run of 63 may hold a whole piece: its part is not used)
+        add_some<In>(a, near, places, base, sum);
+    } else {
+        // the end, by a search in 64 places at a time
+        uint32_t last = first + near - 1, past = a.n;  // `last` has the id, `past` does not
         while (past - last > 1) {
             const uint32_t step = (past - last + 63) / 64, at = last + (lane + 1) * step;
             last += step * static_cast<uint32_t>(__popcll(__ballot(at < past && a.id[at] == id)));
             past = min(past, last + step);
         }
-    }
-    const uint32_t end = last + 1;
-    float sum[kEach] = {};
-    const uint32_t p0 = (first + kPiece - 1) / kPiece, p1 = end / kPiece;  // whole pieces
-    if (p0 < p1) {
+        const uint32_t end = last + 1, p0 = (first + kPiece - 1) / kPiece, p1 = end / kPiece;  // whole pieces
         add_rows<In>(a, first, p0 * kPiece, base, sum);
         constexpr uint32_t kAtOnce = 4;
         for (uint32_t p = p0; p < p1; p += kAtOnce) {
-            float v[kAtOnce][kEach] = {};
+            Raw<float> x[kAtOnce];
 #pragma unroll
             for (uint32_t j = 0; j < kAtOnce; ++j)
-                if (p + j < p1) load_eight(a.part + (p + j) * part_stride(a.d), a.wide, base, a.d, v[j]);
+                if (p + j < p1) x[j].load(a.part + (p + j) * part_stride(a.d), a.wide, base, a.d);
 #pragma unroll
             for (uint32_t j = 0; j < kAtOnce; ++j)
+                if (p + j < p1) {
 #pragma unroll
-                for (uint32_t e = 0; e < kEach; ++e) sum[e] += v[j][e];
+                    for (uint32_t e = 0; e < kEach; ++e) sum[e] += x[j][e];
+                }
         }
         add_rows<In>(a, p1 * kPiece, end, base, sum);
-    } else {
-        add_rows<In>(a, first, end, base, sum);
     }
     Out* row = static_cast<Out*>(a.table) + id * a.table_stride;
 #pragma unroll
     for (uint32_t e = 0; e < kEach; ++e) sum[e] *= a.scale;
     if (a.add) {
-        float old[kEach];
-        load_eight(row, a.wide, base, a.d, old);
+        Raw<Out> old;
+        old.load(row, a.wide, base, a.d);
 #pragma unroll
         for (uint32_t e = 0; e < kEach; ++e) sum[e] += old[e];
     }
@@ -333,18 +372,17 @@ namespace {
 int run(const twd_embedgrad* g, SortArgs sort, const RunArgs& a, int rows_type, int table_type, bool clear, hipStream_t s) {
     sort.lists = over(sort.n, kList);
     const uint64_t size = size_of(table_type);
-    uint32_t fillers = 0;
+    const uint32_t steps = over(a.d, kSpan);
+    Fill f{};
     if (clear && (a.vocab == 1 || a.table_stride == a.d)) {
         const uint64_t bytes = static_cast<uint64_t>(a.vocab) * a.d * size;
         const uintptr_t from = reinterpret_cast<uintptr_t>(a.table);
         const uint64_t before = (16 - from % 16) % 16 < bytes ? (16 - from % 16) % 16 : bytes;
-        sort.fills = (bytes - before) / 16;
-        sort.fill = reinterpret_cast<u32x4_t*>(from + before);
-        sort.edge[0] = static_cast<uint8_t*>(a.table), sort.edge_bytes[0] = static_cast<uint32_t>(before);
-        sort.edge[1] = static_cast<uint8_t*>(a.table) + before + 16 * sort.fills;
-        sort.edge_bytes[1] = static_cast<uint32_t>(bytes - before - 16 * sort.fills);
-        const uint64_t want = (sort.fills + 4 * kListThreads - 1) / (4 * kListThreads);
-        fillers = static_cast<uint32_t>(want < 1 ? 1 : want < 2048 ? want : 2048);
+        f.n = (bytes - before) / 16;
+        f.at = reinterpret_cast<u32x4_t*>(from + before);
+        f.edge[0] = static_cast<uint8_t*>(a.table), f.edge_bytes[0] = static_cast<uint32_t>(before);
+        f.edge[1] = static_cast<uint8_t*>(a.table) + before + 16 * f.n;
+        f.edge_bytes[1] = static_cast<uint32_t>(bytes - before - 16 * f.n);
     } else if (clear) {
         const int rc = with_type(table_type, [&](auto t) -> int {
             using Out = decltype(t);
@@ -354,19 +392,33 @@ int run(const twd_embedgrad* g, SortArgs sort, const RunArgs& a, int rows_type, 
         });
         if (rc) return rc;
     }
-    if (sort.lists + fillers == 0) return TWD_OK;
-    embed_sort_kernel<<<sort.lists + fillers, kListThreads, 0, s>>>(sort);
+    // what is left of the clearing goes with the launches that are left: sorting takes some 6 us, merging 16, the parts 30
+    const bool merges = sort.lists > 1, parts = a.n >= kPiece;
+    auto share = [&](uint32_t percent, uint32_t threads, uint32_t* blocks) {
+        Fill now = f;
+        const uint64_t each = static_cast<uint64_t>(kFillEach) * threads;
+        const uint64_t want = (f.n * percent / 100 + each - 1) / each;
+        now.n = want * each < f.n ? want * each : f.n;
+        *blocks = now.n == 0 && now.edge_bytes[0] + now.edge_bytes[1] == 0 ? 0u : static_cast<uint32_t>(want < 1 ? 1 : want);
+        f.at += now.n, f.n -= now.n, f.edge_bytes[0] = f.edge_bytes[1] = 0;
+        return now;
+    };
+    uint32_t blocks = 0;
+    const Fill first = share(!merges && !parts ? 100 : merges ? 30 : 50, kListThreads, &blocks);
+    if (sort.lists + blocks == 0) return TWD_OK;
+    embed_sort_kernel<<<sort.lists + blocks, kListThreads, 0, s>>>(sort, first);
     TWD_HIP(hipGetLastError());
     if (a.n == 0) return TWD_OK;
-    if (sort.lists > 1) {
-        embed_merge_kernel<<<over(a.n, 256), 256, 0, s>>>(sort);
+    if (merges) {
+        const Fill second = share(parts ? 50 : 100, 256, &blocks);
+        embed_merge_kernel<<<over(a.n, 256) + blocks, 256, 0, s>>>(sort, second);
         TWD_HIP(hipGetLastError());
     }
-    const uint32_t steps = over(a.d, kSpan);
     return with_type(rows_type, [&](auto r) -> int {
         using In = decltype(r);
-        if (a.n >= kPiece) {
-            embed_parts_kernel<In><<<dim3(a.n / kPiece, steps), kEmbedThreads, 0, s>>>(a);
+        if (parts) {
+            const Fill third = share(100, kEmbedThreads, &blocks);
+            embed_parts_kernel<In><<<a.n / kPiece * steps + blocks, kEmbedThreads, 0, s>>>(a, steps, third);
             TWD_HIP(hipGetLastError());
         }
         return with_type(table_type, [&](auto t) -> int {
