@@ -92,25 +92,34 @@ struct LogitArgs {
 // By rows, or with the second operand turned.
 using TileFew = ProductTile<1, 2, 4, 1, 64, 3, false, false>;
 using TileWide = ProductTile<4, 4, 2, 2, 64, 2, false, false, true>;
-using TileMiddle = ProductTile<4, 2, 2, 2, 64, 2, false, false, true>;
-using TileQuarter = ProductTile<2, 2, 4, 1, 64, 3, false, false, true>;
+using TileThree = ProductTile<4, 3, 2, 2, 64, 2, false, false, true>;  // quarters of a wide one
+using TileTwo = ProductTile<4, 2, 2, 2, 64, 2, false, false, true>;
+using TileStripe = ProductTile<2, 2, 4, 1, 64, 3, false, false, true>;
 using TileHidden = ProductTile<4, 4, 2, 2, 32, 4, false, true>;
 using TileWeight = ProductTile<4, 2, 2, 2, 32, 3, true, true>;
 
-// Tiles of logits are of 256 vocabulary rows by 256 hidden rows, or by 128 where no more count. (Narrower tiles for the last
-// hidden rows do not pay: a stage waits for memory as long as a wide one's. 823 rows of 65,537 x 2,880 with 55 in tiles of 64:
-// 437 us.) The few tiles past whole rounds of the units are cut into four and follow in a launch of their own, so that a
-// last round of up to kMostCut costs less than a round (1,023 rows: 459 and 403 us).
+// Tiles of logits are of 256 vocabulary rows by 256, 192 or 128 hidden rows, whichever takes the least time: rounds of the
+// units times a tile's, which goes by its width and some 100 rows more (65,536 x 2,880: 105, 86 and 65 us a round). 518 rows
+// of 32,003 x 2,048 take 139, 113 and 124 us, 1,023 of 65,537 x 2,880 take 427, 476 and 476. The few tiles past whole rounds
+// are cut into stripes of 64 hidden rows and follow in a launch of their own, which costs some 80 rows of a round.
 constexpr uint32_t kVocabTile = 256, kRound = 256, kMostCut = 64, kFewRows = 64;
-static_assert(TileWide::kA == kVocabTile && TileMiddle::kA == kVocabTile && TileQuarter::kA == kVocabTile, "one width");
+static_assert(TileWide::kA == kVocabTile && TileThree::kA == kVocabTile && TileTwo::kA == kVocabTile && TileStripe::kA == kVocabTile, "one width");
 struct LogitTiles {
     TileGrid grid;
-    uint32_t cut;  // of the last tiles
+    uint32_t width;  // hidden rows of a tile
+    uint32_t cut;    // of the last tiles
 };
-__device__ __forceinline__ LogitTiles logit_tiles(uint32_t count, uint32_t na) {
-    const TileGrid g{na, (count + 255) / 256, 1};
-    const uint32_t left = g.tiles() % kRound;
-    return LogitTiles{g, count > 128 && left <= kMostCut ? left : 0};
+__host__ __device__ inline LogitTiles logit_tiles(uint32_t count, uint32_t na) {
+    LogitTiles best{};
+    uint32_t least = ~0u;
+#pragma unroll
+    for (uint32_t width = 256; width >= 128; width -= 64) {
+        const TileGrid g{na, (count + width - 1) / width, 1};
+        const uint32_t left = g.tiles() % kRound, cut = left <= kMostCut ? left : 0;
+        const uint32_t time = g.tiles() / kRound * (width + 100) + (cut > 0 ? 80 : left > 0 ? width + 100 : 0);
+        if (time < least) least = time, best = LogitTiles{g, width, cut};
+    }
+    return best;
 }
 
 template <typename Tile>
@@ -231,22 +240,24 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     const uint32_t tiles = t.grid.tiles() - t.cut, id = stretched(tiles);
     if (id >= tiles) return;
     const TileAt at = tile_at(t.grid, id);
-    if (count > 128) logits_tile<TileWide, GRAD>(a, count, at.a, 256 * at.b, at.share, at.who, s0, s1, nullptr, nullptr, sink);
-    else logits_tile<TileMiddle, GRAD>(a, count, at.a, 0, 1, 0, s0, s1, nullptr, nullptr, sink);
+    const uint32_t m0 = t.width * at.b;
+    if (t.width == 256) logits_tile<TileWide, GRAD>(a, count, at.a, m0, at.share, at.who, s0, s1, nullptr, nullptr, sink);
+    else if (t.width == 192) logits_tile<TileThree, GRAD>(a, count, at.a, m0, at.share, at.who, s0, s1, nullptr, nullptr, sink);
+    else logits_tile<TileTwo, GRAD>(a, count, at.a, m0, at.share, at.who, s0, s1, nullptr, nullptr, sink);
 }
 
 template <bool GRAD>
-__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_quarters_kernel(LogitArgs a) {
-    using Tile = TileQuarter;
+__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_stripes_kernel(LogitArgs a) {
+    using Tile = TileStripe;
     __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces];
     __shared__ uint32_t sink[Tile::kSink];
     const uint32_t count = *a.r.count;
     const LogitTiles t = logit_tiles(count, (a.here + kVocabTile - 1) / kVocabTile);
-    const uint32_t id = stretched(4 * t.cut);
-    if (id >= 4 * t.cut) return;
-    const TileAt at = tile_at(t.grid, t.grid.tiles() - t.cut + id / 4);
-    const uint32_t m0 = 256 * at.b + 64 * (id % 4);
-    if (m0 < count) logits_tile<Tile, GRAD>(a, count, at.a, m0, 4, id % 4, s0, s1, s2, nullptr, sink);
+    const uint32_t each = t.width / 64, id = stretched(each * t.cut);
+    if (id >= each * t.cut) return;
+    const TileAt at = tile_at(t.grid, t.grid.tiles() - t.cut + id / each);
+    const uint32_t m0 = t.width * at.b + 64 * (id % each);
+    if (m0 < count) logits_tile<Tile, GRAD>(a, count, at.a, m0, each, id % each, s0, s1, s2, nullptr, sink);
 }
 
 // Few rows: bound by the read of the weights.
@@ -451,10 +462,15 @@ template <bool GRAD>
 int launch_logits(const LogitArgs& a, uint32_t rows, hipStream_t s) {
     if (rows <= kFewRows) {
         loss_few_kernel<GRAD><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a);
-    } else {  // as many blocks as any number of rows that count needs
-        loss_logits_kernel<GRAD><<<blocks_for(div_up(a.here, kVocabTile) * div_up(rows, 256)), kProductThreads, 0, s>>>(a);
+    } else {
+        uint32_t most = 0;  // blocks, for any number of rows that count
+        for (uint32_t n = 64; n < rows + 64; n += 64) {
+            const uint32_t tiles = logit_tiles(n < rows ? n : rows, div_up(a.here, kVocabTile)).grid.tiles();
+            most = tiles > most ? tiles : most;
+        }
+        loss_logits_kernel<GRAD><<<blocks_for(most), kProductThreads, 0, s>>>(a);
         TWD_HIP(hipGetLastError());
-        loss_quarters_kernel<GRAD><<<4 * kMostCut, kProductThreads, 0, s>>>(a);
+        loss_stripes_kernel<GRAD><<<4 * kMostCut, kProductThreads, 0, s>>>(a);
     }
     TWD_HIP(hipGetLastError());
     return TWD_OK;
