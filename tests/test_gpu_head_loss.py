@@ -101,3 +101,201 @@ def test_loss_and_gradients(vocab, d, rows, cap, share):
     loss.backward(h, w, targets, lse, grad=grad, d_weight=full, need=(False, True))
     check("d_weight fp32", full, want["d_weight"], tol["d_weight"], U)
     loss.close()
+
+
+def test_many_rows():
+    """More rows than the gather takes singly, half of them left out, in many pieces of the vocabulary."""
+    import torch
+    t = twd()
+    vocab, d, rows = 700, 32, 65536
+    h, w, targets, grad = make(vocab, d, rows, rows // 2, 9)
+    want, tol = reference(h, w, targets, 0.0, grad)
+    loss = t.HeadLoss(rows, vocab, d)
+    losses, lse = loss.forward(h, w, targets)
+    check("losses", losses, want["losses"], tol["losses"], U)
+    d_hidden, d_weight = loss.backward(h, w, targets, lse, grad=grad)
+    check("d_hidden", d_hidden, want["d_hidden"], tol["d_hidden"], U16)
+    check("d_weight", d_weight, want["d_weight"], tol["d_weight"], U16)
+    loss.close()
+
+
+@pytest.mark.parametrize("vocab,d,rows", [(1000, 160, 5), (777, 96, 100), (2049, 224, 300)])
+def test_strides_accumulation_and_parts_left_alone(vocab, d, rows):
+    """Rows inside wider buffers on every side; gradients on top of others; either gradient alone; the same results
+    whatever the object's size, run after run."""
+    import torch
+    t = twd()
+    h, w, targets, grad = make(vocab, d, rows, rows // 3, 4)
+    want, tol = reference(h, w, targets, 30.0, grad)
+    nan = float("nan")
+    hw = torch.full((rows, d + 24), nan, dtype=torch.bfloat16, device="cuda:0")
+    ww = torch.full((vocab, d + 8), nan, dtype=torch.bfloat16, device="cuda:0")
+    hw[:, 8:d + 8], ww[:, :d] = h, w
+    loss, large = t.HeadLoss(rows, vocab, d, softcap=30.0), t.HeadLoss(rows + 1000, vocab, d, softcap=30.0)
+    losses, lse = loss.forward(hw[:, 8:d + 8], ww[:, :d], targets)
+    check("losses", losses, want["losses"], tol["losses"], U)
+    again = large.forward(h, w, targets)
+    assert torch.equal(losses, again[0]) and torch.equal(lse, again[1])
+    for dt, step in ((torch.float32, U), (torch.bfloat16, U16)):
+        base = torch.randn(vocab, d, device="cuda:0").to(dt)
+        dw = torch.full((vocab + 1, d + 8), 7.0, dtype=dt, device="cuda:0")
+        dh = torch.full((rows + 1, d + 16), 7.0, dtype=torch.bfloat16, device="cuda:0")
+        dw[:vocab, :d] = base
+        loss.backward(h, w, targets, lse, grad=grad, d_hidden=dh[:rows, 8:d + 8], d_weight=dw[:vocab, :d], accumulate=True)
+        check("d_hidden", dh[:rows, 8:d + 8], want["d_hidden"], tol["d_hidden"], U16)
+        check("d_weight", dw[:vocab, :d], base.double() + want["d_weight"], tol["d_weight"] + U * base.double().abs(), step)
+        assert (dw[vocab] == 7).all() and (dw[:, d:] == 7).all()
+        assert (dh[rows] == 7).all() and (dh[:, :8] == 7).all() and (dh[:, d + 8:] == 7).all()
+    both = loss.backward(h, w, targets, lse, grad=grad)
+    alone = large.backward(h, w, targets, lse, grad=grad, need=(True, False))
+    assert alone[1] is None and torch.equal(alone[0], both[0])
+    alone = large.backward(h, w, targets, lse, grad=grad, need=(False, True))
+    assert alone[0] is None and torch.equal(alone[1], both[1])
+    ones = loss.backward(h, w, targets, lse)
+    assert torch.equal(ones[0], loss.backward(h, w, targets, lse, grad=torch.ones(rows, device="cuda:0"))[0])
+    loss.close(), large.close()
+
+
+@pytest.mark.parametrize("rows", [3, 70, 300])
+def test_nan_and_infinity(rows):
+    """What a row that is left out holds does not matter, nor its weight; a NaN in one that counts is its loss's alone."""
+    import torch
+    t = twd()
+    vocab, d = 600, 96
+    h, w, targets, grad = make(vocab, d, rows, 0, 5)
+    targets[1] = -100
+    clean = [x.clone() for x in (h, grad)]
+    h[1, ::2], h[1, 1::2], grad[1] = float("nan"), float("inf"), float("nan")
+    loss = t.HeadLoss(rows, vocab, d)
+    losses, lse = loss.forward(h, w, targets)
+    d_hidden, d_weight = loss.backward(h, w, targets, lse, grad=grad)
+    losses2, lse2 = loss.forward(clean[0], w, targets)
+    d_hidden2, d_weight2 = loss.backward(clean[0], w, targets, lse2, grad=clean[1])
+    for a, b in ((losses, losses2), (lse, lse2), (d_hidden, d_hidden2), (d_weight, d_weight2)):
+        assert torch.equal(a, b) and bool(torch.isfinite(a).all())
+    h[0, 5] = float("nan")
+    losses, lse = loss.forward(h, w, targets)
+    assert bool(torch.isnan(losses[0])) and torch.equal(losses[1:], losses2[1:])
+    d_hidden, d_weight = loss.backward(h, w, targets, lse, grad=grad)
+    assert bool(torch.isnan(d_hidden[0]).all()) and torch.equal(d_hidden[1:], d_hidden2[1:])
+    assert bool(torch.isnan(d_weight).all())
+    h[0, 5], h[0, 6] = 0.0, float("inf")  # infinite logits: no loss
+    assert bool(torch.isnan(loss.forward(h, w, targets)[0][0]))
+    loss.close()
+
+
+def test_extreme_logits():
+    """Logits far apart and far up: the largest alone counts; the loss of others is their distance."""
+    import torch
+    t = twd()
+    vocab, d = 300, 32
+    w = torch.zeros(vocab, d, dtype=torch.bfloat16, device="cuda:0")
+    w[:, 0] = torch.linspace(-1, 1, vocab, device="cuda:0")
+    h = torch.zeros(4, d, dtype=torch.bfloat16, device="cuda:0")
+    h[0, 0], h[1, 0], h[2, 0], h[3, 0] = 2.0 ** 20, -(2.0 ** 20), 0.0, 2.0 ** 100
+    targets = torch.tensor([vocab - 1, 0, 5, 0], dtype=torch.int32, device="cuda:0")
+    loss = t.HeadLoss(4, vocab, d)
+    losses, lse = loss.forward(h, w, targets)
+    z = h.double() @ w.double().t()
+    want = torch.logsumexp(z, 1)
+    assert bool(((lse.double() - want).abs() <= 4 * U * want.abs() + 1e-6).all())
+    gap = want - z.gather(1, targets.long()[:, None])[:, 0]
+    assert bool(((losses.double() - gap).abs() <= 4 * U * (want.abs() + gap)).all())
+    d_hidden, d_weight = loss.backward(h, w, targets, lse)
+    assert bool(torch.isfinite(d_hidden).all()) and bool(torch.isfinite(d_weight).all())
+    assert bool((d_hidden[:2] == 0).all())  # the target has all of the probability
+    loss.close()
+
+
+def test_gradient_by_differences():
+    """d_weight against central differences of the losses themselves. One logit of a row changes by delta h: the third
+    derivative of the loss by it is p (1 - p) (1 - 2 p), at most 0.0963, so the difference is off by delta^2 |h|^3 0.0963 / 6 a
+    row, and by two losses' errors over 2 delta; the gradient by 2^-8 of its terms."""
+    import torch
+    t = twd()
+    vocab, d, rows, delta = 40, 64, 70, 2.0 ** -4
+    rng = np.random.default_rng(3)
+    h = torch.from_numpy(rng.integers(-4, 5, (rows, d)) / 4.0).cuda().bfloat16()
+    w = torch.from_numpy(rng.integers(-8, 9, (vocab, d)) / 16.0).cuda().bfloat16()  # steps of delta are exact
+    targets = torch.from_numpy(rng.integers(0, vocab, rows)).to(torch.int32).cuda()
+    targets[::7] = -1
+    loss = t.HeadLoss(rows, vocab, d)
+    _, lse = loss.forward(h, w, targets)
+    _, grad = loss.backward(h, w, targets, lse, d_weight=torch.empty(vocab, d, device="cuda:0"))
+    live = (targets >= 0)
+    size = h[live].double().abs()
+    for _ in range(30):
+        v, c = int(rng.integers(vocab)), int(rng.integers(d))
+        ends = []
+        for sign in (1, -1):
+            moved = w.clone()
+            moved[v, c] += sign * delta
+            ends.append(loss.forward(h, moved, targets)[0].double().sum())
+        diff = float((ends[0] - ends[1]) / (2 * delta))
+        tol = float((delta ** 2 * size[:, c] ** 3 * 0.0963 / 6).sum()) + 2 * rows * 30 * U / (2 * delta) + U16 * float(size[:, c].sum())
+        assert abs(diff - float(grad[v, c])) <= tol, (v, c, diff, float(grad[v, c]), tol)
+    loss.close()
+
+
+@pytest.mark.parametrize("rows", [3, 100])
+def test_far_rows(rows):
+    """Weight rows more than 4 GiB from the first, at the widest stride; hidden rows too."""
+    import torch
+    t = twd()
+    vocab, d, far = 600, 32, 1 << 22
+    h, w, targets, grad = make(vocab, d, rows, 1, 6)
+    wide = torch.empty((vocab - 1) * far + d, dtype=torch.bfloat16, device="cuda:0").as_strided((vocab, d), (far, 1))
+    wide.copy_(w)
+    hw = torch.empty((rows - 1) * far + d, dtype=torch.bfloat16, device="cuda:0").as_strided((rows, d), (far, 1))
+    hw.copy_(h)
+    loss = t.HeadLoss(rows, vocab, d)
+    a, b = loss.forward(h, w, targets), loss.forward(hw, wide, targets)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    x, y = loss.backward(h, w, targets, a[1]), loss.backward(hw, wide, targets, a[1], d_weight=wide.clone())
+    assert torch.equal(x[0], y[0]) and torch.equal(x[1], y[1])
+    loss.close()
+
+
+def test_streams_and_graphs():
+    """One object's calls on two streams in turn; captured forward and backward passes replayed with other rows, other
+    targets and another number of rows that count."""
+    import torch
+    t = twd()
+    vocab, d = 3001, 160
+    sets = [make(vocab, d, n, n // 4, n) for n in (200, 30)]
+    loss = t.HeadLoss(200, vocab, d, softcap=30.0)
+    refs = []
+    for h, w, targets, grad in sets:
+        losses, lse = loss.forward(h, w, targets)
+        refs.append((losses, lse) + loss.backward(h, w, targets, lse, grad=grad))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        got = []
+        for s, (h, w, targets, grad) in zip(streams, sets):
+            losses, lse = loss.forward(h, w, targets, stream=s.cuda_stream)
+            got.append((losses, lse) + loss.backward(h, w, targets, lse, grad=grad, stream=s.cuda_stream))
+        torch.cuda.synchronize()
+        for a, b in zip(got, refs):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+    for n in (200, 40):
+        h, w, targets, grad = [x.clone() for x in make(vocab, d, n, 0, 77)]
+        out = [torch.empty(n, device="cuda:0"), torch.empty(n, device="cuda:0"), torch.empty_like(h), torch.empty_like(w)]
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[0]):
+            loss.forward(h, w, targets, losses=out[0], lse=out[1], stream=streams[0].cuda_stream)
+            loss.backward(h, w, targets, out[1], grad=grad, d_hidden=out[2], d_weight=out[3], stream=streams[0].cuda_stream)
+        for rep in range(4):
+            new = make(vocab, d, n, n * rep // 3, 100 + rep)
+            for x, y in zip((h, w, targets, grad), new):
+                x.copy_(y)
+            torch.cuda.synchronize()
+            losses, lse = loss.forward(*new[:3])  # eager work between the replays
+            want = (losses, lse) + loss.backward(*new[:3], lse, grad=new[3])
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(out, want)), (n, rep)
+        del g
+    loss.close()

@@ -169,10 +169,11 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& a, uint32_t count, 
                 }
 #pragma unroll
                 for (int i = 0; i < 16; ++i) most = fmaxf(most, y[i]);
-                const float ref = most > -INFINITY ? most * kLog2e : 0.0f;  // nothing of the vocabulary yet: no infinity less itself
-                sum *= __builtin_amdgcn_exp2f(fmaf(top, kLog2e, -ref));
+                // the differences first: the logits may be large. Nothing of the vocabulary yet: no infinity less itself
+                const float ref = most > -INFINITY ? most : 0.0f;
+                sum *= __builtin_amdgcn_exp2f((top - ref) * kLog2e);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(y[i], kLog2e, -ref));
+                for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f((y[i] - ref) * kLog2e);
                 top = most;
                 __builtin_amdgcn_sched_barrier(0);
             });
@@ -183,14 +184,14 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& a, uint32_t count, 
             sum = sum * __builtin_amdgcn_exp2f((top - ref) * kLog2e) + other_sum * __builtin_amdgcn_exp2f((other_top - ref) * kLog2e);
             if (lane < 32) joint[wa * Tile::kB + in] = make_float2(both, sum);
         } else {
-            const float lse = live ? a.r.lse[m] * -kLog2e : 0.0f, grad = live ? a.r.grad[m] : 0.0f;
+            const float lse = live ? a.r.lse[m] : 0.0f, grad = live ? a.r.grad[m] : 0.0f;
             store_rows<TA, uint16_t>((wave < 2 ? s0 : s1) + wave % 2 * (TA * 128),
                 [&](auto ta) {
                     float y[16];
                     f32x16_t dz;
                     logits(ta, y);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) dz[i] = __builtin_amdgcn_exp2f(fmaf(y[i], kLog2e, lse));
+                    for (int i = 0; i < 16; ++i) dz[i] = __builtin_amdgcn_exp2f((y[i] - lse) * kLog2e);
                     at_target(ta, [&](int i, bool is) { dz[i] = is ? dz[i] - 1.0f : dz[i]; });
                     if (a.softcap.cap > 0.0f) {
 #pragma unroll
@@ -334,15 +335,10 @@ struct GradArgs {
     bool add;
 };
 
-// 16 bytes of a result, on top of what is there.
-__device__ __forceinline__ u32x4_t added(u32x4_t w, u32x4_t old, float) {
-    return __builtin_bit_cast(u32x4_t, __builtin_bit_cast(f32x4_t, w) + __builtin_bit_cast(f32x4_t, old));
-}
-__device__ __forceinline__ u32x4_t added(u32x4_t w, u32x4_t old, uint16_t) {
-    u32x4_t sum;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sum[i] = bf16_pair(bf16_lo(w[i]) + bf16_lo(old[i]), bf16_hi(w[i]) + bf16_hi(old[i]));
-    return sum;
+__device__ __forceinline__ void add4(float* p, f32x4_t v) { *reinterpret_cast<f32x4_t*>(p) += v; }
+__device__ __forceinline__ void add4(uint16_t* p, f32x4_t v) {
+    const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p);
+    *reinterpret_cast<u32x2_t*>(p) = u32x2_t{bf16_pair(v[0] + bf16_lo(w[0]), v[1] + bf16_hi(w[0])), bf16_pair(v[2] + bf16_lo(w[1]), v[3] + bf16_hi(w[1]))};
 }
 
 // d_weight = dz^T H (BY_COUNT: k runs over the rows that count) or a piece's part of d_hidden = dz W.
@@ -380,16 +376,27 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     }
     const uint32_t wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
     Out* const out = static_cast<Out*>(a.out) + at.part * (rows * a.stride);
-    each<TA>([&](auto ta) {
-        store_rows<TB, Out>((wave < 2 ? s0 : s1) + wave % 2 * (TB * 64 * sizeof(Out)), [&](auto tb) { return acc[ta][tb]; },
-            [&](uint32_t row, uint32_t col, u32x4_t w) {
-                const uint32_t r = a0 + 32 * (TA * wa + ta) + row, c = b0 + 32 * TB * wb + col;
-                if (r >= rows || c >= a.cols) return;
-                u32x4_t* const p = reinterpret_cast<u32x4_t*>(out + r * a.stride + c);
-                if (a.add) w = added(w, *p, Out{});
-                *p = w;
-            });
-    });
+    auto place = [&](uint32_t ta, uint32_t row, uint32_t col) -> Out* {
+        const uint32_t r = a0 + 32 * (TA * wa + ta) + row, c = b0 + 32 * TB * wb + col;
+        return r < rows && c < a.cols ? out + r * a.stride + c : nullptr;
+    };
+    if (a.add) {  // on top of what is there, rounded once
+        each<TA>([&](auto ta) {
+            store_rows<TB, float>((wave < 2 ? s0 : s1) + wave % 2 * (TB * 256), [&](auto tb) { return acc[ta][tb]; },
+                [&](uint32_t row, uint32_t col, u32x4_t w) {
+                    Out* const p = place(ta, row, col);
+                    if (p) add4(p, __builtin_bit_cast(f32x4_t, w));
+                });
+        });
+    } else {
+        each<TA>([&](auto ta) {
+            store_rows<TB, Out>((wave < 2 ? s0 : s1) + wave % 2 * (TB * 64 * sizeof(Out)), [&](auto tb) { return acc[ta][tb]; },
+                [&](uint32_t row, uint32_t col, u32x4_t w) {
+                    Out* const p = place(ta, row, col);
+                    if (p) *reinterpret_cast<u32x4_t*>(p) = w;
+                });
+        });
+    }
 }
 
 struct SpreadArgs {
