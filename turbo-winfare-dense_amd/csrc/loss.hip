@@ -91,6 +91,7 @@ struct LogitArgs {
 
 // By rows, or with the second operand turned.
 using TileFew = ProductTile<1, 2, 4, 1, 64, 3, false, false>;
+using TileFewest = ProductTile<1, 1, 2, 2, 64, 4, false, false>;  // 64 vocabulary rows
 using TileWide = ProductTile<4, 4, 2, 2, 64, 2, false, false, true>;
 using TileThree = ProductTile<4, 3, 2, 2, 64, 2, false, false, true>;  // quarters of a wide one
 using TileTwo = ProductTile<4, 2, 2, 2, 64, 2, false, false, true>;
@@ -262,12 +263,11 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
 }
 
 // Few rows: bound by the read of the weights.
-template <bool GRAD>
+template <typename Tile, bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_few_kernel(LogitArgs a) {
-    using Tile = TileFew;
-    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces];
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kPieces3];
     const uint32_t count = *a.r.count, tiles = (a.here + Tile::kA - 1) / Tile::kA, id = stretched(tiles);
-    if (id < tiles && count > 0) logits_tile<Tile, GRAD>(a, count, id, 0, 1, 0, s0, s1, s2, nullptr, nullptr);
+    if (id < tiles && count > 0) logits_tile<Tile, GRAD>(a, count, id, 0, 1, 0, s0, s1, s2, s3, nullptr);
 }
 
 struct JoinArgs {
@@ -431,10 +431,11 @@ uint32_t round_up(uint32_t x, uint32_t y) { return div_up(x, y) * y; }
 
 constexpr uint32_t kLossMaxRows = 65536, kLossMaxVocab = 1u << 24;
 
-// dz holds a piece of the vocabulary: up to 65,536 of it, 2^27 values with all rows (256 MB), a multiple of 256.
+// dz holds a piece of the vocabulary, a multiple of 256 of it: 2^27 values with all rows (256 MB), and rows no further apart
+// than a product takes them.
 uint32_t most_of_piece(uint32_t rows) {
-    const uint32_t most = static_cast<uint32_t>((1ull << 27) / rows) / 256 * 256;
-    return most < 256 ? 256 : most < 65536 ? most : 65536;
+    const uint32_t most = static_cast<uint32_t>((1ull << 27) / rows) / 256 * 256, apart = kMaxProductStride;
+    return most < 256 ? 256 : most < apart ? most : apart;
 }
 uint32_t piece_of(uint32_t rows, uint32_t vocab) {  // pieces alike
     const uint32_t all = round_up(vocab, 256);
@@ -465,10 +466,17 @@ namespace twd {
 
 namespace {
 
+// Vocabulary rows of a tile of few rows: small ones where large ones would not fill the units for two rounds (17 rows of
+// 100,000 x 2,048: 92 and 109 us; of 151,669 x 3,584: 209 and 198).
+uint32_t few_tile(uint32_t vocab) { return vocab > 131072 ? TileFew::kA : TileFewest::kA; }
+
 template <bool GRAD>
 int launch_logits(const LogitArgs& a, uint32_t rows, hipStream_t s) {
     if (rows <= kFewRows) {
-        loss_few_kernel<GRAD><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a);
+        if (few_tile(a.vocab) == TileFew::kA)
+            loss_few_kernel<TileFew, GRAD><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a);
+        else
+            loss_few_kernel<TileFewest, GRAD><<<blocks_for(div_up(a.here, TileFewest::kA)), kProductThreads, 0, s>>>(a);
     } else {
         uint32_t most = 0;  // blocks, for any number of rows that count
         for (uint32_t n = 64; n < rows + 64; n += 64) {
@@ -506,7 +514,7 @@ int forward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, h
     a.d = l->d, a.vocab = a.here = l->vocab, a.softcap = soft_cap(l->softcap), a.part = l->part, a.part_stride = g.rows;
     if (const int rc = launch_logits<false>(a, g.rows, s)) return rc;
     loss_join_kernel<<<div_up(g.rows, kJoinRows), kJoinThreads, 0, s>>>(
-        JoinArgs{l->r, l->part, div_up(l->vocab, g.rows <= kFewRows ? TileFew::kA : kVocabTile), g.rows, g.losses, g.lse_out});
+        JoinArgs{l->r, l->part, div_up(l->vocab, g.rows <= kFewRows ? few_tile(l->vocab) : kVocabTile), g.rows, g.losses, g.lse_out});
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -627,7 +635,7 @@ TWD_API int twd_headloss_create(uint32_t max_rows, uint32_t vocab, uint32_t d_mo
         take(l->r.hit, max_rows);
         take(l->r.h, static_cast<uint64_t>(max_rows) * d_model);
         const uint64_t many = static_cast<uint64_t>(div_up(vocab, kVocabTile)) * max_rows;
-        const uint64_t few = static_cast<uint64_t>(div_up(vocab, TileFew::kA)) * (max_rows < kFewRows ? max_rows : kFewRows);
+        const uint64_t few = static_cast<uint64_t>(div_up(vocab, few_tile(vocab))) * (max_rows < kFewRows ? max_rows : kFewRows);
         take(l->part, many > few ? many : few);
         if (!l->backward) return;
         take(l->dz, dz);
