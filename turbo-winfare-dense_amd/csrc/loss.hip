@@ -134,7 +134,8 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& a, uint32_t count, 
     const uint32_t v_tile = a.v0 + va * Tile::kA;
     Operand w = a.weight, h = a.hidden;  // the piece's rows, and those from m0 on
     w.p += a.v0 * w.stride, w.rows = a.here;
-    h.p += m0 * h.stride, h.rows = count - m0;
+    h.rows = count - m0;
+    if (m0 > 0) h.p += m0 * h.stride;
     f32x16_t acc[TA][TB];
     Tile::template sums<false>(s0, s1, s2, s3, sink, w, h, TileAt{va, 0, 0, share, who}, a.d, acc);
     const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, wa = wave / GB, wb = wave % GB;
@@ -263,11 +264,39 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
 }
 
 // Few rows: bound by the read of the weights.
-template <typename Tile, bool GRAD>
-__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_few_kernel(LogitArgs a) {
+template <typename Tile>
+__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_few_backward_kernel(LogitArgs a) {
     __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kPieces3];
     const uint32_t count = *a.r.count, tiles = (a.here + Tile::kA - 1) / Tile::kA, id = stretched(tiles);
-    if (id < tiles && count > 0) logits_tile<Tile, GRAD>(a, count, id, 0, 1, 0, s0, s1, s2, s3, nullptr);
+    if (id < tiles && count > 0) logits_tile<Tile, true>(a, count, id, 0, 1, 0, s0, s1, s2, s3, nullptr);
+}
+
+// The forward pass of few rows without a gathering before it: a row to a lane.
+template <typename Tile>
+__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_few_forward_kernel(LogitArgs a, GatherArgs g) {
+    static_assert(kFewRows <= 64, "a row to a lane");
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kPieces3];
+    __shared__ uint32_t places[64];
+    __shared__ int32_t targets[64];
+    const uint32_t r = threadIdx.x % 64;
+    const int32_t target = r < g.rows ? g.targets[r] : -1;
+    const uint64_t in = __ballot(static_cast<uint32_t>(target) < g.vocab);
+    const uint32_t count = static_cast<uint32_t>(__popcll(in)), m = static_cast<uint32_t>(__popcll(in & ((1ull << r) - 1)));
+    if (threadIdx.x < 64) {
+        const bool counts = (in >> r & 1) != 0;
+        if (counts) places[m] = r, targets[m] = target;
+        if (blockIdx.x == 0) {
+            if (counts) a.r.at[m] = r;
+            else if (r < g.rows) g.losses[r] = 0.0f, g.lse_out[r] = 0.0f;
+            if (r == 0) *a.r.count = count;
+        }
+    }
+    __syncthreads();
+    const uint32_t tiles = (a.here + Tile::kA - 1) / Tile::kA, id = stretched(tiles);
+    if (id >= tiles || count == 0) return;
+    a.r.target = targets;
+    a.hidden.places = places;
+    logits_tile<Tile, false>(a, count, id, 0, 1, 0, s0, s1, s2, s3, nullptr);
 }
 
 struct JoinArgs {
@@ -472,11 +501,13 @@ uint32_t few_tile(uint32_t vocab) { return vocab > 131072 ? TileFew::kA : TileFe
 
 template <bool GRAD>
 int launch_logits(const LogitArgs& a, uint32_t rows, hipStream_t s) {
-    if (rows <= kFewRows) {
-        if (few_tile(a.vocab) == TileFew::kA)
-            loss_few_kernel<TileFew, GRAD><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a);
-        else
-            loss_few_kernel<TileFewest, GRAD><<<blocks_for(div_up(a.here, TileFewest::kA)), kProductThreads, 0, s>>>(a);
+    if (GRAD && rows <= kFewRows) {
+        if constexpr (GRAD) {  // (the forward pass of few rows has a kernel of its own)
+            if (few_tile(a.vocab) == TileFew::kA)
+                loss_few_backward_kernel<TileFew><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a);
+            else
+                loss_few_backward_kernel<TileFewest><<<blocks_for(div_up(a.here, TileFewest::kA)), kProductThreads, 0, s>>>(a);
+        }
     } else {
         uint32_t most = 0;  // blocks, for any number of rows that count
         for (uint32_t n = 64; n < rows + 64; n += 64) {
@@ -508,11 +539,22 @@ int launch_gather(const twd_headloss* l, GatherArgs a, hipStream_t s) {
 }
 
 int forward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, hipStream_t s) {
-    if (const int rc = launch_gather(l, g, s)) return rc;
     LogitArgs a{};
     a.r = l->r, a.weight = weight, a.hidden = Operand{l->r.h, l->d, g.rows, l->d};
     a.d = l->d, a.vocab = a.here = l->vocab, a.softcap = soft_cap(l->softcap), a.part = l->part, a.part_stride = g.rows;
-    if (const int rc = launch_logits<false>(a, g.rows, s)) return rc;
+    if (g.rows <= kFewRows) {
+        a.hidden = Operand{g.hidden, g.rows > 1 ? g.stride : l->d, g.rows, l->d, nullptr, g.rows};
+        GatherArgs own = g;
+        own.vocab = l->vocab;
+        if (few_tile(l->vocab) == TileFew::kA)
+            loss_few_forward_kernel<TileFew><<<blocks_for(div_up(a.here, TileFew::kA)), kProductThreads, 0, s>>>(a, own);
+        else
+            loss_few_forward_kernel<TileFewest><<<blocks_for(div_up(a.here, TileFewest::kA)), kProductThreads, 0, s>>>(a, own);
+        TWD_HIP(hipGetLastError());
+    } else {
+        if (const int rc = launch_gather(l, g, s)) return rc;
+        if (const int rc = launch_logits<false>(a, g.rows, s)) return rc;
+    }
     loss_join_kernel<<<div_up(g.rows, kJoinRows), kJoinThreads, 0, s>>>(
         JoinArgs{l->r, l->part, div_up(l->vocab, g.rows <= kFewRows ? few_tile(l->vocab) : kVocabTile), g.rows, g.losses, g.lse_out});
     TWD_HIP(hipGetLastError());

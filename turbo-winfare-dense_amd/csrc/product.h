@@ -26,6 +26,9 @@ struct Operand {
     uint64_t stride;
     uint32_t rows;  // [a][k]: a; [k][a]: k
     uint32_t cols;  // [a][k]: k; [k][a]: a; a multiple of 8, as a load of 16 bytes lies inside the range or out of it
+    // [a][k]: where given, row a is row places[a] of `within`, which are at most 64
+    const uint32_t* places = nullptr;
+    uint32_t within = 0;
 };
 constexpr uint64_t kMaxProductStride = 1ull << 22;
 
@@ -86,11 +89,15 @@ struct ProductSide {
             // rows four apart (two, of 64 columns) read the same banks: those exchange their pieces
             column = 16 * (piece ^ (K == 64 ? lane / 16 : lane / 16 % 4));
 #pragma unroll
-            for (uint32_t j = 0; j < kLoads; ++j) off[j] = (kLines * (wave * kLoads + j) + in) * line + column_of(j);
-            const uint32_t here = min(x.rows - first, ROWS);
+            for (uint32_t j = 0; j < kLoads; ++j) off[j] = place_of(kLines * (wave * kLoads + j) + in) + column_of(j);
+            const uint32_t here = x.places ? x.within : min(x.rows - first, ROWS);
             rsrc = make_rsrc(x.p + first * x.stride, (here - 1) * line + 2 * x.cols);
             at = (32 * T * share + lane % 32) * (K / 8);
         }
+    }
+    __device__ __forceinline__ uint32_t place_of(uint32_t row) const {
+        static_assert(kMaxProductStride * 2 * 64 <= 1u << 29, "64 rows lie below a place that is out of every range");
+        return x.places ? (row < x.rows ? x.places[row] * line : 0x40000000u) : row * line;
     }
     __device__ __forceinline__ uint32_t column_of(uint32_t j) const { return K == 64 && j % 2 ? column ^ 64 : column; }
     // Loads from .. last - 1 of a stage into its buffer.
