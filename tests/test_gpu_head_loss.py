@@ -207,6 +207,46 @@ def test_extreme_logits():
     loss.close()
 
 
+@pytest.mark.parametrize("rows", [5, 100])
+def test_logits_below_fp32(rows):
+    """Whole tiles of logits that are minus infinity have no part in a row's sum, as vocabulary rows that are not there."""
+    import torch
+    t = twd()
+    vocab, d, low = 700, 64, 300
+    h, w, targets, grad = make(vocab - low, d, rows, 0, 31)
+    h = h.abs() + 0.5
+    want, tol = reference(h, w, targets, 0.0, grad)
+    all_w = torch.cat([torch.full((low, d), -3e38, dtype=torch.bfloat16, device="cuda:0"), w])
+    loss = t.HeadLoss(rows, vocab, d)
+    losses, lse = loss.forward(h, all_w, targets + low)
+    check("lse", lse, want["lse"], tol["lse"], U)
+    check("losses", losses, want["losses"], tol["losses"], U)
+    d_hidden, d_weight = loss.backward(h, all_w, targets + low, lse, grad=grad)
+    check("d_hidden", d_hidden, want["d_hidden"], tol["d_hidden"], U16)
+    check("d_weight", d_weight[low:], want["d_weight"], tol["d_weight"], U16)
+    assert (d_weight[:low] == 0).all()
+
+
+def test_stride_of_a_single_row_plays_no_part():
+    import torch
+    t = twd()
+    d = 96
+    h, w, targets, grad = make(1, d, 1, 0, 5)
+    loss = t.HeadLoss(1, 1, d)
+    losses, lse = loss.forward(h, w, targets)
+    want = (losses, lse, *loss.backward(h, w, targets, lse, grad=grad))
+    for n in (0, 13, 2 ** 40):
+        got = [torch.full_like(x, float("nan")) for x in want]
+        p = [x.data_ptr() for x in got]
+        torch.cuda.synchronize()
+        assert t.lib.twd_headloss_forward(loss.handle, h.data_ptr(), 1, n, w.data_ptr(), n, targets.data_ptr(), p[0],
+                                          p[1], None) == t.TWD_OK
+        assert t.lib.twd_headloss_backward(loss.handle, h.data_ptr(), 1, n, w.data_ptr(), n, targets.data_ptr(), p[1],
+                                           grad.data_ptr(), p[2], n, p[3], 1, n, 0, None) == t.TWD_OK
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 def test_gradient_by_differences():
     """d_weight against central differences of the losses themselves. One logit of a row changes by delta h: the third
     derivative of the loss by it is p (1 - p) (1 - 2 p), at most 0.0963, so the difference is off by delta^2 |h|^3 0.0963 / 6 a

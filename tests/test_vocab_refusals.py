@@ -35,6 +35,7 @@ def test_head_loss_refusals():
         refused(create(rows, 100, 32, 0.0, 1, C.byref(h)), inv, "max_rows")
     for v in (0, (1 << 24) + 1):
         refused(create(4, v, 32, 0.0, 1, C.byref(h)), inv, "vocab")
+    refused(create(65536, (1 << 22) + 1, 32, 0.0, 1, C.byref(h)), inv, "2^38")
     for d in (0, 16, 40, (1 << 20) + 32):
         refused(create(4, 100, d, 0.0, 1, C.byref(h)), inv, "d_model")
     for cap in (-1.0, float("nan"), float("inf"), 1e-31, 1e31):

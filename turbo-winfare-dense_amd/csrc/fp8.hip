@@ -636,7 +636,7 @@ int launch_logits(const twd_fp8head* h, const Fp8Args& a, hipStream_t s) {
     } else {
         if (a.rows <= 128) return launch_tile<4, Out>(a, s);
         const uint64_t tiles = static_cast<uint64_t>((a.groups + 3) / 4) * ((a.rows + 255) / 256);
-        if (tiles > 0x7FFFFFull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
+        if (tiles > 0x7FFFF8ull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
         fp8_wide_kernel<Out><<<blocks_for(static_cast<uint32_t>(tiles)), kWideThreads, 0, s>>>(a);
         TWD_HIP(hipGetLastError());
         return TWD_OK;
