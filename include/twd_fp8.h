@@ -36,9 +36,11 @@ TWD_API void twd_fp8head_destroy(twd_fp8head* head);
 TWD_API int twd_fp8head_info(const twd_fp8head* head, uint32_t* vocab, uint32_t* d_model, float* softcap,
                              uint64_t* device_bytes);
 /* logits[m][v] = softcap(sum_c w[v][c] h[m][c]) of 1 to 65,536 hidden rows held in the format too (twd_fp8_quantize with
- * block_rows 1: codes [rows][d_model], scales [rows][d_model / 128]), each 128 columns' products summed on 8-bit matrix
- * instructions and added up in fp32; logits_type TWD_F32 or TWD_BF16 with logits_stride >= vocab elements between rows. A
- * row with a NaN scale gives NaN logits. The call keeps no state: calls on one head may overlap, on any streams, and may be
+ * block_rows 1: codes [rows][d_model], scales [rows][d_model / 128]), each 128 columns' products summed on matrix
+ * instructions and the sums, times their scales, added up in fp32; logits_type TWD_F32 or TWD_BF16 with logits_stride >=
+ * vocab elements between rows. The products are exact and added in fp32, but for bf16 logits of more than 128 rows: those run
+ * on 8-bit instructions, which cut the products of eight neighbouring columns at 2^-13 of the largest of the eight (2e-5 of
+ * sum |w h| for normal products). A row with a NaN scale gives NaN logits. The call keeps no state: calls on one head may overlap, on any streams, and may be
  * captured. Asynchronous on `stream`. */
 TWD_API int twd_fp8head_logits(const twd_fp8head* head, const uint8_t* codes, const float* scales, uint32_t rows,
                                void* logits, int logits_type, uint64_t logits_stride, void* stream);

@@ -1,9 +1,12 @@
 """8-bit floating point with a scale for each block of 128: the format bit for bit, and the head's logits against the
 definition in 64 bits.
 
-The matrix instructions add 128 products; a partial sum is at most their magnitudes' sum, and is rounded or truncated 128
+The matrix instructions add 128 products of elements widened to bf16, which are exact; a partial sum is at most their magnitudes' sum, and is rounded or truncated 128
 times, then once for the product with the scales' own rounded product and once where it is added to the others: the bound is
-(130 + 2 + d / 128) 2^-23 sum |w h|, 4 2^-24 |y| for the softcap, and half a step of the output's type. Small integers under
+(130 + 2 + d / 128) 2^-23 sum |w h|, 4 2^-24 |y| for the softcap, and half a step of the output's type. bf16 logits of more
+than 128 rows come from the 8-bit instructions, which align the products of eight neighbouring columns to the largest of them
+and cut them at 2^-13 of it: that takes less than 7 2^-13 of the largest from the other seven, so 7 2^-13 sum |w h| in all
+(the largest, of seven bits, is not cut). Small integers under
 scales that are powers of two are exact in any order and checked bit for bit."""
 import numpy as np
 import pytest
@@ -140,10 +143,35 @@ def test_normal_rows(vocab, d, rows, cap, out_type):
     head.logits(h, out=out)
     z = hv @ wv.T
     want = cap * np.tanh(z / cap) if cap > 0 else z
-    tol = (132 + d // 128) * 2.0 ** -23 * (np.abs(hv) @ np.abs(wv).T) + 4 * 2.0 ** -24 * np.abs(want)
+    cut = 7 * 2.0 ** -13 if out_type == "bfloat16" and rows > 128 else 0.0
+    tol = (cut + (132 + d // 128) * 2.0 ** -23) * (np.abs(hv) @ np.abs(wv).T) + 4 * 2.0 ** -24 * np.abs(want)
     if out_type == "bfloat16":
         tol += 2.0 ** -8 * (np.abs(want) + tol)
     assert (np.abs(out.double().cpu().numpy() - want) <= tol).all()
+    head.close()
+
+
+@pytest.mark.parametrize("rows", [1, 16, 17, 33, 128, 129, 300])
+@pytest.mark.parametrize("out_type", ["float32", "bfloat16"])
+@pytest.mark.parametrize("others", [2.0 ** -10, 2.0 ** -3, 4.0, 8.0])
+def test_small_products_beside_large_ones(rows, out_type, others):
+    """127 products beside one of 2^16 that another block takes away again: the fp32 sums hold them to 2^-7 each (half a
+    step of 2^16, in the sum of whichever they are added to), the 8-bit instructions to 2^3."""
+    import torch
+    t = twd()
+    vocab, d = 70, 256
+    w, h = torch.zeros(vocab, d), torch.zeros(rows, d)
+    w[:, 0], w[:, 128], h[:, 0], h[:, 128] = 256, -256, 256, 256
+    w[:, 1:128], h[:, 1:128] = max(others / 8, 2.0 ** -8), min(others / 2.0 ** -8, 8.0)
+    head = t.Fp8Head(w.to(torch.float8_e4m3fn).cuda(), torch.ones(1, 2, device="cuda:0"))
+    out = torch.empty(rows, vocab, dtype=getattr(torch, out_type), device="cuda:0")
+    head.logits_fp8(h.to(torch.float8_e4m3fn).view(torch.uint8).cuda(), torch.ones(rows, 2, device="cuda:0"), out=out)
+    want = 127 * others
+    cut = out_type == "bfloat16" and rows > 128
+    tol = 7 * 2.0 ** 3 + 2.0 if cut else 127 * 2.0 ** -7
+    if out_type == "bfloat16":
+        tol += 2.0 ** -8 * (want + tol)
+    assert (out.double() - want).abs().max() <= tol
     head.close()
 
 

@@ -1,8 +1,10 @@
 // 8-bit floating point with a scale for each block of 128: rows and weights to the format, and the LM head's product with
 // weights held in it.
 //
+//   code(x) = e4m3(x / s), s = max |x| / 448 of the block    y_mv = softcap(sum_b s_mb s_vb sum_{c in b} w_vc h_mc)
+//
 // An element is an e4m3 code; hidden rows have an fp32 scale for each 128 columns, weights one for each 128 x 128. The product
-// of 128 columns runs on the 8-bit matrix instructions, whose sums are then multiplied by the two scales and added up in fp32.
+// of 128 columns runs on matrix instructions, whose sums are then multiplied by the two scales and added up in fp32.
 #include <hip/hip_runtime.h>
 
 #include <new>
@@ -163,10 +165,12 @@ __device__ __forceinline__ i32x8_t operand(u32x4_t lo, u32x4_t hi) {
     return __builtin_bit_cast(i32x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
 }
 
-// The 8-bit matrix instructions align a step's products to the largest of them before they add, which costs some of the
-// bits: sums of 128 normal products are off by 1.4e-5 of their spread (in bf16, exact products added in fp32: 1e-8). That is
-// far inside a bf16 logit's half step, 2^-8 of itself, and is taken there; for fp32 logits both operands are widened to bf16,
-// which holds every e4m3 value, and multiplied at half the rate. Eight elements of two words:
+// The 8-bit matrix instructions align the products of eight neighbouring columns to the largest of them and cut them at 2^-13
+// of it (seen with one product of 2^16 beside others: those below 2^3 are lost in its eight, kept to 2^-10 elsewhere); for
+// normal products that is 2e-5 of their magnitudes' sum. bf16 logits of many rows, whose own half step is 2^-8, are computed
+// so, at twice the rate. All others widen both operands to bf16, which holds every e4m3 value: exact products, added in fp32.
+// Up to 128 rows that costs little, as the read bounds them (64 rows of 262,144 x 5,376 to bf16: 246 us cut, 267 widened).
+// Eight elements of two words:
 __device__ __forceinline__ bf16x8_t widened(uint32_t lo, uint32_t hi) {
     u32x4_t e;
     e[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.0f, false));
@@ -190,7 +194,7 @@ __device__ __forceinline__ Wide32 widened(i32x8_t v) {
 // Bound by the read of the head. The waves of a block split d_model by quads of chunks; a wave keeps its quad of the hidden
 // rows in registers and streams its quad of one group after another, kAhead chunks (8 KB each) ahead of the arithmetic. The
 // sums over the quads meet in LDS, two buffers in turn.
-constexpr uint32_t kSmallRows = 16;
+constexpr uint32_t kSmallRows = 16, kExactRows = 128;
 constexpr uint32_t kSmallWaves = 12;
 constexpr uint32_t kAhead = 2;
 
@@ -375,44 +379,27 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
         __builtin_amdgcn_sched_barrier(0);
         if (have_group) {
             Wide32 e[2][2];
-            if constexpr (sizeof(Out) == 4) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int s = 0; s < 2; ++s) e[j][s] = widened(operand(w[4 * j + 2 * s], w[4 * j + 2 * s + 1]));
-            }
+                for (int s = 0; s < 2; ++s) e[j][s] = widened(operand(w[4 * j + 2 * s], w[4 * j + 2 * s + 1]));
 #pragma unroll
             for (int n = 0; n < NS; ++n) {
-                i32x8_t y[2];
+                f32x16_t sum[2] = {};
 #pragma unroll
                 for (int s = 0; s < 2; ++s) {
                     const uint32_t row = 32 * n + r, p = 2 * (2 * s + h);
-                    y[s] = operand(x[row * 8 + (p ^ (r / 2 % 8))], x[row * 8 + ((p + 1) ^ (r / 2 % 8))]);
-                }
-                const float f = xs[n] * ws;
-                if constexpr (sizeof(Out) == 4) {
-                    f32x16_t sum[2] = {};
-#pragma unroll
-                    for (int s = 0; s < 2; ++s) {
-                        const Wide32 z = widened(y[s]);
-#pragma unroll
-                        for (int j = 0; j < 2; ++j)
-#pragma unroll
-                            for (int t = 0; t < 4; ++t) sum[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e[j][s].e[t], z.e[t], sum[j], 0, 0, 0);
-                    }
+                    const Wide32 z = widened(operand(x[row * 8 + (p ^ (r / 2 % 8))], x[row * 8 + ((p + 1) ^ (r / 2 % 8))]));
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) acc[j][n][i] = fmaf(sum[j][i], f, acc[j][n][i]);
-                    continue;
+                        for (int t = 0; t < 4; ++t) sum[j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(e[j][s].e[t], z.e[t], sum[j], 0, 0, 0);
                 }
+                const float f = xs[n] * ws;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    f32x16_t sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w[4 * j], w[4 * j + 1]), y[0], f32x16_t{}, 0, 0, 0, 0, 0, 0);
-                    sum = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(w[4 * j + 2], w[4 * j + 3]), y[1], sum, 0, 0, 0, 0, 0, 0);
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) acc[j][n][i] = fmaf(sum[i], f, acc[j][n][i]);
-                }
+                    for (int i = 0; i < 16; ++i) acc[j][n][i] = fmaf(sum[j][i], f, acc[j][n][i]);
             }
         }
         turn_over();
@@ -630,11 +617,10 @@ int launch_logits(const twd_fp8head* h, const Fp8Args& a, hipStream_t s) {
         return TWD_OK;
     }
     if (a.rows <= 32) return launch_tile<1, Out>(a, s);
-    if (a.rows <= 64) return launch_tile<2, Out>(a, s);
     if constexpr (sizeof(Out) == 4) {
-        return launch_tile<2, Out>(a, s);  // widened, 128 rows leave no registers
+        return launch_tile<2, Out>(a, s);
     } else {
-        if (a.rows <= 128) return launch_tile<4, Out>(a, s);
+        if (a.rows <= kExactRows) return launch_tile<2, Out>(a, s);
         const uint64_t tiles = static_cast<uint64_t>((a.groups + 3) / 4) * ((a.rows + 255) / 256);
         if (tiles > 0x7FFFF8ull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
         fp8_wide_kernel<Out><<<blocks_for(static_cast<uint32_t>(tiles)), kWideThreads, 0, s>>>(a);
