@@ -90,7 +90,7 @@ struct LogitArgs {
     uint32_t part_stride, dz_stride;
 };
 
-// By rows, or with the second operand turned.
+// Logits: both operands by rows. d_hidden: the weights turned. d_weight: dz and the hidden rows turned.
 using TileFew = ProductTile<1, 2, 4, 1, 64, 3, false, false>;
 using TileFewest = ProductTile<1, 1, 2, 2, 64, 4, false, false>;  // 64 vocabulary rows
 using TileWide = ProductTile<4, 4, 2, 2, 64, 2, false, false, true>;
@@ -235,6 +235,11 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& a, uint32_t count, 
     }
 }
 
+// One block to a unit, whose waves hold 256 sums a lane each: the widest tile reads least through LDS. 2,048 rows of 262,144 x
+// 5,376 with a softcap take 4.75 ms, 1,215 TFLOP/s (a plain library product of the same rows 1,333): the matrix units are busy
+// in 68% of the cycles, at the clock of some 1.6 GHz that the power leaves, the rest being a tile's first loads and its
+// epilogue, which nothing covers. Tiles of 256 x 128 with two blocks to a unit, one's epilogue beside the other's products,
+// took 6.06 ms where these took 4.90 (32,003 x 2,048 of 777 rows: 145 and 152 us). With dz stored, a piece of 65,536: 1.26 ms.
 template <bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_logits_kernel(LogitArgs a) {
     __shared__ u32x4_t s0[TileWide::kPieces], s1[TileWide::kPieces];
@@ -250,6 +255,8 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     else logits_tile<TileTwo, GRAD>(a, count, at.a, m0, at.share, at.who, s0, s1, nullptr, nullptr, sink);
 }
 
+// The last tiles, a stripe of 64 hidden rows to a block. Bound by its own chain of stages: 16 stripes of 2,880 columns 29 us,
+// as a round of whole tiles takes 95; no tiles to cut, 5 us.
 template <bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_stripes_kernel(LogitArgs a) {
     using Tile = TileStripe;
@@ -264,7 +271,9 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     if (m0 < count) logits_tile<Tile, GRAD>(a, count, at.a, m0, each, id % each, s0, s1, s2, nullptr, sink);
 }
 
-// Few rows: bound by the read of the weights.
+// Up to 64 rows: bound by the read of the weights, so no tile has more hidden rows than those. 17 rows of 262,144 x 5,376 take
+// 496 us forward (5.7 TB/s; a pure read reaches 6.7), 32,003 x 1,024 14 us (4.6 TB/s: the way to a block's first
+// products).
 template <typename Tile>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_few_backward_kernel(LogitArgs a) {
     __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kPieces3];
@@ -308,7 +317,8 @@ struct JoinArgs {
     float* lse;
 };
 
-// The tiles' parts of sixteen rows, 64 tiles at a time; the sum of a row's exponentials in 64 bits.
+// The tiles' parts of sixteen rows, 64 tiles at a time; the sum of a row's exponentials in 64 bits. Little to read (2,048 rows
+// of 1,024 tiles: 17 MB in 13 us), small calls are a chain of loads, exchanges and two logarithms: 5 us.
 constexpr uint32_t kJoinRows = 16, kJoinThreads = 1024;
 
 __global__ __launch_bounds__(kJoinThreads) void loss_join_kernel(JoinArgs a) {
@@ -372,7 +382,10 @@ __device__ __forceinline__ void add4(uint16_t* p, f32x4_t v) {
     *reinterpret_cast<u32x2_t*>(p) = u32x2_t{bf16_pair(v[0] + bf16_lo(w[0]), v[1] + bf16_hi(w[0])), bf16_pair(v[2] + bf16_lo(w[1]), v[3] + bf16_hi(w[1]))};
 }
 
-// d_weight = dz^T H (BY_COUNT: k runs over the rows that count) or a piece's part of d_hidden = dz W.
+// d_weight = dz^T H (BY_COUNT: k runs over the rows that count) or a piece's part of d_hidden = dz W. For 2,048 rows of 65,536
+// x 5,376 1.26 and 1.22 ms: 1,144 and 1,185 TFLOP/s, where the library's products with these operands reach 1,034 and 727.
+// d_weight has no room to wait for its stores, nor few tiles: two blocks to a unit cover each other's. d_hidden has a long sum
+// and few tiles: one large tile a unit, the sum in parts.
 template <typename Tile, typename Out, bool BY_COUNT>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_grad_kernel(GradArgs a) {
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GB = Tile::kGB;
@@ -439,7 +452,8 @@ struct SpreadArgs {
     uint64_t stride;
 };
 
-// d_hidden's parts added up, in the caller's rows; zeros where a row is left out.
+// d_hidden's parts added up, in the caller's rows; zeros where a row is left out. Bound by the read of the parts: 2,048 rows
+// of 5,376 in three parts 30 us, 5.1 TB/s.
 __global__ __launch_bounds__(256) void loss_spread_kernel(SpreadArgs a) {
     const uint32_t c = (blockIdx.y * 256 + threadIdx.x) * 8, b = blockIdx.x;
     if (c >= a.d) return;
