@@ -125,6 +125,26 @@ def test_exact_sums(vocab, d, rows):
     head.close()
 
 
+@pytest.mark.parametrize("rows", [17, 32, 33])
+def test_exact_sums_of_a_head_past_the_memory_cache(rows):
+    import torch
+    t = twd()
+    vocab, d = 70001, 3968
+    g = torch.Generator(device="cuda:0").manual_seed(rows)
+    w = torch.randint(-8, 9, (vocab, d), generator=g, device="cuda:0").half()
+    h = torch.randint(-8, 9, (rows, d), generator=g, device="cuda:0").half()
+    ws = torch.exp2(torch.randint(-2, 3, ((vocab + 127) // 128, d // 128), generator=g, device="cuda:0").float())
+    hs = torch.exp2(torch.randint(-2, 3, (rows, d // 128), generator=g, device="cuda:0").float())
+    head = t.Fp8Head(w.to(torch.float8_e4m3fn), ws)
+    got = head.logits_fp8(h.to(torch.float8_e4m3fn).view(torch.uint8), hs)
+    want = torch.zeros(rows, vocab, dtype=torch.float64, device="cuda:0")
+    for c in range(d // 128):
+        part = h[:, 128 * c:128 * c + 128].double() @ w[:, 128 * c:128 * c + 128].double().t().contiguous()
+        want += part * hs[:, c:c + 1].double() * ws[:, c].double().repeat_interleave(128)[:vocab]
+    assert torch.equal(got.double(), want)
+    head.close()
+
+
 @pytest.mark.parametrize("vocab,d,rows,cap", [(2003, 5376, 1, 30.0), (1000, 2048, 5, 30.0), (513, 5376, 16, 0.0), (600, 3584, 48, 30.0),
                                               (260, 2944, 200, 50.0)])
 @pytest.mark.parametrize("out_type", ["float32", "bfloat16"])

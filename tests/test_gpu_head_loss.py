@@ -18,6 +18,7 @@ SHAPES = [  # vocab, d_model, rows, softcap
     (1, 32, 1, 0.0), (5, 32, 3, 30.0), (257, 96, 2, 0.0), (1000, 160, 64, 30.0), (1003, 1056, 65, 0.0),
     (777, 2880, 129, 30.0), (4099, 512, 300, 50.0), (300, 544, 600, 0.0), (256, 128, 128, 0.0), (2049, 64, 257, 5.0),
     (40001, 64, 40, 30.0), (131075, 32, 1030, 0.0), (515, 5376, 17, 30.0),
+    (131075, 64, 33, 30.0), (40961, 96, 100, 0.0), (2000, 352, 128, 30.0), (70001, 1984, 128, 30.0), (70001, 1984, 21, 0.0),
 ]
 
 

@@ -311,7 +311,7 @@ __global__ __launch_bounds__(kSmallWaves * 64) void fp8_small_kernel(Fp8Args a) 
 // rows stay here, bound by the products: 2,047 rows 5.56 ms, 1,038 TFLOP/s.
 constexpr uint32_t kTileWaves = 4;
 
-template <int NS, typename Out>
+template <int NS, typename Out, bool STREAMED>
 __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu(2))) void fp8_tile_kernel(Fp8Args a) {
     constexpr uint32_t kRows = 32 * NS;
     constexpr uint32_t kStage = kRows * 8;  // 16-byte pieces
@@ -355,7 +355,7 @@ __global__ __launch_bounds__(kTileWaves * 64) __attribute__((amdgpu_waves_per_eu
             for (int s = 0; s < 2; ++s)
 #pragma unroll
                 for (int half = 0; half < 2; ++half)
-                    wn[4 * j + 2 * s + half] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(codes, w_off + 4096 * j + 512 * s + 1024 * half, at, 0));
+                    wn[4 * j + 2 * s + half] = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(codes, w_off + 4096 * j + 512 * s + 1024 * half, at, STREAMED ? kStreamed : 0));
     };
     const float* xs_at[NS];
 #pragma unroll
@@ -607,12 +607,12 @@ namespace twd {
 
 namespace {
 
-template <int NS, typename Out>
+template <int NS, typename Out, bool STREAMED = false>
 int launch_tile(const Fp8Args& a, hipStream_t s) {
     const uint32_t row_tiles = (a.rows + 32 * NS - 1) / (32 * NS), stretches = (a.groups + kTileWaves - 1) / kTileWaves;
     const uint64_t blocks = static_cast<uint64_t>((stretches + 7) / 8) * 8 * row_tiles;
     if (blocks > 0xFFFFFFull) return fail(TWD_E_INVALID, "rows x vocab is too large for one call");
-    fp8_tile_kernel<NS, Out><<<static_cast<uint32_t>(blocks), kTileWaves * 64, 0, s>>>(a);
+    fp8_tile_kernel<NS, Out, STREAMED><<<static_cast<uint32_t>(blocks), kTileWaves * 64, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -626,7 +626,10 @@ int launch_logits(const twd_fp8head* h, const Fp8Args& a, hipStream_t s) {
         TWD_HIP(hipGetLastError());
         return TWD_OK;
     }
-    if (a.rows <= 32) return launch_tile<1, Out>(a, s);
+    // up to 32 rows the weights past the memory's cache are streamed (24 rows of 151,669 x 3,584: 107 us, otherwise 116; of
+    // 32,003 x 2,048, which it holds: 24 and 20); tiles of 64 rows gain nothing (262,144 x 5,376: 290 and 285)
+    const bool streamed = static_cast<uint64_t>(a.vocab) * a.d > kMemoryCache;
+    if (a.rows <= 32) return streamed ? launch_tile<1, Out, true>(a, s) : launch_tile<1, Out>(a, s);
     if constexpr (sizeof(Out) == 4) {
         return launch_tile<2, Out>(a, s);
     } else {

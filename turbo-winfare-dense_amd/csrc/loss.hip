@@ -91,8 +91,12 @@ struct LogitArgs {
 };
 
 // Logits: both operands by rows. d_hidden: the weights turned. d_weight: dz and the hidden rows turned.
-using TileFew = ProductTile<1, 2, 4, 1, 64, 3, false, false>;
-using TileFewest = ProductTile<1, 1, 2, 2, 64, 4, false, false>;  // 64 vocabulary rows
+using TileFew = ProductTile<1, 2, 4, 1, 64, 3, false, false, false, true>;
+template <bool STREAMED>
+using TileFewest = ProductTile<1, 1, 2, 2, 64, 4, false, false, false, STREAMED>;  // 64 vocabulary rows
+template <bool STREAMED>
+using TileMid = ProductTile<4, 2, 2, 2, 64, 3, false, false, false, STREAMED>;  // 128 hidden rows
+using TileMidSmall = ProductTile<2, 2, 2, 2, 64, 4, false, false>;              // and 128 vocabulary rows
 using TileWide = ProductTile<4, 4, 2, 2, 64, 2, false, false, true>;
 using TileThree = ProductTile<4, 3, 2, 2, 64, 2, false, false, true>;
 using TileTwo = ProductTile<4, 2, 2, 2, 64, 2, false, false, true>;
@@ -104,7 +108,7 @@ using TileWeight = ProductTile<4, 2, 2, 2, 32, 3, true, true>;
 // units times a tile's, which goes by its width and some 100 rows more (65,536 x 2,880: 105, 86 and 65 us a round). 518 rows
 // of 32,003 x 2,048 take 139, 113 and 124 us, 1,023 of 65,537 x 2,880 take 427, 476 and 476. The few tiles past whole rounds
 // are cut into stripes of 64 hidden rows and follow in a launch of their own, which costs some 80 rows of a round.
-constexpr uint32_t kVocabTile = 256, kRound = 256, kMostCut = 64, kFewRows = 64;
+constexpr uint32_t kVocabTile = 256, kRound = 256, kMostCut = 64, kFewRows = 64, kMidRows = 128;
 static_assert(TileWide::kA == kVocabTile && TileThree::kA == kVocabTile && TileTwo::kA == kVocabTile && TileStripe::kA == kVocabTile, "one width");
 struct LogitTiles {
     TileGrid grid;
@@ -271,14 +275,15 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
     if (m0 < count) logits_tile<Tile, GRAD>(a, count, at.a, m0, each, id % each, s0, s1, s2, nullptr, sink);
 }
 
-// Up to 64 rows: bound by the read of the weights, so no tile has more hidden rows than those. 17 rows of 262,144 x 5,376 take
-// 496 us forward (5.7 TB/s; a pure read reaches 6.7), 32,003 x 1,024 14 us (4.6 TB/s: the way to a block's first
-// products).
-template <typename Tile>
-__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void loss_few_backward_kernel(LogitArgs a) {
-    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces], s3[Tile::kPieces3];
+// Up to 128 rows: bound by the read of the weights, so a tile has all of the rows. 17 rows of 262,144 x 5,376 take 440 us
+// forward (6.4 TB/s; a pure read reaches 6.7), 128 rows 491 (5.7), 17 of 32,003 x 1,024 14 us (4.6 TB/s: the way to a block's
+// first products).
+template <typename Tile, bool GRAD>
+__global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>)))
+void loss_few_kernel(LogitArgs a) {
+    __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
     const uint32_t count = *a.r.count, tiles = (a.here + Tile::kA - 1) / Tile::kA, id = stretched(tiles);
-    if (id < tiles && count > 0) logits_tile<Tile, true>(a, count, id, 0, 1, 0, s0, s1, s2, s3, nullptr);
+    if (id < tiles && count > 0) logits_tile<Tile, GRAD>(a, count, id, 0, 1, 0, s0, s1, s2, s3, nullptr);
 }
 
 // The forward pass of few rows without a gathering before it: a row to a lane.
@@ -512,34 +517,51 @@ namespace twd {
 
 namespace {
 
-// Vocabulary rows of a tile of few rows: small ones where large ones would not fill the units for two rounds (17 rows of
-// 100,000 x 2,048: 92 and 109 us; of 151,669 x 3,584: 209 and 198).
-uint32_t few_tile(uint32_t vocab) { return vocab > 131072 ? TileFew::kA : TileFewest::kA; }
+// Up to 128 rows have tiles of all of them, so the weights are read once. f(tile): small tiles where large ones would leave
+// units idle or not fill them for two rounds (17 rows of 100,000 x 2,048: 92 and 109 us; of 151,669 x 3,584: 209 and 198; 128
+// rows of 32,003 x 1,024: 27 and 37; of 50,000 x 4,096: 121 and 109). Weights past the memory's cache are streamed (17 rows of
+// 65,537 x 2,880: 84 us, otherwise 91; of 32,003 x 2,048, which it holds: 37 and 30), those of large tiles always, as such
+// heads seldom fit, those of the smallest heads never.
+template <typename F>
+auto with_few_tile(uint32_t rows, uint32_t vocab, uint32_t d, F&& f) {
+    const bool streamed = 2ull * vocab * d > kMemoryCache;
+    if (rows <= kFewRows) {
+        if (vocab > 131072) return f(TileFew{});
+        return streamed ? f(TileFewest<true>{}) : f(TileFewest<false>{});
+    }
+    if (vocab <= 40960) return f(TileMidSmall{});
+    return streamed ? f(TileMid<true>{}) : f(TileMid<false>{});
+}
+// Vocabulary rows of a tile of the forward pass.
+uint32_t vocab_tile(uint32_t rows, uint32_t vocab, uint32_t d) {
+    return rows > kMidRows ? kVocabTile : with_few_tile(rows, vocab, d, [](auto tile) { return decltype(tile)::kA; });
+}
 
-// `g`: forward; without it, backward.
-int launch_few(const LogitArgs& a, const GatherArgs* g, hipStream_t s) {
-    auto go = [&](auto tile) {
+// `g`: forward of so few rows that the tiles gather by themselves.
+template <bool GRAD>
+int launch_few(const LogitArgs& a, uint32_t rows, const GatherArgs* g, hipStream_t s) {
+    return with_few_tile(rows, a.vocab, a.d, [&](auto tile) -> int {
         using Tile = decltype(tile);
         const uint32_t blocks = blocks_for(div_up(a.here, Tile::kA));
-        if (g) loss_few_forward_kernel<Tile><<<blocks, kProductThreads, 0, s>>>(a, *g);
-        else loss_few_backward_kernel<Tile><<<blocks, kProductThreads, 0, s>>>(a);
-    };
-    if (few_tile(a.vocab) == TileFew::kA) go(TileFew{});
-    else go(TileFewest{});
-    TWD_HIP(hipGetLastError());
-    return TWD_OK;
+        if constexpr (!GRAD && Tile::kB <= kFewRows) loss_few_forward_kernel<Tile><<<blocks, kProductThreads, 0, s>>>(a, *g);
+        else loss_few_kernel<Tile, GRAD><<<blocks, kProductThreads, 0, s>>>(a);
+        TWD_HIP(hipGetLastError());
+        return TWD_OK;
+    });
 }
 
 template <bool GRAD>
 int launch_logits(const LogitArgs& a, uint32_t rows, hipStream_t s) {
-    uint32_t most = 0;  // blocks, for any number of rows that count
+    uint32_t most = 0, cut = 0;  // blocks, for any number of rows that count
     for (uint32_t n = 64; n < rows + 64; n += 64) {
-        const uint32_t tiles = logit_tiles(n < rows ? n : rows, div_up(a.here, kVocabTile)).grid.tiles();
-        most = tiles > most ? tiles : most;
+        const LogitTiles t = logit_tiles(n < rows ? n : rows, div_up(a.here, kVocabTile));
+        most = t.grid.tiles() > most ? t.grid.tiles() : most;
+        cut = t.cut > cut ? t.cut : cut;
     }
     loss_logits_kernel<GRAD><<<blocks_for(most), kProductThreads, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
-    loss_stripes_kernel<GRAD><<<4 * kMostCut, kProductThreads, 0, s>>>(a);
+    if (cut == 0) return TWD_OK;
+    loss_stripes_kernel<GRAD><<<blocks_for(4 * cut), kProductThreads, 0, s>>>(a);
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -564,17 +586,19 @@ int forward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, h
     LogitArgs a{};
     a.r = l->r, a.weight = weight, a.hidden = Operand{l->r.h, l->d, g.rows, l->d};
     a.d = l->d, a.vocab = a.here = l->vocab, a.softcap = soft_cap(l->softcap), a.part = l->part, a.part_stride = g.rows;
+    int rc;
     if (g.rows <= kFewRows) {
         a.hidden = Operand{g.hidden, g.rows > 1 ? g.stride : l->d, g.rows, l->d, nullptr, g.rows};
         GatherArgs own = g;
         own.vocab = l->vocab;
-        if (const int rc = launch_few(a, &own, s)) return rc;
+        rc = launch_few<false>(a, g.rows, &own, s);
     } else {
-        if (const int rc = launch_gather(l, g, s)) return rc;
-        if (const int rc = launch_logits<false>(a, g.rows, s)) return rc;
+        if ((rc = launch_gather(l, g, s))) return rc;
+        rc = g.rows <= kMidRows ? launch_few<false>(a, g.rows, nullptr, s) : launch_logits<false>(a, g.rows, s);
     }
+    if (rc) return rc;
     loss_join_kernel<<<div_up(g.rows, kJoinRows), kJoinThreads, 0, s>>>(
-        JoinArgs{l->r, l->part, div_up(l->vocab, g.rows <= kFewRows ? few_tile(l->vocab) : kVocabTile), g.rows, g.losses, g.lse_out});
+        JoinArgs{l->r, l->part, div_up(l->vocab, vocab_tile(g.rows, l->vocab, l->d)), g.rows, g.losses, g.lse_out});
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -603,7 +627,7 @@ int backward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, 
         LogitArgs a{};
         a.r = l->r, a.weight = weight, a.hidden = h;
         a.d = l->d, a.vocab = l->vocab, a.v0 = v0, a.here = here, a.softcap = soft_cap(l->softcap), a.dz = l->dz, a.dz_stride = piece;
-        if ((rc = g.rows <= kFewRows ? launch_few(a, nullptr, s) : launch_logits<true>(a, g.rows, s))) return rc;
+        if ((rc = g.rows <= kMidRows ? launch_few<true>(a, g.rows, nullptr, s) : launch_logits<true>(a, g.rows, s))) return rc;
         if (o.d_weight) {
             GradArgs b{};
             b.count = l->r.count, b.a = Operand{l->dz, piece, g.rows, piece}, b.b = h;
@@ -699,9 +723,13 @@ TWD_API int twd_headloss_create(uint32_t max_rows, uint32_t vocab, uint32_t d_mo
         take(l->r.lse, max_rows);
         take(l->r.hit, max_rows);
         take(l->r.h, static_cast<uint64_t>(max_rows) * d_model);
-        const uint64_t many = static_cast<uint64_t>(div_up(vocab, kVocabTile)) * max_rows;
-        const uint64_t few = static_cast<uint64_t>(div_up(vocab, few_tile(vocab))) * (max_rows < kFewRows ? max_rows : kFewRows);
-        take(l->part, many > few ? many : few);
+        uint64_t parts = 0;
+        for (const uint32_t rows : {kFewRows, kMidRows, max_rows}) {
+            const uint32_t n = rows < max_rows ? rows : max_rows;
+            const uint64_t here = static_cast<uint64_t>(div_up(vocab, vocab_tile(n, vocab, d_model))) * n;
+            parts = here > parts ? here : parts;
+        }
+        take(l->part, parts);
         if (!l->backward) return;
         take(l->dz, dz);
         take(l->dh, part);

@@ -61,7 +61,7 @@ typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) i16x4_t lds_i16x4_t;
 
 // One operand's part of a stage: ROWS of a, K of k, T fragments to a wave.
-template <uint32_t ROWS, uint32_t K, int T, bool TURNED>
+template <uint32_t ROWS, uint32_t K, int T, bool TURNED, bool STREAMED = false>
 struct ProductSide {
     static constexpr uint32_t kLoads = ROWS * K / 2048;                 // of 1 KB, each wave's
     static constexpr uint32_t kLines = 512 / (TURNED ? ROWS : K);       // rows in memory of a load
@@ -115,7 +115,7 @@ struct ProductSide {
             for (uint32_t j = from; j < last; ++j) {
                 const uint32_t go = byte + column_of(j) < 2 * x.cols ? byte : 0x80000000u;  // beyond any range
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + (wave * kLoads + j) * 64), 16,
-                                                         static_cast<int>(off[j] + go), 0, 0, 0);
+                                                         static_cast<int>(off[j] + go), 0, 0, STREAMED ? kStreamed : 0);
             }
         }
     }
@@ -144,8 +144,9 @@ struct ProductSide {
 
 // Where several blocks read the same rows of A from memory at once, TOUCH brings its lines to the L2 three stages ahead: the
 // loads into LDS, of which one stage is on its way, then seldom wait for memory (2,048 x 65,536 x 5,376: 1,285 TFLOP/s without,
-// 1,329 with it; all zeros, where the clock is not held by the power, 1,527 and 1,857; of B's lines too: 1,183).
-template <int TA, int TB, int GA, int GB, uint32_t K, uint32_t BUFS, bool TURNED_A, bool TURNED_B, bool TOUCH = false>
+// 1,329 with it; all zeros, where the clock is not held by the power, 1,527 and 1,857; of B's lines too: 1,183). Where a block
+// alone reads its rows of A, STREAMED lets them pass the L2, which keeps B (17 rows of 262,144 x 5,376: 499 us without, 440).
+template <int TA, int TB, int GA, int GB, uint32_t K, uint32_t BUFS, bool TURNED_A, bool TURNED_B, bool TOUCH = false, bool STREAMED = false>
 struct ProductTile {
     static_assert(GA * GB == 4, "four waves");
     static_assert(BUFS >= 2 && BUFS <= 4, "buffers");
@@ -167,7 +168,7 @@ struct ProductTile {
                                                 const Operand& A, const Operand& B, const TileAt& at, uint32_t k,
                                                 f32x16_t (&acc)[TA][TB]) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        ProductSide<kA, K, TA, TURNED_A> x(A, at.a * kA, wave, wave / GB);
+        ProductSide<kA, K, TA, TURNED_A, STREAMED> x(A, at.a * kA, wave, wave / GB);
         ProductSide<kB, K, TB, TURNED_B> y(B, at.b * kB, wave, wave % GB);
         // whole turns of the buffers; past the operands' ends stages are zero
         const uint32_t turns = (k + BUFS * K - 1) / (BUFS * K);

@@ -172,6 +172,9 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 constexpr int kStreamed = 2;  // a buffer access that is not read again: non-temporal
+// What the cache on the memory's side holds: weights up to this size are found there by the next call, and streaming them
+// would lose that.
+constexpr uint64_t kMemoryCache = 256ull << 20;
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t make_rsrc(const void* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, static_cast<int>(bytes), 0x00027000);
 }
