@@ -102,7 +102,9 @@ using TileThree = ProductTile<4, 3, 2, 2, 64, 2, false, false, true>;
 using TileTwo = ProductTile<4, 2, 2, 2, 64, 2, false, false, true>;
 using TileStripe = ProductTile<2, 2, 4, 1, 64, 3, false, false, true>;  // a quarter of a wide one
 using TileHidden = ProductTile<4, 4, 2, 2, 32, 4, false, true>;
+using TileHiddenFew = ProductTile<4, 2, 1, 4, 32, 3, false, true, false, false, true>;  // up to 128 rows
 using TileWeight = ProductTile<4, 2, 2, 2, 32, 3, true, true>;
+using TileWeightFew = ProductTile<2, 2, 2, 2, 32, 2, true, true>;
 
 // Tiles of logits are of 256 vocabulary rows by 256, 192 or 128 hidden rows, whichever takes the least time: rounds of the
 // units times a tile's, which goes by its width and some 100 rows more (65,536 x 2,880: 105, 86 and 65 us a round). 518 rows
@@ -129,7 +131,7 @@ __host__ __device__ inline LogitTiles logit_tiles(uint32_t count, uint32_t na) {
 }
 
 template <typename Tile>
-constexpr int kWavesPerEu = Tile::kBytes > 81920 ? 1 : 2;  // blocks to a unit
+constexpr int kWavesPerEu = Tile::kBytes > 81920 ? 1 : Tile::kBytes > 40960 ? 2 : 4;  // blocks to a unit
 
 // The tile of vocabulary rows kA va .. and hidden rows m0 ..
 template <typename Tile, bool GRAD>
@@ -362,12 +364,13 @@ __global__ __launch_bounds__(kJoinThreads) void loss_join_kernel(JoinArgs a) {
 }
 
 // d_hidden has few tiles: its sums are cut into the parts, of at least 1,024 columns, that fill the units best, the fewest
-// of those (2,048 rows of 5,376: 168 tiles in 3 parts, two full rounds).
-__host__ __device__ inline uint32_t hidden_parts(uint32_t rows, uint32_t d, uint32_t piece) {
-    const uint64_t tiles = static_cast<uint64_t>((rows + 255) / 256) * ((d + 255) / 256);
+// of those (2,048 rows of 5,376: 168 tiles in 3 parts, two full rounds). A call of few rows has smaller tiles, two to a unit.
+__host__ __device__ inline uint32_t hidden_parts(uint32_t rows, uint32_t d, uint32_t piece, bool few) {
+    const uint32_t most = few ? 32 : 16, least = few ? 512 : 1024, round = few ? 512 : 256;
+    const uint64_t tiles = static_cast<uint64_t>(few ? 1 : (rows + 255) / 256) * ((d + 255) / 256);
     uint32_t best = 1;
-    for (uint32_t n = 2; n <= 16 && n <= (piece + 1023) / 1024; ++n)
-        if (20 * ((tiles * n + 255) / 256 * best) < 19 * ((tiles * best + 255) / 256 * n)) best = n;
+    for (uint32_t n = 2; n <= most && n <= (piece + least - 1) / least; ++n)
+        if (20 * ((tiles * n + round - 1) / round * best) < 19 * ((tiles * best + round - 1) / round * n)) best = n;
     return best;
 }
 
@@ -378,7 +381,7 @@ struct GradArgs {
     uint32_t rows, cols;   // of the result
     void* out;
     uint64_t stride;       // between the result's rows; the parts of d_hidden follow one another
-    bool add;
+    bool add, few;
 };
 
 __device__ __forceinline__ void add4(float* p, f32x4_t v) { *reinterpret_cast<f32x4_t*>(p) += v; }
@@ -394,10 +397,11 @@ __device__ __forceinline__ void add4(uint16_t* p, f32x4_t v) {
 template <typename Tile, typename Out, bool BY_COUNT>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_grad_kernel(GradArgs a) {
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GB = Tile::kGB;
+    static_assert(2 * TB * 256 <= Tile::kPieces, "two waves' fp32 sums change places in a buffer");
     __shared__ u32x4_t s0[Tile::kPieces], s1[Tile::kPieces], s2[Tile::kPieces2], s3[Tile::kPieces3];
     __shared__ uint32_t sink[Tile::kSink];
     const uint32_t count = *a.count, rows = BY_COUNT ? a.rows : count;
-    const uint32_t parts = BY_COUNT ? 1 : hidden_parts(count, a.cols, a.piece);
+    const uint32_t parts = BY_COUNT ? 1 : hidden_parts(count, a.cols, a.piece, a.few);
     const TileGrid grid{(rows + Tile::kA - 1) / Tile::kA, (a.cols + Tile::kB - 1) / Tile::kB, parts};
     const uint32_t id = stretched(grid.tiles());
     if (id >= grid.tiles()) return;
@@ -455,6 +459,7 @@ struct SpreadArgs {
     uint32_t piece, vocab, d;
     uint16_t* out;
     uint64_t stride;
+    bool few;
 };
 
 // d_hidden's parts added up, in the caller's rows; zeros where a row is left out. Bound by the read of the parts: 2,048 rows
@@ -466,8 +471,9 @@ __global__ __launch_bounds__(256) void loss_spread_kernel(SpreadArgs a) {
     if (static_cast<uint32_t>(a.targets[b]) >= a.vocab) *reinterpret_cast<u32x4_t*>(a.out + b * a.stride + c) = u32x4_t{0, 0, 0, 0};
     const uint32_t count = *a.r.count;
     if (b >= count) return;
-    const uint32_t parts = hidden_parts(count, a.d, a.piece);
+    const uint32_t parts = hidden_parts(count, a.d, a.piece, a.few);
     f32x4_t lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+#pragma unroll 4
     for (uint32_t p = 0; p < parts; ++p) {
         const f32x4_t* from = reinterpret_cast<const f32x4_t*>(a.part + (static_cast<uint64_t>(p) * count + b) * a.d + c);
         lo += from[0], hi += from[1];
@@ -616,9 +622,11 @@ int backward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, 
     const uint32_t piece = piece_of(g.rows, l->vocab);
     int rc = launch_gather(l, g, s);
     if (rc) return rc;
+    const bool few = g.rows <= kMidRows;
+    static_assert(TileHiddenFew::kA == kMidRows && TileHiddenFew::kB == 256 && TileHidden::kA == 256 && TileHidden::kB == 256, "as hidden_parts takes them");
     uint32_t most_tiles = 0;  // of d_hidden's product, for any number of rows that count
-    for (uint32_t n = 1; n <= div_up(g.rows, TileHidden::kA); ++n) {
-        const uint32_t tiles = n * div_up(l->d, TileHidden::kB) * hidden_parts(n * TileHidden::kA, l->d, piece);
+    for (uint32_t n = 1; n <= div_up(g.rows, 256); ++n) {
+        const uint32_t tiles = n * div_up(l->d, 256) * hidden_parts(n * 256, l->d, piece, few);
         most_tiles = tiles > most_tiles ? tiles : most_tiles;
     }
     for (uint32_t v0 = 0; v0 < l->vocab; v0 += piece) {
@@ -627,26 +635,28 @@ int backward(const twd_headloss* l, const GatherArgs& g, const Operand& weight, 
         LogitArgs a{};
         a.r = l->r, a.weight = weight, a.hidden = h;
         a.d = l->d, a.vocab = l->vocab, a.v0 = v0, a.here = here, a.softcap = soft_cap(l->softcap), a.dz = l->dz, a.dz_stride = piece;
-        if ((rc = g.rows <= kMidRows ? launch_few<true>(a, g.rows, nullptr, s) : launch_logits<true>(a, g.rows, s))) return rc;
+        if ((rc = few ? launch_few<true>(a, g.rows, nullptr, s) : launch_logits<true>(a, g.rows, s))) return rc;
         if (o.d_weight) {
             GradArgs b{};
             b.count = l->r.count, b.a = Operand{l->dz, piece, g.rows, piece}, b.b = h;
             b.rows = here, b.cols = l->d, b.stride = o.d_weight_stride, b.add = o.add;
             b.out = static_cast<char*>(o.d_weight) + v0 * o.d_weight_stride * (o.type == TWD_F32 ? 4 : 2);
-            rc = o.type == TWD_F32 ? launch_grad<TileWeight, float, true>(b, 0, s) : launch_grad<TileWeight, uint16_t, true>(b, 0, s);
+            if (few) rc = o.type == TWD_F32 ? launch_grad<TileWeightFew, float, true>(b, 0, s) : launch_grad<TileWeightFew, uint16_t, true>(b, 0, s);
+            else rc = o.type == TWD_F32 ? launch_grad<TileWeight, float, true>(b, 0, s) : launch_grad<TileWeight, uint16_t, true>(b, 0, s);
             if (rc) return rc;
         }
         if (o.d_hidden) {
             GradArgs b{};
             b.count = l->r.count, b.a = Operand{l->dz, piece, g.rows, here}, b.b = w;
             b.k = here, b.piece = piece, b.cols = l->d;
-            b.out = l->dh, b.stride = l->d, b.add = v0 > 0;
-            if ((rc = launch_grad<TileHidden, float, false>(b, most_tiles, s))) return rc;
+            b.out = l->dh, b.stride = l->d, b.add = v0 > 0, b.few = few;
+            rc = few ? launch_grad<TileHiddenFew, float, false>(b, most_tiles, s) : launch_grad<TileHidden, float, false>(b, most_tiles, s);
+            if (rc) return rc;
         }
     }
     if (!o.d_hidden) return TWD_OK;
     loss_spread_kernel<<<dim3(g.rows, div_up(l->d, 2048)), 256, 0, s>>>(
-        SpreadArgs{l->r, g.targets, l->dh, piece, l->vocab, l->d, o.d_hidden, o.d_hidden_stride});
+        SpreadArgs{l->r, g.targets, l->dh, piece, l->vocab, l->d, o.d_hidden, o.d_hidden_stride, few});
     TWD_HIP(hipGetLastError());
     return TWD_OK;
 }
@@ -705,7 +715,12 @@ TWD_API int twd_headloss_create(uint32_t max_rows, uint32_t vocab, uint32_t d_mo
     uint64_t dz = 0, part = 0;  // the most that any number of rows, and of those that count, takes
     for (uint32_t rows = 1; l->backward && rows <= max_rows; ++rows) {
         const uint64_t n = static_cast<uint64_t>(rows) * piece_of(rows, vocab);
-        const uint64_t m = static_cast<uint64_t>(rows) * d_model * hidden_parts(rows, d_model, most_of_piece(rows));
+        uint32_t parts = hidden_parts(rows, d_model, most_of_piece(rows), false);
+        if (rows <= kMidRows) {
+            const uint32_t more = hidden_parts(rows, d_model, most_of_piece(rows), true);
+            parts = more > parts ? more : parts;
+        }
+        const uint64_t m = static_cast<uint64_t>(rows) * d_model * parts;
         dz = n > dz ? n : dz, part = m > part ? m : part;
     }
     char* at = nullptr;

@@ -108,7 +108,7 @@ struct ProductSide {
             const auto r = make_rsrc(x.p + k * x.stride + first, left ? (left - 1) * line + 2 * (x.cols - first) : 0);
 #pragma unroll
             for (uint32_t j = from; j < last; ++j)
-                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + (wave * kLoads + j) * 64), 16, static_cast<int>(off[j]), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(to + (wave * kLoads + j) * 64), 16, static_cast<int>(off[j]), 0, 0, STREAMED ? kStreamed : 0);
         } else {
             const uint32_t byte = stage * (2 * K);
 #pragma unroll
@@ -145,8 +145,8 @@ struct ProductSide {
 // Where several blocks read the same rows of A from memory at once, TOUCH brings its lines to the L2 three stages ahead: the
 // loads into LDS, of which one stage is on its way, then seldom wait for memory (2,048 x 65,536 x 5,376: 1,285 TFLOP/s without,
 // 1,329 with it; all zeros, where the clock is not held by the power, 1,527 and 1,857; of B's lines too: 1,183). Where a block
-// alone reads its rows of A, STREAMED lets them pass the L2, which keeps B (17 rows of 262,144 x 5,376: 499 us without, 440).
-template <int TA, int TB, int GA, int GB, uint32_t K, uint32_t BUFS, bool TURNED_A, bool TURNED_B, bool TOUCH = false, bool STREAMED = false>
+// alone reads its part of an operand, STREAMED lets it pass the L2, which keeps the other (17 rows of 262,144 x 5,376: 499 us without, 440).
+template <int TA, int TB, int GA, int GB, uint32_t K, uint32_t BUFS, bool TURNED_A, bool TURNED_B, bool TOUCH = false, bool STREAMED_A = false, bool STREAMED_B = false>
 struct ProductTile {
     static_assert(GA * GB == 4, "four waves");
     static_assert(BUFS >= 2 && BUFS <= 4, "buffers");
@@ -168,8 +168,8 @@ struct ProductTile {
                                                 const Operand& A, const Operand& B, const TileAt& at, uint32_t k,
                                                 f32x16_t (&acc)[TA][TB]) {
         const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
-        ProductSide<kA, K, TA, TURNED_A, STREAMED> x(A, at.a * kA, wave, wave / GB);
-        ProductSide<kB, K, TB, TURNED_B> y(B, at.b * kB, wave, wave % GB);
+        ProductSide<kA, K, TA, TURNED_A, STREAMED_A> x(A, at.a * kA, wave, wave / GB);
+        ProductSide<kB, K, TB, TURNED_B, STREAMED_B> y(B, at.b * kB, wave, wave % GB);
         // whole turns of the buffers; past the operands' ends stages are zero
         const uint32_t turns = (k + BUFS * K - 1) / (BUFS * K);
         auto load = [&](uint32_t stage, u32x4_t* to, uint32_t first, uint32_t last) {
