@@ -446,7 +446,10 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
             store_rows<TB, Out>((wave < 2 ? s0 : s1) + wave % 2 * (TB * 64 * sizeof(Out)), [&](auto tb) { return acc[ta][tb]; },
                 [&](uint32_t row, uint32_t col, u32x4_t w) {
                     Out* const p = place(ta, row, col);
-                    if (p) *reinterpret_cast<u32x4_t*>(p) = w;
+                    if (!p) return;
+                    // d_weight is past the caches' size and not read again here
+                    if constexpr (BY_COUNT) __builtin_nontemporal_store(w, reinterpret_cast<u32x4_t*>(p));
+                    else *reinterpret_cast<u32x4_t*>(p) = w;
                 });
         });
     }
