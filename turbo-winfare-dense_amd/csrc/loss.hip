@@ -242,10 +242,10 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& a, uint32_t count, 
 }
 
 // One block to a unit, whose waves hold 256 sums a lane each: the widest tile reads least through LDS. 2,048 rows of 262,144 x
-// 5,376 with a softcap take 4.75 ms, 1,215 TFLOP/s (a plain library product of the same rows 1,333): the matrix units are busy
+// 5,376 with a softcap take 4.65 to 4.75 ms, 1,215 to 1,240 TFLOP/s (a plain library product of the same rows 1,333): the matrix units are busy
 // in 68% of the cycles, at the clock of some 1.6 GHz that the power leaves, the rest being a tile's first loads and its
 // epilogue, which nothing covers. Tiles of 256 x 128 with two blocks to a unit, one's epilogue beside the other's products,
-// took 6.06 ms where these took 4.90 (32,003 x 2,048 of 777 rows: 145 and 152 us). With dz stored, a piece of 65,536: 1.26 ms.
+// took 6.06 ms where these took 4.90 (32,003 x 2,048 of 777 rows: 145 and 152 us). With dz stored, a piece of 65,536: 1.24 ms.
 template <bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_logits_kernel(LogitArgs a) {
     __shared__ u32x4_t s0[TileWide::kPieces], s1[TileWide::kPieces];
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu
 }
 
 // The last tiles, a stripe of 64 hidden rows to a block. Bound by its own chain of stages: 16 stripes of 2,880 columns 29 us,
-// as a round of whole tiles takes 95; no tiles to cut, 5 us.
+// as a round of whole tiles takes 95; where few rows count and no tile is cut, 5 us.
 template <bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_stripes_kernel(LogitArgs a) {
     using Tile = TileStripe;
@@ -391,9 +391,11 @@ __device__ __forceinline__ void add4(uint16_t* p, f32x4_t v) {
 }
 
 // d_weight = dz^T H (BY_COUNT: k runs over the rows that count) or a piece's part of d_hidden = dz W. For 2,048 rows of 65,536
-// x 5,376 1.26 and 1.22 ms: 1,144 and 1,185 TFLOP/s, where the library's products with these operands reach 1,034 and 727.
-// d_weight has no room to wait for its stores, nor few tiles: two blocks to a unit cover each other's. d_hidden has a long sum
-// and few tiles: one large tile a unit, the sum in parts.
+// x 5,376 1.23 and 1.20 ms: 1,170 and 1,200 TFLOP/s, where the library's products with these operands reach 1,034 and 727.
+// d_weight has many tiles with short sums: two blocks to a unit cover each other's first loads and stores, of up to 128 rows
+// four, whose tiles are a quarter (128 rows of 32,003 x 1,024: 20 us, 24 in large ones). d_hidden has a long sum and few tiles: one
+// large tile to a unit, the sum in parts; of up to 128 rows the read of the weights bounds it, so a tile has just these rows and two
+// blocks share a unit (17 rows of 262,144 x 5,376: 432 us, 6.5 TB/s, 583 in large tiles; the small head 25 and 49).
 template <typename Tile, typename Out, bool BY_COUNT>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(kWavesPerEu<Tile>, kWavesPerEu<Tile>))) void loss_grad_kernel(GradArgs a) {
     constexpr int TA = Tile::kTA, TB = Tile::kTB, GB = Tile::kGB;
