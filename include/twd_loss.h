@@ -26,9 +26,9 @@ extern "C" {
  * An object holds the scratch of calls of up to max_rows (65,536) rows with heads of up to vocab x d_model; d_model is a
  * multiple of 32, at most 2^20, vocab at most 2^24, max_rows x vocab at most 2^38; softcap 0 (none) or in 1e-30..1e30.
  * Without `backward` the scratch is the forward pass's alone: 2 max_rows d_model bytes and 8 max_rows for each 256 of the
- * vocabulary (of up to 64 rows, for each 64). The gradients take, on top of it, up to 256 MB for dz and
- * d_hidden in fp32, once or for each of up to 16 parts that its product is cut into where tiles are few. Its calls are ordered across streams as a selector's are, and replays of captured calls are ordered
- * by the caller. */
+ * vocabulary (of up to 128 rows, for each 64). The gradients take, on top of it, up to 256 MB for dz, and d_hidden in
+ * fp32, once or for each of the up to 16 parts (up to 128 rows: 32) that its product is cut into where tiles are few.
+ * Its calls are ordered across streams as a selector's are, and replays of captured calls are ordered by the caller. */
 typedef struct twd_headloss twd_headloss;
 TWD_API int twd_headloss_create(uint32_t max_rows, uint32_t vocab, uint32_t d_model, float softcap, int backward,
                                 twd_headloss** out);

@@ -19,6 +19,7 @@ SHAPES = [  # vocab, d_model, rows, softcap
     (777, 2880, 129, 30.0), (4099, 512, 300, 50.0), (300, 544, 600, 0.0), (256, 128, 128, 0.0), (2049, 64, 257, 5.0),
     (40001, 64, 40, 30.0), (131075, 32, 1030, 0.0), (515, 5376, 17, 30.0),
     (131075, 64, 33, 30.0), (40961, 96, 100, 0.0), (2000, 352, 128, 30.0), (70001, 1984, 128, 30.0), (70001, 1984, 21, 0.0),
+    (1100003, 32, 128, 30.0),
 ]
 
 
@@ -319,7 +320,7 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         for a, b in zip(got, refs):
             assert all(torch.equal(x, y) for x, y in zip(a, b))
-    for n in (200, 40):
+    for n in (200, 100, 40):
         h, w, targets, grad = [x.clone() for x in make(vocab, d, n, 0, 77)]
         out = [torch.empty(n, device="cuda:0"), torch.empty(n, device="cuda:0"), torch.empty_like(h), torch.empty_like(w)]
         torch.cuda.synchronize()
