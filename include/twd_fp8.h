@@ -27,8 +27,9 @@ TWD_API int twd_fp8_quantize(const void* x, int type, uint64_t rows, uint32_t co
 
 /* An LM head whose weights [vocab][d_model] are held in the format, beside twd_head and twd_mxhead. The codes and scales
  * (device; block_rows 128) are copied into the layout the kernels read and may be freed after the call, which is
- * synchronous. d_model is a multiple of 128, at most 2^20; vocab at most 2^30. Scales that are negative, above 2^100 or NaN
- * are rejected with TWD_E_UNSUPPORTED. softcap 0 (none) or in 1e-30..1e30. */
+ * synchronous. d_model is a multiple of 128, at most 2^20; vocab at most 2^30. Scales that are negative, above 2^8 or NaN
+ * are rejected with TWD_E_UNSUPPORTED: up to 2^8, times the largest scale of a hidden row, they stay within fp32. softcap 0
+ * (none) or in 1e-30..1e30. */
 typedef struct twd_fp8head twd_fp8head;
 TWD_API int twd_fp8head_create(const uint8_t* codes, const float* scales, uint32_t vocab, uint32_t d_model, float softcap,
                                void* stream, twd_fp8head** out);
@@ -40,7 +41,9 @@ TWD_API int twd_fp8head_info(const twd_fp8head* head, uint32_t* vocab, uint32_t*
  * instructions and the sums, times their scales, added up in fp32; logits_type TWD_F32 or TWD_BF16 with logits_stride >=
  * vocab elements between rows. The products are exact and added in fp32, but for bf16 logits of more than 128 rows: those run
  * on 8-bit instructions, which cut the products of eight neighbouring columns at 2^-13 of the largest of the eight (2e-5 of
- * sum |w h| for normal products). A row with a NaN scale gives NaN logits. The call keeps no state: calls on one head may overlap, on any streams, and may be
+ * sum |w h| for normal products). Hidden scales are twd_fp8_quantize's, at most FLT_MAX / 448; the product of two scales is
+ * rounded to fp32 (below 2^-126 to a multiple of 2^-149, which takes less than 2^-125 from a block's sum). A row with a NaN scale
+ * gives NaN logits. The call keeps no state: calls on one head may overlap, on any streams, and may be
  * captured. Asynchronous on `stream`. */
 TWD_API int twd_fp8head_logits(const twd_fp8head* head, const uint8_t* codes, const float* scales, uint32_t rows,
                                void* logits, int logits_type, uint64_t logits_stride, void* stream);

@@ -21,6 +21,10 @@ namespace {
 
 constexpr uint32_t kBlock = 128;
 constexpr float kTop = 448.0f, kLeastScale = 0x1p-126f;
+// A weight scale times the largest that hidden rows get, FLT_MAX / 448, is finite: a sum of zero stays zero, and only logits
+// past fp32 are infinite. Products of scales below 2^-126 are multiples of 2^-149; a sum of 128 products is below 2^24.7, so
+// that takes less than 2^-125 from it.
+constexpr float kMostWeightScale = 0x1p8f;
 
 // ---- to the format --------------------------------------------------------------------------------------
 
@@ -148,7 +152,7 @@ __global__ __launch_bounds__(256) void fp8_repack_kernel(const uint8_t* __restri
 __global__ __launch_bounds__(256) void fp8_check_kernel(const float* scales, float* kept, uint64_t n, uint32_t* bad) {
     for (uint64_t i = blockIdx.x * 256ull + threadIdx.x; i < n; i += gridDim.x * 256ull) {
         const float s = scales[i];
-        if (!(s >= 0.0f && s <= 0x1p100f)) *bad = 1;
+        if (!(s >= 0.0f && s <= kMostWeightScale)) *bad = 1;
         kept[i] = s;
     }
 }
@@ -722,7 +726,7 @@ TWD_API int twd_fp8head_create(const uint8_t* codes, const float* scales, uint32
     if (!h) {
         (void)hipFree(mem);
         if (e != hipSuccess) return hip_fail(e, "repacking the head");
-        if (bad) return fail(TWD_E_UNSUPPORTED, "a block scale is negative, above 2^100 or NaN");
+        if (bad) return fail(TWD_E_UNSUPPORTED, "a block scale is negative, above 2^8 or NaN");
         return fail(TWD_E_INVALID, "out of host memory");
     }
     *out = h;
