@@ -228,8 +228,8 @@ struct ProductTile {
         for (int i = 0; i < TA; ++i)
 #pragma unroll
             for (int j = 0; j < TB; ++j) acc[i][j] = f32x16_t{};
-        constexpr uint32_t kFirst = (BUFS - 2) * kLoads + kLoads / kSpread;
-        __builtin_amdgcn_s_waitcnt(0x0F70 | (kFirst & 15) | (kFirst >> 4) << 14);
+        // all of them: kAhead counts lines of BUFS - 1 stages before, which the first stages do not have
+        __builtin_amdgcn_s_waitcnt(kVmcnt0);
         __syncthreads();
 #pragma unroll
         for (int t = 0; t < TA; ++t) fa[0][t] = x.read(s0, 0, t);
