@@ -16,7 +16,10 @@ extern "C" {
  *   z_mv = softcap(h_m . w_v),  lse_m = ln sum_v exp(z_mv),  losses_m = lse_m - z_m,targets[m]
  * so -losses is the log-probability of each target. Rows whose target lies outside 0..vocab-1 (-100, -1) are left
  * out: their loss and lse are 0, they have no part in d_weight and their row of d_hidden is 0, whatever they hold.
- * A row with a NaN or an infinity gives a NaN loss; the gradients that have a part in it are NaN.
+ * A row with a NaN gives a NaN loss, and the gradients that have a part in it are NaN; so does, without a softcap, one with an
+ * infinity. With a softcap an infinite sum is a logit of +-softcap, as tanh has it: unless one of its sums is NaN (0 times
+ * infinity, infinities of both signs), such a row has a finite loss and d_hidden, and d_weight is not finite in the
+ * infinity's column alone.
  *
  * The logits are computed a piece of the vocabulary at a time, summed in fp32, and again for the gradients, which are
  *   dz_mv = grad_m (exp(z_mv - lse_m) - [v = targets[m]]) softcap'(z_mv)
