@@ -1068,10 +1068,12 @@ class Fp8Head:
             pass
 
     def logits_fp8(self, codes, scales, out=None, stream=None):
-        """Logits of hidden rows that fp8_quantize brought into the format too, in out's float32 or bfloat16 (float32 where
-        none is given)."""
+        """Logits of hidden rows that fp8_quantize brought into the format too (codes uint8 or float8_e4m3fn), in out's
+        float32 or bfloat16 (float32 where none is given)."""
         import torch
         rows = codes.shape[0]
+        if codes.dtype == torch.float8_e4m3fn:
+            codes = codes.view(torch.uint8)
         _buffer(codes, (rows, self.d_model), torch.uint8, "codes")
         _buffer(scales, (rows, self.d_model // 128), torch.float32, "scales")
         with _on_device(codes, scales, out):
