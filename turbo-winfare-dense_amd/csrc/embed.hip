@@ -535,8 +535,9 @@ TWD_API int twd_embedgrad_run(twd_embedgrad* g, const void* d_rows, int rows_typ
     const RunArgs a{d_rows, rows_stride, g->id, g->place, g->part, d_table, table_stride, ids_count, d_model, vocab, scale,
                     wide_rows(d_rows, rows_stride, ids_count, rows_type) && wide_rows(d_table, table_stride, vocab, table_type),
                     accumulate != 0};
-    if ((rc = run(g, sort, a, rows_type, table_type, accumulate == 0, s))) return rc;
-    return order_after(g->order, s);
+    rc = run(g, sort, a, rows_type, table_type, accumulate == 0, s);
+    const int rc2 = order_after(g->order, s);
+    return rc ? rc : rc2;
 }
 
 }  // extern "C"

@@ -792,8 +792,9 @@ TWD_API int twd_headloss_forward(twd_headloss* l, const uint16_t* hidden_bf16, u
     GatherArgs g{};
     g.hidden = hidden_bf16, g.stride = hidden_stride, g.targets = targets, g.losses = losses, g.lse_out = lse, g.rows = rows;
     if ((rc = order_before(l->order, s))) return rc;
-    if ((rc = forward(l, g, weight_of(l, weight_bf16, weight_stride), s))) return rc;
-    return order_after(l->order, s);
+    rc = forward(l, g, weight_of(l, weight_bf16, weight_stride), s);
+    const int rc2 = order_after(l->order, s);
+    return rc ? rc : rc2;
 }
 
 TWD_API int twd_headloss_backward(twd_headloss* l, const uint16_t* hidden_bf16, uint32_t rows, uint64_t hidden_stride,
@@ -816,8 +817,9 @@ TWD_API int twd_headloss_backward(twd_headloss* l, const uint16_t* hidden_bf16, 
     g.hidden = hidden_bf16, g.stride = hidden_stride, g.targets = targets, g.grad = grad, g.lse_in = lse, g.rows = rows;
     const BackOut o{d_hidden_bf16, d_hidden_stride, d_weight, d_weight_type, d_weight_stride, accumulate != 0};
     if ((rc = order_before(l->order, s))) return rc;
-    if ((rc = backward(l, g, weight_of(l, weight_bf16, weight_stride), o, s))) return rc;
-    return order_after(l->order, s);
+    rc = backward(l, g, weight_of(l, weight_bf16, weight_stride), o, s);
+    const int rc2 = order_after(l->order, s);
+    return rc ? rc : rc2;
 }
 
 }  // extern "C"

@@ -1216,8 +1216,8 @@ TWD_API int twd_sampler_sample(twd_sampler* sampler, const void* logits, int typ
     else
         launch<Fp16>(args, rows, s);
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return hip_fail(e, "launching the sampler");
-    return order_after(sampler->order, s);
+    rc = order_after(sampler->order, s);
+    return e != hipSuccess ? hip_fail(e, "launching the sampler") : rc;
 }
 
 }  // extern "C"

@@ -407,7 +407,7 @@ struct StreamOrder {
     hipEvent_t ev = nullptr;
 };
 int order_before(StreamOrder& o, hipStream_t s);  // before enqueueing work that uses the state
-int order_after(StreamOrder& o, hipStream_t s);   // after enqueueing it
+int order_after(StreamOrder& o, hipStream_t s);   // after enqueueing it, also where a launch failed: others may run
 void order_release(StreamOrder& o);
 
 // ---- the fused sample pass ------------------------------------------------------------------------
