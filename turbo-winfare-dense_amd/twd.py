@@ -833,6 +833,8 @@ def _matrix(t, what: str):
     shape, stride = t.shape, t.stride()
     if len(shape) != 2 or (stride[1] != 1 and shape[1] > 1):
         raise ValueError(f"{what} must be two-dimensional with adjacent columns")
+    if (shape[0] | shape[1]) >> 32:  # the library's counts have 32 bits; ctypes would drop the others
+        raise ValueError(f"{what} has 2^32 rows or columns or more")
     return shape[0], shape[1], stride[0] if shape[0] > 1 else shape[1]
 
 
