@@ -135,18 +135,22 @@ __global__ __launch_bounds__(256) void fp8_weights_kernel(QuantArgs a) {
 // 5,376.
 constexpr uint32_t kGroupRows = 64;
 constexpr uint32_t kUnit = 512;  // 16-byte pieces of a group's chunk
+constexpr uint32_t kRepackBlocks = 65536;  // 2^30 rows are 2^24 groups, a block to each 2^32 threads: more than a launch may have
 
 __global__ __launch_bounds__(256) void fp8_repack_kernel(const uint8_t* __restrict__ codes, uint32_t vocab, uint32_t d,
                                                         u32x4_t* __restrict__ out) {
     const uint32_t lane = threadIdx.x % 64, tile = threadIdx.x / 64, kg = lane / 16, chunks = d / kBlock;
-    const uint64_t group = blockIdx.x, row = group * kGroupRows + 16 * tile + lane % 16;
-    for (uint32_t c = 0; c < chunks; ++c)
+    const uint32_t groups = (vocab + kGroupRows - 1) / kGroupRows;
+    for (uint64_t group = blockIdx.x; group < groups; group += gridDim.x) {
+        const uint64_t row = group * kGroupRows + 16 * tile + lane % 16;
+        for (uint32_t c = 0; c < chunks; ++c)
 #pragma unroll
-        for (uint32_t h = 0; h < 2; ++h) {
-            u32x4_t w = {0, 0, 0, 0};
-            if (row < vocab) w = *reinterpret_cast<const u32x4_t*>(codes + row * d + kBlock * c + 32 * kg + 16 * h);
-            out[(group * chunks + c) * kUnit + (2 * tile + h) * 64 + lane] = w;
-        }
+            for (uint32_t h = 0; h < 2; ++h) {
+                u32x4_t w = {0, 0, 0, 0};
+                if (row < vocab) w = *reinterpret_cast<const u32x4_t*>(codes + row * d + kBlock * c + 32 * kg + 16 * h);
+                out[(group * chunks + c) * kUnit + (2 * tile + h) * 64 + lane] = w;
+            }
+    }
 }
 
 __global__ __launch_bounds__(256) void fp8_check_kernel(const float* scales, float* kept, uint64_t n, uint32_t* bad) {
@@ -715,7 +719,7 @@ TWD_API int twd_fp8head_create(const uint8_t* codes, const float* scales, uint32
     hipError_t e = hipMemsetAsync(bad_dev, 0, sizeof(bad), s);
     if (e == hipSuccess) {
         fp8_check_kernel<<<256, 256, 0, s>>>(scales, kept_scales, n_scales, bad_dev);
-        fp8_repack_kernel<<<groups, 256, 0, s>>>(codes, vocab, d_model, kept_codes);
+        fp8_repack_kernel<<<min(groups, kRepackBlocks), 256, 0, s>>>(codes, vocab, d_model, kept_codes);
         e = hipGetLastError();
     }
     if (e == hipSuccess) e = hipMemcpyAsync(&bad, bad_dev, sizeof(bad), hipMemcpyDeviceToHost, s);
