@@ -129,6 +129,7 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedArgs a) {
 // in 24 of them.
 constexpr uint32_t kList = 2048, kListThreads = 1024;
 constexpr uint32_t kFillEach = 4;  // pieces of 16 bytes that a thread clears
+constexpr uint64_t kMostFill = (1ull << 38) - (1u << 20);  // bytes of one launch, which may have fewer than 2^32 threads
 constexpr uint32_t kPiece = 32;
 constexpr uint32_t kNoId = 0xFFFFFFFFu;  // outside the vocabulary: sorted last
 
@@ -326,7 +327,7 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_runs_kernel(RunArgs a) {
     store_eight(row, a.wide, base, a.d, sum);
 }
 
-// Rows apart from one another: cleared one by one.
+// Rows apart from one another, and tables past kMostFill: cleared one by one.
 template <typename Out>
 __global__ __launch_bounds__(kEmbedThreads) void embed_clear_kernel(Out* table, uint64_t stride, uint32_t vocab, uint32_t d, bool wide) {
     const float zero[kEach] = {};
@@ -384,8 +385,8 @@ int run(const twd_embedgrad* g, SortArgs sort, const RunArgs& a, int rows_type, 
     const uint64_t size = size_of(table_type);
     const uint32_t steps = over(a.d, kSpan);
     Fill f{};
-    if (clear && (a.vocab == 1 || a.table_stride == a.d)) {
-        const uint64_t bytes = static_cast<uint64_t>(a.vocab) * a.d * size;
+    const uint64_t bytes = static_cast<uint64_t>(a.vocab) * a.d * size;
+    if (clear && (a.vocab == 1 || a.table_stride == a.d) && bytes <= kMostFill) {
         const uintptr_t from = reinterpret_cast<uintptr_t>(a.table);
         const uint64_t before = (16 - from % 16) % 16 < bytes ? (16 - from % 16) % 16 : bytes;
         f.n = (bytes - before) / 16;
