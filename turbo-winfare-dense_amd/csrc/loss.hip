@@ -106,29 +106,8 @@ using TileHiddenFew = ProductTile<4, 2, 1, 4, 32, 3, false, true, false, false, 
 using TileWeight = ProductTile<4, 2, 2, 2, 32, 3, true, true>;
 using TileWeightFew = ProductTile<2, 2, 2, 2, 32, 2, true, true>;
 
-// Tiles of logits are of 256 vocabulary rows by 256, 192 or 128 hidden rows, whichever takes the least time: rounds of the
-// units times a tile's, which goes by its width and some 100 rows more (65,536 x 2,880: 105, 86 and 65 us a round). 518 rows
-// of 32,003 x 2,048 take 139, 113 and 124 us, 1,023 of 65,537 x 2,880 take 427, 476 and 476. The few tiles past whole rounds
-// are cut into stripes of 64 hidden rows and follow in a launch of their own, which costs some 80 rows of a round.
-constexpr uint32_t kVocabTile = 256, kRound = 256, kMostCut = 64, kFewRows = 64, kMidRows = 128;
 static_assert(TileWide::kA == kVocabTile && TileThree::kA == kVocabTile && TileTwo::kA == kVocabTile && TileStripe::kA == kVocabTile, "one width");
-struct LogitTiles {
-    TileGrid grid;
-    uint32_t width;  // hidden rows of a tile
-    uint32_t cut;    // of the last tiles
-};
-__host__ __device__ inline LogitTiles logit_tiles(uint32_t count, uint32_t na) {
-    LogitTiles best{};
-    uint32_t least = ~0u;
-#pragma unroll
-    for (uint32_t width = 256; width >= 128; width -= 64) {
-        const TileGrid g{na, (count + width - 1) / width, 1};
-        const uint32_t left = g.tiles() % kRound, cut = left <= kMostCut ? left : 0;
-        const uint32_t time = g.tiles() / kRound * (width + 100) + (cut > 0 ? 80 : left > 0 ? width + 100 : 0);
-        if (time < least) least = time, best = LogitTiles{g, width, cut};
-    }
-    return best;
-}
+constexpr uint32_t kFewRows = 64, kMidRows = 128;
 
 template <typename Tile>
 constexpr int kWavesPerEu = Tile::kBytes > 81920 ? 1 : Tile::kBytes > 40960 ? 2 : 4;  // blocks to a unit

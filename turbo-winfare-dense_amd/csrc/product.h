@@ -12,6 +12,7 @@
 // the reads turn 4 (k) x 16 (a) elements over sixteen lanes.
 #pragma once
 
+#include "tiles.h"
 #include "twd_internal.h"
 #include "vocab_core.h"
 
@@ -32,13 +33,9 @@ struct Operand {
 };
 constexpr uint64_t kMaxProductStride = 1ull << 22;
 
-// Which tile a block takes: blocks go to the XCDs in turn, and each XCD takes a contiguous stretch of the tiles, ordered
-// so that a few rows of tiles along A meet up to eight along B at a time: what an XCD's blocks read at once stays in its
-// L2.
-struct TileGrid {
-    uint32_t na, nb, parts;  // tiles along A and B, and parts of the sum
-    __host__ __device__ uint32_t tiles() const { return na * nb * parts; }
-};
+// Which tile of a grid a block takes: blocks go to the XCDs in turn, and each XCD takes a contiguous stretch of the tiles,
+// ordered so that a few rows of tiles along A meet up to eight along B at a time: what an XCD's blocks read at once stays in
+// its L2.
 struct TileAt {
     uint32_t a, b, part;
     uint32_t share, who;  // the blocks that read the same rows of A at once, and which of them this is
