@@ -24,7 +24,7 @@ extern "C" {
  * The logits are computed a piece of the vocabulary at a time, summed in fp32, and again for the gradients, which are
  *   dz_mv = grad_m (exp(z_mv - lse_m) - [v = targets[m]]) softcap'(z_mv)
  *   d_hidden = dz W,  d_weight = dz^T H
- * with dz rounded to bf16 (by at most 2^-8 of each term) for products summed in fp32.
+ * with dz rounded to bf16 (by at most 2^-8 of each term, for a d_weight of fp32 too) for products summed in fp32.
  *
  * An object holds the scratch of calls of up to max_rows (65,536) rows with heads of up to vocab x d_model; d_model is a
  * multiple of 32, at most 2^20, vocab at most 2^24, max_rows x vocab at most 2^38; softcap 0 (none) or in 1e-30..1e30.

@@ -126,7 +126,8 @@ __global__ __launch_bounds__(kEmbedThreads) void embed_kernel(EmbedArgs a) {
 // What bounds it is the clearing of a table that is mostly zeros: 16,384 ids of 262,144 x 5,376 in bf16 take 592 us, 2.8 GB
 // cleared in the first three launches (131 + 170 + 182 us, 5.8 TB/s; a fill reaches 6.8), then the runs, 110 us: their 180 MB of
 // rows, and rows of the table that the clearing has left in no cache. 513 ids of 32,003 x 1,024 to fp32: 36 us, 131 MB cleared
-// in 24 of them.
+// in 24 of them. A run's parts are added by one block, four at a time: 16,384 equal ids of 32,003 x 1,024 in bf16 take 158 us, 72
+// drawn as words are; 262,144 of them 2,065 and 522.
 constexpr uint32_t kList = 2048, kListThreads = 1024;
 constexpr uint32_t kFillEach = 4;  // pieces of 16 bytes that a thread clears
 constexpr uint64_t kMostFill = (1ull << 38) - (1u << 20);  // bytes of one launch, which may have fewer than 2^32 threads

@@ -205,7 +205,9 @@ __device__ __forceinline__ Wide32 widened(i32x8_t v) {
 // Bound by the read of the head. The waves of a block split d_model by quads of chunks; a wave keeps its quad of the hidden
 // rows in registers and streams its quad of one group after another, kAhead chunks (8 KB each) ahead of the arithmetic. The
 // sums over the quads meet in LDS, two buffers in turn. One row of 262,144 x 5,376: 213 us, 6.6 TB/s, where a pure read reaches
-// 6.7; 16 rows 237; seven of 151,669 x 3,584 88 us, 6.2 TB/s.
+// 6.7; 16 rows 237; seven of 151,669 x 3,584 88 us, 6.2 TB/s. A block has the waves for a d_model of up to 6,144; past it rows go to
+// tiles of 32, which read such long rows as fast: of 131,072 rows by 6,144 one takes 120 us and 16 take 130 here, 32 take 129 in a
+// tile; by 7,168 1 to 32 rows take 142 there (6.6 TB/s), by 12,288 246.
 constexpr uint32_t kSmallRows = 16, kExactRows = 128;
 constexpr uint32_t kSmallWaves = 12;
 constexpr uint32_t kAhead = 2;

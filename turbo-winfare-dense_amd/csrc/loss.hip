@@ -6,7 +6,7 @@
 // The rows that count are first gathered one behind another, so rows that are left out cost nothing and cannot spoil a
 // sum. Forward, each tile of logits is reduced where it was summed to its rows' largest value and their sum of
 // exponentials against it; a second kernel joins the tiles. Backward, a piece of the vocabulary after another: the
-// logits again, dz of them in bf16 in both orders, then the two products.
+// logits again, dz of them in bf16 by rows, then the two products.
 #include <hip/hip_runtime.h>
 
 #include <new>
@@ -172,6 +172,9 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& a, uint32_t count, 
             sum = sum * __builtin_amdgcn_exp2f((top - ref) * kLog2e) + other_sum * __builtin_amdgcn_exp2f((other_top - ref) * kLog2e);
             if (lane < 32) joint[wa * Tile::kB + in] = make_float2(both, sum);
         } else {
+            // dz is rounded to bf16, as an operand of the matrix instructions: by at most 2^-8 of each term, of d_weight in fp32
+            // too. To bf16 gradients that adds as much as their own rounding (2,048 rows: errors against 64 bits of 0.0024,
+            // 0.0017 with dz in fp32); two halves of dz would be two products more beside the step's four, a half of its time.
             const float lse = live ? a.r.lse[m] : 0.0f, grad = live ? a.r.grad[m] : 0.0f;
             store_rows<TA, uint16_t>((wave < 2 ? s0 : s1) + wave % 2 * (TA * 128),
                 [&](auto ta) {
@@ -223,7 +226,8 @@ __device__ __forceinline__ void logits_tile(const LogitArgs& a, uint32_t count, 
 // One block to a unit, whose waves hold 256 sums a lane each: the widest tile reads least through LDS. 2,048 rows of 262,144 x
 // 5,376 with a softcap take 4.65 to 4.75 ms, 1,215 to 1,240 TFLOP/s (a plain library product of the same rows 1,333): the matrix units are busy
 // in 68% of the cycles, at the clock of some 1.6 GHz that the power leaves, the rest being a tile's first loads and its
-// epilogue, which nothing covers. Tiles of 256 x 128 with two blocks to a unit, one's epilogue beside the other's products,
+// epilogue, which nothing covers: all 256 sums leave the accumulation registers at once there, and 20 registers (with dz 31) go
+// through scratch memory, none in the loop of products. Tiles of 256 x 128 with two blocks to a unit, one's epilogue beside the other's products,
 // took 6.06 ms where these took 4.90 (32,003 x 2,048 of 777 rows: 145 and 152 us). With dz stored, a piece of 65,536: 1.24 ms.
 template <bool GRAD>
 __global__ __launch_bounds__(kProductThreads) __attribute__((amdgpu_waves_per_eu(1, 1))) void loss_logits_kernel(LogitArgs a) {
@@ -510,8 +514,8 @@ namespace {
 // Up to 128 rows have tiles of all of them, so the weights are read once. f(tile): small tiles where large ones would leave
 // units idle or not fill them for two rounds (17 rows of 100,000 x 2,048: 92 and 109 us; of 151,669 x 3,584: 209 and 198; 128
 // rows of 32,003 x 1,024: 27 and 37; of 50,000 x 4,096: 121 and 109). Weights past the memory's cache are streamed (17 rows of
-// 65,537 x 2,880: 84 us, otherwise 91; of 32,003 x 2,048, which it holds: 37 and 30), those of large tiles always, as such
-// heads seldom fit, those of the smallest heads never.
+// 65,537 x 2,880: 84 us, otherwise 91; of 32,003 x 2,048, which it holds: 37 and 30), those of large tiles always, as heads of
+// more than 131,072 rows seldom fit (below a d_model of 1,024), those of the smallest heads never.
 template <typename F>
 auto with_few_tile(uint32_t rows, uint32_t vocab, uint32_t d, F&& f) {
     const bool streamed = 2ull * vocab * d > kMemoryCache;

@@ -1088,7 +1088,8 @@ class Fp8Head:
         return out
 
     def logits(self, hidden, out=None, stream=None):
-        """Logits of float32, bfloat16 or float16 hidden rows [rows, d_model], quantised on the way."""
+        """Logits of float32, bfloat16 or float16 hidden rows [rows, d_model], quantised on the way (fp8_quantize): the
+        rows are rounded to three mantissa bits first, where MxHead.logits multiplies them as they are."""
         return self.logits_fp8(*fp8_quantize(hidden, stream=stream), out=out, stream=stream)
 
 
@@ -1152,8 +1153,9 @@ class HeadLoss:
                  need=(True, True), stream=None):
         """(d_hidden, d_weight): the gradients of sum(grad * losses) from the forward pass's inputs and lse
         (twd_headloss_backward); grad is float32 [rows], all ones where not given. d_hidden is bfloat16 [rows, d_model],
-        d_weight bfloat16 or float32 [vocab, d_model] (bfloat16 where none is given), added to with accumulate. need says
-        which of the two are wanted; the other is not computed and comes back as None."""
+        d_weight bfloat16 or float32 [vocab, d_model] (bfloat16 where none is given), added to with accumulate: in float32
+        the sums are not rounded again, but each term holds a bfloat16 factor either way. need says which of the two are
+        wanted; the other is not computed and comes back as None."""
         import torch
         rows, stride, w_stride = self._inputs(hidden, weight, targets)
         if accumulate and need[1] and d_weight is None:
